@@ -144,6 +144,91 @@ int dspark_verify_attention_rec(const dspark_attn_args* args, dspark_stream_t st
 int dspark_verify_attention_rec_splits(const dspark_attn_args* args, dspark_stream_t stream);
 int dspark_verify_attention_rec_combine(const dspark_attn_args* args, dspark_stream_t stream);
 
+/* ---------------------------------------------------------------- 8-bit block-scaled K/V cache ("b8" pages)
+ * One byte a value and one fp32 scale for each block of 32 positions (a page) and KV head, K and V apart: half the bytes
+ * of the fp16 pages for either head dimension. Per attention layer code pools [kv_pages][KVH][32][D] of int8 or e4m3 (OCP:
+ * no infinities, 0x7f and 0xff no numbers), scale pools fp32 [kv_pages][KVH], and an int32 block table as above; value =
+ * code * scale, exact in fp32. Pools may pass 4 GiB. A table entry outside [0, kv_pages) is an absent page: it is neither
+ * read nor written, no query sees its positions, and they read back as zeros. Two logical pages that are written must not
+ * share a physical page.
+ * Scale of a block whose largest finite magnitude is A: int8, fp32(A / 127) rounded up to 16 significant bits; e4m3, the
+ * least power of two s with A <= 448 s; 0 for A = 0. Code: x / s rounded once to nearest, ties to even; NaN is coded 0 and
+ * an infinity as the largest code, so that a bad row does not spoil the block it shares. No counterpart in the reference,
+ * whose records hold a scale per position (ops.hip:212-224). */
+enum { DSPARK_B8_INT8 = 0, DSPARK_B8_E4M3 = 1 };
+typedef struct dspark_b8_cache {
+  void* k;                     /* codes, on a 16-byte boundary */
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  const int32_t* block_table;  /* logical -> physical page, NULL = identity */
+  int64_t kv_pages;            /* pages in each pool, < 2^31 */
+  int32_t KVH, D, code;        /* KVH <= 1024; D in {64, 128}; DSPARK_B8_* */
+} dspark_b8_cache;
+
+/* Append: K/V rows of positions pos0 .. pos0 + n - 1 from fp16 k, v [n][row_stride] (head h at h D; both on 16-byte
+ * boundaries, row_stride a multiple of 8 and >= KVH D). A page entered at its first slot starts anew. In a page entered
+ * further on the rows before pos0 stay, the scale becomes the larger of the old one and the new rows', and where it grew the
+ * rows that stay are re-coded to it (rounded once more). The cache then ends at pos0 + n: the slots behind it in the last
+ * page are cleared. A verify block is appended before its attention; rejected rows are dropped by the next append, which
+ * starts before them (their part in the page's scale stays until the page is entered at its first slot). Positions stay
+ * under 2^31 - 64. n = 0 does nothing. */
+int dspark_kv_write_b8(const dspark_b8_cache* cache, const void* k, const void* v, int64_t row_stride, int32_t pos0,
+                       int32_t n, dspark_stream_t stream);
+/* The values of positions pos0 .. pos0 + n - 1 as fp32 rows [n][row_stride] (head h at h D; 16-byte boundaries, row_stride
+ * a multiple of 4): what a prefill over a cached prefix, or a writer of another format, takes. */
+int dspark_kv_read_b8(const dspark_b8_cache* cache, int32_t pos0, int32_t n, float* k, float* v, int64_t row_stride,
+                      dspark_stream_t stream);
+
+/* Verify attention over b8 pages: the tokens, positions and visibility of dspark_verify_attention (a context key kpos < a
+ * by start and window, the block's key a + j by causal), with the rows appended by dspark_kv_write_b8 before. q fp16
+ * [M][q_stride] (head qh at qh D; 16-byte boundary, q_stride a multiple of 8): it may lie inside wider rows. Output fp16
+ * and/or fp32 [M][QH][D] on 16-byte boundaries. lse, if given: fp32 [M][QH], the natural logarithm of the sum of
+ * exp(q k / sqrt(D)) over the keys a row sees (before the gate). A row that sees no key (every page of it absent) gives
+ * zeros and lse -inf. M QH / KVH <= 1024. The workspace needs no clearing and may be shared by stream-ordered calls. The
+ * probabilities are rounded to fp16 once; scores, sums and outputs are fp32. */
+typedef struct dspark_b8_attn_args {
+  const void* q;
+  int64_t q_stride;            /* elements between tokens, >= QH D */
+  void* out;                   /* fp16 [M][QH][D] or NULL */
+  float* out_f32;              /* fp32 [M][QH][D] or NULL */
+  float* lse;                  /* fp32 [M][QH] or NULL */
+  const float* gate;           /* fp32 [M][QH] pre-sigmoid gate or NULL */
+  void* workspace;             /* size from dspark_verify_attention_b8_workspace, on a 16-byte boundary */
+  size_t workspace_bytes;
+  int32_t M, QH;               /* 1 <= M <= DSPARK_MT_MAX; QH % KVH == 0 */
+  int32_t a, start, window, causal;
+  int32_t splits;              /* key-range splits per KV head; 0 = automatic */
+} dspark_b8_attn_args;
+
+size_t dspark_verify_attention_b8_workspace(const dspark_b8_cache* cache, const dspark_b8_attn_args* args);
+int dspark_verify_attention_b8(const dspark_b8_cache* cache, const dspark_b8_attn_args* args, dspark_stream_t stream);
+
+/* The attention weight that keys have drawn, by KV head: for positions p < a + rows
+ *   mass_out[h][p] = (p < a ? mass_in[h][p] : 0) + sum over tokens t < rows and the query heads of h of
+ *                    exp(q k_p / sqrt(D) - lse[t][qh]), 0 where the token does not see p;
+ * positions from a + rows on are left as they are. The same cache and args as the attention call that gave lse (of args it
+ * reads q, q_stride, M, QH, a, start, window and causal); a row with lse -inf adds nothing. rows: device word, clamped to
+ * [0, M], NULL = M -- after dspark_accept_commit the address of State.ctx_new, so that rejected drafts draw nothing.
+ * mass_in NULL = zeros; mass_out may be mass_in itself, and must not overlap it otherwise. mass_stride elements between
+ * heads (>= a + M). Each key's sum is taken by one wave in a fixed order: no atomics. */
+int dspark_attention_mass_b8(const dspark_b8_cache* cache, const dspark_b8_attn_args* args, const float* lse,
+                             const int32_t* rows, const float* mass_in, float* mass_out, int64_t mass_stride,
+                             dspark_stream_t stream);
+
+/* Eviction: of positions 0 .. length - 1 every KV head keeps `keep`: the first `sinks`, the last `recent`, and of those
+ * between them the ones of largest mass[h][p] (among equal ones the lowest positions; NaN ranks below every number). kept
+ * [KVH][keep] receives the kept positions in ascending order, and dst's positions 0 .. keep - 1 their rows in that order: a
+ * cache of `keep` positions for every head (keys keep the rotation they were written with; later calls count positions
+ * from keep). A dst block's scale is the largest of its rows' scales; rows from blocks of a smaller one are re-coded to it
+ * (rounded once more). The slots behind keep in the last page are cleared. mass_out[h][j] = mass[h][kept[h][j]]. dst has
+ * src's KVH, D and code; its pools, kept and mass_out must share no byte with what is read (DSPARK_EINVAL). sinks + recent
+ * <= keep <= length. keep = 0 does nothing. */
+int dspark_kv_evict_b8(const dspark_b8_cache* src, const dspark_b8_cache* dst, int32_t length, int32_t keep, int32_t sinks,
+                       int32_t recent, const float* mass, int64_t mass_stride, int32_t* kept, float* mass_out,
+                       int64_t mass_out_stride, void* workspace, size_t workspace_bytes, dspark_stream_t stream);
+size_t dspark_kv_evict_b8_workspace(int32_t KVH, int32_t length);
+
 /* ---------------------------------------------------------------- verify argmax (greedy head)
  * best_keys[t] = max over r < V of key(pv, r), pv the repetition-penalised fp16-rounded logit (seen[] bitmap, plus
  * drafts tokens[1..t] not yet seen), key = ordered float bits << 32 | (0xFFFFFFFF - r). logits fp32 [M][V] or fp16

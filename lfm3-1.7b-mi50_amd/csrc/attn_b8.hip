@@ -1,0 +1,473 @@
+// Verify attention over the 8-bit block-scaled K/V cache, and the accounts of attention weight its keys draw.
+//
+// o = softmax(q k^T / sqrt(D)) v for the rows of a KV head (row r = token r / G, query head r % G of the head's), keys in
+// blocks of 32 (a page) whose codes carry one scale: x = (q . code) ks log2(e) / sqrt(D), P = 2^(x - ref), and the block's
+// share of o is vs (P . codes). Codes (int8 or e4m3) are exact in fp16, so the products on the matrix cores are of exact
+// operands but for P, which is rounded to fp16 once; scales, running references, sums and outputs are fp32.
+//
+// A wave owns whole pages and all rows of its row group, and takes its operands from memory in registers: nothing is shared
+// until the end. Score product: A = K (16 keys), B = Q, so that a lane holds one row's scores of keys 16 b + 4 g + i
+// (lane = 16 g + n, row n); these eight are, in this order, the lane's B operand of the second product (A = V^T), so P never
+// leaves its lane. The contraction order is free as long as both operands agree: dims go in 16-byte pieces of a K row, and
+// V rows are transposed in registers by byte permutes.
+#include "b8.h"
+#include "dspark.h"
+#include "dspark_internal.h"
+
+namespace dspark {
+
+constexpr int B8_WAVES = 4;
+// Running reference in log2 units: P = 2^(x - ref), ref set to the row's largest x less 8 when some x passes ref + 15:
+// P stays under 2^15, and a P of 2^-22 of the largest is still a normal half.
+constexpr float REF_INIT = -1e30f, REF_BELOW = 8.f, REF_SLACK = 15.f;
+
+template <int D>
+struct B8Tile {
+  u32x4 k[2][D / 64];  // key 16 b + n, dims 64 u + 16 g .. + 16
+  uint32_t v[8][D / 64];  // key 16 (j / 4) + 4 g + j % 4, dims (D / 16) n .. + D / 16
+};
+
+template <int D>
+__device__ __forceinline__ void b8_load_k(const uint8_t* base, int lane, u32x4 (&k)[2][D / 64]) {
+  const uint32_t off = (uint32_t)((lane & 15) * D + (lane >> 4) * 16);
+#pragma unroll
+  for (int b = 0; b < 2; ++b)
+#pragma unroll
+    for (int u = 0; u < D / 64; ++u) k[b][u] = ldg(reinterpret_cast<const u32x4*>(base + off + (16 * b * D + 64 * u)));
+}
+template <int D>
+__device__ __forceinline__ void b8_load_v(const uint8_t* base, int lane, uint32_t (&v)[8][D / 64]) {
+  const uint32_t off = (uint32_t)((lane >> 4) * 4 * D + (lane & 15) * (D / 16));
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint8_t* at = base + off + (16 * (j / 4) + j % 4) * D;
+    if constexpr (D == 64) {
+      v[j][0] = ldg(reinterpret_cast<const uint32_t*>(at));
+    } else {
+      const u32x2 t = ldg(reinterpret_cast<const u32x2*>(at));
+      v[j][0] = t[0];
+      v[j][1] = t[1];
+    }
+  }
+}
+
+// Two codes (bytes 2 H, 2 H + 1 of w) as halves, exactly. int8 codes come with their sign bit flipped (code + 128).
+template <bool FP8, bool H>
+__device__ __forceinline__ half2v b8_half2(uint32_t w) {
+  if constexpr (FP8) {
+    return __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.f, H));
+  } else {
+    const uint32_t u = __builtin_amdgcn_perm(0x64646464u, w, H ? 0x04030402u : 0x04010400u);
+    return __builtin_bit_cast(half2v, u) - half2v{1152, 1152};
+  }
+}
+template <bool FP8>
+__device__ __forceinline__ uint32_t b8_flip(uint32_t w) {
+  if constexpr (FP8) return w;
+  else return w ^ 0x80808080u;
+}
+template <bool FP8>
+__device__ __forceinline__ half8 b8_half8(uint32_t w0, uint32_t w1) {
+  const half2v a = b8_half2<FP8, false>(w0), b = b8_half2<FP8, true>(w0), c = b8_half2<FP8, false>(w1), d = b8_half2<FP8, true>(w1);
+  return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+// V^T operands of dims db and db + 1 (bytes E, E + 1 of the eight keys' words): pairs of keys by one permute for both dims.
+template <bool FP8, int E>
+__device__ __forceinline__ void b8_vt(const uint32_t (&w)[8], half8& v0, half8& v1) {
+  half2v a[4], b[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    // bytes: key 2q dim E, key 2q+1 dim E, key 2q dim E+1, key 2q+1 dim E+1
+    const uint32_t t = __builtin_amdgcn_perm(w[2 * q + 1], w[2 * q], E == 0 ? 0x05010400u : 0x07030602u);
+    a[q] = b8_half2<FP8, false>(t);
+    b[q] = b8_half2<FP8, true>(t);
+  }
+  v0 = half8{a[0][0], a[0][1], a[1][0], a[1][1], a[2][0], a[2][1], a[3][0], a[3][1]};
+  v1 = half8{b[0][0], b[0][1], b[1][0], b[1][1], b[2][0], b[2][1], b[3][0], b[3][1]};
+}
+
+// Largest over the four lanes of a row (lanes n, 16 + n, 32 + n, 48 + n), in all of them; and the sum.
+__device__ __forceinline__ float row_max(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float row_sum(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// Q operands of a row group (row0 = its first row): lane (n, g) holds row n's dims 64 u + 16 g + 8 h .. + 8. Rows past the
+// last repeat it; what is computed of them is stored nowhere.
+template <int D, int RB>
+__device__ __forceinline__ void b8_load_q(const B8Attn& p, int h, int row0, int lane, half8 (&q)[RB][D / 32], int (&tok)[RB]) {
+  const int n = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    const int row = min(row0 + 16 * rb + n, p.R - 1), t = div_by(row, p.g_div);
+    tok[rb] = t;
+    const _Float16* at = p.q + (size_t)t * p.q_stride + (size_t)(h * p.G + row - t * p.G) * D + 16 * g;
+#pragma unroll
+    for (int u = 0; u < D / 64; ++u)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) q[rb][2 * u + e] = as_half8(ldg(reinterpret_cast<const u32x4*>(at + 64 * u + 8 * e)));
+  }
+}
+// What a row sees: context keys from lo on, block keys under hi.
+__device__ __forceinline__ int row_lo(const B8Attn& p, int t) { return max(p.start, p.window > 0 ? p.a + t - p.window + 1 : 0); }
+__device__ __forceinline__ int row_hi(const B8Attn& p, int t) { return p.causal ? p.a + t + 1 : p.a + p.M; }
+
+// Scores (log2 units) of one page: x[rb][b][i] of key 16 b + 4 g + i; -inf where the row does not see it.
+template <int D, int RB, bool FP8>
+__device__ __forceinline__ void b8_scores(const B8Attn& p, const u32x4 (&k)[2][D / 64], const half8 (&q)[RB][D / 32], float ks,
+                                          bool masked, int pos, const int (&tok)[RB], int lane, f32x4 (&x)[RB][2]) {
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    half8 kf[D / 32];
+#pragma unroll
+    for (int u = 0; u < D / 64; ++u) {
+      kf[2 * u] = b8_half8<FP8>(b8_flip<FP8>(k[b][u][0]), b8_flip<FP8>(k[b][u][1]));
+      kf[2 * u + 1] = b8_half8<FP8>(b8_flip<FP8>(k[b][u][2]), b8_flip<FP8>(k[b][u][3]));
+    }
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      f32x4 s = {0, 0, 0, 0};
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e) s = mfma16x16x32(kf[e], q[rb][e], s);
+      x[rb][b] = s * ks;
+    }
+  }
+  if (masked) {
+    const int g = lane >> 4;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      const int lo = row_lo(p, tok[rb]), hi = row_hi(p, tok[rb]);
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int kp = pos + 16 * b + 4 * g + i;
+          if (kp < p.a ? kp < lo : kp >= hi) x[rb][b][i] = -INFINITY;
+        }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- attention
+template <int D, int RB, bool FP8>
+__global__ __launch_bounds__(64 * B8_WAVES) void attn_b8_kernel(B8Attn p) {
+  constexpr int ND = D / 16;
+  __shared__ float s_o[B8_WAVES][16][D + 4];
+  __shared__ f32x2 s_ml[B8_WAVES][RB * 16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+  const int h = blockIdx.y, sp = blockIdx.x, row0 = blockIdx.z * RB * 16;
+  const int end = p.page0 + p.npages;
+  const int sp0 = p.page0 + sp * p.pps, sp1 = min(end, sp0 + p.pps);
+  const int ppw = (p.pps + B8_WAVES - 1) / B8_WAVES;
+  const int w0 = min(sp1, sp0 + wave * ppw), w1 = min(sp1, w0 + ppw);
+
+  half8 q[RB][D / 32];
+  int tok[RB];
+  b8_load_q<D, RB>(p, h, row0, lane, q, tok);
+  float ref[RB], sum[RB];
+  f32x4 o[RB][ND];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    ref[rb] = REF_INIT;
+    sum[rb] = 0.f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[rb][d] = f32x4{0, 0, 0, 0};
+  }
+
+  for (int b0 = w0; b0 < w1; b0 += 64) {
+    // lane i knows page b0 + i
+    const int nb = min(64, w1 - b0);
+    const int pgl = b8_page(p.c, b0 + min(lane, nb - 1));
+    const size_t sat = (size_t)max(pgl, 0) * p.c.KVH + h;
+    const float ksl = ldg(p.c.ks + sat) * p.c2, vsl = ldg(p.c.vs + sat);
+    for (int i = 0; i < nb; ++i) {
+      const int pg = __builtin_amdgcn_readlane(pgl, i), lp = b0 + i;
+      if (pg < 0) continue;
+      const float ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ksl), i));
+      const float vs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vsl), i));
+      const size_t blk = ((size_t)pg * p.c.KVH + h) * (PAGE * D);
+      B8Tile<D> t;
+      b8_load_k<D>(p.c.k + blk, lane, t.k);
+      b8_load_v<D>(p.c.v + blk, lane, t.v);
+      f32x4 x[RB][2];
+      b8_scores<D, RB, FP8>(p, t.k, q, ks, lp < p.full_lo || lp >= p.full_hi, lp * PAGE, tok, lane, x);
+      float top[RB];
+      bool over = false;
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        top[rb] = fmaxf(fmaxf(fmaxf(x[rb][0][0], x[rb][0][1]), fmaxf(x[rb][0][2], x[rb][0][3])),
+                        fmaxf(fmaxf(x[rb][1][0], x[rb][1][1]), fmaxf(x[rb][1][2], x[rb][1][3])));
+        over |= top[rb] > ref[rb] + REF_SLACK;
+      }
+      if (__ballot(over)) {
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+          const float m = row_max(top[rb]);
+          const float to = m > ref[rb] + REF_SLACK ? m - REF_BELOW : ref[rb];
+          const float f = fast_exp2(ref[rb] - to);
+          ref[rb] = to;
+          sum[rb] *= f;
+#pragma unroll
+          for (int d = 0; d < ND; ++d) o[rb][d] *= f;
+        }
+      }
+      half8 pf[RB];
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float e = fast_exp2(x[rb][j / 4][j % 4] - ref[rb]);
+          sum[rb] += e;
+          pf[rb][j] = (_Float16)e;
+        }
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) {
+        uint32_t w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = b8_flip<FP8>(t.v[j][c]);
+        half8 vt[4];
+        b8_vt<FP8, 0>(w, vt[0], vt[1]);
+        b8_vt<FP8, 2>(w, vt[2], vt[3]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb) {
+            const f32x4 y = mfma16x16x32(vt[e], pf[rb], f32x4{0, 0, 0, 0});
+            o[rb][4 * c + e] += y * vs;
+          }
+      }
+    }
+  }
+
+  // The waves' shares, rescaled to the largest reference, added in wave order. Lane (n, g) holds row n's dims
+  // (D / 16) (4 g + i) + db at o[db][i].
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    sum[rb] = row_sum(sum[rb]);
+    if (g == 0) s_ml[wave][16 * rb + n] = f32x2{ref[rb], sum[rb]};
+  }
+  __syncthreads();
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    float m = REF_INIT;
+#pragma unroll
+    for (int w = 0; w < B8_WAVES; ++w) m = fmaxf(m, s_ml[w][16 * rb + n][0]);
+    const float f = fast_exp2(ref[rb] - m);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int d = 0; d < ND; d += 4) {
+        f32x4 y = {o[rb][d][i] * f, o[rb][d + 1][i] * f, o[rb][d + 2][i] * f, o[rb][d + 3][i] * f};
+        *reinterpret_cast<f32x4*>(&s_o[wave][n][ND * (4 * g + i) + d]) = y;
+      }
+    __syncthreads();
+    for (int e = threadIdx.x; e < 16 * (D / 4); e += 64 * B8_WAVES) {
+      const int r = e / (D / 4), c = e % (D / 4), row = row0 + 16 * rb + r;
+      f32x4 acc = {0, 0, 0, 0};
+      float mm = REF_INIT, l = 0.f;
+#pragma unroll
+      for (int w = 0; w < B8_WAVES; ++w) {
+        acc += *reinterpret_cast<const f32x4*>(&s_o[w][r][4 * c]);
+        mm = fmaxf(mm, s_ml[w][16 * rb + r][0]);
+      }
+#pragma unroll
+      for (int w = 0; w < B8_WAVES; ++w) l += s_ml[w][16 * rb + r][1] * fast_exp2(s_ml[w][16 * rb + r][0] - mm);
+      if (row < p.R) {
+        const size_t at = ((size_t)h * p.R + row) * p.S + sp;
+        *reinterpret_cast<f32x4*>(p.part_acc + at * D + 4 * c) = acc;
+        if (c == 0) p.part_ml[at] = f32x2{mm, l};
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// One workgroup per (row, KV head): the splits' shares rescaled and added, 256 / (D / 4) splits side by side, in a fixed
+// order; then 1 / sum, the gate, and the stores.
+template <int D>
+__global__ __launch_bounds__(256) void attn_b8_merge_kernel(B8Attn p) {
+  constexpr int Q = D / 4, SL = 256 / Q;
+  __shared__ f32x4 s_acc[SL][Q];
+  __shared__ float s_m[SL], s_l[SL];
+  const int row = blockIdx.x, h = blockIdx.y, c = threadIdx.x % Q, j = threadIdx.x / Q;
+  const size_t at = ((size_t)h * p.R + row) * p.S;
+  float m = REF_INIT, l = 0.f;
+  f32x4 acc = {0, 0, 0, 0};
+  for (int s = j; s < p.S; s += SL) {
+    const f32x2 ml = ldg(p.part_ml + at + s);
+    const f32x4 a = ldg(reinterpret_cast<const f32x4*>(p.part_acc + (at + s) * D + 4 * c));
+    const float to = fmaxf(m, ml[0]), f0 = fast_exp2(m - to), f1 = fast_exp2(ml[0] - to);
+    acc = acc * f0 + a * f1;
+    l = l * f0 + ml[1] * f1;
+    m = to;
+  }
+  s_acc[j][c] = acc;
+  if (c == 0) {
+    s_m[j] = m;
+    s_l[j] = l;
+  }
+  __syncthreads();
+  if (j) return;
+  for (int s = 0; s < SL; ++s) m = fmaxf(m, s_m[s]);
+  acc = f32x4{0, 0, 0, 0};
+  l = 0.f;
+  for (int s = 0; s < SL; ++s) {
+    const float f = fast_exp2(s_m[s] - m);
+    acc += s_acc[s][c] * f;
+    l += s_l[s] * f;
+  }
+  const int t = row / p.G, qh = h * p.G + row % p.G;
+  const float gv = p.gate ? 1.f / (1.f + __expf(-p.gate[(size_t)t * p.QH + qh])) : 1.f;
+  const f32x4 o = l == 0.f ? f32x4{0, 0, 0, 0} : acc * (gv / l);
+  const size_t e = ((size_t)t * p.QH + qh) * D + 4 * c;
+  if (p.out16) *reinterpret_cast<half4*>(p.out16 + e) = half4{(_Float16)o[0], (_Float16)o[1], (_Float16)o[2], (_Float16)o[3]};
+  if (p.out32) *reinterpret_cast<f32x4*>(p.out32 + e) = o;
+  if (p.lse && c == 0) p.lse[(size_t)t * p.QH + qh] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+}
+
+// ---------------------------------------------------------------- accounts of attention weight
+// mass_out[h][p] = (p < a ? mass_in[h][p] : 0) + sum over the rows of exp(score - lse), p < a + rows. A wave owns whole
+// pages, so every key's sum is one wave's, in a fixed order and without atomics. K alone is read.
+template <int D, int RB, bool FP8>
+__global__ __launch_bounds__(64 * B8_WAVES) void mass_b8_kernel(B8Attn p) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+  const int h = blockIdx.y;
+  const int rows = p.rows ? min(max(ldc(p.rows), 0), p.M) : p.M;
+  const int end = p.page0 + p.npages;
+  const int w0 = min(end, p.page0 + ((int)blockIdx.x * B8_WAVES + wave) * p.pps), w1 = min(end, w0 + p.pps);
+  const float* in = p.mass_in ? p.mass_in + (size_t)h * p.mass_stride : nullptr;
+  float* out = p.mass_out + (size_t)h * p.mass_stride;
+  const int live = p.a + rows, R = rows * p.G;
+  for (int lp = w0; lp < w1; ++lp) {
+    const int pg = b8_page(p.c, lp);
+    const bool seen = pg >= 0 && (lp + 1) * (int64_t)PAGE > p.full_lo;  // full_lo: the first position any row sees
+    f32x4 acc[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+    if (seen) {
+      const float ks = ldg(p.c.ks + (size_t)pg * p.c.KVH + h) * p.c2;
+      u32x4 k[2][D / 64];
+      b8_load_k<D>(p.c.k + ((size_t)pg * p.c.KVH + h) * (PAGE * D), lane, k);
+      for (int row0 = 0; row0 < R; row0 += 16 * RB) {
+        half8 q[RB][D / 32];
+        int tok[RB];
+        b8_load_q<D, RB>(p, h, row0, lane, q, tok);
+        f32x4 x[RB][2];
+        b8_scores<D, RB, FP8>(p, k, q, ks, true, lp * PAGE, tok, lane, x);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+          const int row = row0 + 16 * rb + n;
+          float l2 = -INFINITY;
+          if (row < R) l2 = ldg(p.lse_in + (size_t)tok[rb] * p.QH + h * p.G + row - tok[rb] * p.G) * 1.44269504088896341f;
+          if (l2 == -INFINITY) continue;  // past the rows, or a row that sees nothing
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[b][i] += fast_exp2(x[rb][b][i] - l2);
+        }
+      }
+    }
+    // over the 16 rows of a lane group
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float v = acc[b][i];
+        v += __uint_as_float(row_ror<8>(__float_as_uint(v)));
+        v += __uint_as_float(row_ror<4>(__float_as_uint(v)));
+        v += __uint_as_float(row_ror<2>(__float_as_uint(v)));
+        v += __uint_as_float(row_ror<1>(__float_as_uint(v)));
+        acc[b][i] = v;
+      }
+    if (n < 8) {  // lane (n, g) stores key 16 (n / 4) + 4 g + n % 4
+      const int kp = lp * PAGE + 16 * (n >> 2) + 4 * g + (n & 3);
+      float v = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v = n == j ? acc[j / 4][j % 4] : v;
+      if (kp < live) out[kp] = (kp < p.a && in ? ldg(in + kp) : 0.f) + v;
+    }
+  }
+}
+
+// ---------------------------------------------------------------- plans and launches
+constexpr int B8_ROW_BLOCKS = 4;  // most 16-row blocks of a row group
+
+void b8_attn_plan(B8Attn& p, int D, int splits, int cus) {
+  p.R = p.G * p.M;
+  const int blocks = (p.R + 15) / 16;
+  p.RG = (blocks + B8_ROW_BLOCKS - 1) / B8_ROW_BLOCKS;
+  p.rb = (blocks + p.RG - 1) / p.RG;
+  p.g_div = div_magic((uint32_t)p.G);
+  const int lo = std::min(p.a, std::max(p.start, p.window > 0 ? p.a - p.window + 1 : 0));  // first key any row sees
+  p.page0 = lo / PAGE;
+  p.npages = (p.a + p.M - 1) / PAGE + 1 - p.page0;
+  const int whole = std::max(p.start, p.window > 0 ? p.a + p.M - p.window : 0);            // first context key all rows see
+  p.full_lo = (std::max(whole, 0) + PAGE - 1) / PAGE;
+  p.full_hi = p.a / PAGE;
+  p.c2 = 1.4426950408889634f / std::sqrt((float)D);
+  int S = splits > 0 ? splits : std::max(1, 2 * cus / (p.c.KVH * p.RG));
+  S = std::min(S, (p.npages + B8_WAVES - 1) / B8_WAVES);
+  S = std::max(1, std::min(S, 4096));
+  p.pps = (p.npages + S - 1) / S;
+  p.S = (p.npages + p.pps - 1) / p.pps;
+}
+
+size_t b8_attn_workspace(const B8Attn& p, int D) {
+  const size_t rows = (size_t)p.c.KVH * p.R * p.S;
+  return rows * D * sizeof(float) + rows * sizeof(f32x2);
+}
+
+template <int D, bool FP8>
+static void attn_b8_by_rows(const B8Attn& p, hipStream_t s) {
+  const dim3 grid(p.S, p.c.KVH, p.RG), block(64 * B8_WAVES);
+  switch (p.rb) {
+    case 1: hipLaunchKernelGGL((attn_b8_kernel<D, 1, FP8>), grid, block, 0, s, p); break;
+    case 2: hipLaunchKernelGGL((attn_b8_kernel<D, 2, FP8>), grid, block, 0, s, p); break;
+    case 3: hipLaunchKernelGGL((attn_b8_kernel<D, 3, FP8>), grid, block, 0, s, p); break;
+    default: hipLaunchKernelGGL((attn_b8_kernel<D, 4, FP8>), grid, block, 0, s, p); break;
+  }
+}
+
+int b8_attn_launch(const B8Attn& p, int D, bool fp8, hipStream_t s) {
+  if (D == 64) fp8 ? attn_b8_by_rows<64, true>(p, s) : attn_b8_by_rows<64, false>(p, s);
+  else fp8 ? attn_b8_by_rows<128, true>(p, s) : attn_b8_by_rows<128, false>(p, s);
+  if (const int rc = (int)hipGetLastError()) return rc;
+  const dim3 grid(p.R, p.c.KVH);
+  if (D == 64) hipLaunchKernelGGL(attn_b8_merge_kernel<64>, grid, dim3(256), 0, s, p);
+  else hipLaunchKernelGGL(attn_b8_merge_kernel<128>, grid, dim3(256), 0, s, p);
+  return (int)hipGetLastError();
+}
+
+template <int D, bool FP8>
+static void mass_b8_by_rows(const B8Attn& p, dim3 grid, hipStream_t s) {
+  const dim3 block(64 * B8_WAVES);
+  switch (p.rb) {
+    case 1: hipLaunchKernelGGL((mass_b8_kernel<D, 1, FP8>), grid, block, 0, s, p); break;
+    case 2: hipLaunchKernelGGL((mass_b8_kernel<D, 2, FP8>), grid, block, 0, s, p); break;
+    default: hipLaunchKernelGGL((mass_b8_kernel<D, 4, FP8>), grid, block, 0, s, p); break;
+  }
+}
+
+int b8_mass_launch(const B8Attn& q, int D, bool fp8, int cus, hipStream_t s) {
+  B8Attn p = q;
+  p.R = p.G * p.M;
+  p.rb = std::min(B8_ROW_BLOCKS, (p.R + 15) / 16);
+  p.g_div = div_magic((uint32_t)p.G);
+  p.full_lo = std::min(p.a, std::max(p.start, p.window > 0 ? p.a - p.window + 1 : 0));
+  p.page0 = 0;  // every account is carried over, those of keys out of sight too
+  p.npages = (p.a + p.M - 1) / PAGE + 1;
+  p.c2 = 1.4426950408889634f / std::sqrt((float)D);
+  p.pps = std::max(1, p.npages * p.c.KVH / (8 * cus * 2));
+  const dim3 grid((p.npages + p.pps * B8_WAVES - 1) / (p.pps * B8_WAVES), p.c.KVH);
+  if (D == 64) fp8 ? mass_b8_by_rows<64, true>(p, grid, s) : mass_b8_by_rows<64, false>(p, grid, s);
+  else fp8 ? mass_b8_by_rows<128, true>(p, grid, s) : mass_b8_by_rows<128, false>(p, grid, s);
+  return (int)hipGetLastError();
+}
+
+}  // namespace dspark

@@ -40,6 +40,20 @@ class AttnArgs(ctypes.Structure):
                 ("causal", ctypes.c_int32), ("splits", ctypes.c_int32)]
 
 
+class B8CacheArgs(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+                ("block_table", ctypes.c_void_p), ("kv_pages", ctypes.c_int64), ("KVH", ctypes.c_int32),
+                ("D", ctypes.c_int32), ("code", ctypes.c_int32)]
+
+
+class B8AttnArgs(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("q_stride", ctypes.c_int64), ("out", ctypes.c_void_p), ("out_f32", ctypes.c_void_p),
+                ("lse", ctypes.c_void_p), ("gate", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+                ("workspace_bytes", ctypes.c_size_t), ("M", ctypes.c_int32), ("QH", ctypes.c_int32), ("a", ctypes.c_int32),
+                ("start", ctypes.c_int32), ("window", ctypes.c_int32), ("causal", ctypes.c_int32),
+                ("splits", ctypes.c_int32)]
+
+
 _lib = None
 
 _SIGS = {
@@ -62,6 +76,21 @@ _SIGS = {
     "dspark_verify_attention_rec": (ctypes.c_int, [ctypes.POINTER(AttnArgs), ctypes.c_void_p]),
     "dspark_verify_attention_rec_splits": (ctypes.c_int, [ctypes.POINTER(AttnArgs), ctypes.c_void_p]),
     "dspark_verify_attention_rec_combine": (ctypes.c_int, [ctypes.POINTER(AttnArgs), ctypes.c_void_p]),
+    "dspark_kv_write_b8": (ctypes.c_int, [ctypes.POINTER(B8CacheArgs), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
+                                          ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p]),
+    "dspark_kv_read_b8": (ctypes.c_int, [ctypes.POINTER(B8CacheArgs), ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,
+                                         ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
+    "dspark_verify_attention_b8_workspace": (ctypes.c_size_t, [ctypes.POINTER(B8CacheArgs), ctypes.POINTER(B8AttnArgs)]),
+    "dspark_verify_attention_b8": (ctypes.c_int, [ctypes.POINTER(B8CacheArgs), ctypes.POINTER(B8AttnArgs),
+                                                  ctypes.c_void_p]),
+    "dspark_attention_mass_b8": (ctypes.c_int, [ctypes.POINTER(B8CacheArgs), ctypes.POINTER(B8AttnArgs), ctypes.c_void_p,
+                                                ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
+                                                ctypes.c_void_p]),
+    "dspark_kv_evict_b8": (ctypes.c_int, [ctypes.POINTER(B8CacheArgs), ctypes.POINTER(B8CacheArgs), ctypes.c_int32,
+                                          ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64,
+                                          ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
+                                          ctypes.c_size_t, ctypes.c_void_p]),
+    "dspark_kv_evict_b8_workspace": (ctypes.c_size_t, [ctypes.c_int32, ctypes.c_int32]),
     "dspark_rope_table": (ctypes.c_int, [ctypes.c_float, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
                                          ctypes.c_void_p]),
     "dspark_verify_argmax_workspace": (ctypes.c_size_t, [ctypes.c_int32, ctypes.c_int32]),
@@ -293,6 +322,211 @@ def verify_attention_rec(q, pages, a, start=0, window=0, causal=True, out=None, 
     args.workspace, args.workspace_bytes = ws.data_ptr(), ws.numel()
     check(lib().dspark_verify_attention_rec(ctypes.byref(args), stream_handle(stream)), "dspark_verify_attention_rec")
     return out, out_f32
+
+
+# ---------------------------------------------------------------- 8-bit block-scaled K/V cache
+B8_INT8, B8_E4M3 = 0, 1
+
+
+class B8Cache:
+    """A cache of "b8" pages (include/dspark.h): codes k, v [n_pages][KVH][32][D] as torch.int8 or torch.float8_e4m3fn,
+    scales fp32 [n_pages][KVH], and an int32 block table (None = identity). Holds the tensors and their descriptor."""
+
+    def __init__(self, k, v, k_scale, v_scale, block_table=None):
+        torch = _torch()
+        codes = {torch.int8: B8_INT8, torch.float8_e4m3fn: B8_E4M3}
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in codes or k.shape[2] != PAGE:
+            raise DsparkError("B8Cache: k and v are [n_pages][KVH][32][D] of int8 or float8_e4m3fn")
+        for t in (k_scale, v_scale):
+            if t.shape != k.shape[:2] or t.dtype != torch.float32:
+                raise DsparkError("B8Cache: scales are fp32 [n_pages][KVH]")
+        if block_table is not None and (block_table.dtype != torch.int32 or block_table.dim() != 1):
+            raise DsparkError("B8Cache: the block table is int32 [pages]")
+        every = [t for t in (k, v, k_scale, v_scale, block_table) if t is not None]
+        if any(t.device != k.device or not t.is_contiguous() for t in every):
+            raise DsparkError("B8Cache: contiguous tensors of one device")
+        self.k, self.v, self.k_scale, self.v_scale, self.block_table = k, v, k_scale, v_scale, block_table
+        self.KVH, self.D, self.device = k.shape[1], k.shape[3], k.device
+        self.args = B8CacheArgs(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                                None if block_table is None else block_table.data_ptr(), k.shape[0], self.KVH, self.D,
+                                codes[k.dtype])
+        self.ref = ctypes.byref(self.args)
+
+    def check(self, end, *tensors):
+        """`end` positions have table entries, and the tensors are the cache's device's."""
+        if self.block_table is not None and (end + PAGE - 1) // PAGE > self.block_table.shape[0]:
+            raise DsparkError(f"{end} positions need {(end + PAGE - 1) // PAGE} entries in the block table")
+        for t in tensors:
+            if t is not None and t.device != self.device:
+                raise DsparkError("tensors and cache are on different devices")
+
+
+def b8_cache_alloc(n_pages, KVH, D, dtype=None, device="cuda", block_table=None):
+    """An empty cache; dtype torch.int8 (the default) or torch.float8_e4m3fn."""
+    torch = _torch()
+    codes = [torch.zeros((n_pages, KVH, PAGE, D), dtype=torch.uint8, device=device).view(dtype or torch.int8) for _ in "kv"]
+    scales = [torch.zeros((n_pages, KVH), dtype=torch.float32, device=device) for _ in "kv"]
+    return B8Cache(*codes, *scales, block_table)
+
+
+class _on:
+    """The device of a cache current, and `stream` (default: that device's current stream) the one that allocations belong
+    to; yields the stream's handle. Costs nothing where both are current already."""
+
+    def __init__(self, device, stream):
+        torch = _torch()
+        self.guard = None
+        if stream is None and torch.cuda.current_device() == device.index:
+            self.stream = torch.cuda.current_stream()
+        else:
+            self.stream = stream if stream is not None else torch.cuda.current_stream(device)
+            if self.stream.device != device:
+                raise DsparkError("the stream belongs to another device than the cache")
+            self.guard = torch.cuda.stream(self.stream)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        return self.stream.cuda_stream
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _b8_row(t, KVH, D, what):
+    """Elements between the rows of a [n][KVH][D] (or [n][row]) tensor whose rows are contiguous."""
+    inner = t.stride(-1) == 1 and (t.dim() == 2 or t.stride(1) == D)
+    if t.dim() not in (2, 3) or not inner or (t.shape[1:] != (KVH, D) if t.dim() == 3 else t.shape[1] < KVH * D):
+        raise DsparkError(f"{what}: rows of {KVH} heads x {D}")
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), KVH * D)
+
+
+def kv_write_b8(k, v, cache, pos0, stream=None):
+    """Append k, v fp16 [n][KVH][D] (or [n][row >= KVH*D]; rows may lie inside wider ones) as positions pos0 .. pos0+n-1."""
+    torch = _torch()
+    n = k.shape[0]
+    row = _b8_row(k, cache.KVH, cache.D, "kv_write_b8")
+    if v.shape != k.shape or (n > 1 and _b8_row(v, cache.KVH, cache.D, "kv_write_b8") != row):
+        raise DsparkError("kv_write_b8: k and v of one shape and row stride")
+    if k.dtype != torch.float16 or v.dtype != torch.float16:
+        raise DsparkError("kv_write_b8: k and v are fp16")
+    cache.check(pos0 + n, k, v)
+    with _on(cache.device, stream) as s:
+        check(lib().dspark_kv_write_b8(cache.ref, k.data_ptr(), v.data_ptr(), row, pos0, n, s), "dspark_kv_write_b8")
+
+
+def kv_read_b8(cache, pos0, n, k=None, v=None, stream=None):
+    """The values of positions pos0 .. pos0+n-1 as fp32 [n][KVH][D] tensors (given, as rows, or created)."""
+    torch = _torch()
+    cache.check(pos0 + n, k, v)
+    with _on(cache.device, stream) as s:
+        if k is None or v is None:
+            new = torch.empty((2, n, cache.KVH, cache.D), dtype=torch.float32, device=cache.device)
+            k, v = new[0], new[1]
+        row = _b8_row(k, cache.KVH, cache.D, "kv_read_b8")
+        if k.dtype != torch.float32 or v.dtype != torch.float32 or k.shape[0] < n or v.shape != k.shape \
+                or _b8_row(v, cache.KVH, cache.D, "kv_read_b8") != row:
+            raise DsparkError("kv_read_b8: k and v are fp32 rows of one shape and stride")
+        check(lib().dspark_kv_read_b8(cache.ref, pos0, n, k.data_ptr(), v.data_ptr(), row, s), "dspark_kv_read_b8")
+    return k, v
+
+
+def _b8_attn_args(q, cache, a, start, window, causal):
+    torch = _torch()
+    M, QH, D = q.shape
+    if q.dtype != torch.float16 or D != cache.D or q.stride(2) != 1 or q.stride(1) != D:
+        raise DsparkError("q is fp16 [M][QH][D] of contiguous rows, D the cache's")
+    cache.check(a + M, q)
+    args = B8AttnArgs()
+    args.q, args.q_stride = q.data_ptr(), q.stride(0) if M > 1 else max(q.stride(0), QH * D)
+    args.M, args.QH, args.a, args.start, args.window, args.causal = M, QH, a, start, window, int(causal)
+    return args
+
+
+def _b8_full(t, shape, dtype, cache, what):
+    """The data pointer of an optional tensor that has to be contiguous and of this shape and type."""
+    if t is None:
+        return None
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous() or t.device != cache.device:
+        raise DsparkError(f"{what} is a contiguous {dtype} tensor of shape {tuple(shape)} on the cache's device")
+    return t.data_ptr()
+
+
+def verify_attention_b8(q, cache, a, start=0, window=0, causal=True, out=None, out_f32=None, lse=None, gate=None, splits=0,
+                        workspace=None, stream=None):
+    """verify_attention over a B8Cache that holds positions 0..a+M-1. q fp16 [M][QH][D]; lse (optional) fp32 [M][QH] receives
+    the log-sum-exp of the scores. Returns (out fp16, out_f32) tensors as given/created."""
+    torch = _torch()
+    M, QH, D = q.shape
+    args = _b8_attn_args(q, cache, a, start, window, causal)
+    with _on(cache.device, stream) as s:
+        if out is None and out_f32 is None:
+            out = torch.empty((M, QH, D), dtype=torch.float16, device=q.device)
+        args.out = _b8_full(out, (M, QH, D), torch.float16, cache, "out")
+        args.out_f32 = _b8_full(out_f32, (M, QH, D), torch.float32, cache, "out_f32")
+        args.lse = _b8_full(lse, (M, QH), torch.float32, cache, "lse")
+        args.gate = _b8_full(gate, (M, QH), torch.float32, cache, "gate")
+        args.splits = splits
+        ref = ctypes.byref(args)
+        need = lib().dspark_verify_attention_b8_workspace(cache.ref, ref)
+        if need == 0:
+            raise DsparkError("dspark_verify_attention_b8_workspace rejected the arguments")
+        ws = (workspace or Workspace(q.device)).get(need)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), ws.numel()
+        check(lib().dspark_verify_attention_b8(cache.ref, ref, s), "dspark_verify_attention_b8")
+    return out, out_f32
+
+
+def attention_mass_b8(q, cache, a, lse, mass_out, mass_in=None, rows=None, start=0, window=0, causal=True, stream=None):
+    """Add the attention weights of tokens t < rows (an int32 device word, None = all of q's) to the accounts of the keys they
+    see: mass_out fp32 [KVH][>= a+M] from mass_in (None = zeros, or mass_out itself) and verify_attention_b8's lse."""
+    torch = _torch()
+    M, QH, D = q.shape
+    args = _b8_attn_args(q, cache, a, start, window, causal)
+    lse_ptr = _b8_full(lse, (M, QH), torch.float32, cache, "lse")
+    stride = _b8_accounts(mass_out, a + M, cache, "mass_out")
+    if lse_ptr is None or (mass_in is not None and _b8_accounts(mass_in, a + M, cache, "mass_in") != stride):
+        raise DsparkError("attention_mass_b8: lse is given, and mass_in and mass_out have one stride")
+    if rows is not None and (rows.dtype != torch.int32 or rows.numel() < 1 or rows.device != cache.device):
+        raise DsparkError("attention_mass_b8: rows is an int32 word on the cache's device")
+    with _on(cache.device, stream) as s:
+        check(lib().dspark_attention_mass_b8(cache.ref, ctypes.byref(args), lse_ptr,
+                                             None if rows is None else rows.data_ptr(),
+                                             None if mass_in is None else mass_in.data_ptr(), mass_out.data_ptr(), stride, s),
+              "dspark_attention_mass_b8")
+    return mass_out
+
+
+def _b8_accounts(t, n, cache, what):
+    """Elements between the heads of an fp32 [KVH][>= n] tensor."""
+    if t.dim() != 2 or t.shape[0] != cache.KVH or t.shape[1] < n or t.dtype != _torch().float32 \
+            or (t.shape[1] > 1 and t.stride(1) != 1) or t.device != cache.device:
+        raise DsparkError(f"{what} is fp32 [KVH][>= {n}] on the cache's device")
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def kv_evict_b8(cache, dst, length, keep, mass, sinks=0, recent=0, kept=None, mass_out=None, workspace=None, stream=None):
+    """Keep `keep` of the cache's `length` positions per KV head -- the first `sinks`, the last `recent`, and the rest by mass
+    (fp32 [KVH][>= length]) -- as positions 0..keep-1 of `dst`, another B8Cache of the same heads and codes. Returns
+    (kept int32 [KVH][keep] ascending, their mass), as given/created."""
+    torch = _torch()
+    cache.check(length, mass, kept, mass_out, dst.k)
+    dst.check(keep)
+    stride = _b8_accounts(mass, length, cache, "mass")
+    with _on(cache.device, stream) as s:
+        if kept is None:
+            kept = torch.empty((cache.KVH, keep), dtype=torch.int32, device=cache.device)
+        if mass_out is None:
+            mass_out = torch.empty((cache.KVH, keep), dtype=torch.float32, device=cache.device)
+        kept_ptr = _b8_full(kept, (cache.KVH, keep), torch.int32, cache, "kept")
+        out_stride = _b8_accounts(mass_out, keep, cache, "mass_out")
+        need = lib().dspark_kv_evict_b8_workspace(cache.KVH, length)
+        ws = (workspace or Workspace(cache.device)).get(need) if need else None
+        check(lib().dspark_kv_evict_b8(cache.ref, dst.ref, length, keep, sinks, recent, mass.data_ptr(), stride, kept_ptr,
+                                       mass_out.data_ptr(), out_stride, None if ws is None else ws.data_ptr(),
+                                       0 if ws is None else ws.numel(), s), "dspark_kv_evict_b8")
+    return kept, mass_out
 
 
 # ---------------------------------------------------------------- argmax / accept

@@ -1,0 +1,164 @@
+"""CPU checks of the 8-bit block-scaled cache: what its entry points refuse before any launch (placeholder pointers are never
+dereferenced), what the binding refuses, and the restatement's own properties."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from conftest import load_host
+from oracle import b8
+
+EINVAL, ENOSPACE = 1001, 1002
+
+
+def cache(**kw):
+    h = load_host()
+    c = h.B8CacheArgs(1 << 20, 2 << 20, 3 << 20, 4 << 20, None, 100, 8, 64, 0)
+    for k, v in kw.items():
+        setattr(c, k, v)
+    return c
+
+
+def attn(**kw):
+    h = load_host()
+    a = h.B8AttnArgs(q=16, q_stride=2048, out=16, workspace=16, workspace_bytes=1 << 40, M=16, QH=32, a=1000, causal=1)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+BAD_CACHE = [dict(k=None), dict(v=None), dict(k_scale=None), dict(v_scale=None), dict(k=(1 << 20) + 8), dict(v=(2 << 20) + 4),
+             dict(k_scale=(3 << 20) + 2), dict(block_table=6), dict(kv_pages=0), dict(kv_pages=1 << 31), dict(KVH=0),
+             dict(KVH=1025), dict(D=96), dict(D=0), dict(code=2), dict(code=-1)]
+
+
+@pytest.mark.parametrize("bad", BAD_CACHE)
+def test_every_call_checks_the_cache(bad):
+    L = load_host().lib()
+    c, ok, a = ctypes.byref(cache(**bad)), ctypes.byref(cache()), ctypes.byref(attn())
+    assert L.dspark_kv_write_b8(c, 16, 16, 512, 0, 1, None) == EINVAL
+    assert L.dspark_kv_read_b8(c, 0, 1, 16, 16, 512, None) == EINVAL
+    assert L.dspark_verify_attention_b8(c, a, None) == EINVAL
+    assert L.dspark_verify_attention_b8_workspace(c, a) == 0
+    assert L.dspark_attention_mass_b8(c, a, 16, None, None, 16, 4096, None) == EINVAL
+    for src, dst in ((c, ok), (ok, c)):
+        assert L.dspark_kv_evict_b8(src, dst, 64, 32, 0, 0, 16, 64, 1 << 30, 1 << 31, 64, None, 0, None) == EINVAL
+
+
+def test_writer_and_reader_refuse():
+    L = load_host().lib()
+    c = ctypes.byref(cache())
+    wide = ctypes.byref(cache(block_table=64))
+    for args in ((None, 16, 512, 0, 1), (16, None, 512, 0, 1), (8, 16, 512, 0, 1), (16, 8, 512, 0, 1), (16, 16, 504, 0, 1),
+                 (16, 16, 516, 0, 1), (16, 16, 512, -1, 1), (16, 16, 512, 0, -1), (16, 16, 512, 3199, 2)):
+        assert L.dspark_kv_write_b8(c, *args, None) == EINVAL, args
+    for k, v, row, pos0, n in ((None, 16, 512, 0, 1), (16, None, 512, 0, 1), (8, 16, 512, 0, 1), (16, 16, 508, 0, 1),
+                               (16, 16, 514, 0, 1), (16, 16, 512, -1, 1), (16, 16, 512, 0, -1), (16, 16, 512, 3199, 2)):
+        assert L.dspark_kv_read_b8(c, pos0, n, k, v, row, None) == EINVAL
+    # positions past 2^31 - 64, with a table too
+    assert L.dspark_kv_write_b8(wide, 16, 16, 512, (1 << 31) - 64, 1, None) == EINVAL
+    assert L.dspark_kv_read_b8(wide, (1 << 31) - 64, 1, 16, 16, 512, None) == EINVAL
+    # nothing to do: nothing is launched
+    assert L.dspark_kv_write_b8(c, None, None, 0, 5, 0, None) == 0
+    assert L.dspark_kv_read_b8(c, 5, 0, None, None, 0, None) == 0
+
+
+BAD_ROWS = [dict(M=0), dict(M=65), dict(QH=4), dict(QH=12), dict(QH=0), dict(a=-1), dict(start=-1), dict(window=-1),
+            dict(splits=-1), dict(a=3190), dict(a=(1 << 31) - 70), dict(QH=8 * 17, M=64)]
+
+
+@pytest.mark.parametrize("bad", BAD_ROWS)
+def test_attention_checks_its_shape(bad):
+    L = load_host().lib()
+    c, a = ctypes.byref(cache()), ctypes.byref(attn(q_stride=1 << 20, **bad))
+    assert L.dspark_verify_attention_b8_workspace(c, a) == 0
+    assert L.dspark_verify_attention_b8(c, a, None) == EINVAL
+    assert L.dspark_attention_mass_b8(c, a, 16, None, None, 16, 1 << 40, None) == EINVAL
+
+
+def test_attention_checks_its_pointers_and_workspace():
+    L = load_host().lib()
+    c = ctypes.byref(cache())
+    for bad in (dict(q=None), dict(q=8), dict(q_stride=2040), dict(q_stride=2052), dict(out=None), dict(out=8),
+                dict(out_f32=8)):
+        assert L.dspark_verify_attention_b8(c, ctypes.byref(attn(**bad)), None) == EINVAL, bad
+    need = L.dspark_verify_attention_b8_workspace(c, ctypes.byref(attn()))
+    assert need > 0
+    for bad in (dict(workspace=None), dict(workspace=8), dict(workspace_bytes=need - 1)):
+        assert L.dspark_verify_attention_b8(c, ctypes.byref(attn(**bad)), None) == ENOSPACE, bad
+    a, M = 1000, 16
+    ok = ctypes.byref(attn())
+    for lse, rows, mi, mo, stride in ((None, None, None, 16, 4096), (2, None, None, 16, 4096), (16, 2, None, 16, 4096),
+                                      (16, None, 2, 16, 4096), (16, None, None, None, 4096), (16, None, None, 16, a + M - 1),
+                                      (16, None, 1 << 20, (1 << 20) + 4, 4096), (16, None, (1 << 20) + 4 * 4096, 1 << 20, 4096)):
+        assert L.dspark_attention_mass_b8(c, ok, lse, rows, mi, mo, stride, None) == EINVAL
+
+
+def test_eviction_refuses():
+    L = load_host().lib()
+    src, dst = cache(), cache(k=16 << 20, v=32 << 20, k_scale=48 << 20, v_scale=49 << 20)
+    mass, kept, out = 64 << 20, 65 << 20, 66 << 20
+
+    def call(s=src, d=dst, length=640, keep=320, sinks=4, recent=32, m=mass, ms=640, k=kept, mo=out, mos=320):
+        return L.dspark_kv_evict_b8(ctypes.byref(s), ctypes.byref(d), length, keep, sinks, recent, m, ms, k, mo, mos, None, 0,
+                                    None)
+    assert call(keep=0, sinks=0, recent=0) == 0
+    for bad in (dict(length=-1), dict(keep=-1), dict(keep=641), dict(sinks=-1), dict(recent=-1), dict(sinks=300, recent=21),
+                dict(sinks=(1 << 31) - 1, recent=(1 << 31) - 1), dict(length=3201), dict(m=None), dict(k=None), dict(mo=None),
+                dict(ms=639), dict(mos=319)):
+        assert call(**bad) == EINVAL, bad
+    for d in (cache(k=16 << 20, v=32 << 20, k_scale=48 << 20, v_scale=49 << 20, **x)
+              for x in (dict(KVH=4), dict(D=128), dict(code=1))):
+        assert call(d=d) == EINVAL
+    # nothing that is written may be read: the same pools, K beside V, accounts inside the destination, kept over mass
+    assert call(d=src) == EINVAL
+    assert call(d=cache(k=2 << 20, v=32 << 20, k_scale=48 << 20, v_scale=49 << 20)) == EINVAL
+    assert call(m=(16 << 20) + 100 * 8 * 32 * 64 - 4) == EINVAL
+    assert call(k=mass + 4) == EINVAL and call(mo=mass) == EINVAL
+
+
+def test_the_binding_refuses_on_the_host():
+    import torch
+    h = load_host()
+    k = torch.zeros((4, 2, 32, 64), dtype=torch.int8)
+    s = torch.zeros((4, 2))
+    c = h.B8Cache(k, k.clone(), s, s.clone(), torch.arange(3, dtype=torch.int32))
+    for bad in ((k[:, :, :16], k[:, :, :16], s, s), (k, k.float(), s, s), (k.half(), k.half(), s, s), (k, k, s[:2], s),
+                (k, k, s.double(), s), (k, k, s, s, torch.arange(4)), (k.transpose(0, 1), k.transpose(0, 1), s.t(), s.t()),
+                (k, k[:3], s, s)):
+        with pytest.raises(h.DsparkError):
+            h.B8Cache(*bad)
+    row = torch.zeros((40, 2, 64), dtype=torch.float16)
+    q = torch.zeros((4, 8, 64), dtype=torch.float16)
+    acc = torch.zeros((2, 96))
+    for call in (lambda: h.kv_write_b8(row, row, c, 60),                       # past the table's 3 pages
+                 lambda: h.kv_write_b8(row.float(), row.float(), c, 0), lambda: h.kv_write_b8(row, row[:8], c, 0),
+                 lambda: h.kv_write_b8(row[:, :1], row[:, :1], c, 0), lambda: h.kv_write_b8(row[..., ::2], row[..., ::2], c, 0),
+                 lambda: h.kv_read_b8(c, 90, 7), lambda: h.verify_attention_b8(q, c, 93),
+                 lambda: h.verify_attention_b8(q[..., :32], c, 0), lambda: h.verify_attention_b8(q.float(), c, 0),
+                 lambda: h.attention_mass_b8(q, c, 93, acc, acc), lambda: h.attention_mass_b8(q, c, 0, acc, acc),
+                 lambda: h.attention_mass_b8(q, c, 30, torch.zeros((4, 8)), acc[:, :33]),
+                 lambda: h.kv_evict_b8(c, c, 97, 3, acc), lambda: h.kv_evict_b8(c, c, 96, 3, acc[:, :95])):
+        with pytest.raises(h.DsparkError):
+            call()
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_scales_and_codes_of_the_restatement(code):
+    """A scale takes its block to the code range and no further than need be; codes are the nearest values; code * scale is
+    exact in fp32."""
+    every = np.arange(0x7c00, dtype=np.uint16).view(np.float16).astype(np.float64)  # every non-negative finite half
+    s = b8.scale_of(code, every).astype(np.float64)
+    top = 127 if code == "int8" else 448
+    assert s[0] == 0 and np.all(every <= s * top * (1 + 2.0 ** -23))
+    assert np.all(every[1:] > s[1:] * top * (1 - 2.0 ** -15 if code == "int8" else 0.5))
+    vals = np.unique(b8.values(code, np.arange(256, dtype=np.uint8)))
+    vals = vals[np.isfinite(vals)]
+    prod = vals[None] * s[::97, None]
+    assert np.array_equal(prod.astype(np.float32).astype(np.float64), prod)
+    x = np.random.default_rng(0).uniform(-1, 1, 4000) * top * 0.37
+    got = b8.values(code, b8.codes_of(code, x, np.float64(0.37))) * 0.37
+    inside = vals if code == "e4m3" else vals[vals >= -127]
+    best = np.abs(x[:, None] - inside[None] * 0.37).min(1)
+    assert np.allclose(np.abs(got - x), best, rtol=0, atol=1e-12)
+    assert np.array_equal(b8.codes_of("int8", np.array([0.5, 1.5, -0.5, 2.5, np.nan, np.inf]), 1.0).view(np.int8), [0, 2, 0, 2, 0, 127])

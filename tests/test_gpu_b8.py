@@ -1,0 +1,612 @@
+"""The 8-bit block-scaled K/V cache on the GPU against its restatement in float64 (oracle/b8.py): the writer, reader and
+eviction exactly, the attention and the accounts of attention weight within bounds derived below."""
+import numpy as np
+import pytest
+import torch
+
+from conftest import load_host
+from oracle import b8
+
+pytestmark = pytest.mark.gpu
+KINDS = ["int8", "e4m3"]
+TYPES = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
+
+
+def dev(x):
+    return torch.from_numpy(np.ascontiguousarray(x)).to("cuda")
+
+
+def gpu_cache(c):
+    """A device cache with the oracle cache's contents."""
+    h = load_host()
+    codes = [dev(c.raw[x]).view(TYPES[c.code]) for x in "kv"]
+    table = None if c.table is None else dev(np.asarray(c.table, np.int32))
+    return h.B8Cache(*codes, *(dev(c.scale[x]) for x in "kv"), table)
+
+
+def assert_same(g, c, where=""):
+    """Scales and the values of every code equal (the two zeros of e4m3 are one value)."""
+    for x in "kv":
+        raw = getattr(g, x).view(torch.uint8).cpu().numpy()
+        np.testing.assert_array_equal(getattr(g, x + "_scale").cpu().numpy(), c.scale[x], err_msg=where + x + "_scale")
+        np.testing.assert_array_equal(b8.values(c.code, raw), b8.values(c.code, c.raw[x]), err_msg=where + x)
+
+
+def rows(rng, n, KVH, D, size=1.0):
+    return (rng.standard_normal((n, KVH, D)) * size).astype(np.float16)
+
+
+def filled(code, T, KVH, D, seed, table=None, pages=None, size=1.0):
+    """An oracle cache holding T positions whose blocks differ in size."""
+    rng = np.random.default_rng(seed)
+    n = (T + 31) // 32
+    c = b8.Cache(code, pages or n, KVH, D, table)
+    sz = np.repeat(2.0 ** rng.uniform(-2, 1, (n, KVH, 1)), 32, 0)[:T] * size
+    c.write((rng.standard_normal((T, KVH, D)) * sz).astype(np.float16),
+            (rng.standard_normal((T, KVH, D)) * sz[::-1] + 0.25).astype(np.float16), 0)
+    return c
+
+
+# ------------------------------------------------------------------------------------------------ append and read
+@pytest.mark.parametrize("code", KINDS)
+@pytest.mark.parametrize("KVH,D", [(8, 64), (4, 128), (1, 64), (3, 128)])
+@pytest.mark.parametrize("spans", [[(0, 1)], [(0, 32)], [(0, 33), (33, 31)], [(0, 200), (131, 9), (140, 16), (150, 1)],
+                                   [(0, 70), (64, 3), (95, 2), (96, 32)]])
+def test_appends_and_reads(code, KVH, D, spans):
+    """Appends in turn (some starting before the last one's end, sizes growing and shrinking) through a permuted table."""
+    h = load_host()
+    rng = np.random.default_rng(len(spans) * 1000 + D + KVH)
+    table = rng.permutation(9).astype(np.int32)
+    c = b8.Cache(code, 9, KVH, D, table)
+    for x in "kv":  # what an earlier sequence left
+        c.raw[x][:] = 5
+        c.scale[x][:] = 0.5
+    g = gpu_cache(c)
+    for i, (pos0, n) in enumerate(spans):
+        k, v = rows(rng, n, KVH, D, 2.0 ** (3 * (i % 2) - 1)), rows(rng, n, KVH, D, 2.0 ** -i)
+        wide = torch.zeros((n, 2 * KVH * D + 8), dtype=torch.float16, device="cuda")  # K and V inside wider rows
+        wide[:, :KVH * D], wide[:, KVH * D:2 * KVH * D] = dev(k).view(n, -1), dev(v).view(n, -1)
+        h.kv_write_b8(wide[:, :KVH * D], wide[:, KVH * D:2 * KVH * D], g, pos0)
+        c.write(k, v, pos0)
+        assert_same(g, c, f"after append {i}: ")
+        h.kv_write_b8(wide[:, :KVH * D], wide[:, KVH * D:2 * KVH * D], g, pos0)  # the same rows again change nothing
+        assert_same(g, c, f"after append {i} again: ")
+    end = spans[-1][0] + spans[-1][1]
+    for pos0, n in ((0, end), (max(0, end - 1), 1), (min(5, end - 1), end - min(5, end - 1))):
+        k, v = h.kv_read_b8(g, pos0, n)
+        want = c.read(pos0, n)
+        np.testing.assert_array_equal(k.cpu().numpy().astype(np.float64), want[0])
+        np.testing.assert_array_equal(v.cpu().numpy().astype(np.float64), want[1])
+
+
+@pytest.mark.parametrize("code", KINDS)
+def test_append_special_values(code):
+    """Zeros, subnormals, the largest halves, NaN and infinities, and rows on the borders between two codes."""
+    h = load_host()
+    KVH, D = 2, 64
+    x = np.zeros((160, KVH, D), np.float16)
+    x[0:32] = 0
+    x[32:64] = np.linspace(-6e-8, 6e-8, D).astype(np.float16)
+    x[64:96, 0] = np.linspace(-65504, 65504, D).astype(np.float16)
+    x[64:96, 1] = np.float16(-0.0)
+    x[96:128] = np.arange(-32, 32, dtype=np.float32).astype(np.float16) / 2 + np.float16(0.5)  # borders: scale 2^-3 below
+    x[96, :, 0] = np.float16(127 / 8)
+    x[128:160] = np.random.default_rng(3).standard_normal((32, KVH, D)).astype(np.float16)
+    x[130, 0, 3:6] = [np.nan, np.inf, -np.inf]
+    x[131, 1] = np.nan
+    y = x[::-1].copy()
+    c = b8.Cache(code, 5, KVH, D)
+    g = gpu_cache(c)
+    h.kv_write_b8(dev(x), dev(y), g, 0)
+    c.write(x, y, 0)
+    assert_same(g, c)
+    # a block of nothing but NaN and infinities has scale 0
+    bad = np.full((1, KVH, D), np.inf, np.float16)
+    bad[0, 1] = np.nan
+    h.kv_write_b8(dev(bad), dev(-bad), g, 32)
+    c.write(bad, -bad, 32)
+    assert_same(g, c)
+
+
+@pytest.mark.parametrize("code", KINDS)
+def test_append_borders_between_codes(code):
+    """Values exactly between two codes and one half-precision step to either side, at a scale that is no power of two."""
+    h = load_host()
+    for amax in (1.0, 0.3, 63.5, 1016.0, 40000.0):
+        a = np.float16(amax)
+        s = float(b8.scale_of(code, np.float64(a)))
+        mid = (np.arange(-127, 127) + 0.5) * s if code == "int8" else (b8._E4M3_POS[:-1] + b8._E4M3_POS[1:]) / 2 * s
+        near = mid.astype(np.float16)
+        near = np.concatenate([near, np.nextafter(near, np.float16(np.inf)), np.nextafter(near, np.float16(-np.inf)), -near])
+        near = near[np.abs(near) <= a]
+        x = np.zeros(32 * 128, np.float16)
+        x[:len(near)], x[-1] = near[:len(x) - 1], a
+        x = x.reshape(32, 1, 128)
+        c = b8.Cache(code, 1, 1, 128)
+        g = gpu_cache(c)
+        h.kv_write_b8(dev(x), dev(-x), g, 0)
+        c.write(x, -x, 0)
+        assert_same(g, c, f"amax {amax}: ")
+
+
+@pytest.mark.parametrize("code", KINDS)
+def test_absent_pages_are_neither_written_nor_read(code):
+    h = load_host()
+    rng = np.random.default_rng(5)
+    c = b8.Cache(code, 4, 2, 64, np.array([2, -1, 4, 0, 1 << 30, 3], np.int32))
+    g = gpu_cache(c)
+    k, v = rows(rng, 190, 2, 64), rows(rng, 190, 2, 64)
+    h.kv_write_b8(dev(k), dev(v), g, 1)
+    c.write(k, v, 1)
+    assert_same(g, c)
+    out = [torch.full((190, 2, 64), 7.0, device="cuda") for _ in "kv"]
+    h.kv_read_b8(g, 1, 190, *out)
+    want = c.read(1, 190)
+    np.testing.assert_array_equal(out[0].cpu().numpy(), want[0].astype(np.float32))
+    np.testing.assert_array_equal(out[1].cpu().numpy(), want[1].astype(np.float32))
+
+
+def test_read_into_wider_rows_leaves_the_rest():
+    h = load_host()
+    c = filled("int8", 77, 3, 64, 1)
+    g = gpu_cache(c)
+    out = [torch.full((40, 3 * 64 + 4), 7.0, device="cuda") for _ in "kv"]
+    h.kv_read_b8(g, 30, 39, *out)
+    for o, want in zip(out, c.read(30, 39)):
+        np.testing.assert_array_equal(o[:39, :192].cpu().numpy(), want.reshape(39, -1).astype(np.float32))
+        assert bool((o[39:] == 7).all()) and bool((o[:, 192:] == 7).all())
+
+
+# ------------------------------------------------------------------------------------------------ attention
+# Of a result o = sum P v / sum P with A = sum P |v| / sum P, P is rounded to fp16 once (2^-11 of each P that is a normal
+# half; those below are 2^-22 of the largest at most and off by 2^-33 of it: under 2^-16 A together for 2^17 keys of like
+# size, and under 2^-33 sum |v| always). Scores of up to 64 (log2 units) are sums of exact products in fp32: off by about
+# 2^-24 64 = 2^-18 and their exponential relatively by as much; sums in fp32 add a few 2^-24 more. 2^-16 A covers these.
+# The fp16 output is rounded once more.
+def bound(o, mag, half):
+    return (2.0 ** -11 + 2.0 ** -16) * mag + (2.0 ** -11 * np.abs(o) + 2.0 ** -25 if half else 0) + 1e-9
+
+
+def run_attention(c, q, a, gate=None, splits=0, **mask):
+    h = load_host()
+    g = gpu_cache(c)
+    M, QH, D = q.shape
+    o16, o32 = torch.empty((M, QH, D), dtype=torch.float16, device="cuda"), torch.empty((M, QH, D), device="cuda")
+    lse = torch.empty((M, QH), device="cuda")
+    h.verify_attention_b8(dev(q), g, a, out=o16, out_f32=o32, lse=lse, gate=None if gate is None else dev(gate), splits=splits,
+                          **mask)
+    return o16.cpu().numpy().astype(np.float64), o32.cpu().numpy().astype(np.float64), lse.cpu().numpy().astype(np.float64)
+
+
+def check_attention(c, q, a, gate=None, splits=0, start=0, window=0, causal=True):
+    M = len(q)
+    k, v, here = c.read(0, a + M)
+    see = b8.visible(M, a, start, window, causal, here)
+    o, lse, mag = b8.attention(q, k, v, see, gate)
+    o16, o32, l = run_attention(c, q, a, gate, splits, start=start, window=window, causal=causal)
+    assert np.all(np.abs(o32 - o) <= bound(o, mag, False)), np.max(np.abs(o32 - o) - bound(o, mag, False))
+    assert np.all(np.abs(o16 - o) <= bound(o, mag, True))
+    dead = np.isneginf(lse)
+    assert np.array_equal(np.isneginf(l), dead) and not o32[dead].any() and not o16[dead].any()
+    # a score is off by 2^-18 at most, the logarithm of the sum by a few 2^-24 of its size
+    assert np.all(np.abs(l[~dead] - lse[~dead]) <= 2.0 ** -17 + 2.0 ** -21 * np.abs(lse[~dead]))
+    return lse
+
+
+@pytest.mark.parametrize("code", KINDS)
+@pytest.mark.parametrize("QH,KVH,D", [(32, 8, 64), (16, 4, 128), (2, 2, 64), (20, 1, 128)])
+@pytest.mark.parametrize("M", [1, 5, 16])
+@pytest.mark.parametrize("a", [0, 1, 31, 32, 300])
+def test_attention(code, QH, KVH, D, M, a):
+    rng = np.random.default_rng(a * 100 + M)
+    n = (a + M + 31) // 32
+    c = filled(code, a + M, KVH, D, M, table=rng.permutation(n + 2)[:n].astype(np.int32), pages=n + 2)
+    q = rng.standard_normal((M, QH, D)).astype(np.float16)
+    check_attention(c, q, a, gate=rng.standard_normal((M, QH)).astype(np.float32))
+
+
+@pytest.mark.parametrize("code", KINDS)
+@pytest.mark.parametrize("start,window,causal", [(0, 0, False), (100, 0, True), (0, 17, True), (0, 32, False), (250, 100, True),
+                                                 (400, 0, True), (0, 1, True), (290, 5000, False)])
+@pytest.mark.parametrize("M,D", [(7, 64), (33, 128)])
+def test_attention_masks(code, start, window, causal, M, D):
+    rng = np.random.default_rng(start + window + M)
+    a = 333
+    c = filled(code, a + M, 2, D, 9)
+    check_attention(c, rng.standard_normal((M, 6, D)).astype(np.float16), a, start=start, window=window, causal=causal)
+
+
+@pytest.mark.parametrize("splits", [1, 2, 3, 7, 64, 4096])
+@pytest.mark.parametrize("M,QH,D", [(1, 8, 64), (16, 16, 64), (9, 16, 128), (64, 32, 64), (64, 32, 128)])
+def test_attention_splits_and_rows(splits, M, QH, D):
+    """Any number of splits; up to 1024 rows a KV head (16 query heads, 64 tokens)."""
+    rng = np.random.default_rng(splits)
+    a = 1500
+    c = filled("e4m3", a + M, 2, D, 4)
+    check_attention(c, rng.standard_normal((M, QH, D)).astype(np.float16), a, splits=splits)
+
+
+@pytest.mark.parametrize("code", KINDS)
+def test_attention_sizes_far_apart(code):
+    """Blocks of V up to 2^30 apart and scores up to +-40: no block is lost beside a larger one that the row hardly sees."""
+    rng = np.random.default_rng(8)
+    M, KVH, D, a = 3, 2, 64, 700
+    c = filled(code, a + M, KVH, D, 2)
+    c.scale["v"] *= np.exp2(rng.integers(-20, 10, c.scale["v"].shape)).astype(np.float32)
+    q = (rng.standard_normal((M, 8, D)) * 6).astype(np.float16)
+    check_attention(c, q, a)
+
+
+@pytest.mark.parametrize("code", KINDS)
+def test_attention_growing_and_falling_scores(code):
+    """Scores that climb from page to page (every page moves the running reference) and that fall (none does)."""
+    M, KVH, D, a = 2, 1, 64, 32 * 24
+    c = filled(code, a + M, KVH, D, 2)
+    q = np.full((M, 2, D), 0.5, np.float16)
+    one = b8.codes_of(code, np.ones(1), np.ones(1))[0]
+    c.raw["k"][:] = one
+    for sign in (1, -1):
+        c.scale["k"][:] = (np.arange(len(c.scale["k"]))[::sign, None] * 4).astype(np.float32)  # up to 92 * 64 / 2 / 8
+        check_attention(c, q, a)
+
+
+@pytest.mark.parametrize("code", KINDS)
+def test_attention_absent_pages(code):
+    """Pages that are not there, up to all of them: what is left is attended to, a row that sees nothing gives zeros."""
+    rng = np.random.default_rng(1)
+    M, KVH, D, a = 5, 2, 64, 300
+    q = rng.standard_normal((M, 4, D)).astype(np.float16)
+    for gone in ([0], [1, 2, 3], [9], list(range(9)), list(range(10))):
+        table = np.arange(10).astype(np.int32)
+        c = filled(code, a + M, KVH, D, 3, table=table)
+        c.table = table.copy()
+        c.table[gone] = [-1, 10, 1 << 30, -(1 << 31)][len(gone) % 4]
+        lse = check_attention(c, q, a)
+        assert np.isneginf(lse).all() == (len(gone) == 10)
+
+
+def test_attention_ignores_what_is_masked():
+    """Keys behind the block, and the block's own later keys, may hold anything a writer stores: outputs do not change."""
+    rng = np.random.default_rng(2)
+    M, KVH, D, a = 4, 2, 64, 61
+    q = rng.standard_normal((M, 4, D)).astype(np.float16)
+    got = []
+    for fill in (3, 0x7b):  # the block's last key (position 64, page 2), the slots behind it and the page behind that
+        c = b8.Cache("int8", 4, KVH, D)
+        c.write(rows(np.random.default_rng(7), a + M, KVH, D), rows(np.random.default_rng(6), a + M, KVH, D), 0)
+        for x in "kv":
+            c.raw[x][2:] = fill
+        got.append(run_attention(c, q, a)[1])
+    assert np.array_equal(got[0][:3], got[1][:3]) and not np.array_equal(got[0][3], got[1][3])
+
+
+def test_attention_query_rows_apart():
+    """A NaN query head spoils its own row alone; q inside wider rows; a single token's stride is not read."""
+    h = load_host()
+    rng = np.random.default_rng(2)
+    c = filled("e4m3", 210, 2, 64, 1)
+    g = gpu_cache(c)
+    q = rng.standard_normal((9, 8, 64)).astype(np.float16)
+    wide = torch.zeros((9, 8 * 64 + 40), dtype=torch.float16, device="cuda")
+    wide[:, :512] = dev(q).view(9, -1)
+    qs = wide[:, :512].unflatten(1, (8, 64))
+    want, _ = h.verify_attention_b8(dev(q), g, 200)
+    got, _ = h.verify_attention_b8(qs, g, 200)
+    assert torch.equal(want, got)
+    wide[4, 64:128] = float("nan")
+    bad, _ = h.verify_attention_b8(qs, g, 200)
+    keep = torch.ones((9, 8), dtype=torch.bool, device="cuda")
+    keep[4, 1] = False
+    assert torch.equal(bad[keep], want[keep]) and bool(bad[4, 1].isnan().all())
+    one, _ = h.verify_attention_b8(qs[2:3], g, 202)
+    assert one.shape == (1, 8, 64)
+
+
+@pytest.mark.parametrize("code,QH,KVH,D,M,a", [("e4m3", 32, 8, 64, 16, 32768), ("int8", 16, 4, 128, 9, 20011)])
+def test_attention_long(code, QH, KVH, D, M, a):
+    """Long caches against the same attention in float64 on the GPU."""
+    h = load_host()
+    rng = np.random.default_rng(4)
+    n = (a + M + 31) // 32
+    c = b8.Cache(code, n, KVH, D, rng.permutation(n).astype(np.int32))
+    g = gpu_cache(c)
+    kv = torch.randn((2, a + M, KVH, D), device="cuda").half()
+    h.kv_write_b8(kv[0], kv[1], g, 0)
+    k, v = (x.double().transpose(0, 1) for x in h.kv_read_b8(g, 0, a + M))
+    q = torch.randn((M, QH, D), device="cuda").half()
+    out, o32, lse = None, torch.empty((M, QH, D), device="cuda"), torch.empty((M, QH), device="cuda")
+    h.verify_attention_b8(q, g, a, out_f32=o32, lse=lse)
+    x = q.double().view(M, KVH, -1, D).transpose(0, 1).reshape(KVH, -1, D) @ k.transpose(1, 2).contiguous() / D ** 0.5
+    x = x.view(KVH, M, -1, a + M)
+    p, t = torch.arange(a + M, device="cuda"), torch.arange(M, device="cuda")[:, None]
+    x = x.masked_fill((p - a > t)[:, None], -float("inf"))
+    want = (torch.softmax(x, -1).view(KVH, -1, a + M) @ v).view(KVH, M, -1, D).transpose(0, 1).reshape(M, QH, D)
+    mag = (torch.softmax(x, -1).view(KVH, -1, a + M) @ v.abs()).view(KVH, M, -1, D).transpose(0, 1).reshape(M, QH, D)
+    assert bool(((o32 - want).abs() <= (2.0 ** -11 + 2.0 ** -16) * mag).all())
+    wl = torch.logsumexp(x, -1).transpose(0, 1).reshape(M, QH)
+    assert float((lse - wl).abs().max()) <= 2.0 ** -17 + 2.0 ** -21 * 16
+
+
+def test_pool_past_4_gib():
+    """Pages behind byte 2^32 of a pool: written, read, attended to and evicted from."""
+    h = load_host()
+    KVH, D, pages = 8, 64, (1 << 32) // (8 * 32 * 64) + 40
+    far = np.array([pages - 1, 7, pages - 2, 0, pages - 5], np.int32)
+    big = h.b8_cache_alloc(pages, KVH, D, dtype=torch.int8, block_table=dev(far))
+    near = b8.Cache("int8", 5, KVH, D)
+    g = gpu_cache(near)
+    rng = np.random.default_rng(3)
+    k, v, q = rows(rng, 150, KVH, D), rows(rng, 150, KVH, D), rng.standard_normal((4, 32, D)).astype(np.float16)
+    got = []
+    for c in (big, g):
+        h.kv_write_b8(dev(k), dev(v), c, 0)
+        lse = torch.empty((4, 32), device="cuda")
+        o, _ = h.verify_attention_b8(dev(q), c, 146, lse=lse)
+        m = h.attention_mass_b8(dev(q), c, 146, lse, torch.zeros((KVH, 160), device="cuda"))
+        d = h.b8_cache_alloc(3, KVH, D)
+        kept, km = h.kv_evict_b8(c, d, 150, 70, m, sinks=2, recent=4)
+        got.append([o, lse, m, kept, km, d.k, d.v, d.k_scale, d.v_scale, *h.kv_read_b8(c, 0, 150)])
+    for x, y in zip(*got):
+        assert torch.equal(x, y)
+
+
+# ------------------------------------------------------------------------------------------------ accounts
+# Every weight exp(score - lse) is relatively off by the error of its exponent: a score of up to 64 (log2 units) and lse
+# rounded and scaled in fp32, 2^-24 64 each, three roundings: 2^-16. Sums of non-negative numbers keep that.
+def check_mass(c, q, a, rows_, start=0, window=0, causal=True, with_in=True, alias=False):
+    h = load_host()
+    g = gpu_cache(c)
+    M = len(q)
+    k, v, here = c.read(0, a + M)
+    see = b8.visible(M, a, start, window, causal, here)
+    lse = b8.attention(q, k, v, see)[1].astype(np.float32)
+    rng = np.random.default_rng(a)
+    m_in = rng.exponential(1.0, (c.KVH, a + M + 5)).astype(np.float32) if with_in else None
+    out = dev(m_in) if alias else torch.full((c.KVH, a + M + 5), -3.0, device="cuda")
+    word = torch.tensor([rows_], dtype=torch.int32, device="cuda")
+    before = out.clone()
+    h.attention_mass_b8(dev(q), g, a, dev(lse), out, mass_in=out if alias else None if m_in is None else dev(m_in), rows=word,
+                        start=start, window=window, causal=causal)
+    n = min(max(rows_, 0), M)
+    want = b8.mass(q, k, see, lse, n, a, m_in)
+    got = out[:, :a + n].cpu().numpy().astype(np.float64)
+    assert np.all(np.abs(got - want) <= 2.0 ** -16 * want + 1e-9), np.max(np.abs(got - want) / (want + 1e-9))
+    assert torch.equal(out[:, a + n:], before[:, a + n:])
+
+
+@pytest.mark.parametrize("code", KINDS)
+@pytest.mark.parametrize("QH,KVH,D,M,a", [(32, 8, 64, 16, 300), (16, 4, 128, 9, 1001), (2, 2, 64, 1, 0), (2, 2, 64, 1, 32),
+                                          (20, 1, 128, 5, 95), (32, 2, 64, 64, 200)])
+def test_mass(code, QH, KVH, D, M, a):
+    rng = np.random.default_rng(M)
+    c = filled(code, a + M, KVH, D, a, table=rng.permutation((a + M + 31) // 32).astype(np.int32))
+    q = rng.standard_normal((M, QH, D)).astype(np.float16)
+    check_mass(c, q, a, M)
+    check_mass(c, q, a, (M + 1) // 2, with_in=False)
+    check_mass(c, q, a, 0, alias=True)
+    check_mass(c, q, a, M + 7, alias=True)
+    check_mass(c, q, a, -1)
+
+
+@pytest.mark.parametrize("start,window,causal", [(0, 0, False), (100, 0, True), (0, 17, True), (400, 0, True), (0, 1, True)])
+def test_mass_masks(start, window, causal):
+    rng = np.random.default_rng(start + window)
+    c = filled("int8", 333 + 7, 2, 64, 9)
+    check_mass(c, rng.standard_normal((7, 6, 64)).astype(np.float16), 333, 5, start=start, window=window, causal=causal)
+
+
+def test_mass_absent_pages():
+    """Absent pages draw nothing and keep their accounts; rows that saw nothing (lse -inf) add nothing."""
+    rng = np.random.default_rng(0)
+    for gone in ([2], list(range(11))):
+        table = np.arange(11).astype(np.int32)
+        c = filled("e4m3", 340, 2, 64, 9, table=table)
+        c.table = table.copy()
+        c.table[gone] = -1
+        check_mass(c, rng.standard_normal((7, 6, 64)).astype(np.float16), 333, 5)
+
+
+# ------------------------------------------------------------------------------------------------ eviction
+def check_evict(c, length, keep, m, sinks, recent, dst_table=None):
+    h = load_host()
+    g = gpu_cache(c)
+    n = (keep + 31) // 32
+    d = b8.Cache(c.code, n if dst_table is None else len(dst_table), c.KVH, c.D, dst_table)
+    for x in "kv":
+        d.raw[x][:] = 9
+    gd = gpu_cache(d)
+    kept, mass = h.kv_evict_b8(g, gd, length, keep, dev(m), sinks=sinks, recent=recent)
+    wk, wm = b8.evict(c, d, length, keep, m, sinks, recent)
+    np.testing.assert_array_equal(kept.cpu().numpy(), wk)
+    np.testing.assert_array_equal(mass.cpu().numpy(), wm)
+    assert_same(gd, d)
+
+
+@pytest.mark.parametrize("code", KINDS)
+@pytest.mark.parametrize("KVH,D", [(8, 64), (3, 128)])
+@pytest.mark.parametrize("length,keep,sinks,recent", [(1, 1, 0, 0), (40, 39, 0, 0), (333, 100, 4, 30), (333, 333, 0, 0),
+                                                      (333, 333, 100, 233), (1030, 64, 0, 64), (1030, 65, 64, 1),
+                                                      (2100, 1025, 7, 0), (5000, 31, 1, 1)])
+def test_evict(code, KVH, D, length, keep, sinks, recent):
+    rng = np.random.default_rng(length + keep)
+    n = (length + 31) // 32
+    c = filled(code, length, KVH, D, keep, table=rng.permutation(n).astype(np.int32))
+    m = np.exp(2 * rng.standard_normal((KVH, length + 3))).astype(np.float16).astype(np.float32)
+    check_evict(c, length, keep, m, sinks, recent, rng.permutation((keep + 31) // 32 + 1).astype(np.int32))
+
+
+@pytest.mark.parametrize("name", ["equal", "few", "special", "negative", "subnormal", "bits"])
+def test_evict_order(name):
+    """Ties, infinities, NaN, both zeros, subnormal and negative accounts, and neighbours one bit apart."""
+    rng = np.random.default_rng(12)
+    KVH, T = 2, 1500
+    m = np.ones((KVH, T), np.float32)
+    if name == "few":
+        m = rng.integers(0, 3, (KVH, T)).astype(np.float32)
+    elif name == "special":
+        m = rng.choice(np.array([np.nan, np.inf, -np.inf, 0.0, -0.0, 1.0], np.float32), (KVH, T))
+        m.view(np.uint32)[:, 5] = 0xFFC00001  # a NaN with its sign bit set
+    elif name == "negative":
+        m = -rng.exponential(1.0, (KVH, T)).astype(np.float32)
+    elif name == "subnormal":
+        m = (rng.integers(0, 1 << 22, (KVH, T)).astype(np.uint32)).view(np.float32)
+    elif name == "bits":
+        m = (np.uint32(0x3F800000) + rng.integers(0, 700, (KVH, T)).astype(np.uint32)).view(np.float32)
+    c = filled("int8", T, KVH, 64, 3)
+    for keep, sinks, recent in ((700, 3, 40), (1400, 0, 0), (44, 4, 39)):
+        check_evict(c, T, keep, m, sinks, recent)
+
+
+def test_evict_absent_pages():
+    """Rows of absent pages are kept as zeros; a destination page that is absent is not written."""
+    rng = np.random.default_rng(12)
+    table = np.arange(7).astype(np.int32)
+    c = filled("e4m3", 200, 2, 64, 3, table=table)
+    c.table = table.copy()
+    c.table[[1, 4]] = [-1, 99]
+    m = rng.exponential(1.0, (2, 200)).astype(np.float32)
+    check_evict(c, 200, 130, m, 2, 5, np.array([3, -1, 0, 7, 1], np.int32))
+
+
+@pytest.mark.parametrize("length,keep", [(16384, 5000), (40000, 39000), (131072, 16384), (300001, 1000)])
+def test_evict_long(length, keep):
+    """Long accounts, kept positions against a stable sort."""
+    h = load_host()
+    KVH, D = 2, 64
+    g = h.b8_cache_alloc((length + 31) // 32, KVH, D, dtype=torch.float8_e4m3fn)
+    d = h.b8_cache_alloc((keep + 31) // 32, KVH, D, dtype=torch.float8_e4m3fn)
+    m = torch.randn((KVH, length), device="cuda").mul_(2).exp_().half().float()
+    kept, mass = h.kv_evict_b8(g, d, length, keep, m, sinks=4, recent=100)
+    for i in range(KVH):
+        np.testing.assert_array_equal(kept[i].cpu().numpy(), b8.kept(m[i].cpu().numpy(), length, keep, 4, 100))
+    assert torch.equal(mass, m.gather(1, kept.long()))
+
+
+# ------------------------------------------------------------------------------------------------ together
+@pytest.mark.parametrize("code,QH,KVH,D", [("int8", 32, 8, 64), ("e4m3", 16, 4, 128)])
+def test_rounds_with_a_bounded_cache(code, QH, KVH, D):
+    """Speculative rounds over one layer: append a block, attend, accept some drafts (accept_commit on the device State),
+    account for the committed rows alone, and evict whenever the cache passes its limit."""
+    h = load_host()
+    rng = np.random.default_rng(21)
+    M, limit, keep, V = 6, 130, 96, 4096
+    pools = [b8.Cache(code, 6, KVH, D, rng.permutation(6).astype(np.int32)) for _ in range(2)]
+    dev_pools = [gpu_cache(c) for c in pools]
+    acc = [torch.zeros((KVH, 192), device="cuda") for _ in range(2)]
+    cur, a = 0, 90
+    k, v = rows(rng, a, KVH, D), rows(rng, a, KVH, D)
+    pools[0].write(k, v, 0)
+    h.kv_write_b8(dev(k), dev(v), dev_pools[0], 0)
+    want_acc = np.zeros((KVH, 192))
+    ws, seen = h.Workspace("cuda"), torch.zeros(V // 32, dtype=torch.int32, device="cuda")
+    evictions = 0
+    for r in range(14):
+        c, g = pools[cur], dev_pools[cur]
+        k, v, q = rows(rng, M, KVH, D), rows(rng, M, KVH, D), rng.standard_normal((M, QH, D)).astype(np.float16)
+        c.write(k, v, a)
+        h.kv_write_b8(dev(k), dev(v), g, a)
+        o32, lse = torch.empty((M, QH, D), device="cuda"), torch.empty((M, QH), device="cuda")
+        h.verify_attention_b8(dev(q), g, a, out_f32=o32, lse=lse, workspace=ws)
+        kk, vv, here = c.read(0, a + M)
+        see = b8.visible(M, a, 0, 0, True, here)
+        o, wl, mag = b8.attention(q, kk, vv, see)
+        assert np.all(np.abs(o32.cpu().numpy() - o) <= bound(o, mag, False))
+        # drafts accepted up to a chosen one
+        good = int(rng.integers(0, M))
+        tokens = rng.integers(0, V, M)
+        logits = np.zeros((M, V), np.float32)
+        for t in range(M):
+            logits[t, (tokens[t + 1] if t < good else (tokens[(t + 1) % M] + 1) % V)] = 5
+        st = h.state_tensor(a=a, anchor=int(tokens[0]), tokens=tokens.tolist(), rounds_left=9, budget=500, eos=-1,
+                            stop_at=10000, run=1, skip_rounds=1)
+        best = h.verify_argmax(dev(logits), seen, st)
+        h.accept_commit(st, best, M, torch.zeros(64, dtype=torch.int32, device="cuda"), seen)
+        ctx_new = h.STATE_FIELDS.index("ctx_new")
+        h.attention_mass_b8(dev(q), g, a, lse, acc[cur], mass_in=acc[cur], rows=st[ctx_new:ctx_new + 1])
+        n = good + 1
+        want_acc[:, :a + n] = b8.mass(q, kk, see, lse.cpu().numpy(), n, a, want_acc)
+        a += n
+        got = acc[cur][:, :a].cpu().numpy()
+        assert np.all(np.abs(got - want_acc[:, :a]) <= 2.0 ** -15 * want_acc[:, :a] + 1e-9), r
+        if a > limit:
+            m = acc[cur].cpu().numpy()
+            kept, _ = h.kv_evict_b8(g, dev_pools[1 - cur], a, keep, acc[cur], sinks=4, recent=32, mass_out=acc[1 - cur])
+            wk, wm = b8.evict(c, pools[1 - cur], a, keep, m, 4, 32)
+            np.testing.assert_array_equal(kept.cpu().numpy(), wk)
+            cur, a = 1 - cur, keep
+            np.testing.assert_array_equal(acc[cur][:, :keep].cpu().numpy(), wm)
+            want_acc[:] = 0
+            want_acc[:, :keep] = wm
+            evictions += 1
+    assert evictions >= 1
+    n = (a + 31) // 32
+    k, v = h.kv_read_b8(dev_pools[cur], 0, a)
+    want = pools[cur].read(0, a)
+    np.testing.assert_array_equal(k.cpu().numpy(), want[0].astype(np.float32))
+    np.testing.assert_array_equal(v.cpu().numpy(), want[1].astype(np.float32))
+
+
+def test_side_stream_and_repeats():
+    """Calls on a stream that is not current (their buffers allocated there), and the same bits every time."""
+    h = load_host()
+    rng = np.random.default_rng(2)
+    c = filled("int8", 2010, 4, 64, 1)
+    g = gpu_cache(c)
+    q = dev(rng.standard_normal((10, 16, 64)).astype(np.float16))
+    lse = torch.empty((10, 16), device="cuda")
+    want, _ = h.verify_attention_b8(q, g, 2000, lse=lse)
+    want_mass = h.attention_mass_b8(q, g, 2000, lse, torch.zeros((4, 2010), device="cuda"))
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(5):
+        got, _ = h.verify_attention_b8(q, g, 2000, stream=side)
+        fill = torch.full((1 << 20,), 3.0, device="cuda")  # the current stream keeps allocating meanwhile
+        mass = torch.zeros((4, 2010), device="cuda")
+        side.wait_stream(torch.cuda.current_stream())
+        h.attention_mass_b8(q, g, 2000, lse, mass, stream=side)
+        side.synchronize()
+        assert torch.equal(got, want) and torch.equal(mass, want_mass) and bool((fill == 3).all())
+
+
+def test_graph_replays():
+    """The whole chain captured once and replayed with other inputs between eager calls; every replay against eager calls."""
+    h = load_host()
+    rng = np.random.default_rng(5)
+    KVH, D, M, a = 2, 64, 4, 500
+    base = filled("e4m3", a, KVH, D, 1)
+    g, eager = gpu_cache(base), gpu_cache(base)
+    kv = torch.zeros((2, M, KVH, D), dtype=torch.float16, device="cuda")
+    q = torch.zeros((M, 8, D), dtype=torch.float16, device="cuda")
+    dst, dst_e = h.b8_cache_alloc(8, KVH, D, dtype=torch.float8_e4m3fn), h.b8_cache_alloc(8, KVH, D, dtype=torch.float8_e4m3fn)
+    acc, word = torch.zeros((KVH, 512), device="cuda"), torch.tensor([3], dtype=torch.int32, device="cuda")
+    out, lse = torch.empty((M, 8, D), dtype=torch.float16, device="cuda"), torch.empty((M, 8), device="cuda")
+    kept, mout = torch.empty((KVH, 250), dtype=torch.int32, device="cuda"), torch.empty((KVH, 250), device="cuda")
+    ws, ws_e = h.Workspace("cuda"), h.Workspace("cuda")
+
+    def chain(c, d, o, l, m, ws, kept, mout):
+        h.kv_write_b8(kv[0], kv[1], c, a)
+        h.verify_attention_b8(q, c, a, out=o, lse=l, workspace=ws)
+        h.attention_mass_b8(q, c, a, l, m, mass_in=m, rows=word)
+        h.kv_evict_b8(c, d, a + 3, 250, m, sinks=2, recent=20, kept=kept, mass_out=mout, workspace=ws)
+
+    chain(g, dst, out, lse, acc, ws, kept, mout)  # sizes the workspace
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        chain(g, dst, out, lse, acc, ws, kept, mout)
+    acc.zero_()
+    acc_e, out_e, lse_e = torch.zeros_like(acc), torch.empty_like(out), torch.empty_like(lse)
+    kept_e, mout_e = torch.empty_like(kept), torch.empty_like(mout)
+    for x in ("k", "v", "k_scale", "v_scale"):
+        getattr(g, x).view(torch.uint8).copy_(getattr(eager, x).view(torch.uint8))
+    for r in range(4):
+        kv.copy_(torch.randn(kv.shape, device="cuda"))
+        q.copy_(torch.randn(q.shape, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        chain(eager, dst_e, out_e, lse_e, acc_e, ws_e, kept_e, mout_e)
+        torch.cuda.synchronize()
+        for x, y in ((out, out_e), (lse, lse_e), (acc, acc_e), (kept, kept_e), (mout, mout_e), (dst.k_scale, dst_e.k_scale),
+                     (dst.v.view(torch.uint8), dst_e.v.view(torch.uint8)), (dst.k.view(torch.uint8), dst_e.k.view(torch.uint8)),
+                     (g.k.view(torch.uint8), eager.k.view(torch.uint8))):
+            assert torch.equal(x, y), r
