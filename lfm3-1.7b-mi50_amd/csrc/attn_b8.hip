@@ -16,7 +16,7 @@
 
 namespace dspark {
 
-constexpr int B8_WAVES = 4;
+constexpr int B8_WAVES = 8, MASS_WAVES = 4;
 // Running reference in log2 units: P = 2^(x - ref), ref set to the row's largest x less 8 when some x passes ref + 15:
 // P stays under 2^15, and a P of 2^-22 of the largest is still a normal half.
 constexpr float REF_INIT = -1e30f, REF_BELOW = 8.f, REF_SLACK = 15.f;
@@ -120,10 +120,9 @@ __device__ __forceinline__ void b8_load_q(const B8Attn& p, int h, int row0, int 
 __device__ __forceinline__ int row_lo(const B8Attn& p, int t) { return max(p.start, p.window > 0 ? p.a + t - p.window + 1 : 0); }
 __device__ __forceinline__ int row_hi(const B8Attn& p, int t) { return p.causal ? p.a + t + 1 : p.a + p.M; }
 
-// Scores (log2 units) of one page: x[rb][b][i] of key 16 b + 4 g + i; -inf where the row does not see it.
+// q . code of one page: s[rb][b][i] of key 16 b + 4 g + i, still to be multiplied by the block's scale.
 template <int D, int RB, bool FP8>
-__device__ __forceinline__ void b8_scores(const B8Attn& p, const u32x4 (&k)[2][D / 64], const half8 (&q)[RB][D / 32], float ks,
-                                          bool masked, int pos, const int (&tok)[RB], int lane, f32x4 (&x)[RB][2]) {
+__device__ __forceinline__ void b8_scores(const u32x4 (&k)[2][D / 64], const half8 (&q)[RB][D / 32], f32x4 (&s)[RB][2]) {
 #pragma unroll
   for (int b = 0; b < 2; ++b) {
     half8 kf[D / 32];
@@ -134,31 +133,107 @@ __device__ __forceinline__ void b8_scores(const B8Attn& p, const u32x4 (&k)[2][D
     }
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      f32x4 s = {0, 0, 0, 0};
+      s[rb][b] = f32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int e = 0; e < D / 32; ++e) s = mfma16x16x32(kf[e], q[rb][e], s);
-      x[rb][b] = s * ks;
+      for (int e = 0; e < D / 32; ++e) s[rb][b] = mfma16x16x32(kf[e], q[rb][e], s[rb][b]);
     }
   }
-  if (masked) {
-    const int g = lane >> 4;
+}
+// The scores of a page that some row does not see whole, scaled (a block of zeros has scale 0: -inf comes after it), with -inf
+// where the row does not see the key.
+template <int RB>
+__device__ __forceinline__ void b8_mask(const B8Attn& p, float ks, int pos, const int (&tok)[RB], int lane, f32x4 (&s)[RB][2]) {
+  const int g = lane >> 4;
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      const int lo = row_lo(p, tok[rb]), hi = row_hi(p, tok[rb]);
+  for (int rb = 0; rb < RB; ++rb) {
+    const int lo = row_lo(p, tok[rb]), hi = row_hi(p, tok[rb]);
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int kp = pos + 16 * b + 4 * g + i;
-          if (kp < p.a ? kp < lo : kp >= hi) x[rb][b][i] = -INFINITY;
-        }
-    }
+      for (int i = 0; i < 4; ++i) {
+        const int kp = pos + 16 * b + 4 * g + i;
+        s[rb][b][i] = (kp < p.a ? kp < lo : kp >= hi) ? -INFINITY : s[rb][b][i] * ks;
+      }
   }
 }
 
 // ---------------------------------------------------------------- attention
+template <int D>
+__device__ __forceinline__ void b8_load_tile(const B8Attn& p, int h, int pg, int lane, B8Tile<D>& t) {
+  const size_t blk = ((size_t)max(pg, 0) * p.c.KVH + h) * (PAGE * D);  // an absent page's loads go to page 0, unused
+  b8_load_k<D>(p.c.k + blk, lane, t.k);
+  b8_load_v<D>(p.c.v + blk, lane, t.v);
+}
+
+// Running state of a wave's rows: o[rb][d] of row 16 rb + n, dims (D / 16) (4 g + i) + d; l the lane's part of the sum of P,
+// before P's rounding (the log-sum-exp is an fp32 output: a sum of rounded P, from a product with ones, is 2^-12 off).
+template <int D, int RB>
+struct B8Rows {
+  float ref[RB];
+  float l[RB];
+  f32x4 o[RB][D / 16];
+};
+
 template <int D, int RB, bool FP8>
-__global__ __launch_bounds__(64 * B8_WAVES) void attn_b8_kernel(B8Attn p) {
+__device__ __forceinline__ void b8_page(const B8Attn& p, const B8Tile<D>& t, const half8 (&q)[RB][D / 32], const int (&tok)[RB],
+                                        float ks, float vs, int lp, int lane, B8Rows<D, RB>& st) {
+  f32x4 s[RB][2];
+  b8_scores<D, RB, FP8>(t.k, q, s);
+  if (lp < p.full_lo || lp >= p.full_hi) {
+    b8_mask<RB>(p, ks, lp * PAGE, tok, lane, s);
+    ks = 1.f;
+  }
+  float top[RB];
+  bool over = false;
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    top[rb] = ks * fmaxf(fmaxf(fmaxf(s[rb][0][0], s[rb][0][1]), fmaxf(s[rb][0][2], s[rb][0][3])),
+                         fmaxf(fmaxf(s[rb][1][0], s[rb][1][1]), fmaxf(s[rb][1][2], s[rb][1][3])));
+    over |= top[rb] > st.ref[rb] + REF_SLACK;
+  }
+  if (__ballot(over)) {
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      const float m = row_max(top[rb]);
+      const float to = m > st.ref[rb] + REF_SLACK ? m - REF_BELOW : st.ref[rb];
+      const float f = fast_exp2(st.ref[rb] - to);
+      st.ref[rb] = to;
+      st.l[rb] *= f;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) st.o[rb][d] *= f;
+    }
+  }
+  half8 pf[RB];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    float e[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      e[j] = fast_exp2(fmaf(s[rb][j / 4][j % 4], ks, -st.ref[rb]));
+      pf[rb][j] = (_Float16)e[j];
+    }
+    st.l[rb] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+  }
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c) {
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = b8_flip<FP8>(t.v[j][c]);
+    half8 vt[4];
+    b8_vt<FP8, 0>(w, vt[0], vt[1]);
+    b8_vt<FP8, 2>(w, vt[2], vt[3]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        const f32x4 y = mfma16x16x32(vt[e], pf[rb], f32x4{0, 0, 0, 0});
+        st.o[rb][4 * c + e] += y * vs;
+      }
+  }
+}
+
+template <int D, int RB, bool FP8>
+__global__ __launch_bounds__(64 * B8_WAVES, 2) void attn_b8_kernel(B8Attn p) {
   constexpr int ND = D / 16;
   __shared__ float s_o[B8_WAVES][16][D + 4];
   __shared__ f32x2 s_ml[B8_WAVES][RB * 16];
@@ -172,14 +247,13 @@ __global__ __launch_bounds__(64 * B8_WAVES) void attn_b8_kernel(B8Attn p) {
   half8 q[RB][D / 32];
   int tok[RB];
   b8_load_q<D, RB>(p, h, row0, lane, q, tok);
-  float ref[RB], sum[RB];
-  f32x4 o[RB][ND];
+  B8Rows<D, RB> st;
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
-    ref[rb] = REF_INIT;
-    sum[rb] = 0.f;
+    st.ref[rb] = REF_INIT;
+    st.l[rb] = 0.f;
 #pragma unroll
-    for (int d = 0; d < ND; ++d) o[rb][d] = f32x4{0, 0, 0, 0};
+    for (int d = 0; d < ND; ++d) st.o[rb][d] = f32x4{0, 0, 0, 0};
   }
 
   for (int b0 = w0; b0 < w1; b0 += 64) {
@@ -187,72 +261,27 @@ __global__ __launch_bounds__(64 * B8_WAVES) void attn_b8_kernel(B8Attn p) {
     const int nb = min(64, w1 - b0);
     const int pgl = b8_page(p.c, b0 + min(lane, nb - 1));
     const size_t sat = (size_t)max(pgl, 0) * p.c.KVH + h;
+    B8Tile<D> t[2];
+    b8_load_tile<D>(p, h, __builtin_amdgcn_readlane(pgl, 0), lane, t[0]);
     const float ksl = ldg(p.c.ks + sat) * p.c2, vsl = ldg(p.c.vs + sat);
-    for (int i = 0; i < nb; ++i) {
-      const int pg = __builtin_amdgcn_readlane(pgl, i), lp = b0 + i;
-      if (pg < 0) continue;
-      const float ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ksl), i));
-      const float vs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vsl), i));
-      const size_t blk = ((size_t)pg * p.c.KVH + h) * (PAGE * D);
-      B8Tile<D> t;
-      b8_load_k<D>(p.c.k + blk, lane, t.k);
-      b8_load_v<D>(p.c.v + blk, lane, t.v);
-      f32x4 x[RB][2];
-      b8_scores<D, RB, FP8>(p, t.k, q, ks, lp < p.full_lo || lp >= p.full_hi, lp * PAGE, tok, lane, x);
-      float top[RB];
-      bool over = false;
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb) {
-        top[rb] = fmaxf(fmaxf(fmaxf(x[rb][0][0], x[rb][0][1]), fmaxf(x[rb][0][2], x[rb][0][3])),
-                        fmaxf(fmaxf(x[rb][1][0], x[rb][1][1]), fmaxf(x[rb][1][2], x[rb][1][3])));
-        over |= top[rb] > ref[rb] + REF_SLACK;
-      }
-      if (__ballot(over)) {
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-          const float m = row_max(top[rb]);
-          const float to = m > ref[rb] + REF_SLACK ? m - REF_BELOW : ref[rb];
-          const float f = fast_exp2(ref[rb] - to);
-          ref[rb] = to;
-          sum[rb] *= f;
-#pragma unroll
-          for (int d = 0; d < ND; ++d) o[rb][d] *= f;
-        }
-      }
-      half8 pf[RB];
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float e = fast_exp2(x[rb][j / 4][j % 4] - ref[rb]);
-          sum[rb] += e;
-          pf[rb][j] = (_Float16)e;
-        }
-#pragma unroll
-      for (int c = 0; c < D / 64; ++c) {
-        uint32_t w[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = b8_flip<FP8>(t.v[j][c]);
-        half8 vt[4];
-        b8_vt<FP8, 0>(w, vt[0], vt[1]);
-        b8_vt<FP8, 2>(w, vt[2], vt[3]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-          for (int rb = 0; rb < RB; ++rb) {
-            const f32x4 y = mfma16x16x32(vt[e], pf[rb], f32x4{0, 0, 0, 0});
-            o[rb][4 * c + e] += y * vs;
-          }
-      }
+    // the next page's loads are in flight while a page is worked on (past the last one: that page again, from L2)
+    auto step = [&](int i, const B8Tile<D>& now, B8Tile<D>& next) {
+      b8_load_tile<D>(p, h, __builtin_amdgcn_readlane(pgl, min(i + 1, nb - 1)), lane, next);
+      if (__builtin_amdgcn_readlane(pgl, i) >= 0)
+        b8_page<D, RB, FP8>(p, now, q, tok, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ksl), i)),
+                            __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vsl), i)), b0 + i, lane, st);
+    };
+    for (int i = 0; i < nb; i += 2) {
+      step(i, t[0], t[1]);
+      if (i + 1 < nb) step(i + 1, t[1], t[0]);
     }
   }
 
-  // The waves' shares, rescaled to the largest reference, added in wave order. Lane (n, g) holds row n's dims
-  // (D / 16) (4 g + i) + db at o[db][i].
+  // The waves' shares, rescaled to the largest reference, added in wave order.
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
-    sum[rb] = row_sum(sum[rb]);
-    if (g == 0) s_ml[wave][16 * rb + n] = f32x2{ref[rb], sum[rb]};
+    const float l = row_sum(st.l[rb]);
+    if (g == 0) s_ml[wave][16 * rb + n] = f32x2{st.ref[rb], l};
   }
   __syncthreads();
 #pragma unroll
@@ -260,12 +289,12 @@ __global__ __launch_bounds__(64 * B8_WAVES) void attn_b8_kernel(B8Attn p) {
     float m = REF_INIT;
 #pragma unroll
     for (int w = 0; w < B8_WAVES; ++w) m = fmaxf(m, s_ml[w][16 * rb + n][0]);
-    const float f = fast_exp2(ref[rb] - m);
+    const float f = fast_exp2(st.ref[rb] - m);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int d = 0; d < ND; d += 4) {
-        f32x4 y = {o[rb][d][i] * f, o[rb][d + 1][i] * f, o[rb][d + 2][i] * f, o[rb][d + 3][i] * f};
+        f32x4 y = {st.o[rb][d][i] * f, st.o[rb][d + 1][i] * f, st.o[rb][d + 2][i] * f, st.o[rb][d + 3][i] * f};
         *reinterpret_cast<f32x4*>(&s_o[wave][n][ND * (4 * g + i) + d]) = y;
       }
     __syncthreads();
@@ -337,81 +366,104 @@ __global__ __launch_bounds__(256) void attn_b8_merge_kernel(B8Attn p) {
 // mass_out[h][p] = (p < a ? mass_in[h][p] : 0) + sum over the rows of exp(score - lse), p < a + rows. A wave owns whole
 // pages, so every key's sum is one wave's, in a fixed order and without atomics. K alone is read.
 template <int D, int RB, bool FP8>
-__global__ __launch_bounds__(64 * B8_WAVES) void mass_b8_kernel(B8Attn p) {
+__global__ __launch_bounds__(64 * MASS_WAVES) void mass_b8_kernel(B8Attn p) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
   const int h = blockIdx.y;
   const int rows = p.rows ? min(max(ldc(p.rows), 0), p.M) : p.M;
   const int end = p.page0 + p.npages;
-  const int w0 = min(end, p.page0 + ((int)blockIdx.x * B8_WAVES + wave) * p.pps), w1 = min(end, w0 + p.pps);
+  const int w0 = min(end, p.page0 + ((int)blockIdx.x * MASS_WAVES + wave) * p.pps), w1 = min(end, w0 + p.pps);
+  const int live = p.a + rows, R = rows * p.G;
   const float* in = p.mass_in ? p.mass_in + (size_t)h * p.mass_stride : nullptr;
   float* out = p.mass_out + (size_t)h * p.mass_stride;
-  const int live = p.a + rows, R = rows * p.G;
-  for (int lp = w0; lp < w1; ++lp) {
-    const int pg = b8_page(p.c, lp);
-    const bool seen = pg >= 0 && (lp + 1) * (int64_t)PAGE > p.full_lo;  // full_lo: the first position any row sees
-    f32x4 acc[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
-    if (seen) {
-      const float ks = ldg(p.c.ks + (size_t)pg * p.c.KVH + h) * p.c2;
-      u32x4 k[2][D / 64];
-      b8_load_k<D>(p.c.k + ((size_t)pg * p.c.KVH + h) * (PAGE * D), lane, k);
-      for (int row0 = 0; row0 < R; row0 += 16 * RB) {
-        half8 q[RB][D / 32];
-        int tok[RB];
-        b8_load_q<D, RB>(p, h, row0, lane, q, tok);
-        f32x4 x[RB][2];
-        b8_scores<D, RB, FP8>(p, k, q, ks, true, lp * PAGE, tok, lane, x);
+  // Every group of 16 RB rows in turn over the wave's pages: the first group stores in + sum, later ones add to that.
+  for (int row0 = 0; row0 == 0 || row0 < R; row0 += 16 * RB) {
+    half8 q[RB][D / 32];
+    int tok[RB];
+    float l2[RB];
+    b8_load_q<D, RB>(p, h, row0, lane, q, tok);
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-          const int row = row0 + 16 * rb + n;
-          float l2 = -INFINITY;
-          if (row < R) l2 = ldg(p.lse_in + (size_t)tok[rb] * p.QH + h * p.G + row - tok[rb] * p.G) * 1.44269504088896341f;
-          if (l2 == -INFINITY) continue;  // past the rows, or a row that sees nothing
-#pragma unroll
-          for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[b][i] += fast_exp2(x[rb][b][i] - l2);
-        }
-      }
+    for (int rb = 0; rb < RB; ++rb) {
+      const int row = row0 + 16 * rb + n;
+      const float l = ldg(p.lse_in + (size_t)tok[rb] * p.QH + h * p.G + min(row, p.R - 1) - tok[rb] * p.G);
+      // past the rows, or a row that saw nothing: 2^(x - inf) adds nothing
+      l2[rb] = row < R && l != -INFINITY ? l * 1.44269504088896341f : INFINITY;
     }
-    // over the 16 rows of a lane group
+    for (int b0 = w0; b0 < w1; b0 += 64) {
+      const int nb = min(64, w1 - b0);
+      const int pgl = b8_page(p.c, b0 + min(lane, nb - 1));
+      const float ksl = ldg(p.c.ks + (size_t)max(pgl, 0) * p.c.KVH + h) * p.c2;
+      u32x4 k[2][2][D / 64];
+      auto load = [&](int i, u32x4 (&t)[2][D / 64]) {
+        const int pg = max(__builtin_amdgcn_readlane(pgl, i), 0);
+        b8_load_k<D>(p.c.k + ((size_t)pg * p.c.KVH + h) * (PAGE * D), lane, t);
+      };
+      load(0, k[0]);
+      auto step = [&](int i, const u32x4 (&now)[2][D / 64], u32x4 (&next)[2][D / 64]) {
+        load(min(i + 1, nb - 1), next);
+        const int lp = b0 + i;
+        // lane (n, g), n < 8, stores key 16 (n / 4) + 4 g + n % 4
+        const int kp = lp * PAGE + 16 * ((n >> 2) & 1) + 4 * g + (n & 3);
+        const bool mine = n < 8 && kp < live;
+        const float* from = row0 ? out : in;
+        const float old = mine && from && (row0 || kp < p.a) ? ldg(from + kp) : 0.f;
+        f32x4 acc[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+        if (__builtin_amdgcn_readlane(pgl, i) >= 0 && lp >= p.seen_lo && R > 0) {
+          float ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ksl), i));
+          f32x4 s[RB][2];
+          b8_scores<D, RB, FP8>(now, q, s);
+          if (lp < p.full_lo || lp >= p.full_hi) {
+            b8_mask<RB>(p, ks, lp * PAGE, tok, lane, s);
+            ks = 1.f;
+          }
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+          for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float v = acc[b][i];
-        v += __uint_as_float(row_ror<8>(__float_as_uint(v)));
-        v += __uint_as_float(row_ror<4>(__float_as_uint(v)));
-        v += __uint_as_float(row_ror<2>(__float_as_uint(v)));
-        v += __uint_as_float(row_ror<1>(__float_as_uint(v)));
-        acc[b][i] = v;
+            for (int j = 0; j < 8; ++j) acc[j / 4][j % 4] += fast_exp2(fmaf(s[rb][j / 4][j % 4], ks, -l2[rb]));
+        }
+        // over the 16 rows of a lane group
+        float v = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float y = acc[j / 4][j % 4];
+          y += __uint_as_float(row_ror<8>(__float_as_uint(y)));
+          y += __uint_as_float(row_ror<4>(__float_as_uint(y)));
+          y += __uint_as_float(row_ror<2>(__float_as_uint(y)));
+          y += __uint_as_float(row_ror<1>(__float_as_uint(y)));
+          v = n == j ? y : v;
+        }
+        if (mine) out[kp] = old + v;
+      };
+      for (int i = 0; i < nb; i += 2) {
+        step(i, k[0], k[1]);
+        if (i + 1 < nb) step(i + 1, k[1], k[0]);
       }
-    if (n < 8) {  // lane (n, g) stores key 16 (n / 4) + 4 g + n % 4
-      const int kp = lp * PAGE + 16 * (n >> 2) + 4 * g + (n & 3);
-      float v = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v = n == j ? acc[j / 4][j % 4] : v;
-      if (kp < live) out[kp] = (kp < p.a && in ? ldg(in + kp) : 0.f) + v;
     }
   }
 }
 
 // ---------------------------------------------------------------- plans and launches
-constexpr int B8_ROW_BLOCKS = 4;  // most 16-row blocks of a row group
+constexpr int B8_ROW_BLOCKS = 4;  // most 16-row blocks of a row group (2 at D = 128)
 
-void b8_attn_plan(B8Attn& p, int D, int splits, int cus) {
-  p.R = p.G * p.M;
-  const int blocks = (p.R + 15) / 16;
-  p.RG = (blocks + B8_ROW_BLOCKS - 1) / B8_ROW_BLOCKS;
-  p.rb = (blocks + p.RG - 1) / p.RG;
-  p.g_div = div_magic((uint32_t)p.G);
+// Which pages any row sees, and which every row sees whole.
+static void b8_sight(B8Attn& p, int D) {
   const int lo = std::min(p.a, std::max(p.start, p.window > 0 ? p.a - p.window + 1 : 0));  // first key any row sees
   p.page0 = lo / PAGE;
   p.npages = (p.a + p.M - 1) / PAGE + 1 - p.page0;
   const int whole = std::max(p.start, p.window > 0 ? p.a + p.M - p.window : 0);            // first context key all rows see
-  p.full_lo = (std::max(whole, 0) + PAGE - 1) / PAGE;
+  p.full_lo = whole / PAGE + (whole % PAGE > 0);
   p.full_hi = p.a / PAGE;
   p.c2 = 1.4426950408889634f / std::sqrt((float)D);
-  int S = splits > 0 ? splits : std::max(1, 2 * cus / (p.c.KVH * p.RG));
+}
+
+void b8_attn_plan(B8Attn& p, int D, int splits, int cus) {
+  p.R = p.G * p.M;
+  const int blocks = (p.R + 15) / 16;
+  const int most = D == 64 ? B8_ROW_BLOCKS : 2;
+  p.RG = (blocks + most - 1) / most;
+  p.rb = (blocks + p.RG - 1) / p.RG;
+  p.g_div = div_magic((uint32_t)p.G);
+  b8_sight(p, D);
+  int S = splits > 0 ? splits : std::max(1, (p.rb == 1 ? 2 : 1) * cus / (p.c.KVH * p.RG));
   S = std::min(S, (p.npages + B8_WAVES - 1) / B8_WAVES);
   S = std::max(1, std::min(S, 4096));
   p.pps = (p.npages + S - 1) / S;
@@ -423,14 +475,17 @@ size_t b8_attn_workspace(const B8Attn& p, int D) {
   return rows * D * sizeof(float) + rows * sizeof(f32x2);
 }
 
+template <int D, int RB, bool FP8>
+static void attn_b8_rows(const B8Attn& p, hipStream_t s) {
+  hipLaunchKernelGGL((attn_b8_kernel<D, RB, FP8>), dim3(p.S, p.c.KVH, p.RG), dim3(64 * B8_WAVES), 0, s, p);
+}
 template <int D, bool FP8>
 static void attn_b8_by_rows(const B8Attn& p, hipStream_t s) {
-  const dim3 grid(p.S, p.c.KVH, p.RG), block(64 * B8_WAVES);
-  switch (p.rb) {
-    case 1: hipLaunchKernelGGL((attn_b8_kernel<D, 1, FP8>), grid, block, 0, s, p); break;
-    case 2: hipLaunchKernelGGL((attn_b8_kernel<D, 2, FP8>), grid, block, 0, s, p); break;
-    case 3: hipLaunchKernelGGL((attn_b8_kernel<D, 3, FP8>), grid, block, 0, s, p); break;
-    default: hipLaunchKernelGGL((attn_b8_kernel<D, 4, FP8>), grid, block, 0, s, p); break;
+  if (p.rb == 1) return attn_b8_rows<D, 1, FP8>(p, s);
+  if (p.rb == 2) return attn_b8_rows<D, 2, FP8>(p, s);
+  if constexpr (D == 64) {
+    if (p.rb == 3) return attn_b8_rows<D, 3, FP8>(p, s);
+    return attn_b8_rows<D, 4, FP8>(p, s);
   }
 }
 
@@ -446,10 +501,11 @@ int b8_attn_launch(const B8Attn& p, int D, bool fp8, hipStream_t s) {
 
 template <int D, bool FP8>
 static void mass_b8_by_rows(const B8Attn& p, dim3 grid, hipStream_t s) {
-  const dim3 block(64 * B8_WAVES);
+  const dim3 block(64 * MASS_WAVES);
   switch (p.rb) {
     case 1: hipLaunchKernelGGL((mass_b8_kernel<D, 1, FP8>), grid, block, 0, s, p); break;
     case 2: hipLaunchKernelGGL((mass_b8_kernel<D, 2, FP8>), grid, block, 0, s, p); break;
+    case 3: hipLaunchKernelGGL((mass_b8_kernel<D, 3, FP8>), grid, block, 0, s, p); break;
     default: hipLaunchKernelGGL((mass_b8_kernel<D, 4, FP8>), grid, block, 0, s, p); break;
   }
 }
@@ -459,12 +515,12 @@ int b8_mass_launch(const B8Attn& q, int D, bool fp8, int cus, hipStream_t s) {
   p.R = p.G * p.M;
   p.rb = std::min(B8_ROW_BLOCKS, (p.R + 15) / 16);
   p.g_div = div_magic((uint32_t)p.G);
-  p.full_lo = std::min(p.a, std::max(p.start, p.window > 0 ? p.a - p.window + 1 : 0));
+  b8_sight(p, D);
+  p.seen_lo = p.page0;
   p.page0 = 0;  // every account is carried over, those of keys out of sight too
   p.npages = (p.a + p.M - 1) / PAGE + 1;
-  p.c2 = 1.4426950408889634f / std::sqrt((float)D);
-  p.pps = std::max(1, p.npages * p.c.KVH / (8 * cus * 2));
-  const dim3 grid((p.npages + p.pps * B8_WAVES - 1) / (p.pps * B8_WAVES), p.c.KVH);
+  p.pps = std::max(1, (int)((int64_t)p.npages * p.c.KVH / (8 * cus)));
+  const dim3 grid((p.npages + p.pps * MASS_WAVES - 1) / (p.pps * MASS_WAVES), p.c.KVH);
   if (D == 64) fp8 ? mass_b8_by_rows<64, true>(p, grid, s) : mass_b8_by_rows<64, false>(p, grid, s);
   else fp8 ? mass_b8_by_rows<128, true>(p, grid, s) : mass_b8_by_rows<128, false>(p, grid, s);
   return (int)hipGetLastError();

@@ -135,6 +135,7 @@ struct B8Attn {
   int rb;               // 16-row blocks of a row group
   float c2;             // log2(e) / sqrt(D)
   // the key accounts
+  int seen_lo;          // first logical page any row sees
   const float* lse_in;
   const int32_t* rows;
   const float* mass_in;
