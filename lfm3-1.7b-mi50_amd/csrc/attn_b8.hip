@@ -1,9 +1,12 @@
 // Verify attention over the 8-bit block-scaled K/V cache, and the accounts of attention weight its keys draw.
 //
 // o = softmax(q k^T / sqrt(D)) v for the rows of a KV head (row r = token r / G, query head r % G of the head's), keys in
-// blocks of 32 (a page) whose codes carry one scale: x = (q . code) ks log2(e) / sqrt(D), P = 2^(x - ref), and the block's
-// share of o is vs (P . codes). Codes (int8 or e4m3) are exact in fp16, so the products on the matrix cores are of exact
-// operands but for P, which is rounded to fp16 once; scales, running references, sums and outputs are fp32.
+// blocks of 32 (a page) whose codes carry one scale: x = (q . code) ks log2(e) / sqrt(D). V's scale goes into the exponent:
+// P = 2^(x + log2 vs - ref) with the row's running reference over x + log2 vs, so that o += P . codes accumulates in the matrix
+// cores whatever the blocks' scales, and l += (sum of P) / vs keeps the softmax sum in the same units (with o += vs (P . codes)
+// instead, D / 4 multiply-adds a row block and page: 79 -> 58 us at 128k keys and 33 tokens). Codes (int8 or e4m3) are exact
+// in fp16, so the products are of exact operands but for P, which is rounded to fp16 once; scales, references, sums and
+// outputs are fp32.
 //
 // A wave owns whole pages and all rows of its row group, and takes its operands from memory in registers: nothing is shared
 // until the end. Score product: A = K (16 keys), B = Q, so that a lane holds one row's scores of keys 16 b + 4 g + i
@@ -17,8 +20,8 @@
 namespace dspark {
 
 constexpr int B8_WAVES = 8, MASS_WAVES = 4;
-// Running reference in log2 units: P = 2^(x - ref), ref set to the row's largest x less 8 when some x passes ref + 15:
-// P stays under 2^15, and a P of 2^-22 of the largest is still a normal half.
+// Running reference in log2 units, set to the row's largest x + log2 vs less 8 when one passes ref + 15: P stays under 2^15,
+// and a P of 2^-22 of the largest is still a normal half (one below is off by 2^-33 of the largest at most).
 constexpr float REF_INIT = -1e30f, REF_BELOW = 8.f, REF_SLACK = 15.f;
 
 template <int D>
@@ -86,12 +89,15 @@ __device__ __forceinline__ void b8_vt(const uint32_t (&w)[8], half8& v0, half8& 
   v1 = half8{b[0][0], b[0][1], b[1][0], b[1][1], b[2][0], b[2][1], b[3][0], b[3][1]};
 }
 
+// The larger one by the instruction that passes a NaN on: fmaxf costs a second one to quiet its operands.
+__device__ __forceinline__ float max_of(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+__device__ __forceinline__ float max3(float a, float b, float c) { return max_of(max_of(a, b), c); }
 // Largest over the four lanes of a row (lanes n, 16 + n, 32 + n, 48 + n), in all of them; and the sum.
 __device__ __forceinline__ float row_max(float v) {
   const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  v = max_of(__uint_as_float(a[0]), __uint_as_float(a[1]));
   const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+  return max_of(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 __device__ __forceinline__ float row_sum(float v) {
   const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -120,17 +126,21 @@ __device__ __forceinline__ void b8_load_q(const B8Attn& p, int h, int row0, int 
 __device__ __forceinline__ int row_lo(const B8Attn& p, int t) { return max(p.start, p.window > 0 ? p.a + t - p.window + 1 : 0); }
 __device__ __forceinline__ int row_hi(const B8Attn& p, int t) { return p.causal ? p.a + t + 1 : p.a + p.M; }
 
+template <int D, bool FP8>
+__device__ __forceinline__ void b8_k_operand(const u32x4 (&k)[D / 64], half8 (&kf)[D / 32]) {
+#pragma unroll
+  for (int u = 0; u < D / 64; ++u) {
+    kf[2 * u] = b8_half8<FP8>(b8_flip<FP8>(k[u][0]), b8_flip<FP8>(k[u][1]));
+    kf[2 * u + 1] = b8_half8<FP8>(b8_flip<FP8>(k[u][2]), b8_flip<FP8>(k[u][3]));
+  }
+}
 // q . code of one page: s[rb][b][i] of key 16 b + 4 g + i, still to be multiplied by the block's scale.
 template <int D, int RB, bool FP8>
 __device__ __forceinline__ void b8_scores(const u32x4 (&k)[2][D / 64], const half8 (&q)[RB][D / 32], f32x4 (&s)[RB][2]) {
 #pragma unroll
   for (int b = 0; b < 2; ++b) {
     half8 kf[D / 32];
-#pragma unroll
-    for (int u = 0; u < D / 64; ++u) {
-      kf[2 * u] = b8_half8<FP8>(b8_flip<FP8>(k[b][u][0]), b8_flip<FP8>(k[b][u][1]));
-      kf[2 * u + 1] = b8_half8<FP8>(b8_flip<FP8>(k[b][u][2]), b8_flip<FP8>(k[b][u][3]));
-    }
+    b8_k_operand<D, FP8>(k[b], kf);
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
       s[rb][b] = f32x4{0, 0, 0, 0};
@@ -176,19 +186,19 @@ struct B8Rows {
 
 template <int D, int RB, bool FP8>
 __device__ __forceinline__ void b8_page(const B8Attn& p, const B8Tile<D>& t, const half8 (&q)[RB][D / 32], const int (&tok)[RB],
-                                        float ks, float vs, int lp, int lane, B8Rows<D, RB>& st) {
+                                        float ks, float lv, float iv, int lp, int lane, B8Rows<D, RB>& st) {
   f32x4 s[RB][2];
   b8_scores<D, RB, FP8>(t.k, q, s);
   if (lp < p.full_lo || lp >= p.full_hi) {
     b8_mask<RB>(p, ks, lp * PAGE, tok, lane, s);
     ks = 1.f;
   }
-  float top[RB];
+  float top[RB], at[RB];
   bool over = false;
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
-    top[rb] = ks * fmaxf(fmaxf(fmaxf(s[rb][0][0], s[rb][0][1]), fmaxf(s[rb][0][2], s[rb][0][3])),
-                         fmaxf(fmaxf(s[rb][1][0], s[rb][1][1]), fmaxf(s[rb][1][2], s[rb][1][3])));
+    top[rb] = fmaf(ks, max3(max3(s[rb][0][0], s[rb][0][1], s[rb][0][2]), max3(s[rb][0][3], s[rb][1][0], s[rb][1][1]),
+                            max_of(s[rb][1][2], s[rb][1][3])), lv);
     over |= top[rb] > st.ref[rb] + REF_SLACK;
   }
   if (__ballot(over)) {
@@ -203,16 +213,18 @@ __device__ __forceinline__ void b8_page(const B8Attn& p, const B8Tile<D>& t, con
       for (int d = 0; d < D / 16; ++d) st.o[rb][d] *= f;
     }
   }
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) at[rb] = lv - st.ref[rb];
   half8 pf[RB];
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
     float e[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      e[j] = fast_exp2(fmaf(s[rb][j / 4][j % 4], ks, -st.ref[rb]));
+      e[j] = fast_exp2(fmaf(s[rb][j / 4][j % 4], ks, at[rb]));
       pf[rb][j] = (_Float16)e[j];
     }
-    st.l[rb] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+    st.l[rb] = fmaf(((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7])), iv, st.l[rb]);
   }
 #pragma unroll
   for (int c = 0; c < D / 64; ++c) {
@@ -225,10 +237,7 @@ __device__ __forceinline__ void b8_page(const B8Attn& p, const B8Tile<D>& t, con
 #pragma unroll
     for (int e = 0; e < 4; ++e)
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb) {
-        const f32x4 y = mfma16x16x32(vt[e], pf[rb], f32x4{0, 0, 0, 0});
-        st.o[rb][4 * c + e] += y * vs;
-      }
+      for (int rb = 0; rb < RB; ++rb) st.o[rb][4 * c + e] = mfma16x16x32(vt[e], pf[rb], st.o[rb][4 * c + e]);
   }
 }
 
@@ -264,12 +273,18 @@ __global__ __launch_bounds__(64 * B8_WAVES, 2) void attn_b8_kernel(B8Attn p) {
     B8Tile<D> t[2];
     b8_load_tile<D>(p, h, __builtin_amdgcn_readlane(pgl, 0), lane, t[0]);
     const float ksl = ldg(p.c.ks + sat) * p.c2, vsl = ldg(p.c.vs + sat);
+    // log2 vs, and 1 / vs as its very inverse. A block of zeros (scale 0) takes the smallest scale about: any will do for its
+    // sum, and the smallest moves no reference.
+    const bool some = vsl > 0.f;
+    const float low = -wave_max(some ? -__builtin_amdgcn_logf(vsl) : -INFINITY);
+    const float lvl = some ? __builtin_amdgcn_logf(vsl) : low < INFINITY ? low : 0.f, ivl = fast_exp2(-lvl);
     // the next page's loads are in flight while a page is worked on (past the last one: that page again, from L2)
     auto step = [&](int i, const B8Tile<D>& now, B8Tile<D>& next) {
       b8_load_tile<D>(p, h, __builtin_amdgcn_readlane(pgl, min(i + 1, nb - 1)), lane, next);
       if (__builtin_amdgcn_readlane(pgl, i) >= 0)
         b8_page<D, RB, FP8>(p, now, q, tok, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ksl), i)),
-                            __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vsl), i)), b0 + i, lane, st);
+                            __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lvl), i)),
+                            __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ivl), i)), b0 + i, lane, st);
     };
     for (int i = 0; i < nb; i += 2) {
       step(i, t[0], t[1]);
@@ -363,8 +378,11 @@ __global__ __launch_bounds__(256) void attn_b8_merge_kernel(B8Attn p) {
 }
 
 // ---------------------------------------------------------------- accounts of attention weight
-// mass_out[h][p] = (p < a ? mass_in[h][p] : 0) + sum over the rows of exp(score - lse), p < a + rows. A wave owns whole
-// pages, so every key's sum is one wave's, in a fixed order and without atomics. K alone is read.
+// mass_out[h][p] = (p < a ? mass_in[h][p] : 0) + sum over the rows of 2^(x - lse log2(e)), p < a + rows. A wave owns whole
+// pages, so every key's sum is one wave's, in a fixed order and without atomics. K alone is read. The score product has its
+// operands the other way round than the attention's (A = Q, B = K): a lane holds one key's scores of rows 4 g + i, adds them
+// up in place over all row blocks, and only the four lanes of a key are added across (sums over the rows' lanes instead, with
+// A = K: eight row reductions a page, 39 -> 25 us at 128k keys and 64 rows a head).
 template <int D, int RB, bool FP8>
 __global__ __launch_bounds__(64 * MASS_WAVES) void mass_b8_kernel(B8Attn p) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
@@ -379,63 +397,69 @@ __global__ __launch_bounds__(64 * MASS_WAVES) void mass_b8_kernel(B8Attn p) {
   for (int row0 = 0; row0 == 0 || row0 < R; row0 += 16 * RB) {
     half8 q[RB][D / 32];
     int tok[RB];
-    float l2[RB];
     b8_load_q<D, RB>(p, h, row0, lane, q, tok);
+    f32x4 l2[RB];
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      const int row = row0 + 16 * rb + n;
-      const float l = ldg(p.lse_in + (size_t)tok[rb] * p.QH + h * p.G + min(row, p.R - 1) - tok[rb] * p.G);
-      // past the rows, or a row that saw nothing: 2^(x - inf) adds nothing
-      l2[rb] = row < R && l != -INFINITY ? l * 1.44269504088896341f : INFINITY;
-    }
+    for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = row0 + 16 * rb + 4 * g + i, rc = min(row, p.R - 1), t = div_by(rc, p.g_div);
+        const float l = ldg(p.lse_in + (size_t)t * p.QH + h * p.G + rc - t * p.G);
+        // past the rows, or a row that saw nothing: 2^(x - inf) adds nothing
+        l2[rb][i] = row < R && l != -INFINITY ? l * -1.44269504088896341f : -INFINITY;
+      }
     for (int b0 = w0; b0 < w1; b0 += 64) {
       const int nb = min(64, w1 - b0);
       const int pgl = b8_page(p.c, b0 + min(lane, nb - 1));
       const float ksl = ldg(p.c.ks + (size_t)max(pgl, 0) * p.c.KVH + h) * p.c2;
       u32x4 k[2][2][D / 64];
-      auto load = [&](int i, u32x4 (&t)[2][D / 64]) {
-        const int pg = max(__builtin_amdgcn_readlane(pgl, i), 0);
+      float old[2];
+      // lane (n, g), g < 2, stores key 16 g + n
+      auto load = [&](int i, u32x4 (&t)[2][D / 64], float& was) {
+        const int pg = max(__builtin_amdgcn_readlane(pgl, i), 0), kp = (b0 + i) * PAGE + 16 * (g & 1) + n;
         b8_load_k<D>(p.c.k + ((size_t)pg * p.c.KVH + h) * (PAGE * D), lane, t);
-      };
-      load(0, k[0]);
-      auto step = [&](int i, const u32x4 (&now)[2][D / 64], u32x4 (&next)[2][D / 64]) {
-        load(min(i + 1, nb - 1), next);
-        const int lp = b0 + i;
-        // lane (n, g), n < 8, stores key 16 (n / 4) + 4 g + n % 4
-        const int kp = lp * PAGE + 16 * ((n >> 2) & 1) + 4 * g + (n & 3);
-        const bool mine = n < 8 && kp < live;
         const float* from = row0 ? out : in;
-        const float old = mine && from && (row0 || kp < p.a) ? ldg(from + kp) : 0.f;
-        f32x4 acc[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+        was = from && kp < (row0 ? live : p.a) ? ldg(from + kp) : 0.f;
+      };
+      load(0, k[0], old[0]);
+      auto step = [&](int i, const u32x4 (&now)[2][D / 64], float was, u32x4 (&next)[2][D / 64], float& then) {
+        load(min(i + 1, nb - 1), next, then);
+        const int lp = b0 + i;
+        float acc[2] = {0.f, 0.f};
         if (__builtin_amdgcn_readlane(pgl, i) >= 0 && lp >= p.seen_lo && R > 0) {
-          float ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ksl), i));
-          f32x4 s[RB][2];
-          b8_scores<D, RB, FP8>(now, q, s);
-          if (lp < p.full_lo || lp >= p.full_hi) {
-            b8_mask<RB>(p, ks, lp * PAGE, tok, lane, s);
-            ks = 1.f;
+          const float ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ksl), i));
+          const bool edge = lp < p.full_lo || lp >= p.full_hi;
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            half8 kf[D / 32];
+            b8_k_operand<D, FP8>(now[b], kf);
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+              f32x4 s = {0, 0, 0, 0}, x;
+#pragma unroll
+              for (int e = 0; e < D / 32; ++e) s = mfma16x16x32(q[rb][e], kf[e], s);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) x[i] = fmaf(s[i], ks, l2[rb][i]);
+              if (edge) {
+                const int kp = lp * PAGE + 16 * b + n;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const int t = div_by(min(row0 + 16 * rb + 4 * g + i, p.R - 1), p.g_div);
+                  if (kp < p.a ? kp < row_lo(p, t) : kp >= row_hi(p, t)) x[i] = -INFINITY;
+                }
+              }
+#pragma unroll
+              for (int i = 0; i < 4; ++i) acc[b] += fast_exp2(x[i]);
+            }
           }
-#pragma unroll
-          for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) acc[j / 4][j % 4] += fast_exp2(fmaf(s[rb][j / 4][j % 4], ks, -l2[rb]));
         }
-        // over the 16 rows of a lane group
-        float v = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          float y = acc[j / 4][j % 4];
-          y += __uint_as_float(row_ror<8>(__float_as_uint(y)));
-          y += __uint_as_float(row_ror<4>(__float_as_uint(y)));
-          y += __uint_as_float(row_ror<2>(__float_as_uint(y)));
-          y += __uint_as_float(row_ror<1>(__float_as_uint(y)));
-          v = n == j ? y : v;
-        }
-        if (mine) out[kp] = old + v;
+        const float v0 = row_sum(acc[0]), v1 = row_sum(acc[1]);  // (the exchanges take every lane: no branch around them)
+        const int kp = lp * PAGE + 16 * (g & 1) + n;
+        if (g < 2 && kp < live) out[kp] = was + (g ? v1 : v0);
       };
       for (int i = 0; i < nb; i += 2) {
-        step(i, k[0], k[1]);
-        if (i + 1 < nb) step(i + 1, k[1], k[0]);
+        step(i, k[0], old[0], k[1], old[1]);
+        if (i + 1 < nb) step(i + 1, k[1], old[1], k[0], old[0]);
       }
     }
   }

@@ -158,13 +158,20 @@ def test_read_into_wider_rows_leaves_the_rest():
 
 
 # ------------------------------------------------------------------------------------------------ attention
-# Of a result o = sum P v / sum P with A = sum P |v| / sum P, P is rounded to fp16 once (2^-11 of each P that is a normal
-# half; those below are 2^-22 of the largest at most and off by 2^-33 of it: under 2^-16 A together for 2^17 keys of like
-# size, and under 2^-33 sum |v| always). Scores of up to 64 (log2 units) are sums of exact products in fp32: off by about
-# 2^-24 64 = 2^-18 and their exponential relatively by as much; sums in fp32 add a few 2^-24 more. 2^-16 A covers these.
-# The fp16 output is rounded once more.
-def bound(o, mag, half):
-    return (2.0 ** -11 + 2.0 ** -16) * mag + (2.0 ** -11 * np.abs(o) + 2.0 ** -25 if half else 0) + 1e-9
+# Of a result o = sum p v with A = sum p |v| (p the softmax): V's scale vs goes into the exponent and p vs, times a power of two
+# that takes the row's largest to at least 2^8, is rounded to fp16 once: by 2^-11 of itself where that is a normal half, and
+# by 2^-25 below 2^-14, which is 2^-33 of the row's largest. Codes c are up to T = 127 or 448, so the latter errors of N keys
+# are under 2^-33 N max(p vs) T, and max(p vs T) <= B = sum p vs T. Scores of up to 64 (log2 units) are sums of exact products
+# in fp32, off by about 2^-24 64 = 2^-18, log2 vs (up to 32) by 2^-19, and their exponential relatively by as much; sums in
+# fp32 add a few 2^-24 more. 2^-16 A covers these. The fp16 output is rounded once more.
+def bound(o, mag, half, N, B):
+    return ((2.0 ** -11 + 2.0 ** -16) * mag + 2.0 ** -33 * N * B + (2.0 ** -11 * np.abs(o) + 2.0 ** -25 if half else 0) + 1e-9)
+
+
+def tops(c, n):
+    """What the largest code of each position's V block stands for, [n][KVH][1]."""
+    pg = np.array([c.page(i // 32) for i in range(n)])
+    return (np.where(pg[:, None] >= 0, c.scale["v"][pg], 0) * (127 if c.code == "int8" else 448))[..., None]
 
 
 def run_attention(c, q, a, gate=None, splits=0, **mask):
@@ -184,8 +191,9 @@ def check_attention(c, q, a, gate=None, splits=0, start=0, window=0, causal=True
     see = b8.visible(M, a, start, window, causal, here)
     o, lse, mag = b8.attention(q, k, v, see, gate)
     o16, o32, l = run_attention(c, q, a, gate, splits, start=start, window=window, causal=causal)
-    assert np.all(np.abs(o32 - o) <= bound(o, mag, False)), np.max(np.abs(o32 - o) - bound(o, mag, False))
-    assert np.all(np.abs(o16 - o) <= bound(o, mag, True))
+    B = b8.attention(q, k, np.broadcast_to(tops(c, a + M), v.shape), see, gate)[2]
+    assert np.all(np.abs(o32 - o) <= bound(o, mag, False, a + M, B)), np.max(np.abs(o32 - o) - bound(o, mag, False, a + M, B))
+    assert np.all(np.abs(o16 - o) <= bound(o, mag, True, a + M, B))
     dead = np.isneginf(lse)
     assert np.array_equal(np.isneginf(l), dead) and not o32[dead].any() and not o16[dead].any()
     # a score is off by 2^-18 at most, the logarithm of the sum by a few 2^-24 of its size
@@ -228,13 +236,26 @@ def test_attention_splits_and_rows(splits, M, QH, D):
 
 @pytest.mark.parametrize("code", KINDS)
 def test_attention_sizes_far_apart(code):
-    """Blocks of V up to 2^30 apart and scores up to +-40: no block is lost beside a larger one that the row hardly sees."""
+    """Blocks of V up to 2^30 apart and scores up to +-40: no block's weight is lost from the sum beside larger ones."""
     rng = np.random.default_rng(8)
     M, KVH, D, a = 3, 2, 64, 700
     c = filled(code, a + M, KVH, D, 2)
     c.scale["v"] *= np.exp2(rng.integers(-20, 10, c.scale["v"].shape)).astype(np.float32)
     q = (rng.standard_normal((M, 8, D)) * 6).astype(np.float16)
     check_attention(c, q, a)
+
+
+@pytest.mark.parametrize("code", KINDS)
+def test_attention_blocks_of_zeros(code):
+    """Blocks of V (or K) that are all zeros, the first and the last of a cache, single and all: they weigh in the sum."""
+    rng = np.random.default_rng(8)
+    M, KVH, D, a = 3, 2, 64, 400
+    for x in "vk":
+        for gone in ([0], [3, 4], list(range(12)), list(range(13))):
+            c = filled(code, a + M, KVH, D, 2)
+            c.scale[x][gone] = 0
+            c.raw[x][gone] = 0
+            check_attention(c, rng.standard_normal((M, 8, D)).astype(np.float16), a)
 
 
 @pytest.mark.parametrize("code", KINDS)
@@ -510,7 +531,8 @@ def test_rounds_with_a_bounded_cache(code, QH, KVH, D):
         kk, vv, here = c.read(0, a + M)
         see = b8.visible(M, a, 0, 0, True, here)
         o, wl, mag = b8.attention(q, kk, vv, see)
-        assert np.all(np.abs(o32.cpu().numpy() - o) <= bound(o, mag, False))
+        B = b8.attention(q, kk, np.broadcast_to(tops(c, a + M), vv.shape), see)[2]
+        assert np.all(np.abs(o32.cpu().numpy() - o) <= bound(o, mag, False, a + M, B))
         # drafts accepted up to a chosen one
         good = int(rng.integers(0, M))
         tokens = rng.integers(0, V, M)
