@@ -19,7 +19,9 @@
 
 namespace dspark {
 
-constexpr int B8_WAVES = 8, MASS_WAVES = 4;
+// Waves of a workgroup, which fills a CU: as many as the registers of RB row blocks leave (o alone takes D RB / 4).
+constexpr int b8_waves(int D, int RB) { return D == 64 ? (RB == 1 ? 16 : RB <= 3 ? 12 : 8) : RB == 1 ? 12 : 8; }
+constexpr int MASS_WAVES = 4;
 // Running reference in log2 units, set to the row's largest x + log2 vs less 8 when one passes ref + 15: P stays under 2^15,
 // and a P of 2^-22 of the largest is still a normal half (one below is off by 2^-33 of the largest at most).
 constexpr float REF_INIT = -1e30f, REF_BELOW = 8.f, REF_SLACK = 15.f;
@@ -241,18 +243,35 @@ __device__ __forceinline__ void b8_page(const B8Attn& p, const B8Tile<D>& t, con
   }
 }
 
-template <int D, int RB, bool FP8>
-__global__ __launch_bounds__(64 * B8_WAVES, 2) void attn_b8_kernel(B8Attn p) {
-  constexpr int ND = D / 16;
-  __shared__ float s_o[B8_WAVES][16][D + 4];
-  __shared__ f32x2 s_ml[B8_WAVES][RB * 16];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
-  const int h = blockIdx.y, sp = blockIdx.x, row0 = blockIdx.z * RB * 16;
-  const int end = p.page0 + p.npages;
-  const int sp0 = p.page0 + sp * p.pps, sp1 = min(end, sp0 + p.pps);
-  const int ppw = (p.pps + B8_WAVES - 1) / B8_WAVES;
-  const int w0 = min(sp1, sp0 + wave * ppw), w1 = min(sp1, w0 + ppw);
+// Four dims (4 c ...) of a row's result from its sums: 1 / l, the gate, the stores.
+template <int D>
+__device__ __forceinline__ void b8_store(const B8Attn& p, int h, int row, int c, f32x4 acc, float ref, float l, float gate) {
+  const int t = div_by(row, p.g_div), qh = h * p.G + row - t * p.G;
+  const f32x4 o = l == 0.f ? f32x4{0, 0, 0, 0} : acc * (gate / l);
+  const size_t e = ((size_t)t * p.QH + qh) * D + 4 * c;
+  if (p.out16) *reinterpret_cast<half4*>(p.out16 + e) = half4{(_Float16)o[0], (_Float16)o[1], (_Float16)o[2], (_Float16)o[3]};
+  if (p.out32) *reinterpret_cast<f32x4*>(p.out32 + e) = o;
+  if (p.lse && c == 0) p.lse[(size_t)t * p.QH + qh] = l == 0.f ? -INFINITY : (ref + log2f(l)) * 0.69314718055994531f;
+}
+__device__ __forceinline__ float b8_gate(const B8Attn& p, int h, int row) {
+  const int t = div_by(row, p.g_div), qh = h * p.G + row - t * p.G;
+  return p.gate ? 1.f / (1.f + __expf(-ldg(p.gate + (size_t)t * p.QH + qh))) : 1.f;
+}
 
+// One workgroup per (KV head, key split, row group), the split's pages spread evenly over its waves. Splits go to the
+// workspace and a second kernel adds them; a single split is finished here.
+template <int D, int RB, bool FP8>
+__global__ __launch_bounds__(64 * b8_waves(D, RB), b8_waves(D, RB) / 4) void attn_b8_kernel(B8Attn p) {
+  constexpr int ND = D / 16, NW = b8_waves(D, RB), ROWS = 16 * RB, NT = 64 * NW;
+  __shared__ float s_o[NW][ROWS][D + 4];  // (rows 4 banks apart)
+  __shared__ f32x2 s_ml[NW][ROWS];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+  const int h = blockIdx.y, sp = blockIdx.x, row0 = blockIdx.z * ROWS;
+  // wave gw of the head's S NW waves: pps pages, one more for the first `more` waves
+  const int gw = sp * NW + wave;
+  const int w0 = p.page0 + gw * p.pps + min(gw, p.more), w1 = w0 + p.pps + (gw < p.more ? 1 : 0);
+
+  int pgl = b8_page(p.c, min(w0 + lane, p.page0 + p.npages - 1));  // lane i knows page b0 + i
   half8 q[RB][D / 32];
   int tok[RB];
   b8_load_q<D, RB>(p, h, row0, lane, q, tok);
@@ -266,9 +285,8 @@ __global__ __launch_bounds__(64 * B8_WAVES, 2) void attn_b8_kernel(B8Attn p) {
   }
 
   for (int b0 = w0; b0 < w1; b0 += 64) {
-    // lane i knows page b0 + i
     const int nb = min(64, w1 - b0);
-    const int pgl = b8_page(p.c, b0 + min(lane, nb - 1));
+    if (b0 > w0) pgl = b8_page(p.c, min(b0 + lane, w1 - 1));
     const size_t sat = (size_t)max(pgl, 0) * p.c.KVH + h;
     B8Tile<D> t[2];
     b8_load_tile<D>(p, h, __builtin_amdgcn_readlane(pgl, 0), lane, t[0]);
@@ -292,89 +310,111 @@ __global__ __launch_bounds__(64 * B8_WAVES, 2) void attn_b8_kernel(B8Attn p) {
     }
   }
 
-  // The waves' shares, rescaled to the largest reference, added in wave order.
+  // Every wave's sums into LDS at once, then each thread adds up some rows' quads, rescaled to the row's largest reference,
+  // in wave order. (Row block by row block with 16 rows of LDS: two more barriers and a drain each, 5 us instead of 1.5.)
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
     const float l = row_sum(st.l[rb]);
     if (g == 0) s_ml[wave][16 * rb + n] = f32x2{st.ref[rb], l};
-  }
-  __syncthreads();
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    float m = REF_INIT;
-#pragma unroll
-    for (int w = 0; w < B8_WAVES; ++w) m = fmaxf(m, s_ml[w][16 * rb + n][0]);
-    const float f = fast_exp2(st.ref[rb] - m);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int d = 0; d < ND; d += 4) {
-        f32x4 y = {st.o[rb][d][i] * f, st.o[rb][d + 1][i] * f, st.o[rb][d + 2][i] * f, st.o[rb][d + 3][i] * f};
-        *reinterpret_cast<f32x4*>(&s_o[wave][n][ND * (4 * g + i) + d]) = y;
-      }
-    __syncthreads();
-    for (int e = threadIdx.x; e < 16 * (D / 4); e += 64 * B8_WAVES) {
-      const int r = e / (D / 4), c = e % (D / 4), row = row0 + 16 * rb + r;
-      f32x4 acc = {0, 0, 0, 0};
-      float mm = REF_INIT, l = 0.f;
+      for (int d = 0; d < ND; d += 4)
+        *reinterpret_cast<f32x4*>(&s_o[wave][16 * rb + n][ND * (4 * g + i) + d]) =
+            f32x4{st.o[rb][d][i], st.o[rb][d + 1][i], st.o[rb][d + 2][i], st.o[rb][d + 3][i]};
+  }
+  constexpr int QUADS = D / 4, PER = NT / QUADS;  // rows side by side
+  const int c = threadIdx.x % QUADS;
+  float gate[(ROWS + PER - 1) / PER];
+  if (p.S == 1)
 #pragma unroll
-      for (int w = 0; w < B8_WAVES; ++w) {
-        acc += *reinterpret_cast<const f32x4*>(&s_o[w][r][4 * c]);
-        mm = fmaxf(mm, s_ml[w][16 * rb + r][0]);
-      }
+    for (int k = 0; k < (ROWS + PER - 1) / PER; ++k) gate[k] = b8_gate(p, h, min(row0 + (int)threadIdx.x / QUADS + k * PER, p.R - 1));
+  lds_barrier();
 #pragma unroll
-      for (int w = 0; w < B8_WAVES; ++w) l += s_ml[w][16 * rb + r][1] * fast_exp2(s_ml[w][16 * rb + r][0] - mm);
-      if (row < p.R) {
-        const size_t at = ((size_t)h * p.R + row) * p.S + sp;
-        *reinterpret_cast<f32x4*>(p.part_acc + at * D + 4 * c) = acc;
-        if (c == 0) p.part_ml[at] = f32x2{mm, l};
-      }
+  for (int k = 0; k < (ROWS + PER - 1) / PER; ++k) {
+    const int r = threadIdx.x / QUADS + k * PER, row = row0 + r;
+    if (r >= ROWS || row >= p.R) break;
+    f32x2 ml[NW];
+    float m = REF_INIT, l = 0.f;
+    f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      ml[w] = s_ml[w][r];
+      m = max_of(m, ml[w][0]);
     }
-    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float f = fast_exp2(ml[w][0] - m);
+      l = fmaf(ml[w][1], f, l);
+      acc += *reinterpret_cast<const f32x4*>(&s_o[w][r][4 * c]) * f;
+    }
+    if (p.S == 1) {
+      b8_store<D>(p, h, row, c, acc, m, l, gate[k]);
+    } else {
+      const size_t at = ((size_t)h * p.R + row) * p.S + sp;
+      *reinterpret_cast<f32x4*>(p.part_acc + at * D + 4 * c) = acc;
+      if (c == 0) p.part_ml[at] = f32x2{m, l};
+    }
   }
 }
 
-// One workgroup per (row, KV head): the splits' shares rescaled and added, 256 / (D / 4) splits side by side, in a fixed
-// order; then 1 / sum, the gate, and the stores.
+// One workgroup per (row, KV head): the splits' sums rescaled and added, 256 / (D / 4) splits side by side, in a fixed
+// order, and finished.
 template <int D>
 __global__ __launch_bounds__(256) void attn_b8_merge_kernel(B8Attn p) {
-  constexpr int Q = D / 4, SL = 256 / Q;
+  constexpr int Q = D / 4, SL = 256 / Q, PER = 4;
   __shared__ f32x4 s_acc[SL][Q];
-  __shared__ float s_m[SL], s_l[SL];
+  __shared__ f32x2 s_ml[SL];
   const int row = blockIdx.x, h = blockIdx.y, c = threadIdx.x % Q, j = threadIdx.x / Q;
   const size_t at = ((size_t)h * p.R + row) * p.S;
   float m = REF_INIT, l = 0.f;
   f32x4 acc = {0, 0, 0, 0};
-  for (int s = j; s < p.S; s += SL) {
-    const f32x2 ml = ldg(p.part_ml + at + s);
-    const f32x4 a = ldg(reinterpret_cast<const f32x4*>(p.part_acc + (at + s) * D + 4 * c));
-    const float to = fmaxf(m, ml[0]), f0 = fast_exp2(m - to), f1 = fast_exp2(ml[0] - to);
-    acc = acc * f0 + a * f1;
-    l = l * f0 + ml[1] * f1;
+  const float gate = b8_gate(p, h, row);
+  for (int s0 = j; s0 < p.S; s0 += SL * PER) {
+    f32x2 ml[PER];
+    f32x4 a[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int s = min(s0 + i * SL, p.S - 1);
+      ml[i] = ldg(p.part_ml + at + s);
+      a[i] = ldg(reinterpret_cast<const f32x4*>(p.part_acc + (at + s) * D + 4 * c));
+    }
+    float to = m;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (s0 + i * SL >= p.S) ml[i][0] = REF_INIT, ml[i][1] = 0.f, a[i] = f32x4{0, 0, 0, 0};
+      to = max_of(to, ml[i][0]);
+    }
+    const float f0 = fast_exp2(m - to);
+    acc *= f0;
+    l *= f0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const float f = fast_exp2(ml[i][0] - to);
+      acc += a[i] * f;
+      l = fmaf(ml[i][1], f, l);
+    }
     m = to;
   }
   s_acc[j][c] = acc;
-  if (c == 0) {
-    s_m[j] = m;
-    s_l[j] = l;
-  }
-  __syncthreads();
+  if (c == 0) s_ml[j] = f32x2{m, l};
+  lds_barrier();
   if (j) return;
-  for (int s = 0; s < SL; ++s) m = fmaxf(m, s_m[s]);
+  f32x2 ml[SL];
+#pragma unroll
+  for (int s = 0; s < SL; ++s) {
+    ml[s] = s_ml[s];
+    m = max_of(m, ml[s][0]);
+  }
   acc = f32x4{0, 0, 0, 0};
   l = 0.f;
+#pragma unroll
   for (int s = 0; s < SL; ++s) {
-    const float f = fast_exp2(s_m[s] - m);
+    const float f = fast_exp2(ml[s][0] - m);
     acc += s_acc[s][c] * f;
-    l += s_l[s] * f;
+    l = fmaf(ml[s][1], f, l);
   }
-  const int t = row / p.G, qh = h * p.G + row % p.G;
-  const float gv = p.gate ? 1.f / (1.f + __expf(-p.gate[(size_t)t * p.QH + qh])) : 1.f;
-  const f32x4 o = l == 0.f ? f32x4{0, 0, 0, 0} : acc * (gv / l);
-  const size_t e = ((size_t)t * p.QH + qh) * D + 4 * c;
-  if (p.out16) *reinterpret_cast<half4*>(p.out16 + e) = half4{(_Float16)o[0], (_Float16)o[1], (_Float16)o[2], (_Float16)o[3]};
-  if (p.out32) *reinterpret_cast<f32x4*>(p.out32 + e) = o;
-  if (p.lse && c == 0) p.lse[(size_t)t * p.QH + qh] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+  b8_store<D>(p, h, row, c, acc, m, l, gate);
 }
 
 // ---------------------------------------------------------------- accounts of attention weight
@@ -487,21 +527,23 @@ void b8_attn_plan(B8Attn& p, int D, int splits, int cus) {
   p.rb = (blocks + p.RG - 1) / p.RG;
   p.g_div = div_magic((uint32_t)p.G);
   b8_sight(p, D);
-  int S = splits > 0 ? splits : std::max(1, (p.rb == 1 ? 2 : 1) * cus / (p.c.KVH * p.RG));
-  S = std::min(S, (p.npages + B8_WAVES - 1) / B8_WAVES);
-  S = std::max(1, std::min(S, 4096));
-  p.pps = (p.npages + S - 1) / S;
-  p.S = (p.npages + p.pps - 1) / p.pps;
+  const int waves = b8_waves(D, p.rb);
+  int S = splits > 0 ? splits : std::max(1, cus / (p.c.KVH * p.RG));
+  S = std::max(1, std::min(std::min(S, 4096), (p.npages + waves - 1) / waves));
+  p.S = S;
+  p.pps = p.npages / (S * waves);
+  p.more = p.npages % (S * waves);
 }
 
 size_t b8_attn_workspace(const B8Attn& p, int D) {
+  if (p.S == 1) return 0;
   const size_t rows = (size_t)p.c.KVH * p.R * p.S;
   return rows * D * sizeof(float) + rows * sizeof(f32x2);
 }
 
 template <int D, int RB, bool FP8>
 static void attn_b8_rows(const B8Attn& p, hipStream_t s) {
-  hipLaunchKernelGGL((attn_b8_kernel<D, RB, FP8>), dim3(p.S, p.c.KVH, p.RG), dim3(64 * B8_WAVES), 0, s, p);
+  hipLaunchKernelGGL((attn_b8_kernel<D, RB, FP8>), dim3(p.S, p.c.KVH, p.RG), dim3(64 * b8_waves(D, RB)), 0, s, p);
 }
 template <int D, bool FP8>
 static void attn_b8_by_rows(const B8Attn& p, hipStream_t s) {
@@ -517,6 +559,7 @@ int b8_attn_launch(const B8Attn& p, int D, bool fp8, hipStream_t s) {
   if (D == 64) fp8 ? attn_b8_by_rows<64, true>(p, s) : attn_b8_by_rows<64, false>(p, s);
   else fp8 ? attn_b8_by_rows<128, true>(p, s) : attn_b8_by_rows<128, false>(p, s);
   if (const int rc = (int)hipGetLastError()) return rc;
+  if (p.S == 1) return 0;
   const dim3 grid(p.R, p.c.KVH);
   if (D == 64) hipLaunchKernelGGL(attn_b8_merge_kernel<64>, grid, dim3(256), 0, s, p);
   else hipLaunchKernelGGL(attn_b8_merge_kernel<128>, grid, dim3(256), 0, s, p);

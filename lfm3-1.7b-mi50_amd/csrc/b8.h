@@ -131,7 +131,8 @@ struct B8Attn {
   int a, start, window, causal;
   int page0, npages;    // logical pages any row sees
   int full_lo, full_hi; // pages in [full_lo, full_hi) are seen whole by every row
-  int S, pps, RG;       // key splits, pages of a split, row groups
+  int S, RG;            // key splits, row groups
+  int pps, more;        // pages of a wave, and waves that take one more
   int rb;               // 16-row blocks of a row group
   float c2;             // log2(e) / sqrt(D)
   // the key accounts

@@ -2,6 +2,8 @@
 // range and alignment a kernel assumes is checked here, on the host, before anything is launched.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "dspark.h"
 #include "dspark_internal.h"
 #include "b8.h"
@@ -127,7 +129,7 @@ size_t dspark_verify_attention_b8_workspace(const dspark_b8_cache* c, const dspa
   if (!rows_ok(c, a)) return 0;
   B8Attn p = attn(c, a);
   b8_attn_plan(p, c->D, a->splits, device_cus());
-  return b8_attn_workspace(p, c->D);
+  return std::max(b8_attn_workspace(p, c->D), (size_t)256);  // (0 says that the arguments are refused)
 }
 
 int dspark_verify_attention_b8(const dspark_b8_cache* c, const dspark_b8_attn_args* a, dspark_stream_t stream) {
@@ -136,7 +138,7 @@ int dspark_verify_attention_b8(const dspark_b8_cache* c, const dspark_b8_attn_ar
   if ((a->out && !on(a->out, 16)) || (a->out_f32 && !on(a->out_f32, 16))) return DSPARK_EINVAL;
   B8Attn p = attn(c, a);
   b8_attn_plan(p, c->D, a->splits, device_cus());
-  if (!on(a->workspace, 16) || a->workspace_bytes < b8_attn_workspace(p, c->D)) return DSPARK_ENOSPACE;
+  if (!on(a->workspace, 16) || a->workspace_bytes < std::max(b8_attn_workspace(p, c->D), (size_t)256)) return DSPARK_ENOSPACE;
   p.part_acc = static_cast<float*>(a->workspace);
   p.part_ml = reinterpret_cast<f32x2*>(p.part_acc + (size_t)p.c.KVH * p.R * p.S * c->D);
   return b8_attn_launch(p, c->D, c->code == DSPARK_B8_E4M3, S(stream));
