@@ -124,9 +124,17 @@ __device__ __forceinline__ void b8_load_q(const B8Attn& p, int h, int row0, int 
       for (int e = 0; e < 2; ++e) q[rb][2 * u + e] = as_half8(ldg(reinterpret_cast<const u32x4*>(at + 64 * u + 8 * e)));
   }
 }
-// What a row sees: context keys from lo on, block keys under hi.
-__device__ __forceinline__ int row_lo(const B8Attn& p, int t) { return max(p.start, p.window > 0 ? p.a + t - p.window + 1 : 0); }
-__device__ __forceinline__ int row_hi(const B8Attn& p, int t) { return p.causal ? p.a + t + 1 : p.a + p.M; }
+// What token t sees: the keys lo, lo + 1, ... of the range's `n` (context keys from start and the window on, then the block's;
+// one comparison a key).
+struct B8Sight {
+  int lo;
+  uint32_t n;
+  __device__ __forceinline__ bool sees(int kp) const { return (uint32_t)(kp - lo) < n; }
+};
+__device__ __forceinline__ B8Sight b8_sight(const B8Attn& p, int t) {
+  const int lo = min(p.a, max(p.start, p.window > 0 ? p.a + t - p.window + 1 : 0));
+  return B8Sight{lo, (uint32_t)((p.causal ? p.a + t + 1 : p.a + p.M) - lo)};
+}
 
 template <int D, bool FP8>
 __device__ __forceinline__ void b8_k_operand(const u32x4 (&k)[D / 64], half8 (&kf)[D / 32]) {
@@ -158,13 +166,13 @@ __device__ __forceinline__ void b8_mask(const B8Attn& p, float ks, int pos, cons
   const int g = lane >> 4;
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
-    const int lo = row_lo(p, tok[rb]), hi = row_hi(p, tok[rb]);
+    const B8Sight sight = b8_sight(p, tok[rb]);
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int kp = pos + 16 * b + 4 * g + i;
-        s[rb][b][i] = (kp < p.a ? kp < lo : kp >= hi) ? -INFINITY : s[rb][b][i] * ks;
+        const float x = s[rb][b][i] * ks;
+        s[rb][b][i] = sight.sees(pos + 16 * b + 4 * g + i) ? x : -INFINITY;
       }
   }
 }
@@ -265,7 +273,7 @@ __global__ __launch_bounds__(64 * b8_waves(D, RB), b8_waves(D, RB) / 4) void att
   constexpr int ND = D / 16, NW = b8_waves(D, RB), ROWS = 16 * RB, NT = 64 * NW;
   __shared__ float s_o[NW][ROWS][D + 4];  // (rows 4 banks apart)
   __shared__ f32x2 s_ml[NW][ROWS];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   const int h = blockIdx.y, sp = blockIdx.x, row0 = blockIdx.z * ROWS;
   // wave gw of the head's S NW waves: pps pages, one more for the first `more` waves
   const int gw = sp * NW + wave;
@@ -293,9 +301,12 @@ __global__ __launch_bounds__(64 * b8_waves(D, RB), b8_waves(D, RB) / 4) void att
     const float ksl = ldg(p.c.ks + sat) * p.c2, vsl = ldg(p.c.vs + sat);
     // log2 vs, and 1 / vs as its very inverse. A block of zeros (scale 0) takes the smallest scale about: any will do for its
     // sum, and the smallest moves no reference.
-    const bool some = vsl > 0.f;
-    const float low = -wave_max(some ? -__builtin_amdgcn_logf(vsl) : -INFINITY);
-    const float lvl = some ? __builtin_amdgcn_logf(vsl) : low < INFINITY ? low : 0.f, ivl = fast_exp2(-lvl);
+    float lvl = __builtin_amdgcn_logf(vsl);
+    if (__ballot(!(vsl > 0.f))) {
+      const float low = -wave_max(vsl > 0.f ? -lvl : -INFINITY);
+      if (!(vsl > 0.f)) lvl = low < INFINITY ? low : 0.f;
+    }
+    const float ivl = fast_exp2(-lvl);
     // the next page's loads are in flight while a page is worked on (past the last one: that page again, from L2)
     auto step = [&](int i, const B8Tile<D>& now, B8Tile<D>& next) {
       b8_load_tile<D>(p, h, __builtin_amdgcn_readlane(pgl, min(i + 1, nb - 1)), lane, next);
@@ -304,7 +315,12 @@ __global__ __launch_bounds__(64 * b8_waves(D, RB), b8_waves(D, RB) / 4) void att
                             __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lvl), i)),
                             __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ivl), i)), b0 + i, lane, st);
     };
+    // Of the waves of a SIMD the oldest would run ahead and leave the others to finish alone: who is further on yields.
+    __builtin_amdgcn_s_setprio(3);
     for (int i = 0; i < nb; i += 2) {
+      if (4 * i >= nb) __builtin_amdgcn_s_setprio(2);
+      if (2 * i >= nb) __builtin_amdgcn_s_setprio(1);
+      if (4 * i >= 3 * nb) __builtin_amdgcn_s_setprio(0);
       step(i, t[0], t[1]);
       if (i + 1 < nb) step(i + 1, t[1], t[0]);
     }
@@ -425,7 +441,7 @@ __global__ __launch_bounds__(256) void attn_b8_merge_kernel(B8Attn p) {
 // A = K: eight row reductions a page, 39 -> 25 us at 128k keys and 64 rows a head).
 template <int D, int RB, bool FP8>
 __global__ __launch_bounds__(64 * MASS_WAVES) void mass_b8_kernel(B8Attn p) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   const int h = blockIdx.y;
   const int rows = p.rows ? min(max(ldc(p.rows), 0), p.M) : p.M;
   const int end = p.page0 + p.npages;
@@ -484,8 +500,8 @@ __global__ __launch_bounds__(64 * MASS_WAVES) void mass_b8_kernel(B8Attn p) {
                 const int kp = lp * PAGE + 16 * b + n;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                  const int t = div_by(min(row0 + 16 * rb + 4 * g + i, p.R - 1), p.g_div);
-                  if (kp < p.a ? kp < row_lo(p, t) : kp >= row_hi(p, t)) x[i] = -INFINITY;
+                  const B8Sight sight = b8_sight(p, div_by(min(row0 + 16 * rb + 4 * g + i, p.R - 1), p.g_div));
+                  x[i] = sight.sees(kp) ? x[i] : -INFINITY;
                 }
               }
 #pragma unroll
@@ -509,7 +525,7 @@ __global__ __launch_bounds__(64 * MASS_WAVES) void mass_b8_kernel(B8Attn p) {
 constexpr int B8_ROW_BLOCKS = 4;  // most 16-row blocks of a row group (2 at D = 128)
 
 // Which pages any row sees, and which every row sees whole.
-static void b8_sight(B8Attn& p, int D) {
+static void b8_range(B8Attn& p, int D) {
   const int lo = std::min(p.a, std::max(p.start, p.window > 0 ? p.a - p.window + 1 : 0));  // first key any row sees
   p.page0 = lo / PAGE;
   p.npages = (p.a + p.M - 1) / PAGE + 1 - p.page0;
@@ -526,7 +542,7 @@ void b8_attn_plan(B8Attn& p, int D, int splits, int cus) {
   p.RG = (blocks + most - 1) / most;
   p.rb = (blocks + p.RG - 1) / p.RG;
   p.g_div = div_magic((uint32_t)p.G);
-  b8_sight(p, D);
+  b8_range(p, D);
   const int waves = b8_waves(D, p.rb);
   int S = splits > 0 ? splits : std::max(1, cus / (p.c.KVH * p.RG));
   S = std::max(1, std::min(std::min(S, 4096), (p.npages + waves - 1) / waves));
@@ -582,7 +598,7 @@ int b8_mass_launch(const B8Attn& q, int D, bool fp8, int cus, hipStream_t s) {
   p.R = p.G * p.M;
   p.rb = std::min(B8_ROW_BLOCKS, (p.R + 15) / 16);
   p.g_div = div_magic((uint32_t)p.G);
-  b8_sight(p, D);
+  b8_range(p, D);
   p.seen_lo = p.page0;
   p.page0 = 0;  // every account is carried over, those of keys out of sight too
   p.npages = (p.a + p.M - 1) / PAGE + 1;

@@ -19,7 +19,7 @@ constexpr int WPB = 4;  // waves per workgroup; a wave owns one block
 template <int D, bool FP8>
 __global__ __launch_bounds__(64 * WPB) void kv_write_b8_kernel(B8Write p, int nwaves) {
   constexpr int LPR = D / 8, RPI = 64 / LPR, NI = PAGE / RPI;  // lanes per row, rows per instruction, instructions
-  const int w = blockIdx.x * WPB + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int w = blockIdx.x * WPB + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (w >= nwaves) return;
   const int KVH = p.c.KVH, h = w % KVH, kv = (w / KVH) & 1, lp = p.pos0 / PAGE + w / (2 * KVH);
   const int pg = b8_page(p.c, lp);
@@ -78,7 +78,7 @@ __global__ __launch_bounds__(64 * WPB) void kv_write_b8_kernel(B8Write p, int nw
 template <int D, bool FP8>
 __global__ __launch_bounds__(64 * WPB) void kv_read_b8_kernel(B8Read p, int nwaves) {
   constexpr int LPR = D / 4, RPI = 64 / LPR, NI = PAGE / RPI;
-  const int w = blockIdx.x * WPB + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int w = blockIdx.x * WPB + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (w >= nwaves) return;
   const int KVH = p.c.KVH, h = w % KVH, kv = (w / KVH) & 1, lp = p.pos0 / PAGE + w / (2 * KVH);
   const int pg = b8_page(p.c, lp);
@@ -194,7 +194,7 @@ __global__ __launch_bounds__(SEL_T) void evict_select_kernel(B8Evict p) {
 template <int D, bool FP8>
 __global__ __launch_bounds__(64 * WPB) void evict_move_kernel(B8Evict p, int nwaves) {
   constexpr int LPR = D / 16, RPI = 64 / LPR, NI = PAGE / RPI;
-  const int w = blockIdx.x * WPB + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int w = blockIdx.x * WPB + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (w >= nwaves) return;
   const int KVH = p.src.KVH, h = w % KVH, kv = (w / KVH) & 1, lp = w / (2 * KVH);
   const int slot0 = lp * PAGE, live = min(PAGE, p.keep - slot0);
