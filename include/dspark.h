@@ -223,7 +223,7 @@ int dspark_attention_mass_b8(const dspark_b8_cache* cache, const dspark_b8_attn_
  * from keep). A dst block's scale is the largest of its rows' scales; rows from blocks of a smaller one are re-coded to it
  * (rounded once more). The slots behind keep in the last page are cleared. mass_out[h][j] = mass[h][kept[h][j]]. dst has
  * src's KVH, D and code; its pools, kept and mass_out must share no byte with what is read (DSPARK_EINVAL). sinks + recent
- * <= keep <= length. keep = 0 does nothing. */
+ * <= keep <= length <= 2^30. keep = 0 does nothing. The workspace (a size of 0: none is needed) needs no clearing. */
 int dspark_kv_evict_b8(const dspark_b8_cache* src, const dspark_b8_cache* dst, int32_t length, int32_t keep, int32_t sinks,
                        int32_t recent, const float* mass, int64_t mass_stride, int32_t* kept, float* mass_out,
                        int64_t mass_out_stride, void* workspace, size_t workspace_bytes, dspark_stream_t stream);

@@ -45,14 +45,14 @@ __device__ __forceinline__ float b8_inv(float scale) { return scale > 0.f ? __fd
 // The int8 code of x at scale s: x / s rounded to nearest, ties to even, decided exactly. t = rint(x inv) is off by at
 // most one next to a border; the sign of x - (t +- 1/2) s, from one fma (t +- 1/2 is exact, and rounding keeps a sign
 // and a zero), says on which side x lies. NaN is coded 0, what lies past the codes +-127.
-__device__ __forceinline__ int b8_code_i8(float x, float s, float inv) {
+__device__ __forceinline__ uint32_t b8_code_i8(float x, float s, float inv) {
   x = x != x ? 0.f : fminf(fmaxf(x, -127.f * s), 127.f * s);
   float t = rintf(x * inv);
   const float up = fmaf(-(t + 0.5f), s, x), dn = fmaf(-(t - 0.5f), s, x);
   const bool odd = ((int)t & 1) != 0;
   if (up > 0.f || (up == 0.f && odd && s > 0.f)) t += 1.f;
   else if (dn < 0.f || (dn == 0.f && odd && s > 0.f)) t -= 1.f;
-  return (int)t;
+  return (uint32_t)(int)t;
 }
 
 // Four values as four codes (one word, the first in the low byte). x inv is exact for e4m3 (inv a power of two).
@@ -66,8 +66,24 @@ __device__ __forceinline__ uint32_t b8_code4(float x0, float x1, float x2, float
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(y(x0), y(x1), 0, false);
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y(x2), y(x3), w, true);
   } else {
-    return (uint32_t)(b8_code_i8(x0, s, inv) & 255) | (uint32_t)(b8_code_i8(x1, s, inv) & 255) << 8 |
-           (uint32_t)(b8_code_i8(x2, s, inv) & 255) << 16 | (uint32_t)(b8_code_i8(x3, s, inv) & 255) << 24;
+    // y = x inv + 1.5 2^23 holds the rounded code in its low byte. x inv is off by 2^-16 at most (codes up to 127, two
+    // roundings), so only values within 2^-14 of a border, and those that are no numbers, are decided anew.
+    constexpr float MAGIC = 12582912.f;
+    const float x[4] = {x0, x1, x2, x3};
+    uint32_t y[4];
+    bool near = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float r = fmaf(x[i], inv, MAGIC);
+      y[i] = __float_as_uint(r);
+      near |= !(fabsf(fmaf(x[i], inv, MAGIC - r)) < 0.5f - 0x1p-14f);
+    }
+    if (__builtin_expect(__ballot(near) != 0, 0)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = b8_code_i8(x[i], s, inv);
+    }
+    const uint32_t lo = __builtin_amdgcn_perm(y[1], y[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(y[3], y[2], 0x04000c0cu);
+    return lo | hi;
   }
 }
 
@@ -114,7 +130,8 @@ struct B8Evict {
 };
 int b8_write_launch(const B8Write& p, int D, bool fp8, hipStream_t s);
 int b8_read_launch(const B8Read& p, int D, bool fp8, hipStream_t s);
-int b8_evict_launch(const B8Evict& p, int D, bool fp8, hipStream_t s);
+int b8_evict_launch(const B8Evict& p, int D, bool fp8, void* ws, hipStream_t s);
+size_t b8_evict_workspace(int KVH, int length);
 
 struct B8Attn {
   B8Pool c;

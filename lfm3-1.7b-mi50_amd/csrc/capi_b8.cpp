@@ -160,19 +160,16 @@ int dspark_attention_mass_b8(const dspark_b8_cache* c, const dspark_b8_attn_args
 }
 
 size_t dspark_kv_evict_b8_workspace(int32_t KVH, int32_t length) {
-  (void)KVH;
-  (void)length;
-  return 0;
+  if (KVH < 1 || KVH > HEADS_MAX || length < 0) return 0;
+  return b8_evict_workspace(KVH, length);
 }
 
 int dspark_kv_evict_b8(const dspark_b8_cache* src, const dspark_b8_cache* dst, int32_t length, int32_t keep, int32_t sinks,
                        int32_t recent, const float* mass, int64_t mass_stride, int32_t* kept, float* mass_out,
                        int64_t mass_out_stride, void* workspace, size_t workspace_bytes, dspark_stream_t stream) {
-  (void)workspace;
-  (void)workspace_bytes;
   if (!cache_ok(src) || !cache_ok(dst) || src->KVH != dst->KVH || src->D != dst->D || src->code != dst->code) return DSPARK_EINVAL;
   if (length < 0 || keep < 0 || keep > length || sinks < 0 || recent < 0 || (int64_t)sinks + recent > keep) return DSPARK_EINVAL;
-  if (!fits(src, length) || !fits(dst, keep) || !waves_fit(dst, pages_of(keep))) return DSPARK_EINVAL;
+  if (length > 1 << 30 || !fits(src, length) || !fits(dst, keep) || !waves_fit(dst, pages_of(keep))) return DSPARK_EINVAL;
   if (keep == 0) return 0;
   if (!on(mass, 4) || !on(kept, 4) || !on(mass_out, 4) || mass_stride < length || mass_out_stride < keep) return DSPARK_EINVAL;
   // the rows move between pools that share nothing: a destination page may be written while other rows are still read
@@ -181,9 +178,11 @@ int dspark_kv_evict_b8(const dspark_b8_cache* src, const dspark_b8_cache* dst, i
   const struct { const void* p; size_t n; } reads[6] = {
       {src->k, from[1]}, {src->v, from[1]}, {src->k_scale, from[0] * 4}, {src->v_scale, from[0] * 4},
       {mass, ((size_t)(src->KVH - 1) * mass_stride + length) * 4}, {src->block_table, src->block_table ? (size_t)pages_of(length) * 4 : 0}};
-  const struct { const void* p; size_t n; } writes[6] = {
+  const size_t need = b8_evict_workspace(src->KVH, length);
+  if (need && (!on(workspace, 16) || workspace_bytes < need)) return DSPARK_ENOSPACE;
+  const struct { const void* p; size_t n; } writes[7] = {
       {dst->k, to[1]}, {dst->v, to[1]}, {dst->k_scale, to[0] * 4}, {dst->v_scale, to[0] * 4},
-      {mass_out, ((size_t)(src->KVH - 1) * mass_out_stride + keep) * 4}, {kept, (size_t)src->KVH * keep * 4}};
+      {mass_out, ((size_t)(src->KVH - 1) * mass_out_stride + keep) * 4}, {kept, (size_t)src->KVH * keep * 4}, {workspace, need}};
   for (const auto& r : reads)
     for (const auto& w : writes)
       if (r.n && w.n && overlap(r.p, r.n, w.p, w.n)) return DSPARK_EINVAL;
@@ -199,7 +198,7 @@ int dspark_kv_evict_b8(const dspark_b8_cache* src, const dspark_b8_cache* dst, i
   p.kept = kept;
   p.mass_out = mass_out;
   p.mass_out_stride = mass_out_stride;
-  return b8_evict_launch(p, src->D, src->code == DSPARK_B8_E4M3, S(stream));
+  return b8_evict_launch(p, src->D, src->code == DSPARK_B8_E4M3, workspace, S(stream));
 }
 
 }  // extern "C"

@@ -102,91 +102,254 @@ __global__ __launch_bounds__(64 * WPB) void kv_read_b8_kernel(B8Read p, int nwav
 // Order of the accounts: as the values are, NaN below all of them, -0 as 0.
 __device__ __forceinline__ uint32_t mass_key(float v) { return v != v ? 0u : argmax_ord(v + 0.f); }
 
-constexpr int SEL_T = 1024, SEL_W = SEL_T / 64;
+constexpr int SEL_T = 1024, SEL_W = SEL_T / 64, SEL_BINS = 2048;
+// Radix selection over the keys' bits 31-21, 20-10 and 9-0.
+constexpr int sel_shift(int pass) { return pass == 0 ? 21 : pass == 1 ? 10 : 0; }
+constexpr int sel_bins(int pass) { return pass == 2 ? 1024 : 2048; }
 
-// One workgroup per KV head finds the keep - sinks - recent largest accounts of the middle positions and lists what is
-// kept in position order. The threshold (the least kept key) by radix selection over 11, 11 and 10 bits with LDS
-// histograms; of the keys equal to it the first positions are kept. Wave w owns a contiguous range of positions, 64 in
-// a row at a time, so that the places come from ballots and one scan over the waves.
-__global__ __launch_bounds__(SEL_T) void evict_select_kernel(B8Evict p) {
-  __shared__ uint32_t hist[2048];
-  __shared__ uint32_t wsum[SEL_W];
-  __shared__ uint32_t found[2];  // digit, keys above it
-  __shared__ uint32_t wgt[SEL_W], weq[SEL_W];
-  const int h = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const float* mass = p.mass + (size_t)h * p.mass_stride + p.sinks;
-  int32_t* kept = p.kept + (size_t)h * p.keep;
-  const int N = p.T - p.sinks - p.recent, k = p.keep - p.sinks - p.recent;
-  for (int i = tid; i < p.sinks; i += SEL_T) kept[i] = i;
-  for (int i = tid; i < p.recent; i += SEL_T) kept[p.keep - p.recent + i] = p.T - p.recent + i;
-  if (k <= 0) return;
-  uint32_t prefix = 0, mask = 0;  // the threshold's bits found so far
-  uint32_t need = (uint32_t)k;    // how many of the keys with that prefix are kept
-#pragma unroll 1
-  for (int pass = 0; pass < 3; ++pass) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
-    for (int i = tid; i < bins; i += SEL_T) hist[i] = 0;
-    __syncthreads();
-    for (int i = tid; i < N; i += SEL_T) {
-      const uint32_t u = mass_key(ldg(mass + i));
-      if ((u & mask) == prefix) atomicAdd(&hist[(u >> shift) & (bins - 1)], 1u);
-    }
-    __syncthreads();
-    // thread t owns bins 2 t, 2 t + 1 counted from the top; an inclusive scan over the threads
-    const int b1 = bins - 1 - 2 * tid, b0 = b1 - 1;
-    const uint32_t n1 = b1 >= 0 ? hist[b1] : 0u, n0 = b0 >= 0 ? hist[b0] : 0u;
-    uint32_t sum = n1 + n0;
+// Where the need-th largest of the counted keys lies: its bin and how many lie in higher bins. hist [bins] in LDS (complete
+// and visible), thread t owning bins 2 t, 2 t + 1 counted from the top; 1 <= need <= the number counted.
+struct SelLds {
+  uint32_t hist[SEL_BINS];
+  uint32_t wsum[SEL_W];
+  uint32_t found[2];
+};
+__device__ __forceinline__ void sel_find(SelLds& s, int bins, uint32_t need, uint32_t& bin, uint32_t& above) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int b1 = bins - 1 - 2 * tid, b0 = b1 - 1;
+  const uint32_t n1 = b1 >= 0 ? s.hist[b1] : 0u, n0 = b0 >= 0 ? s.hist[b0] : 0u;
+  uint32_t sum = n1 + n0;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint32_t o = __shfl_up(sum, d);
-      if (lane >= d) sum += o;
-    }
-    if (lane == 63) wsum[wave] = sum;
-    __syncthreads();
-    uint32_t before = sum - n1 - n0;
-    for (int w = 0; w < wave; ++w) before += wsum[w];
-    if (before < need && need <= before + n1) {
-      found[0] = (uint32_t)b1;
-      found[1] = before;
-    } else if (before + n1 < need && need <= before + n1 + n0) {
-      found[0] = (uint32_t)b0;
-      found[1] = before + n1;
-    }
-    __syncthreads();
-    prefix |= found[0] << shift;
-    mask |= (uint32_t)(bins - 1) << shift;
-    need -= found[1];
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t o = __shfl_up(sum, d);
+    if (lane >= d) sum += o;
   }
-  // every key above the threshold, and the first `need` of those equal to it
-  const int per = ((N + SEL_W - 1) / SEL_W + 63) / 64 * 64;
-  const int lo = min(N, wave * per), hi = min(N, lo + per);
-  uint32_t gt = 0, eq = 0;
-  for (int i = lo + lane; i - lane < hi; i += 64) {
-    const uint32_t u = i < hi ? mass_key(ldg(mass + i)) : 0u;
-    gt += __popcll(__ballot(i < hi && u > prefix));
-    eq += __popcll(__ballot(i < hi && u == prefix));
-  }
-  if (lane == 0) {
-    wgt[wave] = gt;
-    weq[wave] = eq;
+  if (lane == 63) s.wsum[wave] = sum;
+  __syncthreads();
+  uint32_t before = sum - n1 - n0;
+  for (int w = 0; w < wave; ++w) before += s.wsum[w];
+  if (before < need && need <= before + n1) {
+    s.found[0] = (uint32_t)b1;
+    s.found[1] = before;
+  } else if (before + n1 < need && need <= before + n1 + n0) {
+    s.found[0] = (uint32_t)b0;
+    s.found[1] = before + n1;
   }
   __syncthreads();
-  uint32_t at = 0, used = 0;
-  for (int w = 0; w < wave; ++w) {
-    const uint32_t e = min(weq[w], need - used);
-    at += wgt[w] + e;
-    used += e;
-  }
+  bin = s.found[0];
+  above = s.found[1];
+}
+
+__device__ __forceinline__ void sel_edges(const B8Evict& p, int32_t* kept, int first, int step) {
+  for (int i = first; i < p.sinks; i += step) kept[i] = i;
+  for (int i = first; i < p.recent; i += step) kept[p.keep - p.recent + i] = p.T - p.recent + i;
+}
+
+// The kept ones of a wave's 64 NPL keys (u[j] of position i0 + 64 j + lane): those above the threshold and the first `need`
+// equal ones of the head, `used` of which lie before; stored from place `at` on.
+template <int NPL>
+__device__ __forceinline__ void sel_emit(const uint32_t (&u)[NPL], int i0, int N, uint32_t thr, uint32_t need, uint32_t used,
+                                         uint32_t at, int sinks, int32_t* kept) {
+  const int lane = threadIdx.x & 63;
   const uint64_t below = (1ull << lane) - 1;
-  for (int i = lo + lane; i - lane < hi; i += 64) {
-    const uint32_t u = i < hi ? mass_key(ldg(mass + i)) : 0u;
-    const uint64_t be = __ballot(i < hi && u == prefix);
-    const bool take = i < hi && (u > prefix || (u == prefix && used + __popcll(be & below) < need));
+#pragma unroll
+  for (int j = 0; j < NPL; ++j) {
+    const int i = i0 + 64 * j + lane;
+    const uint64_t be = __ballot(i < N && u[j] == thr);
+    const bool take = i < N && (u[j] > thr || (u[j] == thr && used + __popcll(be & below) < need));
     const uint64_t bt = __ballot(take);
-    if (take) kept[p.sinks + at + __popcll(bt & below)] = p.sinks + i;
+    if (take) kept[at + __popcll(bt & below)] = sinks + i;
     at += __popcll(bt);
     used = min(need, used + (uint32_t)__popcll(be));
   }
+}
+template <int NPL>
+__device__ __forceinline__ void sel_count(const uint32_t (&u)[NPL], int i0, int N, uint32_t thr, uint32_t& gt, uint32_t& eq) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int j = 0; j < NPL; ++j) {
+    const bool in = i0 + 64 * j + lane < N;
+    gt += __popcll(__ballot(in && u[j] > thr));
+    eq += __popcll(__ballot(in && u[j] == thr));
+  }
+}
+// Places of a wave's first kept key from the waves' counts (wc: above and equal, complete and visible), behind `at0` kept ones
+// and `eq0` equal ones.
+__device__ __forceinline__ void sel_places(const uint32_t (*wc)[2], int wave, uint32_t need, uint32_t eq0, uint32_t& at, uint32_t& used) {
+  used = min(need, eq0);
+  for (int w = 0; w < wave; ++w) {
+    const uint32_t e = min(wc[w][1], need - used);
+    at += wc[w][0] + e;
+    used += e;
+  }
+}
+
+// One workgroup per KV head finds the keep - sinks - recent largest accounts of up to 1024 NPL middle positions, held in
+// registers, and lists what is kept in position order.
+template <int NPL>
+__global__ __launch_bounds__(SEL_T) void evict_select_kernel(B8Evict p) {
+  __shared__ SelLds s;
+  __shared__ uint32_t wc[SEL_W][2];
+  const int h = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const float* mass = p.mass + (size_t)h * p.mass_stride + p.sinks;
+  int32_t* kept = p.kept + (size_t)h * p.keep;
+  const int N = p.T - p.sinks - p.recent, k = p.keep - p.sinks - p.recent;
+  const int i0 = wave * 64 * NPL;
+  float v[NPL];
+#pragma unroll
+  for (int j = 0; j < NPL; ++j) v[j] = N > 0 ? ldg(mass + min(i0 + 64 * j + lane, N - 1)) : 0.f;
+  sel_edges(p, kept, tid, SEL_T);
+  if (k <= 0) return;
+  uint32_t u[NPL];
+#pragma unroll
+  for (int j = 0; j < NPL; ++j) u[j] = mass_key(v[j]);
+  uint32_t thr = 0, mask = 0, need = (uint32_t)k;
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = sel_shift(pass), bins = sel_bins(pass);
+    for (int i = tid; i < bins; i += SEL_T) s.hist[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < NPL; ++j)
+      if (i0 + 64 * j + lane < N && (u[j] & mask) == thr) atomicAdd(&s.hist[(u[j] >> shift) & (bins - 1)], 1u);
+    __syncthreads();
+    uint32_t bin, above;
+    sel_find(s, bins, need, bin, above);
+    thr |= bin << shift;
+    mask |= (uint32_t)(bins - 1) << shift;
+    need -= above;
+  }
+  uint32_t gt = 0, eq = 0, at = p.sinks, used = 0;
+  sel_count<NPL>(u, i0, N, thr, gt, eq);
+  if (lane == 0) {
+    wc[wave][0] = gt;
+    wc[wave][1] = eq;
+  }
+  __syncthreads();
+  sel_places(wc, wave, need, 0, at, used);
+  sel_emit<NPL>(u, i0, N, thr, need, used, at, p.sinks, kept);
+}
+
+// More positions: `parts` workgroups a head, each a contiguous range of them (whole tiles of 8192), and a launch for each
+// digit. A workgroup stores its own histogram; the next launch's workgroups each add up all of the head's (from L2), find the
+// digit, and count the next one among their keys that match so far. The last launch knows from the parts' counts where each
+// part's first kept key goes. No atomics in memory, and no state from one call to the next.
+constexpr int SEL_NPL = 8, SEL_TILE = SEL_T * SEL_NPL, SEL_PARTS = 32;
+struct SelHead {  // a head's part of the workspace, a u32 each
+  uint32_t hist[3][SEL_PARTS][SEL_BINS];
+  uint32_t above[2][SEL_PARTS];  // a part's keys over the threshold by digit 0, by digit 1
+  uint32_t state[2][2];          // after digit 0 and 1: threshold so far, keys still needed at it
+};
+template <int PASS>
+__global__ __launch_bounds__(SEL_T) void evict_pass_kernel(B8Evict p, SelHead* ws, int parts, int per) {
+  __shared__ SelLds s;
+  __shared__ uint32_t wc[SEL_W][2];
+  __shared__ uint32_t red[2];
+  const int h = blockIdx.y, part = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  SelHead& w = ws[h];
+  const float* mass = p.mass + (size_t)h * p.mass_stride + p.sinks;
+  int32_t* kept = p.kept + (size_t)h * p.keep;
+  const int N = p.T - p.sinks - p.recent;
+  const int lo = part * per, hi = min(N, lo + per);
+  auto load = [&](int t0, uint32_t (&u)[SEL_NPL]) {
+    float v[SEL_NPL];
+#pragma unroll
+    for (int j = 0; j < SEL_NPL; ++j) v[j] = ldg(mass + min(t0 + wave * 64 * SEL_NPL + 64 * j + lane, N - 1));
+#pragma unroll
+    for (int j = 0; j < SEL_NPL; ++j) u[j] = mass_key(v[j]);
+  };
+  uint32_t u[SEL_NPL];
+  load(min(lo, N - 1), u);  // the first tile's keys, in flight while the digit is found
+  uint32_t thr = 0, mask = 0, need = (uint32_t)(p.keep - p.sinks - p.recent);
+  if constexpr (PASS > 0) {  // the digit before
+    constexpr int prev = PASS - 1;
+    if (PASS > 1) {
+      thr = w.state[prev - 1][0];
+      need = w.state[prev - 1][1];
+      mask = PASS == 2 ? (uint32_t)(sel_bins(0) - 1) << sel_shift(0) : ~(uint32_t)(sel_bins(2) - 1);
+    }
+    for (int i = tid; i < sel_bins(prev); i += SEL_T) {
+      uint32_t n = 0;
+#pragma unroll 8
+      for (int q = 0; q < parts; ++q) n += ldg(&w.hist[prev][q][i]);
+      s.hist[i] = n;
+    }
+    __syncthreads();
+    uint32_t bin, above;
+    sel_find(s, sel_bins(prev), need, bin, above);
+    thr |= bin << sel_shift(prev);
+    need -= above;
+    if constexpr (PASS < 3) {
+      // keys that the digit puts over the threshold
+      mask |= (uint32_t)(sel_bins(prev) - 1) << sel_shift(prev);
+      if (tid == 0) red[0] = 0;
+      __syncthreads();
+      uint32_t gt = 0;
+      for (int i = tid; i < sel_bins(prev); i += SEL_T)
+        if (i > (int)bin) gt += ldg(&w.hist[prev][part][i]);
+      if (gt) atomicAdd(&red[0], gt);
+      if (part == 0 && tid == 0) {
+        w.state[prev][0] = thr;
+        w.state[prev][1] = need;
+      }
+      __syncthreads();
+      if (tid == 0) w.above[prev][part] = red[0];
+    }
+  }
+  if constexpr (PASS < 3) {
+    constexpr int bins = sel_bins(PASS), shift = sel_shift(PASS);
+    for (int i = tid; i < bins; i += SEL_T) s.hist[i] = 0;
+    __syncthreads();
+    for (int t0 = lo; t0 < hi; t0 += SEL_TILE) {
+      if (t0 > lo) load(t0, u);
+#pragma unroll
+      for (int j = 0; j < SEL_NPL; ++j)
+        if (t0 + wave * 64 * SEL_NPL + 64 * j + lane < hi && (u[j] & mask) == thr) atomicAdd(&s.hist[(u[j] >> shift) & (bins - 1)], 1u);
+    }
+    __syncthreads();
+    for (int i = tid; i < bins; i += SEL_T) w.hist[PASS][part][i] = s.hist[i];
+  } else {
+    // kept and equal keys in the parts before
+    constexpr int bins = sel_bins(2);
+    const uint32_t bin = thr & (bins - 1);
+    if (tid < 2) red[tid] = 0;
+    __syncthreads();
+    uint32_t gt = 0, eq = 0;
+    for (int i = tid; i < part * bins; i += SEL_T) {
+      const uint32_t n = (uint32_t)(i % bins) >= bin ? ldg(&w.hist[2][i / bins][i % bins]) : 0u;
+      if ((uint32_t)(i % bins) == bin) eq += n;
+      else gt += n;
+    }
+    if (tid < part) gt += ldg(&w.above[0][tid]) + ldg(&w.above[1][tid]);
+    if (gt) atomicAdd(&red[0], gt);
+    if (eq) atomicAdd(&red[1], eq);
+    if (part == 0) sel_edges(p, kept, tid, SEL_T);
+    __syncthreads();
+    uint32_t eq0 = red[1], at0 = p.sinks + red[0] + min(need, red[1]);
+    for (int t0 = lo; t0 < hi; t0 += SEL_TILE) {
+      if (t0 > lo) load(t0, u);
+      const int i0 = t0 + wave * 64 * SEL_NPL;
+      uint32_t g = 0, e = 0, at = at0, used;
+      sel_count<SEL_NPL>(u, i0, hi, thr, g, e);
+      if (lane == 0) {
+        wc[wave][0] = g;
+        wc[wave][1] = e;
+      }
+      __syncthreads();
+      sel_places(wc, wave, need, eq0, at, used);
+      sel_emit<SEL_NPL>(u, i0, hi, thr, need, used, at, p.sinks, kept);
+      for (int x = 0; x < SEL_W; ++x) {  // on to the next tile
+        const uint32_t more = min(wc[x][1], need - min(need, eq0));
+        at0 += wc[x][0] + more;
+        eq0 += wc[x][1];
+      }
+      __syncthreads();
+    }
+  }
+}
+
+__global__ __launch_bounds__(SEL_T) void evict_edges_kernel(B8Evict p) {
+  sel_edges(p, p.kept + (size_t)blockIdx.x * p.keep, threadIdx.x, SEL_T);
 }
 
 // One wave per (destination page, K or V, head): 32 kept rows gathered 16 bytes a lane into one block. Its scale is the
@@ -257,8 +420,31 @@ int b8_read_launch(const B8Read& p, int D, bool fp8, hipStream_t s) {
                        s, p, nw);
   });
 }
-int b8_evict_launch(const B8Evict& p, int D, bool fp8, hipStream_t s) {
-  hipLaunchKernelGGL(evict_select_kernel, dim3(p.src.KVH), dim3(SEL_T), 0, s, p);
+// Up to 16384 middle positions in one launch, from 16 keys a lane; more by parts (8449 positions 18 -> 7 us against passes
+// over memory; 130044 positions 160 -> 20).
+constexpr int SEL_ONE = 16 * SEL_T;
+size_t b8_evict_workspace(int KVH, int length) { return length > SEL_ONE ? (size_t)KVH * sizeof(SelHead) : 0; }
+
+int b8_evict_launch(const B8Evict& p, int D, bool fp8, void* ws, hipStream_t s) {
+  const int N = p.T - p.sinks - p.recent, KVH = p.src.KVH;
+  if (N <= 4 * SEL_T) {
+    hipLaunchKernelGGL(evict_select_kernel<4>, dim3(KVH), dim3(SEL_T), 0, s, p);
+  } else if (N <= SEL_ONE) {
+    hipLaunchKernelGGL(evict_select_kernel<16>, dim3(KVH), dim3(SEL_T), 0, s, p);
+  } else {
+    const int tiles = (N + SEL_TILE - 1) / SEL_TILE, each = (tiles + SEL_PARTS - 1) / SEL_PARTS;
+    const int parts = (tiles + each - 1) / each, per = each * SEL_TILE;
+    SelHead* w = static_cast<SelHead*>(ws);
+    const dim3 grid(parts, KVH), block(SEL_T);
+    if (p.keep > p.sinks + p.recent) {
+      hipLaunchKernelGGL(evict_pass_kernel<0>, grid, block, 0, s, p, w, parts, per);
+      hipLaunchKernelGGL(evict_pass_kernel<1>, grid, block, 0, s, p, w, parts, per);
+      hipLaunchKernelGGL(evict_pass_kernel<2>, grid, block, 0, s, p, w, parts, per);
+      hipLaunchKernelGGL(evict_pass_kernel<3>, grid, block, 0, s, p, w, parts, per);
+    } else {  // nothing of the middle is kept
+      hipLaunchKernelGGL(evict_edges_kernel, dim3(KVH), block, 0, s, p);
+    }
+  }
   if (const int rc = (int)hipGetLastError()) return rc;
   const int nw = (p.keep + PAGE - 1) / PAGE * 2 * p.src.KVH;
   return by_kind(D, fp8, [&](auto d, auto f) {
