@@ -107,33 +107,40 @@ constexpr int SEL_T = 1024, SEL_W = SEL_T / 64, SEL_BINS = 2048;
 constexpr int sel_shift(int pass) { return pass == 0 ? 21 : pass == 1 ? 10 : 0; }
 constexpr int sel_bins(int pass) { return pass == 2 ? 1024 : 2048; }
 
-// Where the need-th largest of the counted keys lies: its bin and how many lie in higher bins. hist [bins] in LDS (complete
-// and visible), thread t owning bins 2 t, 2 t + 1 counted from the top; 1 <= need <= the number counted.
+// Inclusive sum over the lanes of a row of 16 up to this one, and over the lanes of the wave up to this one.
+template <int N>
+__device__ __forceinline__ uint32_t row_shr_add(uint32_t v) {
+  return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x110 + N, 0xf, 0xf, true);
+}
+__device__ __forceinline__ uint32_t row_scan(uint32_t v) { return row_shr_add<8>(row_shr_add<4>(row_shr_add<2>(row_shr_add<1>(v)))); }
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  v = row_scan(v);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);  // row 0's last lane to row 1, 2's to 3
+  return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);  // lane 31 to rows 2 and 3
+}
+__device__ __forceinline__ uint32_t wave_total(uint32_t v) {
+  return wave_butterfly(v, [](uint32_t a, uint32_t b) { return a + b; });
+}
+
+// Where the need-th largest of the counted keys lies: its bin and how many lie in higher bins. Thread t holds the counts n1, n0
+// of bins b1 = bins - 1 - 2 t and b1 - 1 (0 past the bins); 1 <= need <= the number counted.
 struct SelLds {
-  uint32_t hist[SEL_BINS];
   uint32_t wsum[SEL_W];
   uint32_t found[2];
 };
-__device__ __forceinline__ void sel_find(SelLds& s, int bins, uint32_t need, uint32_t& bin, uint32_t& above) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int b1 = bins - 1 - 2 * tid, b0 = b1 - 1;
-  const uint32_t n1 = b1 >= 0 ? s.hist[b1] : 0u, n0 = b0 >= 0 ? s.hist[b0] : 0u;
-  uint32_t sum = n1 + n0;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t o = __shfl_up(sum, d);
-    if (lane >= d) sum += o;
-  }
+__device__ __forceinline__ void sel_find(SelLds& s, int bins, uint32_t n1, uint32_t n0, uint32_t need, uint32_t& bin,
+                                         uint32_t& above) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t sum = wave_scan(n1 + n0);
   if (lane == 63) s.wsum[wave] = sum;
   __syncthreads();
-  uint32_t before = sum - n1 - n0;
-  for (int w = 0; w < wave; ++w) before += s.wsum[w];
-  if (before < need && need <= before + n1) {
-    s.found[0] = (uint32_t)b1;
-    s.found[1] = before;
-  } else if (before + n1 < need && need <= before + n1 + n0) {
-    s.found[0] = (uint32_t)b0;
-    s.found[1] = before + n1;
+  const uint32_t upto = row_scan(s.wsum[lane % SEL_W]);
+  const uint32_t before = sum - n1 - n0 + (wave ? (uint32_t)__builtin_amdgcn_readlane((int)upto, max(wave - 1, 0)) : 0u);
+  const int b1 = bins - 1 - 2 * tid;
+  if (before < need && need <= before + n1 + n0) {
+    const bool low = need > before + n1;
+    s.found[0] = (uint32_t)(b1 - low);
+    s.found[1] = before + (low ? n1 : 0u);
   }
   __syncthreads();
   bin = s.found[0];
@@ -189,6 +196,7 @@ __device__ __forceinline__ void sel_places(const uint32_t (*wc)[2], int wave, ui
 template <int NPL>
 __global__ __launch_bounds__(SEL_T) void evict_select_kernel(B8Evict p) {
   __shared__ SelLds s;
+  __shared__ __align__(16) uint32_t hist[SEL_BINS];
   __shared__ uint32_t wc[SEL_W][2];
   const int h = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const float* mass = p.mass + (size_t)h * p.mass_stride + p.sinks;
@@ -207,14 +215,15 @@ __global__ __launch_bounds__(SEL_T) void evict_select_kernel(B8Evict p) {
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = sel_shift(pass), bins = sel_bins(pass);
-    for (int i = tid; i < bins; i += SEL_T) s.hist[i] = 0;
+    for (int i = tid; i < bins; i += SEL_T) hist[i] = 0;
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < NPL; ++j)
-      if (i0 + 64 * j + lane < N && (u[j] & mask) == thr) atomicAdd(&s.hist[(u[j] >> shift) & (bins - 1)], 1u);
+      if (i0 + 64 * j + lane < N && (u[j] & mask) == thr) atomicAdd(&hist[(u[j] >> shift) & (bins - 1)], 1u);
     __syncthreads();
+    const u32x2 n = 2 * tid < bins ? *reinterpret_cast<const u32x2*>(&hist[bins - 2 - 2 * tid]) : u32x2{0, 0};
     uint32_t bin, above;
-    sel_find(s, bins, need, bin, above);
+    sel_find(s, bins, n[1], n[0], need, bin, above);
     thr |= bin << shift;
     mask |= (uint32_t)(bins - 1) << shift;
     need -= above;
@@ -243,6 +252,7 @@ struct SelHead {  // a head's part of the workspace, a u32 each
 template <int PASS>
 __global__ __launch_bounds__(SEL_T) void evict_pass_kernel(B8Evict p, SelHead* ws, int parts, int per) {
   __shared__ SelLds s;
+  __shared__ __align__(16) uint32_t hist[SEL_BINS];
   __shared__ uint32_t wc[SEL_W][2];
   __shared__ uint32_t red[2];
   const int h = blockIdx.y, part = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -261,71 +271,69 @@ __global__ __launch_bounds__(SEL_T) void evict_pass_kernel(B8Evict p, SelHead* w
   uint32_t u[SEL_NPL];
   load(min(lo, N - 1), u);  // the first tile's keys, in flight while the digit is found
   uint32_t thr = 0, mask = 0, need = (uint32_t)(p.keep - p.sinks - p.recent);
-  if constexpr (PASS > 0) {  // the digit before
-    constexpr int prev = PASS - 1;
+  uint32_t gt = 0, eq = 0;  // PASS 3: kept and equal keys in the parts before
+  if constexpr (PASS > 0) {  // the digit of the launch before
+    constexpr int prev = PASS - 1, bins = sel_bins(prev);
     if (PASS > 1) {
-      thr = w.state[prev - 1][0];
-      need = w.state[prev - 1][1];
-      mask = PASS == 2 ? (uint32_t)(sel_bins(0) - 1) << sel_shift(0) : ~(uint32_t)(sel_bins(2) - 1);
+      thr = ldg(&w.state[PASS - 2][0]);
+      need = ldg(&w.state[PASS - 2][1]);
+      mask = (uint32_t)(sel_bins(0) - 1) << sel_shift(0);
     }
-    for (int i = tid; i < sel_bins(prev); i += SEL_T) {
-      uint32_t n = 0;
-#pragma unroll 8
-      for (int q = 0; q < parts; ++q) n += ldg(&w.hist[prev][q][i]);
-      s.hist[i] = n;
+    if (tid < 2) red[tid] = 0;
+    // this thread's two bins in every part: all of them, this part's own, and those of the parts before it
+    u32x2 all = {0, 0}, mine = {0, 0}, ahead = {0, 0};
+    if (2 * tid < bins) {
+      const u32x2* at = reinterpret_cast<const u32x2*>(&w.hist[prev][0][bins - 2 - 2 * tid]);
+#pragma unroll 16
+      for (int q = 0; q < parts; ++q) {
+        const u32x2 n = ldg(at + (size_t)q * (SEL_BINS / 2));
+        all += n;
+        if (q == part) mine = n;
+        if (q < part) ahead += n;
+      }
     }
-    __syncthreads();
     uint32_t bin, above;
-    sel_find(s, sel_bins(prev), need, bin, above);
+    sel_find(s, bins, all[1], all[0], need, bin, above);
     thr |= bin << sel_shift(prev);
     need -= above;
-    if constexpr (PASS < 3) {
-      // keys that the digit puts over the threshold
-      mask |= (uint32_t)(sel_bins(prev) - 1) << sel_shift(prev);
-      if (tid == 0) red[0] = 0;
-      __syncthreads();
-      uint32_t gt = 0;
-      for (int i = tid; i < sel_bins(prev); i += SEL_T)
-        if (i > (int)bin) gt += ldg(&w.hist[prev][part][i]);
-      if (gt) atomicAdd(&red[0], gt);
-      if (part == 0 && tid == 0) {
-        w.state[prev][0] = thr;
-        w.state[prev][1] = need;
+    mask |= (uint32_t)(bins - 1) << sel_shift(prev);
+    const uint32_t b1 = (uint32_t)(bins - 1 - 2 * tid);
+    if (2 * tid < bins) {
+      const u32x2 n = PASS < 3 ? mine : ahead;
+      gt = (b1 > bin ? n[1] : 0u) + (b1 - 1 > bin ? n[0] : 0u);
+      eq = (b1 == bin ? n[1] : 0u) + (b1 - 1 == bin ? n[0] : 0u);
+    }
+    if (PASS == 3 && tid < part) gt += ldg(&w.above[0][tid]) + ldg(&w.above[1][tid]);
+    gt = wave_total(gt);
+    eq = wave_total(eq);
+    if (lane == 0 && gt) atomicAdd(&red[0], gt);
+    if (lane == 0 && eq) atomicAdd(&red[1], eq);
+    __syncthreads();
+    gt = red[0];
+    eq = red[1];
+    if (PASS < 3 && tid == 0) {
+      w.above[PASS - 1][part] = gt;  // keys of this part that the digit puts over the threshold
+      if (part == 0) {
+        w.state[PASS - 1][0] = thr;
+        w.state[PASS - 1][1] = need;
       }
-      __syncthreads();
-      if (tid == 0) w.above[prev][part] = red[0];
     }
   }
   if constexpr (PASS < 3) {
     constexpr int bins = sel_bins(PASS), shift = sel_shift(PASS);
-    for (int i = tid; i < bins; i += SEL_T) s.hist[i] = 0;
+    for (int i = tid; i < bins; i += SEL_T) hist[i] = 0;
     __syncthreads();
     for (int t0 = lo; t0 < hi; t0 += SEL_TILE) {
       if (t0 > lo) load(t0, u);
 #pragma unroll
       for (int j = 0; j < SEL_NPL; ++j)
-        if (t0 + wave * 64 * SEL_NPL + 64 * j + lane < hi && (u[j] & mask) == thr) atomicAdd(&s.hist[(u[j] >> shift) & (bins - 1)], 1u);
+        if (t0 + wave * 64 * SEL_NPL + 64 * j + lane < hi && (u[j] & mask) == thr) atomicAdd(&hist[(u[j] >> shift) & (bins - 1)], 1u);
     }
     __syncthreads();
-    for (int i = tid; i < bins; i += SEL_T) w.hist[PASS][part][i] = s.hist[i];
+    for (int i = tid; i < bins; i += SEL_T) w.hist[PASS][part][i] = hist[i];
   } else {
-    // kept and equal keys in the parts before
-    constexpr int bins = sel_bins(2);
-    const uint32_t bin = thr & (bins - 1);
-    if (tid < 2) red[tid] = 0;
-    __syncthreads();
-    uint32_t gt = 0, eq = 0;
-    for (int i = tid; i < part * bins; i += SEL_T) {
-      const uint32_t n = (uint32_t)(i % bins) >= bin ? ldg(&w.hist[2][i / bins][i % bins]) : 0u;
-      if ((uint32_t)(i % bins) == bin) eq += n;
-      else gt += n;
-    }
-    if (tid < part) gt += ldg(&w.above[0][tid]) + ldg(&w.above[1][tid]);
-    if (gt) atomicAdd(&red[0], gt);
-    if (eq) atomicAdd(&red[1], eq);
     if (part == 0) sel_edges(p, kept, tid, SEL_T);
-    __syncthreads();
-    uint32_t eq0 = red[1], at0 = p.sinks + red[0] + min(need, red[1]);
+    uint32_t eq0 = eq, at0 = p.sinks + gt + min(need, eq);
     for (int t0 = lo; t0 < hi; t0 += SEL_TILE) {
       if (t0 > lo) load(t0, u);
       const int i0 = t0 + wave * 64 * SEL_NPL;
