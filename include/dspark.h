@@ -187,6 +187,7 @@ int dspark_kv_read_b8(const dspark_b8_cache* cache, int32_t pos0, int32_t n, flo
  * exp(q k / sqrt(D)) over the keys a row sees (before the gate). A row that sees no key (every page of it absent) gives
  * zeros and lse -inf. M QH / KVH <= 1024. The workspace needs no clearing and may be shared by stream-ordered calls. The
  * probabilities are rounded to fp16 once; scores, sums and outputs are fp32. */
+#define DSPARK_B8_ARRIVALS 32
 typedef struct dspark_b8_attn_args {
   const void* q;
   int64_t q_stride;            /* elements between tokens, >= QH D */
@@ -196,6 +197,9 @@ typedef struct dspark_b8_attn_args {
   const float* gate;           /* fp32 [M][QH] pre-sigmoid gate or NULL */
   void* workspace;             /* size from dspark_verify_attention_b8_workspace, on a 16-byte boundary */
   size_t workspace_bytes;
+  uint32_t* arrivals;          /* KVH x DSPARK_B8_ARRIVALS words or NULL: with them the splits of few rows are added by the
+                                  last of them to finish instead of a second launch, to the same bits. Zero before their first use; every call leaves them zero. Like the workspace they
+                                  serve any number of stream-ordered calls, not calls that overlap, but nothing else. */
   int32_t M, QH;               /* 1 <= M <= DSPARK_MT_MAX; QH % KVH == 0 */
   int32_t a, start, window, causal;
   int32_t splits;              /* key-range splits per KV head; 0 = automatic */

@@ -22,6 +22,11 @@ namespace dspark {
 // Waves of a workgroup, which fills a CU: as many as the registers of RB row blocks leave (o alone takes D RB / 4).
 constexpr int b8_waves(int D, int RB) { return D == 64 ? (RB == 1 ? 16 : RB <= 3 ? 12 : 8) : RB == 1 ? 12 : 8; }
 constexpr int MASS_WAVES = 4;
+#ifndef B8_SHORT
+#define B8_SHORT 4
+#endif
+constexpr int B8_COHERENT = 16;    // buffer cache policy SC1: device-scope coherent store / load
+constexpr int B8_FUSED_BYTES = 64 << 10;  // sums of one row block's splits that the last of them adds (b8_attn_plan)
 // Running reference in log2 units, set to the row's largest x + log2 vs less 8 when one passes ref + 15: P stays under 2^15,
 // and a P of 2^-22 of the largest is still a normal half (one below is off by 2^-33 of the largest at most).
 constexpr float REF_INIT = -1e30f, REF_BELOW = 8.f, REF_SLACK = 15.f;
@@ -32,24 +37,31 @@ struct B8Tile {
   uint32_t v[8][D / 64];  // key 16 (j / 4) + 4 g + j % 4, dims (D / 16) n .. + D / 16
 };
 
+// A block as a buffer (wave-uniform), so that a load is the lane's 32-bit offset and registers of pending loads are not needed
+// for addresses; an absent page (pg < 0) is an empty one, whose loads return zeros.
 template <int D>
-__device__ __forceinline__ void b8_load_k(const uint8_t* base, int lane, u32x4 (&k)[2][D / 64]) {
-  const uint32_t off = (uint32_t)((lane & 15) * D + (lane >> 4) * 16);
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t b8_block(const uint8_t* pool, int KVH, int h, int pg) {
+  const size_t blk = ((size_t)max(pg, 0) * KVH + h) * (PAGE * D);
+  return __builtin_amdgcn_make_buffer_rsrc((void*)(pool + blk), (short)0, pg < 0 ? 0 : PAGE * D, 0x00020000);
+}
+template <int D>
+__device__ __forceinline__ void b8_load_k(__amdgpu_buffer_rsrc_t r, int lane, u32x4 (&k)[2][D / 64]) {
+  const int off = (lane & 15) * D + (lane >> 4) * 16;
 #pragma unroll
   for (int b = 0; b < 2; ++b)
 #pragma unroll
-    for (int u = 0; u < D / 64; ++u) k[b][u] = ldg(reinterpret_cast<const u32x4*>(base + off + (16 * b * D + 64 * u)));
+    for (int u = 0; u < D / 64; ++u) k[b][u] = __builtin_amdgcn_raw_buffer_load_b128(r, off + (16 * b * D + 64 * u), 0, 0);
 }
 template <int D>
-__device__ __forceinline__ void b8_load_v(const uint8_t* base, int lane, uint32_t (&v)[8][D / 64]) {
-  const uint32_t off = (uint32_t)((lane >> 4) * 4 * D + (lane & 15) * (D / 16));
+__device__ __forceinline__ void b8_load_v(__amdgpu_buffer_rsrc_t r, int lane, uint32_t (&v)[8][D / 64]) {
+  const int off = (lane >> 4) * 4 * D + (lane & 15) * (D / 16);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const uint8_t* at = base + off + (16 * (j / 4) + j % 4) * D;
+    const int at = off + (16 * (j / 4) + j % 4) * D;
     if constexpr (D == 64) {
-      v[j][0] = ldg(reinterpret_cast<const uint32_t*>(at));
+      v[j][0] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0);
     } else {
-      const u32x2 t = ldg(reinterpret_cast<const u32x2*>(at));
+      const u32x2 t = __builtin_amdgcn_raw_buffer_load_b64(r, at, 0, 0);
       v[j][0] = t[0];
       v[j][1] = t[1];
     }
@@ -124,6 +136,7 @@ __device__ __forceinline__ void b8_load_q(const B8Attn& p, int h, int row0, int 
       for (int e = 0; e < 2; ++e) q[rb][2 * u + e] = as_half8(ldg(reinterpret_cast<const u32x4*>(at + 64 * u + 8 * e)));
   }
 }
+constexpr int NOWHERE = 0x7fffffff - PAGE;  // the position of an absent page's first key: past every range
 // What token t sees: the keys lo, lo + 1, ... of the range's `n` (context keys from start and the window on, then the block's;
 // one comparison a key).
 struct B8Sight {
@@ -180,9 +193,8 @@ __device__ __forceinline__ void b8_mask(const B8Attn& p, float ks, int pos, cons
 // ---------------------------------------------------------------- attention
 template <int D>
 __device__ __forceinline__ void b8_load_tile(const B8Attn& p, int h, int pg, int lane, B8Tile<D>& t) {
-  const size_t blk = ((size_t)max(pg, 0) * p.c.KVH + h) * (PAGE * D);  // an absent page's loads go to page 0, unused
-  b8_load_k<D>(p.c.k + blk, lane, t.k);
-  b8_load_v<D>(p.c.v + blk, lane, t.v);
+  b8_load_k<D>(b8_block<D>(p.c.k, p.c.KVH, h, pg), lane, t.k);
+  b8_load_v<D>(b8_block<D>(p.c.v, p.c.KVH, h, pg), lane, t.v);
 }
 
 // Running state of a wave's rows: o[rb][d] of row 16 rb + n, dims (D / 16) (4 g + i) + d; l the lane's part of the sum of P,
@@ -194,13 +206,14 @@ struct B8Rows {
   f32x4 o[RB][D / 16];
 };
 
+// One page; lp < 0: an absent one, which no row sees.
 template <int D, int RB, bool FP8>
 __device__ __forceinline__ void b8_page(const B8Attn& p, const B8Tile<D>& t, const half8 (&q)[RB][D / 32], const int (&tok)[RB],
                                         float ks, float lv, float iv, int lp, int lane, B8Rows<D, RB>& st) {
   f32x4 s[RB][2];
   b8_scores<D, RB, FP8>(t.k, q, s);
   if (lp < p.full_lo || lp >= p.full_hi) {
-    b8_mask<RB>(p, ks, lp * PAGE, tok, lane, s);
+    b8_mask<RB>(p, ks, lp < 0 ? NOWHERE : lp * PAGE, tok, lane, s);
     ks = 1.f;
   }
   float top[RB], at[RB];
@@ -266,6 +279,61 @@ __device__ __forceinline__ float b8_gate(const B8Attn& p, int h, int row) {
   return p.gate ? 1.f / (1.f + __expf(-ldg(p.gate + (size_t)t * p.QH + qh))) : 1.f;
 }
 
+// The splits of a row are added in an order of its own, whoever adds them: split lane j takes splits j, j + 4, ... in batches
+// of 8, each batch rescaled to the largest reference so far; then the lanes in order.
+constexpr int SPLIT_LANES = 4, SPLIT_BATCH = 8;
+template <int D>
+__device__ __forceinline__ void b8_add_splits(const B8Attn& p, __amdgpu_buffer_rsrc_t racc, __amdgpu_buffer_rsrc_t rml, int first, int j,
+                                              int c, float* o, f32x2* ml_out) {
+  float m = REF_INIT, l = 0.f;
+  f32x4 acc = {0, 0, 0, 0};
+  for (int s0 = j; s0 < p.S; s0 += SPLIT_LANES * SPLIT_BATCH) {
+    f32x2 ml[SPLIT_BATCH];
+    f32x4 v[SPLIT_BATCH];
+#pragma unroll
+    for (int i = 0; i < SPLIT_BATCH; ++i) {  // (past the last split: the last again)
+      const int at = first + min(s0 + i * SPLIT_LANES, p.S - 1);
+      ml[i] = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(rml, at * (int)sizeof(f32x2), 0, B8_COHERENT));
+      v[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(racc, (at * D + 4 * c) * (int)sizeof(float), 0, B8_COHERENT));
+    }
+    float to = m;
+#pragma unroll
+    for (int i = 0; i < SPLIT_BATCH; ++i) {
+      if (s0 + i * SPLIT_LANES >= p.S) ml[i] = f32x2{REF_INIT, 0.f}, v[i] = f32x4{0, 0, 0, 0};
+      to = max_of(to, ml[i][0]);
+    }
+    const float f0 = fast_exp2(m - to);
+    acc *= f0;
+    l *= f0;
+#pragma unroll
+    for (int i = 0; i < SPLIT_BATCH; ++i) {
+      const float f = fast_exp2(ml[i][0] - to);
+      acc += v[i] * f;
+      l = fmaf(ml[i][1], f, l);
+    }
+    m = to;
+  }
+  *reinterpret_cast<f32x4*>(o) = acc;
+  if (c == 0) *ml_out = f32x2{m, l};
+}
+// The split lanes' sums (o_lane and ml_lane apart from lane to lane) added, the row finished.
+template <int D>
+__device__ __forceinline__ void b8_finish_row(const B8Attn& p, int h, int row, int c, const float* o, const f32x2* ml, int o_lane,
+                                              int ml_lane) {
+  const float gate = b8_gate(p, h, row);
+  float m = REF_INIT, l = 0.f;
+  f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+  for (int w = 0; w < SPLIT_LANES; ++w) m = max_of(m, ml[w * ml_lane][0]);
+#pragma unroll
+  for (int w = 0; w < SPLIT_LANES; ++w) {
+    const float f = fast_exp2(ml[w * ml_lane][0] - m);
+    acc += *reinterpret_cast<const f32x4*>(o + w * o_lane) * f;
+    l = fmaf(ml[w * ml_lane][1], f, l);
+  }
+  b8_store<D>(p, h, row, c, acc, m, l, gate);
+}
+
 // One workgroup per (KV head, key split, row group), the split's pages spread evenly over its waves. Splits go to the
 // workspace and a second kernel adds them; a single split is finished here.
 template <int D, int RB, bool FP8>
@@ -310,10 +378,10 @@ __global__ __launch_bounds__(64 * b8_waves(D, RB), b8_waves(D, RB) / 4) void att
     // the next page's loads are in flight while a page is worked on (past the last one: that page again, from L2)
     auto step = [&](int i, const B8Tile<D>& now, B8Tile<D>& next) {
       b8_load_tile<D>(p, h, __builtin_amdgcn_readlane(pgl, min(i + 1, nb - 1)), lane, next);
-      if (__builtin_amdgcn_readlane(pgl, i) >= 0)
-        b8_page<D, RB, FP8>(p, now, q, tok, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ksl), i)),
-                            __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lvl), i)),
-                            __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ivl), i)), b0 + i, lane, st);
+      b8_page<D, RB, FP8>(p, now, q, tok, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ksl), i)),
+                          __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lvl), i)),
+                          __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ivl), i)),
+                          __builtin_amdgcn_readlane(pgl, i) < 0 ? -1 : b0 + i, lane, st);
     };
     // Of the waves of a SIMD the oldest would run ahead and leave the others to finish alone: who is further on yields.
     __builtin_amdgcn_s_setprio(3);
@@ -345,11 +413,18 @@ __global__ __launch_bounds__(64 * b8_waves(D, RB), b8_waves(D, RB) / 4) void att
   if (p.S == 1)
 #pragma unroll
     for (int k = 0; k < (ROWS + PER - 1) / PER; ++k) gate[k] = b8_gate(p, h, min(row0 + (int)threadIdx.x / QUADS + k * PER, p.R - 1));
+  // the row group's part of the workspace (rows past the last have none; under 2 GiB: at most 64 rows and 4096 splits)
+  const size_t first = ((size_t)h * p.R + row0) * p.S;
+  const int held = min(ROWS, p.R - row0) * p.S;
+  const __amdgpu_buffer_rsrc_t racc =
+      __builtin_amdgcn_make_buffer_rsrc((void*)(p.part_acc + first * D), (short)0, held * D * (int)sizeof(float), 0x00020000);
+  const __amdgpu_buffer_rsrc_t rml =
+      __builtin_amdgcn_make_buffer_rsrc((void*)(p.part_ml + first), (short)0, held * (int)sizeof(f32x2), 0x00020000);
   lds_barrier();
 #pragma unroll
   for (int k = 0; k < (ROWS + PER - 1) / PER; ++k) {
     const int r = threadIdx.x / QUADS + k * PER, row = row0 + r;
-    if (r >= ROWS || row >= p.R) break;
+    if (r >= ROWS || row >= p.R) continue;
     f32x2 ml[NW];
     float m = REF_INIT, l = 0.f;
     f32x4 acc = {0, 0, 0, 0};
@@ -367,70 +442,56 @@ __global__ __launch_bounds__(64 * b8_waves(D, RB), b8_waves(D, RB) / 4) void att
     if (p.S == 1) {
       b8_store<D>(p, h, row, c, acc, m, l, gate[k]);
     } else {
-      const size_t at = ((size_t)h * p.R + row) * p.S + sp;
-      *reinterpret_cast<f32x4*>(p.part_acc + at * D + 4 * c) = acc;
-      if (c == 0) p.part_ml[at] = f32x2{m, l};
+      const uint32_t at = (uint32_t)(r * p.S + sp);
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc), racc, (int)((at * D + 4 * c) * sizeof(float)), 0, B8_COHERENT);
+      if (c == 0) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, f32x2{m, l}), rml, (int)(at * sizeof(f32x2)), 0, B8_COHERENT);
+    }
+  }
+  if constexpr (RB == 1) {
+    // The last split of a row group to arrive adds all of them. Sums are stored and loaded device-coherent; every store of a
+    // split is complete (vmcnt 0, then the workgroup's barrier) before its arrival is counted, and the last one's loads come
+    // after its own count. It leaves the counter at zero.
+    if (!p.arrivals) return;
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    __shared__ int last_s;
+    if (threadIdx.x == 0) {
+      uint32_t* counter = p.arrivals + h * p.RG + blockIdx.z;
+      last_s = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(p.S - 1);
+      if (last_s) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!last_s) return;
+    constexpr int RP = PER / SPLIT_LANES;  // rows side by side
+    static_assert(RP >= 1 && NW >= SPLIT_LANES, "the split lanes' sums fit where the waves' were");
+    const int u = threadIdx.x / QUADS, j = u / RP;
+#pragma unroll 1
+    for (int r0 = 0; r0 < ROWS && row0 + r0 < p.R; r0 += RP) {
+      const int r = r0 + u % RP;
+      const bool mine = j < SPLIT_LANES && r < ROWS && row0 + r < p.R;
+      if (mine) b8_add_splits<D>(p, racc, rml, r * p.S, j, c, &s_o[j][r][4 * c], &s_ml[j][r]);
+      lds_barrier();
+      if (mine && j == 0) b8_finish_row<D>(p, h, row0 + r, c, &s_o[0][r][4 * c], &s_ml[0][r], ROWS * (D + 4), ROWS);
     }
   }
 }
 
-// One workgroup per (row, KV head): the splits' sums rescaled and added, 256 / (D / 4) splits side by side, in a fixed
-// order, and finished.
+// One workgroup for some rows of a KV head: the splits' sums added and finished.
 template <int D>
 __global__ __launch_bounds__(256) void attn_b8_merge_kernel(B8Attn p) {
-  constexpr int Q = D / 4, SL = 256 / Q, PER = 4;
-  __shared__ f32x4 s_acc[SL][Q];
-  __shared__ f32x2 s_ml[SL];
-  const int row = blockIdx.x, h = blockIdx.y, c = threadIdx.x % Q, j = threadIdx.x / Q;
-  const size_t at = ((size_t)h * p.R + row) * p.S;
-  float m = REF_INIT, l = 0.f;
-  f32x4 acc = {0, 0, 0, 0};
-  const float gate = b8_gate(p, h, row);
-  for (int s0 = j; s0 < p.S; s0 += SL * PER) {
-    f32x2 ml[PER];
-    f32x4 a[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int s = min(s0 + i * SL, p.S - 1);
-      ml[i] = ldg(p.part_ml + at + s);
-      a[i] = ldg(reinterpret_cast<const f32x4*>(p.part_acc + (at + s) * D + 4 * c));
-    }
-    float to = m;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      if (s0 + i * SL >= p.S) ml[i][0] = REF_INIT, ml[i][1] = 0.f, a[i] = f32x4{0, 0, 0, 0};
-      to = max_of(to, ml[i][0]);
-    }
-    const float f0 = fast_exp2(m - to);
-    acc *= f0;
-    l *= f0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const float f = fast_exp2(ml[i][0] - to);
-      acc += a[i] * f;
-      l = fmaf(ml[i][1], f, l);
-    }
-    m = to;
-  }
-  s_acc[j][c] = acc;
-  if (c == 0) s_ml[j] = f32x2{m, l};
+  constexpr int Q = D / 4, RP = 256 / Q / SPLIT_LANES;
+  __shared__ float s_acc[SPLIT_LANES][RP][D];
+  __shared__ f32x2 s_ml[SPLIT_LANES][RP];
+  const int h = blockIdx.y, c = threadIdx.x % Q, u = threadIdx.x / Q, r = u % RP, j = u / RP, row = blockIdx.x * RP + r;
+  const size_t first = ((size_t)h * p.R + blockIdx.x * RP) * p.S;
+  const int held = min(RP, p.R - (int)blockIdx.x * RP) * p.S;
+  const __amdgpu_buffer_rsrc_t racc =
+      __builtin_amdgcn_make_buffer_rsrc((void*)(p.part_acc + first * D), (short)0, held * D * (int)sizeof(float), 0x00020000);
+  const __amdgpu_buffer_rsrc_t rml =
+      __builtin_amdgcn_make_buffer_rsrc((void*)(p.part_ml + first), (short)0, held * (int)sizeof(f32x2), 0x00020000);
+  if (row < p.R) b8_add_splits<D>(p, racc, rml, r * p.S, j, c, &s_acc[j][r][4 * c], &s_ml[j][r]);
   lds_barrier();
-  if (j) return;
-  f32x2 ml[SL];
-#pragma unroll
-  for (int s = 0; s < SL; ++s) {
-    ml[s] = s_ml[s];
-    m = max_of(m, ml[s][0]);
-  }
-  acc = f32x4{0, 0, 0, 0};
-  l = 0.f;
-#pragma unroll
-  for (int s = 0; s < SL; ++s) {
-    const float f = fast_exp2(ml[s][0] - m);
-    acc += s_acc[s][c] * f;
-    l = fmaf(ml[s][1], f, l);
-  }
-  b8_store<D>(p, h, row, c, acc, m, l, gate);
+  if (row < p.R && j == 0) b8_finish_row<D>(p, h, row, c, &s_acc[0][r][4 * c], &s_ml[0][r], RP * D, RP);
 }
 
 // ---------------------------------------------------------------- accounts of attention weight
@@ -472,8 +533,8 @@ __global__ __launch_bounds__(64 * MASS_WAVES) void mass_b8_kernel(B8Attn p) {
       float old[2];
       // lane (n, g), g < 2, stores key 16 g + n
       auto load = [&](int i, u32x4 (&t)[2][D / 64], float& was) {
-        const int pg = max(__builtin_amdgcn_readlane(pgl, i), 0), kp = (b0 + i) * PAGE + 16 * (g & 1) + n;
-        b8_load_k<D>(p.c.k + ((size_t)pg * p.c.KVH + h) * (PAGE * D), lane, t);
+        const int kp = (b0 + i) * PAGE + 16 * (g & 1) + n;
+        b8_load_k<D>(b8_block<D>(p.c.k, p.c.KVH, h, __builtin_amdgcn_readlane(pgl, i)), lane, t);
         const float* from = row0 ? out : in;
         was = from && kp < (row0 ? live : p.a) ? ldg(from + kp) : 0.f;
       };
@@ -537,16 +598,25 @@ static void b8_range(B8Attn& p, int D) {
 
 void b8_attn_plan(B8Attn& p, int D, int splits, int cus) {
   p.R = p.G * p.M;
-  const int blocks = (p.R + 15) / 16;
-  const int most = D == 64 ? B8_ROW_BLOCKS : 2;
-  p.RG = (blocks + most - 1) / most;
-  p.rb = (blocks + p.RG - 1) / p.RG;
   p.g_div = div_magic((uint32_t)p.G);
   b8_range(p, D);
+  const int blocks = (p.R + 15) / 16, most = D == 64 ? B8_ROW_BLOCKS : 2;
+  p.RG = (blocks + most - 1) / most;
+  p.rb = (blocks + p.RG - 1) / p.RG;
+  // Few pages: a row block a workgroup and no splits, while that leaves a wave few of them (SHORT).
+  if (splits == 0 && p.npages <= B8_SHORT * b8_waves(D, 1) && p.c.KVH * blocks <= cus) {
+    p.rb = 1;
+    p.RG = blocks;
+    splits = 1;
+  }
   const int waves = b8_waves(D, p.rb);
   int S = splits > 0 ? splits : std::max(1, cus / (p.c.KVH * p.RG));
   S = std::max(1, std::min(std::min(S, 4096), (p.npages + waves - 1) / waves));
   p.S = S;
+  // The last split to arrive adds the others (if the caller has counters) where they are little to read for one workgroup:
+  // one token of 32768 keys 12.3 us against 11.7 with a second launch, which costs its caller 4 more; 36 rows of 131063
+  // keys, 64 KB at D = 128 and four splits ... 46 against 38.
+  if (S == 1 || p.rb > 1 || std::min(p.R, 16) * S * D * (int)sizeof(float) > B8_FUSED_BYTES) p.arrivals = nullptr;
   p.pps = p.npages / (S * waves);
   p.more = p.npages % (S * waves);
 }
@@ -575,8 +645,9 @@ int b8_attn_launch(const B8Attn& p, int D, bool fp8, hipStream_t s) {
   if (D == 64) fp8 ? attn_b8_by_rows<64, true>(p, s) : attn_b8_by_rows<64, false>(p, s);
   else fp8 ? attn_b8_by_rows<128, true>(p, s) : attn_b8_by_rows<128, false>(p, s);
   if (const int rc = (int)hipGetLastError()) return rc;
-  if (p.S == 1) return 0;
-  const dim3 grid(p.R, p.c.KVH);
+  if (p.S == 1 || p.arrivals) return 0;
+  const int rows = 256 / (D / 4) / SPLIT_LANES;
+  const dim3 grid((p.R + rows - 1) / rows, p.c.KVH);
   if (D == 64) hipLaunchKernelGGL(attn_b8_merge_kernel<64>, grid, dim3(256), 0, s, p);
   else hipLaunchKernelGGL(attn_b8_merge_kernel<128>, grid, dim3(256), 0, s, p);
   return (int)hipGetLastError();

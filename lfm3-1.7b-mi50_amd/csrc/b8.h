@@ -143,6 +143,7 @@ struct B8Attn {
   const float* gate;    // [M][QH]
   float* part_acc;      // [KVH][rows][S][D]
   f32x2* part_ml;       // [KVH][rows][S] (reference exponent, sum)
+  uint32_t* arrivals;   // [KVH][RG] zero between calls, or nullptr
   int M, QH, G, R;      // R = G M rows per KV head, row r = token r / G, query head r % G of the KV head's
   uint32_t g_div;
   int a, start, window, causal;

@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "dspark.h"
 #include "dspark_internal.h"
@@ -47,10 +48,16 @@ B8Pool pool(const dspark_b8_cache* c) {
   return p;
 }
 
+// Compute units of the current device (queried once per device).
 int device_cus() {
-  int dev = 0, n = 0;
-  if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0)
-    return 256;
+  static std::atomic<int> cached[64];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+  int n = cached[dev].load(std::memory_order_relaxed);
+  if (!n) {
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
+    cached[dev].store(n, std::memory_order_relaxed);
+  }
   return n;
 }
 
@@ -73,6 +80,7 @@ B8Attn attn(const dspark_b8_cache* c, const dspark_b8_attn_args* a) {
   p.out32 = a->out_f32;
   p.lse = a->lse;
   p.gate = a->gate;
+  p.arrivals = a->arrivals;
   p.M = a->M;
   p.QH = a->QH;
   p.G = a->QH / c->KVH;
@@ -135,6 +143,7 @@ size_t dspark_verify_attention_b8_workspace(const dspark_b8_cache* c, const dspa
 int dspark_verify_attention_b8(const dspark_b8_cache* c, const dspark_b8_attn_args* a, dspark_stream_t stream) {
   if (!rows_ok(c, a) || !query_ok(c, a)) return DSPARK_EINVAL;
   if (!a->out && !a->out_f32) return DSPARK_EINVAL;
+  if (a->arrivals && !on(a->arrivals, 4)) return DSPARK_EINVAL;
   if ((a->out && !on(a->out, 16)) || (a->out_f32 && !on(a->out_f32, 16))) return DSPARK_EINVAL;
   B8Attn p = attn(c, a);
   b8_attn_plan(p, c->D, a->splits, device_cus());

@@ -49,8 +49,8 @@ class B8CacheArgs(ctypes.Structure):
 class B8AttnArgs(ctypes.Structure):
     _fields_ = [("q", ctypes.c_void_p), ("q_stride", ctypes.c_int64), ("out", ctypes.c_void_p), ("out_f32", ctypes.c_void_p),
                 ("lse", ctypes.c_void_p), ("gate", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
-                ("workspace_bytes", ctypes.c_size_t), ("M", ctypes.c_int32), ("QH", ctypes.c_int32), ("a", ctypes.c_int32),
-                ("start", ctypes.c_int32), ("window", ctypes.c_int32), ("causal", ctypes.c_int32),
+                ("workspace_bytes", ctypes.c_size_t), ("arrivals", ctypes.c_void_p), ("M", ctypes.c_int32),
+                ("QH", ctypes.c_int32), ("a", ctypes.c_int32), ("start", ctypes.c_int32), ("window", ctypes.c_int32), ("causal", ctypes.c_int32),
                 ("splits", ctypes.c_int32)]
 
 
@@ -166,6 +166,7 @@ class Workspace:
     def __init__(self, device="cuda"):
         self.device = device
         self.buf = None
+        self.words = None
 
     def get(self, nbytes):
         torch = _torch()
@@ -174,6 +175,13 @@ class Workspace:
             # zero-filled: the split-K GEMM keeps its arrival counters here (left at zero by every call)
             self.buf = torch.zeros(nbytes, dtype=torch.uint8, device=self.device)
         return self.buf
+
+    def arrivals(self, n):
+        """n words apart from the buffer, zeroed once: arrival counters, which their user leaves at zero."""
+        torch = _torch()
+        if self.words is None or self.words.numel() < n:
+            self.words = torch.zeros(n, dtype=torch.int32, device=self.device)
+        return self.words
 
 
 # ---------------------------------------------------------------- KV pages
@@ -326,6 +334,7 @@ def verify_attention_rec(q, pages, a, start=0, window=0, causal=True, out=None, 
 
 # ---------------------------------------------------------------- 8-bit block-scaled K/V cache
 B8_INT8, B8_E4M3 = 0, 1
+B8_ARRIVALS = 32
 
 
 class B8Cache:
@@ -346,7 +355,8 @@ class B8Cache:
         if any(t.device != k.device or not t.is_contiguous() for t in every):
             raise DsparkError("B8Cache: contiguous tensors of one device")
         self.k, self.v, self.k_scale, self.v_scale, self.block_table = k, v, k_scale, v_scale, block_table
-        self.KVH, self.D, self.device = k.shape[1], k.shape[3], k.device
+        self.KVH, self.D, self.device, self.index = k.shape[1], k.shape[3], k.device, k.get_device()
+        self.positions = None if block_table is None else block_table.shape[0] * PAGE  # that the table has entries for
         self.args = B8CacheArgs(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                                 None if block_table is None else block_table.data_ptr(), k.shape[0], self.KVH, self.D,
                                 codes[k.dtype])
@@ -354,10 +364,10 @@ class B8Cache:
 
     def check(self, end, *tensors):
         """`end` positions have table entries, and the tensors are the cache's device's."""
-        if self.block_table is not None and (end + PAGE - 1) // PAGE > self.block_table.shape[0]:
+        if self.positions is not None and end > self.positions:
             raise DsparkError(f"{end} positions need {(end + PAGE - 1) // PAGE} entries in the block table")
         for t in tensors:
-            if t is not None and t.device != self.device:
+            if t is not None and t.get_device() != self.index:
                 raise DsparkError("tensors and cache are on different devices")
 
 
@@ -369,164 +379,167 @@ def b8_cache_alloc(n_pages, KVH, D, dtype=None, device="cuda", block_table=None)
     return B8Cache(*codes, *scales, block_table)
 
 
-class _on:
-    """The device of a cache current, and `stream` (default: that device's current stream) the one that allocations belong
-    to; yields the stream's handle. Costs nothing where both are current already."""
-
-    def __init__(self, device, stream):
-        torch = _torch()
-        self.guard = None
-        if stream is None and torch.cuda.current_device() == device.index:
-            self.stream = torch.cuda.current_stream()
-        else:
-            self.stream = stream if stream is not None else torch.cuda.current_stream(device)
-            if self.stream.device != device:
-                raise DsparkError("the stream belongs to another device than the cache")
-            self.guard = torch.cuda.stream(self.stream)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return self.stream.cuda_stream
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _b8_on(cache, stream, call, *args):
+    """call(handle of the stream, cache, *args) with the cache's device current and `stream` (default: that device's current
+    one) the stream that allocations belong to."""
+    torch = _torch()
+    if stream is None and torch.cuda.current_device() == cache.index:
+        return call(torch._C._cuda_getCurrentRawStream(cache.index), cache, *args)
+    stream = stream if stream is not None else torch.cuda.current_stream(cache.device)
+    if stream.device_index != cache.index:
+        raise DsparkError("the stream belongs to another device than the cache")
+    with torch.cuda.stream(stream):
+        return call(stream.cuda_stream, cache, *args)
 
 
-def _b8_row(t, KVH, D, what):
+def _b8_row(t, cache, what):
     """Elements between the rows of a [n][KVH][D] (or [n][row]) tensor whose rows are contiguous."""
-    inner = t.stride(-1) == 1 and (t.dim() == 2 or t.stride(1) == D)
-    if t.dim() not in (2, 3) or not inner or (t.shape[1:] != (KVH, D) if t.dim() == 3 else t.shape[1] < KVH * D):
-        raise DsparkError(f"{what}: rows of {KVH} heads x {D}")
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), KVH * D)
+    shape, stride, H, D = t.shape, t.stride(), cache.KVH, cache.D
+    if len(shape) == 3 and shape[1] == H and shape[2] == D and stride[2] == 1 and (H == 1 or stride[1] == D) \
+            or len(shape) == 2 and shape[1] >= H * D and stride[1] == 1:
+        return stride[0] if shape[0] > 1 else max(stride[0], H * D)
+    raise DsparkError(f"{what}: rows of {H} heads x {D}")
+
+
+def _kv_write_b8(s, cache, k, v, row, pos0, n):
+    check(lib().dspark_kv_write_b8(cache.ref, k.data_ptr(), v.data_ptr(), row, pos0, n, s), "dspark_kv_write_b8")
 
 
 def kv_write_b8(k, v, cache, pos0, stream=None):
     """Append k, v fp16 [n][KVH][D] (or [n][row >= KVH*D]; rows may lie inside wider ones) as positions pos0 .. pos0+n-1."""
-    torch = _torch()
-    n = k.shape[0]
-    row = _b8_row(k, cache.KVH, cache.D, "kv_write_b8")
-    if v.shape != k.shape or (n > 1 and _b8_row(v, cache.KVH, cache.D, "kv_write_b8") != row):
-        raise DsparkError("kv_write_b8: k and v of one shape and row stride")
-    if k.dtype != torch.float16 or v.dtype != torch.float16:
-        raise DsparkError("kv_write_b8: k and v are fp16")
+    f16 = _torch().float16
+    row, n = _b8_row(k, cache, "kv_write_b8"), k.shape[0]
+    if v.shape != k.shape or _b8_row(v, cache, "kv_write_b8") != row or k.dtype != f16 or v.dtype != f16:
+        raise DsparkError("kv_write_b8: k and v are fp16, of one shape and row stride")
     cache.check(pos0 + n, k, v)
-    with _on(cache.device, stream) as s:
-        check(lib().dspark_kv_write_b8(cache.ref, k.data_ptr(), v.data_ptr(), row, pos0, n, s), "dspark_kv_write_b8")
+    _b8_on(cache, stream, _kv_write_b8, k, v, row, pos0, n)
+
+
+def _kv_read_b8(s, cache, pos0, n, k, v):
+    torch = _torch()
+    if k is None or v is None:
+        k, v = torch.empty((2, n, cache.KVH, cache.D), dtype=torch.float32, device=cache.device).unbind()
+    row = _b8_row(k, cache, "kv_read_b8")
+    if k.dtype != torch.float32 or v.dtype != torch.float32 or k.shape[0] < n or v.shape != k.shape \
+            or _b8_row(v, cache, "kv_read_b8") != row:
+        raise DsparkError("kv_read_b8: k and v are fp32 rows of one shape and stride")
+    check(lib().dspark_kv_read_b8(cache.ref, pos0, n, k.data_ptr(), v.data_ptr(), row, s), "dspark_kv_read_b8")
+    return k, v
 
 
 def kv_read_b8(cache, pos0, n, k=None, v=None, stream=None):
     """The values of positions pos0 .. pos0+n-1 as fp32 [n][KVH][D] tensors (given, as rows, or created)."""
-    torch = _torch()
     cache.check(pos0 + n, k, v)
-    with _on(cache.device, stream) as s:
-        if k is None or v is None:
-            new = torch.empty((2, n, cache.KVH, cache.D), dtype=torch.float32, device=cache.device)
-            k, v = new[0], new[1]
-        row = _b8_row(k, cache.KVH, cache.D, "kv_read_b8")
-        if k.dtype != torch.float32 or v.dtype != torch.float32 or k.shape[0] < n or v.shape != k.shape \
-                or _b8_row(v, cache.KVH, cache.D, "kv_read_b8") != row:
-            raise DsparkError("kv_read_b8: k and v are fp32 rows of one shape and stride")
-        check(lib().dspark_kv_read_b8(cache.ref, pos0, n, k.data_ptr(), v.data_ptr(), row, s), "dspark_kv_read_b8")
-    return k, v
+    return _b8_on(cache, stream, _kv_read_b8, pos0, n, k, v)
 
 
 def _b8_attn_args(q, cache, a, start, window, causal):
-    torch = _torch()
-    M, QH, D = q.shape
-    if q.dtype != torch.float16 or D != cache.D or q.stride(2) != 1 or q.stride(1) != D:
+    shape, stride = q.shape, q.stride()
+    if len(shape) != 3 or shape[2] != cache.D or q.dtype != _torch().float16 or stride[2] != 1 \
+            or (shape[1] > 1 and stride[1] != cache.D):
         raise DsparkError("q is fp16 [M][QH][D] of contiguous rows, D the cache's")
+    M, QH, D = shape
     cache.check(a + M, q)
-    args = B8AttnArgs()
-    args.q, args.q_stride = q.data_ptr(), q.stride(0) if M > 1 else max(q.stride(0), QH * D)
-    args.M, args.QH, args.a, args.start, args.window, args.causal = M, QH, a, start, window, int(causal)
-    return args
+    return B8AttnArgs(q=q.data_ptr(), q_stride=stride[0] if M > 1 else max(stride[0], QH * D), M=M, QH=QH, a=a, start=start,
+                      window=window, causal=int(causal))
 
 
 def _b8_full(t, shape, dtype, cache, what):
     """The data pointer of an optional tensor that has to be contiguous and of this shape and type."""
     if t is None:
         return None
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous() or t.device != cache.device:
+    if t.shape != shape or t.dtype != dtype or not t.is_contiguous() or t.get_device() != cache.index:
         raise DsparkError(f"{what} is a contiguous {dtype} tensor of shape {tuple(shape)} on the cache's device")
     return t.data_ptr()
+
+
+def _verify_attention_b8(s, cache, q, args, out, out_f32, workspace):
+    torch = _torch()
+    if out is None and out_f32 is None:
+        out = torch.empty(q.shape, dtype=torch.float16, device=q.device)
+    args.out = _b8_full(out, q.shape, torch.float16, cache, "out")
+    args.out_f32 = _b8_full(out_f32, q.shape, torch.float32, cache, "out_f32")
+    ref = ctypes.byref(args)
+    need = lib().dspark_verify_attention_b8_workspace(cache.ref, ref)
+    if need == 0:
+        raise DsparkError("dspark_verify_attention_b8_workspace rejected the arguments")
+    ws = (workspace or Workspace(q.device)).get(need)
+    args.workspace, args.workspace_bytes = ws.data_ptr(), ws.numel()
+    # The counters save a launch, which costs the host more than the last split's work the GPU; a graph's launch costs little,
+    # and zeroing counters for one call a launch itself.
+    if workspace is not None and not torch.cuda.is_current_stream_capturing():
+        args.arrivals = workspace.arrivals(cache.KVH * B8_ARRIVALS).data_ptr()
+    check(lib().dspark_verify_attention_b8(cache.ref, ref, s), "dspark_verify_attention_b8")
+    return out, out_f32
 
 
 def verify_attention_b8(q, cache, a, start=0, window=0, causal=True, out=None, out_f32=None, lse=None, gate=None, splits=0,
                         workspace=None, stream=None):
     """verify_attention over a B8Cache that holds positions 0..a+M-1. q fp16 [M][QH][D]; lse (optional) fp32 [M][QH] receives
-    the log-sum-exp of the scores. Returns (out fp16, out_f32) tensors as given/created."""
-    torch = _torch()
-    M, QH, D = q.shape
+    the log-sum-exp of the scores. A workspace that is kept saves a launch for few rows: it holds the counters by which the
+    last key split to finish adds them all. Returns (out fp16, out_f32) tensors as given/created."""
     args = _b8_attn_args(q, cache, a, start, window, causal)
-    with _on(cache.device, stream) as s:
-        if out is None and out_f32 is None:
-            out = torch.empty((M, QH, D), dtype=torch.float16, device=q.device)
-        args.out = _b8_full(out, (M, QH, D), torch.float16, cache, "out")
-        args.out_f32 = _b8_full(out_f32, (M, QH, D), torch.float32, cache, "out_f32")
-        args.lse = _b8_full(lse, (M, QH), torch.float32, cache, "lse")
-        args.gate = _b8_full(gate, (M, QH), torch.float32, cache, "gate")
-        args.splits = splits
-        ref = ctypes.byref(args)
-        need = lib().dspark_verify_attention_b8_workspace(cache.ref, ref)
-        if need == 0:
-            raise DsparkError("dspark_verify_attention_b8_workspace rejected the arguments")
-        ws = (workspace or Workspace(q.device)).get(need)
-        args.workspace, args.workspace_bytes = ws.data_ptr(), ws.numel()
-        check(lib().dspark_verify_attention_b8(cache.ref, ref, s), "dspark_verify_attention_b8")
-    return out, out_f32
+    f32 = _torch().float32
+    args.lse = _b8_full(lse, q.shape[:2], f32, cache, "lse")
+    args.gate = _b8_full(gate, q.shape[:2], f32, cache, "gate")
+    args.splits = splits
+    return _b8_on(cache, stream, _verify_attention_b8, q, args, out, out_f32, workspace)
+
+
+def _b8_accounts(t, n, cache, what):
+    """Elements between the heads of an fp32 [KVH][>= n] tensor."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or shape[0] != cache.KVH or shape[1] < n or t.dtype != _torch().float32 \
+            or (shape[1] > 1 and stride[1] != 1) or t.get_device() != cache.index:
+        raise DsparkError(f"{what} is fp32 [KVH][>= {n}] on the cache's device")
+    return stride[0] if shape[0] > 1 else max(stride[0], shape[1])
+
+
+def _attention_mass_b8(s, cache, args, lse, rows, mass_in, mass_out, stride):
+    check(lib().dspark_attention_mass_b8(cache.ref, ctypes.byref(args), lse, None if rows is None else rows.data_ptr(),
+                                         None if mass_in is None else mass_in.data_ptr(), mass_out.data_ptr(), stride, s),
+          "dspark_attention_mass_b8")
+    return mass_out
 
 
 def attention_mass_b8(q, cache, a, lse, mass_out, mass_in=None, rows=None, start=0, window=0, causal=True, stream=None):
     """Add the attention weights of tokens t < rows (an int32 device word, None = all of q's) to the accounts of the keys they
     see: mass_out fp32 [KVH][>= a+M] from mass_in (None = zeros, or mass_out itself) and verify_attention_b8's lse."""
     torch = _torch()
-    M, QH, D = q.shape
     args = _b8_attn_args(q, cache, a, start, window, causal)
-    lse_ptr = _b8_full(lse, (M, QH), torch.float32, cache, "lse")
-    stride = _b8_accounts(mass_out, a + M, cache, "mass_out")
-    if lse_ptr is None or (mass_in is not None and _b8_accounts(mass_in, a + M, cache, "mass_in") != stride):
+    lse_ptr = _b8_full(lse, q.shape[:2], torch.float32, cache, "lse")
+    stride = _b8_accounts(mass_out, a + args.M, cache, "mass_out")
+    if lse_ptr is None or (mass_in is not None and _b8_accounts(mass_in, a + args.M, cache, "mass_in") != stride):
         raise DsparkError("attention_mass_b8: lse is given, and mass_in and mass_out have one stride")
-    if rows is not None and (rows.dtype != torch.int32 or rows.numel() < 1 or rows.device != cache.device):
+    if rows is not None and (rows.dtype != torch.int32 or rows.numel() < 1 or rows.get_device() != cache.index):
         raise DsparkError("attention_mass_b8: rows is an int32 word on the cache's device")
-    with _on(cache.device, stream) as s:
-        check(lib().dspark_attention_mass_b8(cache.ref, ctypes.byref(args), lse_ptr,
-                                             None if rows is None else rows.data_ptr(),
-                                             None if mass_in is None else mass_in.data_ptr(), mass_out.data_ptr(), stride, s),
-              "dspark_attention_mass_b8")
-    return mass_out
+    return _b8_on(cache, stream, _attention_mass_b8, args, lse_ptr, rows, mass_in, mass_out, stride)
 
 
-def _b8_accounts(t, n, cache, what):
-    """Elements between the heads of an fp32 [KVH][>= n] tensor."""
-    if t.dim() != 2 or t.shape[0] != cache.KVH or t.shape[1] < n or t.dtype != _torch().float32 \
-            or (t.shape[1] > 1 and t.stride(1) != 1) or t.device != cache.device:
-        raise DsparkError(f"{what} is fp32 [KVH][>= {n}] on the cache's device")
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+def _kv_evict_b8(s, cache, dst, length, keep, mass, stride, sinks, recent, kept, mass_out, workspace):
+    torch = _torch()
+    if kept is None:
+        kept = torch.empty((cache.KVH, keep), dtype=torch.int32, device=cache.device)
+    if mass_out is None:
+        mass_out = torch.empty((cache.KVH, keep), dtype=torch.float32, device=cache.device)
+    kept_ptr = _b8_full(kept, (cache.KVH, keep), torch.int32, cache, "kept")
+    out_stride = _b8_accounts(mass_out, keep, cache, "mass_out")
+    need = lib().dspark_kv_evict_b8_workspace(cache.KVH, length)
+    ws = (workspace or Workspace(cache.device)).get(need) if need else None
+    check(lib().dspark_kv_evict_b8(cache.ref, dst.ref, length, keep, sinks, recent, mass.data_ptr(), stride, kept_ptr,
+                                   mass_out.data_ptr(), out_stride, None if ws is None else ws.data_ptr(),
+                                   0 if ws is None else ws.numel(), s), "dspark_kv_evict_b8")
+    return kept, mass_out
 
 
 def kv_evict_b8(cache, dst, length, keep, mass, sinks=0, recent=0, kept=None, mass_out=None, workspace=None, stream=None):
     """Keep `keep` of the cache's `length` positions per KV head -- the first `sinks`, the last `recent`, and the rest by mass
     (fp32 [KVH][>= length]) -- as positions 0..keep-1 of `dst`, another B8Cache of the same heads and codes. Returns
     (kept int32 [KVH][keep] ascending, their mass), as given/created."""
-    torch = _torch()
-    cache.check(length, mass, kept, mass_out, dst.k)
+    cache.check(length, dst.k)
     dst.check(keep)
     stride = _b8_accounts(mass, length, cache, "mass")
-    with _on(cache.device, stream) as s:
-        if kept is None:
-            kept = torch.empty((cache.KVH, keep), dtype=torch.int32, device=cache.device)
-        if mass_out is None:
-            mass_out = torch.empty((cache.KVH, keep), dtype=torch.float32, device=cache.device)
-        kept_ptr = _b8_full(kept, (cache.KVH, keep), torch.int32, cache, "kept")
-        out_stride = _b8_accounts(mass_out, keep, cache, "mass_out")
-        need = lib().dspark_kv_evict_b8_workspace(cache.KVH, length)
-        ws = (workspace or Workspace(cache.device)).get(need) if need else None
-        check(lib().dspark_kv_evict_b8(cache.ref, dst.ref, length, keep, sinks, recent, mass.data_ptr(), stride, kept_ptr,
-                                       mass_out.data_ptr(), out_stride, None if ws is None else ws.data_ptr(),
-                                       0 if ws is None else ws.numel(), s), "dspark_kv_evict_b8")
-    return kept, mass_out
+    return _b8_on(cache, stream, _kv_evict_b8, dst, length, keep, mass, stride, sinks, recent, kept, mass_out, workspace)
 
 
 # ---------------------------------------------------------------- argmax / accept

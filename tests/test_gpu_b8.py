@@ -174,14 +174,21 @@ def tops(c, n):
     return (np.where(pg[:, None] >= 0, c.scale["v"][pg], 0) * (127 if c.code == "int8" else 448))[..., None]
 
 
-def run_attention(c, q, a, gate=None, splits=0, **mask):
+KEPT = []  # one workspace (and its arrival counters) for every shape
+
+
+def run_attention(c, q, a, gate=None, splits=0, kept=False, **mask):
     h = load_host()
+    if kept and not KEPT:
+        KEPT.append(h.Workspace("cuda"))
     g = gpu_cache(c)
     M, QH, D = q.shape
     o16, o32 = torch.empty((M, QH, D), dtype=torch.float16, device="cuda"), torch.empty((M, QH, D), device="cuda")
     lse = torch.empty((M, QH), device="cuda")
     h.verify_attention_b8(dev(q), g, a, out=o16, out_f32=o32, lse=lse, gate=None if gate is None else dev(gate), splits=splits,
-                          **mask)
+                          workspace=KEPT[0] if kept else None, **mask)
+    if kept:
+        assert not KEPT[0].words.any()
     return o16.cpu().numpy().astype(np.float64), o32.cpu().numpy().astype(np.float64), lse.cpu().numpy().astype(np.float64)
 
 
@@ -190,14 +197,18 @@ def check_attention(c, q, a, gate=None, splits=0, start=0, window=0, causal=True
     k, v, here = c.read(0, a + M)
     see = b8.visible(M, a, start, window, causal, here)
     o, lse, mag = b8.attention(q, k, v, see, gate)
-    o16, o32, l = run_attention(c, q, a, gate, splits, start=start, window=window, causal=causal)
     B = b8.attention(q, k, np.broadcast_to(tops(c, a + M), v.shape), see, gate)[2]
-    assert np.all(np.abs(o32 - o) <= bound(o, mag, False, a + M, B)), np.max(np.abs(o32 - o) - bound(o, mag, False, a + M, B))
-    assert np.all(np.abs(o16 - o) <= bound(o, mag, True, a + M, B))
     dead = np.isneginf(lse)
-    assert np.array_equal(np.isneginf(l), dead) and not o32[dead].any() and not o16[dead].any()
-    # a score is off by 2^-18 at most, the logarithm of the sum by a few 2^-24 of its size
-    assert np.all(np.abs(l[~dead] - lse[~dead]) <= 2.0 ** -17 + 2.0 ** -21 * np.abs(lse[~dead]))
+    for kept in (False, True):
+        o16, o32, l = run_attention(c, q, a, gate, splits, kept, start=start, window=window, causal=causal)
+        assert np.all(np.abs(o32 - o) <= bound(o, mag, False, a + M, B)), np.max(np.abs(o32 - o) - bound(o, mag, False, a + M, B))
+        assert np.all(np.abs(o16 - o) <= bound(o, mag, True, a + M, B))
+        assert np.array_equal(np.isneginf(l), dead) and not o32[dead].any() and not o16[dead].any()
+        # a score is off by 2^-18 at most, the logarithm of the sum by a few 2^-24 of its size
+        assert np.all(np.abs(l[~dead] - lse[~dead]) <= 2.0 ** -17 + 2.0 ** -21 * np.abs(lse[~dead]))
+        if kept:  # whoever adds the splits, the bits are the same
+            assert np.array_equal(o32, first[0]) and np.array_equal(l, first[1])
+        first = o32, l
     return lse
 
 
