@@ -22,9 +22,6 @@ namespace dspark {
 // Waves of a workgroup, which fills a CU: as many as the registers of RB row blocks leave (o alone takes D RB / 4).
 constexpr int b8_waves(int D, int RB) { return D == 64 ? (RB == 1 ? 16 : RB <= 3 ? 12 : 8) : RB == 1 ? 12 : 8; }
 constexpr int MASS_WAVES = 4;
-#ifndef B8_SHORT
-#define B8_SHORT 4
-#endif
 constexpr int B8_COHERENT = 16;    // buffer cache policy SC1: device-scope coherent store / load
 constexpr int B8_FUSED_BYTES = 64 << 10;  // sums of one row block's splits that the last of them adds (b8_attn_plan)
 // Running reference in log2 units, set to the row's largest x + log2 vs less 8 when one passes ref + 15: P stays under 2^15,
@@ -603,19 +600,23 @@ void b8_attn_plan(B8Attn& p, int D, int splits, int cus) {
   const int blocks = (p.R + 15) / 16, most = D == 64 ? B8_ROW_BLOCKS : 2;
   p.RG = (blocks + most - 1) / most;
   p.rb = (blocks + p.RG - 1) / p.RG;
-  // Few pages: a row block a workgroup and no splits, while that leaves a wave few of them (SHORT).
-  if (splits == 0 && p.npages <= B8_SHORT * b8_waves(D, 1) && p.c.KVH * blocks <= cus) {
+  // Few pages: a row block a workgroup, and splits of a page a wave as far as there are CUs -- at D = 64 up to four pages a wave
+  // (16 tokens, 32/8/64 heads: 1000 keys 9.8 -> 8.0 us, 4000 10.3 -> 8.9, 8000 11.5 -> 10.4, 16000 13.1 -> 12.7), at
+  // D = 128 to one (8 tokens, 16/4/128: 250 keys 10.5 -> 7.0, 1001 10.7 -> 10.9 but without a second launch, 16000 13.1 -> 14.2
+  // with two).
+  const int w1 = b8_waves(D, 1), most1 = cus / (p.c.KVH * blocks);
+  if (splits == 0 && most1 > 0 && p.npages <= (D == 64 ? 4 : 1) * w1 * most1) {
     p.rb = 1;
     p.RG = blocks;
-    splits = 1;
+    splits = std::min(most1, (p.npages + w1 - 1) / w1);
   }
   const int waves = b8_waves(D, p.rb);
   int S = splits > 0 ? splits : std::max(1, cus / (p.c.KVH * p.RG));
   S = std::max(1, std::min(std::min(S, 4096), (p.npages + waves - 1) / waves));
   p.S = S;
-  // The last split to arrive adds the others (if the caller has counters) where they are little to read for one workgroup:
-  // one token of 32768 keys 12.3 us against 11.7 with a second launch, which costs its caller 4 more; 36 rows of 131063
-  // keys, 64 KB at D = 128 and four splits ... 46 against 38.
+  // The last split to arrive adds the others (if the caller has counters) where they are little to read for one workgroup: a
+  // token of 32768 keys takes 12.8 us instead of 11.9 with a second launch, whose caller spends 4 more on it; 32 rows of
+  // 131063 keys in one workgroup 46 against 38.
   if (S == 1 || p.rb > 1 || std::min(p.R, 16) * S * D * (int)sizeof(float) > B8_FUSED_BYTES) p.arrivals = nullptr;
   p.pps = p.npages / (S * waves);
   p.more = p.npages % (S * waves);
