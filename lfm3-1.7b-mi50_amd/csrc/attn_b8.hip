@@ -210,7 +210,9 @@ __device__ __forceinline__ void b8_page(const B8Attn& p, const B8Tile<D>& t, con
   f32x4 s[RB][2];
   b8_scores<D, RB, FP8>(t.k, q, s);
   if (lp < p.full_lo || lp >= p.full_hi) {
-    b8_mask<RB>(p, ks, lp < 0 ? NOWHERE : lp * PAGE, tok, lane, s);
+    int pos = lp < 0 ? NOWHERE : lp * PAGE;
+    asm volatile("" : "+s"(pos));  // (keeps the comparisons in this branch: they were made for every page)
+    b8_mask<RB>(p, ks, pos, tok, lane, s);
     ks = 1.f;
   }
   float top[RB], at[RB];
@@ -498,7 +500,7 @@ __global__ __launch_bounds__(256) void attn_b8_merge_kernel(B8Attn p) {
 // up in place over all row blocks, and only the four lanes of a key are added across (sums over the rows' lanes instead, with
 // A = K: eight row reductions a page, 39 -> 25 us at 128k keys and 64 rows a head).
 template <int D, int RB, bool FP8>
-__global__ __launch_bounds__(64 * MASS_WAVES) void mass_b8_kernel(B8Attn p) {
+__global__ __launch_bounds__(64 * MASS_WAVES, 2) void mass_b8_kernel(B8Attn p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   const int h = blockIdx.y;
   const int rows = p.rows ? min(max(ldc(p.rows), 0), p.M) : p.M;
@@ -542,36 +544,51 @@ __global__ __launch_bounds__(64 * MASS_WAVES) void mass_b8_kernel(B8Attn p) {
         float acc[2] = {0.f, 0.f};
         if (__builtin_amdgcn_readlane(pgl, i) >= 0 && lp >= p.seen_lo && R > 0) {
           const float ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ksl), i));
-          const bool edge = lp < p.full_lo || lp >= p.full_hi;
+          f32x4 x[RB][2];
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
             half8 kf[D / 32];
             b8_k_operand<D, FP8>(now[b], kf);
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
-              f32x4 s = {0, 0, 0, 0}, x;
+              f32x4 s = {0, 0, 0, 0};
 #pragma unroll
               for (int e = 0; e < D / 32; ++e) s = mfma16x16x32(q[rb][e], kf[e], s);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) x[i] = fmaf(s[i], ks, l2[rb][i]);
-              if (edge) {
-                const int kp = lp * PAGE + 16 * b + n;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const B8Sight sight = b8_sight(p, div_by(min(row0 + 16 * rb + 4 * g + i, p.R - 1), p.g_div));
-                  x[i] = sight.sees(kp) ? x[i] : -INFINITY;
-                }
-              }
-#pragma unroll
-              for (int i = 0; i < 4; ++i) acc[b] += fast_exp2(x[i]);
+              for (int i = 0; i < 4; ++i) x[rb][b][i] = fmaf(s[i], ks, l2[rb][i]);
             }
+          }
+          if (lp < p.full_lo || lp >= p.full_hi) {
+            int pos = lp * PAGE;
+            asm volatile("" : "+s"(pos));  // (keeps the comparisons in this branch: they were made for every page)
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const B8Sight sight = b8_sight(p, div_by(min(row0 + 16 * rb + 4 * g + i, p.R - 1), p.g_div));
+#pragma unroll
+                for (int b = 0; b < 2; ++b) x[rb][b][i] = sight.sees(pos + 16 * b + n) ? x[rb][b][i] : -INFINITY;
+              }
+          }
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            f32x4 sum = {0, 0, 0, 0};
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) sum[i] += fast_exp2(x[rb][b][i]);
+            acc[b] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
           }
         }
         const float v0 = row_sum(acc[0]), v1 = row_sum(acc[1]);  // (the exchanges take every lane: no branch around them)
         const int kp = lp * PAGE + 16 * (g & 1) + n;
         if (g < 2 && kp < live) out[kp] = was + (g ? v1 : v0);
       };
+      __builtin_amdgcn_s_setprio(3);  // (as in the attention: who is further on yields)
       for (int i = 0; i < nb; i += 2) {
+        if (4 * i >= nb) __builtin_amdgcn_s_setprio(2);
+        if (2 * i >= nb) __builtin_amdgcn_s_setprio(1);
+        if (4 * i >= 3 * nb) __builtin_amdgcn_s_setprio(0);
         step(i, k[0], old[0], k[1], old[1]);
         if (i + 1 < nb) step(i + 1, k[1], old[1], k[0], old[0]);
       }
@@ -674,7 +691,9 @@ int b8_mass_launch(const B8Attn& q, int D, bool fp8, int cus, hipStream_t s) {
   p.seen_lo = p.page0;
   p.page0 = 0;  // every account is carried over, those of keys out of sight too
   p.npages = (p.a + p.M - 1) / PAGE + 1;
-  p.pps = std::max(1, (int)((int64_t)p.npages * p.c.KVH / (8 * cus)));
+  // as many pages a wave as let every workgroup start at once (a few over: 27.8 us instead of MASSNEW)
+  const int64_t waves = (int64_t)cus * (p.rb > 2 ? 12 : 16);
+  p.pps = (int)std::max<int64_t>(1, ((int64_t)p.npages * p.c.KVH + waves - 1) / waves);
   const dim3 grid((p.npages + p.pps * MASS_WAVES - 1) / (p.pps * MASS_WAVES), p.c.KVH);
   if (D == 64) fp8 ? mass_b8_by_rows<64, true>(p, grid, s) : mass_b8_by_rows<64, false>(p, grid, s);
   else fp8 ? mass_b8_by_rows<128, true>(p, grid, s) : mass_b8_by_rows<128, false>(p, grid, s);

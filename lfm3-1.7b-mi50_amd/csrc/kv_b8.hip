@@ -152,43 +152,72 @@ __device__ __forceinline__ void sel_edges(const B8Evict& p, int32_t* kept, int f
   for (int i = first; i < p.recent; i += step) kept[p.keep - p.recent + i] = p.T - p.recent + i;
 }
 
-// The kept ones of a wave's 64 NPL keys (u[j] of position i0 + 64 j + lane): those above the threshold and the first `need`
-// equal ones of the head, `used` of which lie before; stored from place `at` on.
+// A wave's 64 NPL keys: u[4 j + e] of position i0 + 256 j + 4 lane + e, so that a lane's four are one load and places come from
+// one scan over the lanes for 256 positions.
 template <int NPL>
-__device__ __forceinline__ void sel_emit(const uint32_t (&u)[NPL], int i0, int N, uint32_t thr, uint32_t need, uint32_t used,
-                                         uint32_t at, int sinks, int32_t* kept) {
-  const int lane = threadIdx.x & 63;
-  const uint64_t below = (1ull << lane) - 1;
+__device__ __forceinline__ void sel_load(const float* mass, int i0, int N, uint32_t (&u)[NPL]) {
+  typedef __attribute__((address_space(1))) const f32x4 __attribute__((aligned(4))) GV;  // the accounts' rows start at any word
+  f32x4 v[NPL / 4];
 #pragma unroll
-  for (int j = 0; j < NPL; ++j) {
-    const int i = i0 + 64 * j + lane;
-    const uint64_t be = __ballot(i < N && u[j] == thr);
-    const bool take = i < N && (u[j] > thr || (u[j] == thr && used + __popcll(be & below) < need));
-    const uint64_t bt = __ballot(take);
-    if (take) kept[at + __popcll(bt & below)] = sinks + i;
-    at += __popcll(bt);
-    used = min(need, used + (uint32_t)__popcll(be));
+  for (int j = 0; j < NPL / 4; ++j) {
+    const int i = i0 + 256 * j + 4 * (threadIdx.x & 63);
+    if (i + 4 <= N) {
+      v[j] = *(GV*)(mass + i);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[j][e] = i + e < N ? ldg(mass + i + e) : 0.f;
+    }
   }
+#pragma unroll
+  for (int k = 0; k < NPL; ++k) u[k] = mass_key(v[k / 4][k % 4]);
+}
+__device__ __forceinline__ int sel_pos(int i0, int k) { return i0 + 256 * (k / 4) + 4 * (int)(threadIdx.x & 63) + k % 4; }
+// A lane's keys above the threshold (low half) and equal to it (high half) among its four of group j.
+template <int NPL>
+__device__ __forceinline__ uint32_t sel_mark(const uint32_t (&u)[NPL], int j, int i0, int N, uint32_t thr) {
+  uint32_t c = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t x = u[4 * j + e];
+    c += sel_pos(i0, 4 * j + e) < N ? (x > thr ? 1u : 0u) + (x == thr ? 0x10000u : 0u) : 0u;
+  }
+  return c;
 }
 template <int NPL>
-__device__ __forceinline__ void sel_count(const uint32_t (&u)[NPL], int i0, int N, uint32_t thr, uint32_t& gt, uint32_t& eq) {
-  const int lane = threadIdx.x & 63;
+__device__ __forceinline__ uint32_t sel_count(const uint32_t (&u)[NPL], int i0, int N, uint32_t thr) {
+  uint32_t c = 0;
 #pragma unroll
-  for (int j = 0; j < NPL; ++j) {
-    const bool in = i0 + 64 * j + lane < N;
-    gt += __popcll(__ballot(in && u[j] > thr));
-    eq += __popcll(__ballot(in && u[j] == thr));
+  for (int j = 0; j < NPL / 4; ++j) c += sel_mark<NPL>(u, j, i0, N, thr);
+  return wave_total(c);
+}
+// Stores the kept ones: a key above the threshold, or one of the first `need` equal to it, goes to place
+// sinks + (keys above before it) + min(need, equal ones before it); gt, eq: those before the wave's first.
+template <int NPL>
+__device__ __forceinline__ void sel_emit(const uint32_t (&u)[NPL], int i0, int N, uint32_t thr, uint32_t need, uint32_t gt, uint32_t eq,
+                                         int sinks, int32_t* kept) {
+#pragma unroll
+  for (int j = 0; j < NPL / 4; ++j) {
+    if (i0 + 256 * j >= N) break;
+    const uint32_t c = sel_mark<NPL>(u, j, i0, N, thr), upto = wave_scan(c);
+    uint32_t g = gt + ((upto - c) & 0xffffu), q = eq + ((upto - c) >> 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = sel_pos(i0, 4 * j + e);
+      const bool above = i < N && u[4 * j + e] > thr, same = i < N && u[4 * j + e] == thr;
+      if (above || (same && q < need)) kept[sinks + g + min(q, need)] = sinks + i;
+      g += above;
+      q += same;
+    }
+    const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+    gt += all & 0xffffu;
+    eq += all >> 16;
   }
 }
-// Places of a wave's first kept key from the waves' counts (wc: above and equal, complete and visible), behind `at0` kept ones
-// and `eq0` equal ones.
-__device__ __forceinline__ void sel_places(const uint32_t (*wc)[2], int wave, uint32_t need, uint32_t eq0, uint32_t& at, uint32_t& used) {
-  used = min(need, eq0);
-  for (int w = 0; w < wave; ++w) {
-    const uint32_t e = min(wc[w][1], need - used);
-    at += wc[w][0] + e;
-    used += e;
-  }
+// The counts of the waves before this one (wc: every wave's, complete and visible), and of all of them.
+__device__ __forceinline__ uint32_t sel_before(const uint32_t* wc, int wave, uint32_t& all) {
+  const uint32_t upto = row_scan(wc[threadIdx.x % SEL_W]);
+  all = (uint32_t)__builtin_amdgcn_readlane((int)upto, SEL_W - 1);
+  return wave ? (uint32_t)__builtin_amdgcn_readlane((int)upto, max(wave - 1, 0)) : 0u;
 }
 
 // One workgroup per KV head finds the keep - sinks - recent largest accounts of up to 1024 NPL middle positions, held in
@@ -197,20 +226,16 @@ template <int NPL>
 __global__ __launch_bounds__(SEL_T) void evict_select_kernel(B8Evict p) {
   __shared__ SelLds s;
   __shared__ __align__(16) uint32_t hist[SEL_BINS];
-  __shared__ uint32_t wc[SEL_W][2];
+  __shared__ uint32_t wc[SEL_W];
   const int h = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const float* mass = p.mass + (size_t)h * p.mass_stride + p.sinks;
   int32_t* kept = p.kept + (size_t)h * p.keep;
   const int N = p.T - p.sinks - p.recent, k = p.keep - p.sinks - p.recent;
-  const int i0 = wave * 64 * NPL;
-  float v[NPL];
-#pragma unroll
-  for (int j = 0; j < NPL; ++j) v[j] = N > 0 ? ldg(mass + min(i0 + 64 * j + lane, N - 1)) : 0.f;
+  const int per = (N + 256 * SEL_W - 1) / (256 * SEL_W) * 256, i0 = wave * per, hi = min(N, i0 + per);  // whole groups a wave
+  uint32_t u[NPL];
+  sel_load<NPL>(mass, i0, hi, u);
   sel_edges(p, kept, tid, SEL_T);
   if (k <= 0) return;
-  uint32_t u[NPL];
-#pragma unroll
-  for (int j = 0; j < NPL; ++j) u[j] = mass_key(v[j]);
   uint32_t thr = 0, mask = 0, need = (uint32_t)k;
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
@@ -219,7 +244,7 @@ __global__ __launch_bounds__(SEL_T) void evict_select_kernel(B8Evict p) {
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < NPL; ++j)
-      if (i0 + 64 * j + lane < N && (u[j] & mask) == thr) atomicAdd(&hist[(u[j] >> shift) & (bins - 1)], 1u);
+      if (sel_pos(i0, j) < hi && (u[j] & mask) == thr) atomicAdd(&hist[(u[j] >> shift) & (bins - 1)], 1u);
     __syncthreads();
     const u32x2 n = 2 * tid < bins ? *reinterpret_cast<const u32x2*>(&hist[bins - 2 - 2 * tid]) : u32x2{0, 0};
     uint32_t bin, above;
@@ -228,15 +253,12 @@ __global__ __launch_bounds__(SEL_T) void evict_select_kernel(B8Evict p) {
     mask |= (uint32_t)(bins - 1) << shift;
     need -= above;
   }
-  uint32_t gt = 0, eq = 0, at = p.sinks, used = 0;
-  sel_count<NPL>(u, i0, N, thr, gt, eq);
-  if (lane == 0) {
-    wc[wave][0] = gt;
-    wc[wave][1] = eq;
-  }
+  const uint32_t c = sel_count<NPL>(u, i0, hi, thr);
+  if (lane == 0) wc[wave] = c;
   __syncthreads();
-  sel_places(wc, wave, need, 0, at, used);
-  sel_emit<NPL>(u, i0, N, thr, need, used, at, p.sinks, kept);
+  uint32_t all;
+  const uint32_t before = sel_before(wc, wave, all);  // (up to 16384 of each: the halves do not meet)
+  sel_emit<NPL>(u, i0, hi, thr, need, before & 0xffffu, before >> 16, p.sinks, kept);
 }
 
 // More positions: `parts` workgroups a head, each a contiguous range of them (whole tiles of 8192), and a launch for each
@@ -253,7 +275,7 @@ template <int PASS>
 __global__ __launch_bounds__(SEL_T) void evict_pass_kernel(B8Evict p, SelHead* ws, int parts, int per) {
   __shared__ SelLds s;
   __shared__ __align__(16) uint32_t hist[SEL_BINS];
-  __shared__ uint32_t wc[SEL_W][2];
+  __shared__ uint32_t wc[SEL_W];
   __shared__ uint32_t red[2];
   const int h = blockIdx.y, part = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   SelHead& w = ws[h];
@@ -261,15 +283,9 @@ __global__ __launch_bounds__(SEL_T) void evict_pass_kernel(B8Evict p, SelHead* w
   int32_t* kept = p.kept + (size_t)h * p.keep;
   const int N = p.T - p.sinks - p.recent;
   const int lo = part * per, hi = min(N, lo + per);
-  auto load = [&](int t0, uint32_t (&u)[SEL_NPL]) {
-    float v[SEL_NPL];
-#pragma unroll
-    for (int j = 0; j < SEL_NPL; ++j) v[j] = ldg(mass + min(t0 + wave * 64 * SEL_NPL + 64 * j + lane, N - 1));
-#pragma unroll
-    for (int j = 0; j < SEL_NPL; ++j) u[j] = mass_key(v[j]);
-  };
   uint32_t u[SEL_NPL];
-  load(min(lo, N - 1), u);  // the first tile's keys, in flight while the digit is found
+  const int w0 = wave * 64 * SEL_NPL;
+  sel_load<SEL_NPL>(mass, lo + w0, N, u);  // the first tile's keys, in flight while the digit is found
   uint32_t thr = 0, mask = 0, need = (uint32_t)(p.keep - p.sinks - p.recent);
   uint32_t gt = 0, eq = 0;  // PASS 3: kept and equal keys in the parts before
   if constexpr (PASS > 0) {  // the digit of the launch before
@@ -324,33 +340,25 @@ __global__ __launch_bounds__(SEL_T) void evict_pass_kernel(B8Evict p, SelHead* w
     for (int i = tid; i < bins; i += SEL_T) hist[i] = 0;
     __syncthreads();
     for (int t0 = lo; t0 < hi; t0 += SEL_TILE) {
-      if (t0 > lo) load(t0, u);
+      if (t0 > lo) sel_load<SEL_NPL>(mass, t0 + w0, N, u);
 #pragma unroll
       for (int j = 0; j < SEL_NPL; ++j)
-        if (t0 + wave * 64 * SEL_NPL + 64 * j + lane < hi && (u[j] & mask) == thr) atomicAdd(&hist[(u[j] >> shift) & (bins - 1)], 1u);
+        if (sel_pos(t0 + w0, j) < hi && (u[j] & mask) == thr) atomicAdd(&hist[(u[j] >> shift) & (bins - 1)], 1u);
     }
     __syncthreads();
     for (int i = tid; i < bins; i += SEL_T) w.hist[PASS][part][i] = hist[i];
   } else {
     if (part == 0) sel_edges(p, kept, tid, SEL_T);
-    uint32_t eq0 = eq, at0 = p.sinks + gt + min(need, eq);
     for (int t0 = lo; t0 < hi; t0 += SEL_TILE) {
-      if (t0 > lo) load(t0, u);
-      const int i0 = t0 + wave * 64 * SEL_NPL;
-      uint32_t g = 0, e = 0, at = at0, used;
-      sel_count<SEL_NPL>(u, i0, hi, thr, g, e);
-      if (lane == 0) {
-        wc[wave][0] = g;
-        wc[wave][1] = e;
-      }
+      if (t0 > lo) sel_load<SEL_NPL>(mass, t0 + w0, N, u);
+      const uint32_t c = sel_count<SEL_NPL>(u, t0 + w0, hi, thr);
+      if (lane == 0) wc[wave] = c;
       __syncthreads();
-      sel_places(wc, wave, need, eq0, at, used);
-      sel_emit<SEL_NPL>(u, i0, hi, thr, need, used, at, p.sinks, kept);
-      for (int x = 0; x < SEL_W; ++x) {  // on to the next tile
-        const uint32_t more = min(wc[x][1], need - min(need, eq0));
-        at0 += wc[x][0] + more;
-        eq0 += wc[x][1];
-      }
+      uint32_t all;
+      const uint32_t before = sel_before(wc, wave, all);
+      sel_emit<SEL_NPL>(u, t0 + w0, hi, thr, need, gt + (before & 0xffffu), eq + (before >> 16), p.sinks, kept);
+      gt += all & 0xffffu;  // on to the next tile
+      eq += all >> 16;
       __syncthreads();
     }
   }
