@@ -55,13 +55,15 @@ __device__ __forceinline__ uint32_t b8_code_i8(float x, float s, float inv) {
   return (uint32_t)(int)t;
 }
 
-// Four values as four codes (one word, the first in the low byte). x inv is exact for e4m3 (inv a power of two).
-template <bool FP8>
+// Four values as four codes (one word, the first in the low byte). ANY: values may be infinite or no numbers; without it they
+// are finite and the block's scale covers them.
+template <bool FP8, bool ANY>
 __device__ __forceinline__ uint32_t b8_code4(float x0, float x1, float x2, float x3, float s, float inv) {
-  if constexpr (FP8) {
+  if constexpr (FP8) {  // x inv is exact: inv is a power of two
     auto y = [&](float x) {
       const float z = x * inv;
-      return z != z ? 0.f : fminf(fmaxf(z, -448.f), 448.f);
+      if constexpr (ANY) return z != z ? 0.f : fminf(fmaxf(z, -448.f), 448.f);
+      else return z;
     };
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(y(x0), y(x1), 0, false);
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y(x2), y(x3), w, true);
@@ -102,7 +104,7 @@ __device__ __forceinline__ f32x4 b8_value4(uint32_t w) {
 template <bool FP8>
 __device__ __forceinline__ uint32_t b8_recode4(uint32_t w, float from, float to, float inv_to) {
   const f32x4 x = b8_value4<FP8>(w) * from;
-  return b8_code4<FP8>(x[0], x[1], x[2], x[3], to, inv_to);
+  return b8_code4<FP8, false>(x[0], x[1], x[2], x[3], to, inv_to);
 }
 
 struct B8Write {

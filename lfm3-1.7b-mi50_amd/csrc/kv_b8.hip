@@ -38,18 +38,35 @@ __global__ __launch_bounds__(64 * WPB) void kv_write_b8_kernel(B8Write p, int nw
   }
   const bool entered = base < 0;  // the page holds earlier rows
   const float was = entered ? ldg(scale) : 0.f;
-  uint32_t top = 0;  // largest finite magnitude: for non-negative halves the order of the patterns is that of the values
+  // Largest magnitude: for non-negative halves the order of the patterns is that of the values, so two are compared by one
+  // packed maximum. Patterns from 0x7c00 on are infinities and NaN: only if there is one are the finite values picked out.
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  u16x2 most = {0, 0};
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
     const int row = base + r + RPI * i;
-    if (row >= 0 && row < p.n)
+    u32x4 w;
+    __builtin_memcpy(&w, &x[i], 16);
+    if (row < 0 || row >= p.n) w = u32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t b = __builtin_bit_cast(uint16_t, (_Float16)x[i][j]) & 0x7fffu;
-        top = max(top, b < 0x7c00u ? b : 0u);
-      }
+    for (int j = 0; j < 4; ++j) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, w[j] & 0x7fff7fffu));
   }
-  top = wave_max_u32(top);
+  uint32_t top = wave_max_u32(max((uint32_t)most[0], (uint32_t)most[1]));
+  const bool any = top >= 0x7c00u;
+  if (any) {
+    top = 0;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int row = base + r + RPI * i;
+      if (row >= 0 && row < p.n)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t b = __builtin_bit_cast(uint16_t, (_Float16)x[i][j]) & 0x7fffu;
+          top = max(top, b < 0x7c00u ? b : 0u);
+        }
+    }
+    top = wave_max_u32(top);
+  }
   const float s = fmaxf(was, b8_scale<FP8>((float)__builtin_bit_cast(_Float16, (uint16_t)top)));
   const float inv = b8_inv(s);
   if (lane == 0) *scale = s;
@@ -60,8 +77,13 @@ __global__ __launch_bounds__(64 * WPB) void kv_write_b8_kernel(B8Write p, int nw
     u32x2 y;
     if (row >= 0) {
       const half8 v = x[i];
-      y[0] = b8_code4<FP8>((float)v[0], (float)v[1], (float)v[2], (float)v[3], s, inv);
-      y[1] = b8_code4<FP8>((float)v[4], (float)v[5], (float)v[6], (float)v[7], s, inv);
+      if (any) {
+        y[0] = b8_code4<FP8, true>((float)v[0], (float)v[1], (float)v[2], (float)v[3], s, inv);
+        y[1] = b8_code4<FP8, true>((float)v[4], (float)v[5], (float)v[6], (float)v[7], s, inv);
+      } else {
+        y[0] = b8_code4<FP8, false>((float)v[0], (float)v[1], (float)v[2], (float)v[3], s, inv);
+        y[1] = b8_code4<FP8, false>((float)v[4], (float)v[5], (float)v[6], (float)v[7], s, inv);
+      }
       if (row >= p.n) y = u32x2{0, 0};
       *at = y;
     } else if (s != was) {
