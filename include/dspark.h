@@ -186,8 +186,8 @@ int dspark_kv_read_b8(const dspark_b8_cache* cache, int32_t pos0, int32_t n, flo
  * and/or fp32 [M][QH][D] on 16-byte boundaries. lse, if given: fp32 [M][QH], the natural logarithm of the sum of
  * exp(q k / sqrt(D)) over the keys a row sees (before the gate). A row that sees no key (every page of it absent) gives
  * zeros and lse -inf. M QH / KVH <= 1024. The workspace needs no clearing and may be shared by stream-ordered calls. The
- * probabilities are rounded to fp16 once; scores, sums and outputs are fp32. */
-#define DSPARK_B8_ARRIVALS 32
+ * probabilities are rounded to fp16 once; scores, sums and outputs are fp32. Outputs must not overlap q (DSPARK_EINVAL). */
+#define DSPARK_B8_ARRIVALS 64 /* row groups of a KV head at most: 1024 rows by 16 */
 typedef struct dspark_b8_attn_args {
   const void* q;
   int64_t q_stride;            /* elements between tokens, >= QH D */
@@ -226,7 +226,8 @@ int dspark_attention_mass_b8(const dspark_b8_cache* cache, const dspark_b8_attn_
  * cache of `keep` positions for every head (keys keep the rotation they were written with; later calls count positions
  * from keep). A dst block's scale is the largest of its rows' scales; rows from blocks of a smaller one are re-coded to it
  * (rounded once more). The slots behind keep in the last page are cleared. mass_out[h][j] = mass[h][kept[h][j]]. dst has
- * src's KVH, D and code; its pools, kept and mass_out must share no byte with what is read (DSPARK_EINVAL). sinks + recent
+ * src's KVH, D and code; its pools, kept, mass_out and the workspace must share no byte with what is read, nor with one
+ * another (DSPARK_EINVAL). sinks + recent
  * <= keep <= length <= 2^30. keep = 0 does nothing. The workspace (a size of 0: none is needed) needs no clearing. */
 int dspark_kv_evict_b8(const dspark_b8_cache* src, const dspark_b8_cache* dst, int32_t length, int32_t keep, int32_t sinks,
                        int32_t recent, const float* mass, int64_t mass_stride, int32_t* kept, float* mass_out,

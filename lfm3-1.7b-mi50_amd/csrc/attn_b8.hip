@@ -369,9 +369,10 @@ __global__ __launch_bounds__(64 * b8_waves(D, RB), b8_waves(D, RB) / 4) void att
     // log2 vs, and 1 / vs as its very inverse. A block of zeros (scale 0) takes the smallest scale about: any will do for its
     // sum, and the smallest moves no reference.
     float lvl = __builtin_amdgcn_logf(vsl);
-    if (__ballot(!(vsl > 0.f))) {
-      const float low = -wave_max(vsl > 0.f ? -lvl : -INFINITY);
-      if (!(vsl > 0.f)) lvl = low < INFINITY ? low : 0.f;
+    const bool none = !(vsl > 1e-30f);  // (no scale of a block that holds anything is as small)
+    if (__ballot(none)) {
+      const float low = -wave_max(none ? -INFINITY : -lvl);
+      if (none) lvl = low < INFINITY ? low : 0.f;
     }
     const float ivl = fast_exp2(-lvl);
     // the next page's loads are in flight while a page is worked on (past the last one: that page again, from L2)

@@ -144,6 +144,9 @@ int dspark_verify_attention_b8(const dspark_b8_cache* c, const dspark_b8_attn_ar
   if (!rows_ok(c, a) || !query_ok(c, a)) return DSPARK_EINVAL;
   if (!a->out && !a->out_f32) return DSPARK_EINVAL;
   if (a->arrivals && !on(a->arrivals, 4)) return DSPARK_EINVAL;
+  // every workgroup reads its rows of q by itself, also after others have stored theirs
+  const size_t n = (size_t)a->M * a->QH * c->D, qn = ((size_t)(a->M - 1) * a->q_stride + (size_t)a->QH * c->D) * 2;
+  if ((a->out && overlap(a->out, 2 * n, a->q, qn)) || (a->out_f32 && overlap(a->out_f32, 4 * n, a->q, qn))) return DSPARK_EINVAL;
   if ((a->out && !on(a->out, 16)) || (a->out_f32 && !on(a->out_f32, 16))) return DSPARK_EINVAL;
   B8Attn p = attn(c, a);
   b8_attn_plan(p, c->D, a->splits, device_cus());
@@ -184,9 +187,10 @@ int dspark_kv_evict_b8(const dspark_b8_cache* src, const dspark_b8_cache* dst, i
   // the rows move between pools that share nothing: a destination page may be written while other rows are still read
   const size_t from[2] = {(size_t)src->kv_pages * src->KVH, (size_t)src->kv_pages * src->KVH * DSPARK_PAGE_TOKENS * src->D};
   const size_t to[2] = {(size_t)dst->kv_pages * dst->KVH, (size_t)dst->kv_pages * dst->KVH * DSPARK_PAGE_TOKENS * dst->D};
-  const struct { const void* p; size_t n; } reads[6] = {
+  const struct { const void* p; size_t n; } reads[7] = {
       {src->k, from[1]}, {src->v, from[1]}, {src->k_scale, from[0] * 4}, {src->v_scale, from[0] * 4},
-      {mass, ((size_t)(src->KVH - 1) * mass_stride + length) * 4}, {src->block_table, src->block_table ? (size_t)pages_of(length) * 4 : 0}};
+      {mass, ((size_t)(src->KVH - 1) * mass_stride + length) * 4}, {src->block_table, src->block_table ? (size_t)pages_of(length) * 4 : 0},
+      {dst->block_table, dst->block_table ? (size_t)pages_of(keep) * 4 : 0}};
   const size_t need = b8_evict_workspace(src->KVH, length);
   if (need && (!on(workspace, 16) || workspace_bytes < need)) return DSPARK_ENOSPACE;
   const struct { const void* p; size_t n; } writes[7] = {
@@ -195,6 +199,9 @@ int dspark_kv_evict_b8(const dspark_b8_cache* src, const dspark_b8_cache* dst, i
   for (const auto& r : reads)
     for (const auto& w : writes)
       if (r.n && w.n && overlap(r.p, r.n, w.p, w.n)) return DSPARK_EINVAL;
+  for (const auto& v : writes)
+    for (const auto& w : writes)
+      if (&v < &w && v.n && w.n && overlap(v.p, v.n, w.p, w.n)) return DSPARK_EINVAL;
   B8Evict p;
   p.src = pool(src);
   p.dst = pool(dst);

@@ -334,7 +334,7 @@ def verify_attention_rec(q, pages, a, start=0, window=0, causal=True, out=None, 
 
 # ---------------------------------------------------------------- 8-bit block-scaled K/V cache
 B8_INT8, B8_E4M3 = 0, 1
-B8_ARRIVALS = 32
+B8_ARRIVALS = 64
 
 
 class B8Cache:
@@ -383,8 +383,10 @@ def _b8_on(cache, stream, call, *args):
     """call(handle of the stream, cache, *args) with the cache's device current and `stream` (default: that device's current
     one) the stream that allocations belong to."""
     torch = _torch()
-    if stream is None and torch.cuda.current_device() == cache.index:
+    if stream is None and cache.index >= 0 and torch.cuda.current_device() == cache.index:
         return call(torch._C._cuda_getCurrentRawStream(cache.index), cache, *args)
+    if cache.index < 0:
+        raise DsparkError("the cache is not on a GPU")
     stream = stream if stream is not None else torch.cuda.current_stream(cache.device)
     if stream.device_index != cache.index:
         raise DsparkError("the stream belongs to another device than the cache")
@@ -453,6 +455,13 @@ def _b8_full(t, shape, dtype, cache, what):
     return t.data_ptr()
 
 
+def _b8_workspace(cache, workspace, need):
+    ws = (workspace or Workspace(cache.device)).get(need)
+    if ws.get_device() != cache.index:
+        raise DsparkError("workspace and cache are on different devices")
+    return ws
+
+
 def _verify_attention_b8(s, cache, q, args, out, out_f32, workspace):
     torch = _torch()
     if out is None and out_f32 is None:
@@ -463,7 +472,7 @@ def _verify_attention_b8(s, cache, q, args, out, out_f32, workspace):
     need = lib().dspark_verify_attention_b8_workspace(cache.ref, ref)
     if need == 0:
         raise DsparkError("dspark_verify_attention_b8_workspace rejected the arguments")
-    ws = (workspace or Workspace(q.device)).get(need)
+    ws = _b8_workspace(cache, workspace, need)
     args.workspace, args.workspace_bytes = ws.data_ptr(), ws.numel()
     # The counters save a launch, which costs the host more than the last split's work the GPU; a graph's launch costs little,
     # and zeroing counters for one call a launch itself.
@@ -525,7 +534,7 @@ def _kv_evict_b8(s, cache, dst, length, keep, mass, stride, sinks, recent, kept,
     kept_ptr = _b8_full(kept, (cache.KVH, keep), torch.int32, cache, "kept")
     out_stride = _b8_accounts(mass_out, keep, cache, "mass_out")
     need = lib().dspark_kv_evict_b8_workspace(cache.KVH, length)
-    ws = (workspace or Workspace(cache.device)).get(need) if need else None
+    ws = _b8_workspace(cache, workspace, need) if need else None
     check(lib().dspark_kv_evict_b8(cache.ref, dst.ref, length, keep, sinks, recent, mass.data_ptr(), stride, kept_ptr,
                                    mass_out.data_ptr(), out_stride, None if ws is None else ws.data_ptr(),
                                    0 if ws is None else ws.numel(), s), "dspark_kv_evict_b8")

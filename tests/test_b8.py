@@ -21,7 +21,7 @@ def cache(**kw):
 
 def attn(**kw):
     h = load_host()
-    a = h.B8AttnArgs(q=16, q_stride=2048, out=16, workspace=16, workspace_bytes=1 << 40, M=16, QH=32, a=1000, causal=1)
+    a = h.B8AttnArgs(q=16, q_stride=2048, out=1 << 30, workspace=16, workspace_bytes=1 << 40, M=16, QH=32, a=1000, causal=1)
     for k, v in kw.items():
         setattr(a, k, v)
     return a
@@ -82,6 +82,10 @@ def test_attention_checks_its_pointers_and_workspace():
     for bad in (dict(q=None), dict(q=8), dict(q_stride=2040), dict(q_stride=2052), dict(out=None), dict(out=8),
                 dict(out_f32=8)):
         assert L.dspark_verify_attention_b8(c, ctypes.byref(attn(**bad)), None) == EINVAL, bad
+    q = 1 << 22  # outputs over the last and the first byte of q
+    for bad in (dict(q=q, out=q + (15 * 2048 + 32 * 64) * 2 - 16), dict(q=q, out=q - 16 * 32 * 64 * 2 + 16),
+                dict(q=q, out_f32=q), dict(q=q, out=None, out_f32=q - 16), dict(arrivals=2)):
+        assert L.dspark_verify_attention_b8(c, ctypes.byref(attn(**bad)), None) == EINVAL, bad
     need = L.dspark_verify_attention_b8_workspace(c, ctypes.byref(attn()))
     assert need > 0
     for bad in (dict(workspace=None), dict(workspace=8), dict(workspace_bytes=need - 1)):
@@ -115,6 +119,15 @@ def test_eviction_refuses():
     assert call(d=cache(k=2 << 20, v=32 << 20, k_scale=48 << 20, v_scale=49 << 20)) == EINVAL
     assert call(m=(16 << 20) + 100 * 8 * 32 * 64 - 4) == EINVAL
     assert call(k=mass + 4) == EINVAL and call(mo=mass) == EINVAL
+    assert call(mo=kept) == EINVAL and call(k=16 << 20) == EINVAL
+    assert call(d=cache(k=16 << 20, v=(16 << 20) + 64, k_scale=48 << 20, v_scale=49 << 20)) == EINVAL
+    assert call(d=cache(k=16 << 20, v=32 << 20, k_scale=48 << 20, v_scale=49 << 20, block_table=kept)) == EINVAL
+    # a selection by parts has a workspace
+    big = dict(s=cache(block_table=1 << 10), length=100000, ms=100000)
+    need = L.dspark_kv_evict_b8_workspace(8, 100000)
+    assert need > 0 and L.dspark_kv_evict_b8_workspace(8, 8000) == 0 and L.dspark_kv_evict_b8_workspace(0, 100000) == 0
+    assert call(**big) == ENOSPACE
+    assert call(length=(1 << 30) + 1, ms=1 << 40, s=cache(block_table=1 << 10)) == EINVAL
 
 
 def test_the_binding_refuses_on_the_host():

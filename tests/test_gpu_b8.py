@@ -235,13 +235,14 @@ def test_attention_masks(code, start, window, causal, M, D):
     check_attention(c, rng.standard_normal((M, 6, D)).astype(np.float16), a, start=start, window=window, causal=causal)
 
 
-@pytest.mark.parametrize("splits", [1, 2, 3, 7, 64, 4096])
-@pytest.mark.parametrize("M,QH,D", [(1, 8, 64), (16, 16, 64), (9, 16, 128), (64, 32, 64), (64, 32, 128)])
-def test_attention_splits_and_rows(splits, M, QH, D):
+@pytest.mark.parametrize("splits", [0, 1, 2, 3, 7, 64, 4096])
+@pytest.mark.parametrize("M,QH,KVH,D", [(1, 8, 2, 64), (16, 16, 2, 64), (9, 16, 2, 128), (64, 32, 2, 64), (64, 32, 2, 128),
+                                        (64, 16, 1, 64), (64, 16, 1, 128), (3, 40, 2, 64), (3, 70, 2, 128)])
+def test_attention_splits_and_rows(splits, M, QH, KVH, D):
     """Any number of splits; up to 1024 rows a KV head (16 query heads, 64 tokens)."""
     rng = np.random.default_rng(splits)
     a = 1500
-    c = filled("e4m3", a + M, 2, D, 4)
+    c = filled("e4m3", a + M, KVH, D, 4)
     check_attention(c, rng.standard_normal((M, QH, D)).astype(np.float16), a, splits=splits)
 
 
@@ -599,6 +600,40 @@ def test_side_stream_and_repeats():
         h.attention_mass_b8(q, g, 2000, lse, mass, stream=side)
         side.synchronize()
         assert torch.equal(got, want) and torch.equal(mass, want_mass) and bool((fill == 3).all())
+
+
+def test_two_streams_at_once():
+    """Calls that overlap, each with its own workspace, caches, accounts and destination."""
+    h = load_host()
+    rng = np.random.default_rng(9)
+    jobs = []
+    for i, (QH, KVH, D, M, a) in enumerate([(32, 8, 64, 4, 20000), (16, 4, 128, 9, 17000)]):
+        n = (a + M + 31) // 32
+        g = h.b8_cache_alloc(n, KVH, D, dtype=TYPES[KINDS[i]])
+        kv = torch.randn((2, a + M, KVH, D), device="cuda").half()
+        q = torch.randn((M, QH, D), device="cuda").half()
+
+        def run(stream, ws, g=g, kv=kv, q=q, KVH=KVH, D=D, M=M, a=a, kind=KINDS[i]):
+            with torch.cuda.stream(stream):
+                lse, acc = torch.empty(q.shape[:2], device="cuda"), torch.zeros((KVH, a + M), device="cuda")
+                dst = h.b8_cache_alloc(40, KVH, D, dtype=TYPES[kind])
+                h.kv_write_b8(kv[0, a:], kv[1, a:], g, a)
+                o, _ = h.verify_attention_b8(q, g, a, lse=lse, workspace=ws)
+                h.attention_mass_b8(q, g, a, lse, acc, mass_in=acc)
+                kept, m = h.kv_evict_b8(g, dst, a + M, 1270, acc, sinks=4, recent=64, workspace=ws)
+                return [o, lse, acc, kept, m, dst.k.view(torch.uint8), dst.v.view(torch.uint8), dst.k_scale, dst.v_scale]
+        h.kv_write_b8(kv[0], kv[1], g, 0)
+        jobs.append(run)
+    torch.cuda.synchronize()
+    alone = [run(torch.cuda.current_stream(), h.Workspace("cuda")) for run in jobs]
+    torch.cuda.synchronize()
+    streams, spaces = [torch.cuda.Stream() for _ in jobs], [h.Workspace("cuda") for _ in jobs]
+    for _ in range(4):
+        both = [[run(s, w) for _ in range(3)][-1] for run, s, w in zip(jobs, streams, spaces)]
+        torch.cuda.synchronize()
+        for x, y in zip(alone, both):
+            for u, v in zip(x, y):
+                assert torch.equal(u, v)
 
 
 def test_graph_replays():
