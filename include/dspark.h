@@ -150,7 +150,8 @@ int dspark_verify_attention_rec_combine(const dspark_attn_args* args, dspark_str
  * no infinities, 0x7f and 0xff no numbers), scale pools fp32 [kv_pages][KVH], and an int32 block table as above; value =
  * code * scale, exact in fp32. Pools may pass 4 GiB. A table entry outside [0, kv_pages) is an absent page: it is neither
  * read nor written, no query sees its positions, and they read back as zeros. Two logical pages that are written must not
- * share a physical page.
+ * share a physical page. What one of these calls writes (workspaces too) shares no byte with what it reads, nor with anything
+ * else it writes, unless said otherwise (DSPARK_EINVAL).
  * Scale of a block whose largest finite magnitude is A: int8, fp32(A / 127) rounded up to 16 significant bits; e4m3, the
  * least power of two s with A <= 448 s; 0 for A = 0. Code: x / s rounded once to nearest, ties to even; NaN is coded 0 and
  * an infinity as the largest code, so that a bad row does not spoil the block it shares. No counterpart in the reference,
@@ -176,7 +177,8 @@ typedef struct dspark_b8_cache {
 int dspark_kv_write_b8(const dspark_b8_cache* cache, const void* k, const void* v, int64_t row_stride, int32_t pos0,
                        int32_t n, dspark_stream_t stream);
 /* The values of positions pos0 .. pos0 + n - 1 as fp32 rows [n][row_stride] (head h at h D; 16-byte boundaries, row_stride
- * a multiple of 4): what a prefill over a cached prefix, or a writer of another format, takes. */
+ * a multiple of 4; k and v may lie side by side in wider rows): what a prefill over a cached prefix, or a writer of another
+ * format, takes. */
 int dspark_kv_read_b8(const dspark_b8_cache* cache, int32_t pos0, int32_t n, float* k, float* v, int64_t row_stride,
                       dspark_stream_t stream);
 
@@ -186,7 +188,7 @@ int dspark_kv_read_b8(const dspark_b8_cache* cache, int32_t pos0, int32_t n, flo
  * and/or fp32 [M][QH][D] on 16-byte boundaries. lse, if given: fp32 [M][QH], the natural logarithm of the sum of
  * exp(q k / sqrt(D)) over the keys a row sees (before the gate). A row that sees no key (every page of it absent) gives
  * zeros and lse -inf. M QH / KVH <= 1024. The workspace needs no clearing and may be shared by stream-ordered calls. The
- * probabilities are rounded to fp16 once; scores, sums and outputs are fp32. Outputs must not overlap q (DSPARK_EINVAL). */
+ * probabilities are rounded to fp16 once; scores, sums and outputs are fp32. */
 #define DSPARK_B8_ARRIVALS 64 /* row groups of a KV head at most: 1024 rows by 16 */
 typedef struct dspark_b8_attn_args {
   const void* q;
@@ -198,8 +200,9 @@ typedef struct dspark_b8_attn_args {
   void* workspace;             /* size from dspark_verify_attention_b8_workspace, on a 16-byte boundary */
   size_t workspace_bytes;
   uint32_t* arrivals;          /* KVH x DSPARK_B8_ARRIVALS words or NULL: with them the splits of few rows are added by the
-                                  last of them to finish instead of a second launch, to the same bits. Zero before their first use; every call leaves them zero. Like the workspace they
-                                  serve any number of stream-ordered calls, not calls that overlap, but nothing else. */
+                                  last of them to finish instead of a second launch, to the same bits. Zero before their
+                                  first use; every call leaves them zero. Like the workspace they serve any number of
+                                  stream-ordered calls, not calls that overlap, but nothing else. */
   int32_t M, QH;               /* 1 <= M <= DSPARK_MT_MAX; QH % KVH == 0 */
   int32_t a, start, window, causal;
   int32_t splits;              /* key-range splits per KV head; 0 = automatic */
@@ -214,7 +217,7 @@ int dspark_verify_attention_b8(const dspark_b8_cache* cache, const dspark_b8_att
  * positions from a + rows on are left as they are. The same cache and args as the attention call that gave lse (of args it
  * reads q, q_stride, M, QH, a, start, window and causal); a row with lse -inf adds nothing. rows: device word, clamped to
  * [0, M], NULL = M -- after dspark_accept_commit the address of State.ctx_new, so that rejected drafts draw nothing.
- * mass_in NULL = zeros; mass_out may be mass_in itself, and must not overlap it otherwise. mass_stride elements between
+ * mass_in NULL = zeros; mass_out may be mass_in itself. mass_stride elements between
  * heads (>= a + M). Each key's sum is taken by one wave in a fixed order: no atomics. */
 int dspark_attention_mass_b8(const dspark_b8_cache* cache, const dspark_b8_attn_args* args, const float* lse,
                              const int32_t* rows, const float* mass_in, float* mass_out, int64_t mass_stride,
@@ -226,9 +229,7 @@ int dspark_attention_mass_b8(const dspark_b8_cache* cache, const dspark_b8_attn_
  * cache of `keep` positions for every head (keys keep the rotation they were written with; later calls count positions
  * from keep). A dst block's scale is the largest of its rows' scales; rows from blocks of a smaller one are re-coded to it
  * (rounded once more). The slots behind keep in the last page are cleared. mass_out[h][j] = mass[h][kept[h][j]]. dst has
- * src's KVH, D and code; its pools, kept, mass_out and the workspace must share no byte with what is read, nor with one
- * another (DSPARK_EINVAL). sinks + recent
- * <= keep <= length <= 2^30. keep = 0 does nothing. The workspace (a size of 0: none is needed) needs no clearing. */
+ * src's KVH, D and code, and pools of its own. sinks + recent <= keep <= length <= 2^30. keep = 0 does nothing. The workspace (a size of 0: none is needed) needs no clearing. */
 int dspark_kv_evict_b8(const dspark_b8_cache* src, const dspark_b8_cache* dst, int32_t length, int32_t keep, int32_t sinks,
                        int32_t recent, const float* mass, int64_t mass_stride, int32_t* kept, float* mass_out,
                        int64_t mass_out_stride, void* workspace, size_t workspace_bytes, dspark_stream_t stream);

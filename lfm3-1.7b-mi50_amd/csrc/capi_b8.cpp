@@ -91,10 +91,42 @@ B8Attn attn(const dspark_b8_cache* c, const dspark_b8_attn_args* a) {
   return p;
 }
 
-// [p, p + pn) and [q, q + qn) share a byte.
-bool overlap(const void* p, size_t pn, const void* q, size_t qn) {
-  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
-  return a < b + qn && b < a + pn;
+// Memory that a call reads or writes; p NULL or n 0: none.
+struct Span {
+  const void* p;
+  size_t n;
+};
+bool overlap(const Span& x, const Span& y) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(x.p), b = reinterpret_cast<uintptr_t>(y.p);
+  return a && b && x.n && y.n && a < b + y.n && b < a + x.n;
+}
+// Nothing that is written shares a byte with what is read, nor with anything else that is written: workgroups read and store in
+// no order among each other.
+template <size_t NR, size_t NW>
+bool apart(const Span (&reads)[NR], const Span (&writes)[NW]) {
+  for (size_t i = 0; i < NW; ++i) {
+    for (const Span& r : reads)
+      if (overlap(r, writes[i])) return false;
+    for (size_t j = 0; j < i; ++j)
+      if (overlap(writes[j], writes[i])) return false;
+  }
+  return true;
+}
+size_t scale_bytes(const dspark_b8_cache* c) { return (size_t)c->kv_pages * c->KVH * sizeof(float); }
+size_t code_bytes(const dspark_b8_cache* c) { return (size_t)c->kv_pages * c->KVH * DSPARK_PAGE_TOKENS * c->D; }
+Span table(const dspark_b8_cache* c, int64_t positions) { return {c->block_table, (size_t)pages_of(positions) * sizeof(int32_t)}; }
+// Rows of KVH D elements, row_stride apart.
+Span rows_of(const dspark_b8_cache* c, const void* p, int64_t n, int64_t row_stride, size_t element) {
+  return {p, ((size_t)(n - 1) * row_stride + (size_t)c->KVH * c->D) * element};
+}
+Span query(const dspark_b8_cache* c, const dspark_b8_attn_args* a) {
+  return {a->q, ((size_t)(a->M - 1) * a->q_stride + (size_t)a->QH * c->D) * 2};
+}
+// Two sets of n such rows share a byte (they may lie in turn in wider rows).
+bool rows_meet(const Span& x, const Span& y, int64_t n, size_t row, size_t stride) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(x.p), b = reinterpret_cast<uintptr_t>(y.p);
+  const size_t d = a < b ? b - a : a - b, q = d / stride, m = d % stride;
+  return (m < row && q < (size_t)n) || (stride - m < row && q + 1 < (size_t)n);
 }
 
 }  // namespace
@@ -107,6 +139,9 @@ int dspark_kv_write_b8(const dspark_b8_cache* c, const void* k, const void* v, i
   if (n == 0) return 0;
   if (!on(k, 16) || !on(v, 16) || row_stride < (int64_t)c->KVH * c->D || row_stride % 8) return DSPARK_EINVAL;
   if (!waves_fit(c, pages_of((int64_t)n) + 1)) return DSPARK_EINVAL;
+  const Span reads[3] = {rows_of(c, k, n, row_stride, 2), rows_of(c, v, n, row_stride, 2), table(c, (int64_t)pos0 + n)};
+  const Span writes[4] = {{c->k, code_bytes(c)}, {c->v, code_bytes(c)}, {c->k_scale, scale_bytes(c)}, {c->v_scale, scale_bytes(c)}};
+  if (!apart(reads, writes)) return DSPARK_EINVAL;
   B8Write p;
   p.c = pool(c);
   p.k = static_cast<const _Float16*>(k);
@@ -123,6 +158,11 @@ int dspark_kv_read_b8(const dspark_b8_cache* c, int32_t pos0, int32_t n, float* 
   if (n == 0) return 0;
   if (!on(k, 16) || !on(v, 16) || row_stride < (int64_t)c->KVH * c->D || row_stride % 4) return DSPARK_EINVAL;
   if (!waves_fit(c, pages_of((int64_t)n) + 1)) return DSPARK_EINVAL;
+  const Span reads[5] = {{c->k, code_bytes(c)}, {c->v, code_bytes(c)}, {c->k_scale, scale_bytes(c)}, {c->v_scale, scale_bytes(c)},
+                         table(c, (int64_t)pos0 + n)};
+  const Span ks[1] = {rows_of(c, k, n, row_stride, 4)}, vs[1] = {rows_of(c, v, n, row_stride, 4)};
+  if (!apart(reads, ks) || !apart(reads, vs)) return DSPARK_EINVAL;
+  if (rows_meet(ks[0], vs[0], n, (size_t)c->KVH * c->D * 4, (size_t)row_stride * 4)) return DSPARK_EINVAL;
   B8Read p;
   p.c = pool(c);
   p.k = k;
@@ -144,13 +184,16 @@ int dspark_verify_attention_b8(const dspark_b8_cache* c, const dspark_b8_attn_ar
   if (!rows_ok(c, a) || !query_ok(c, a)) return DSPARK_EINVAL;
   if (!a->out && !a->out_f32) return DSPARK_EINVAL;
   if (a->arrivals && !on(a->arrivals, 4)) return DSPARK_EINVAL;
-  // every workgroup reads its rows of q by itself, also after others have stored theirs
-  const size_t n = (size_t)a->M * a->QH * c->D, qn = ((size_t)(a->M - 1) * a->q_stride + (size_t)a->QH * c->D) * 2;
-  if ((a->out && overlap(a->out, 2 * n, a->q, qn)) || (a->out_f32 && overlap(a->out_f32, 4 * n, a->q, qn))) return DSPARK_EINVAL;
   if ((a->out && !on(a->out, 16)) || (a->out_f32 && !on(a->out_f32, 16))) return DSPARK_EINVAL;
   B8Attn p = attn(c, a);
   b8_attn_plan(p, c->D, a->splits, device_cus());
-  if (!on(a->workspace, 16) || a->workspace_bytes < std::max(b8_attn_workspace(p, c->D), (size_t)256)) return DSPARK_ENOSPACE;
+  const size_t need = b8_attn_workspace(p, c->D), heads = (size_t)a->M * a->QH;
+  if (!on(a->workspace, 16) || a->workspace_bytes < std::max(need, (size_t)256)) return DSPARK_ENOSPACE;
+  const Span reads[7] = {query(c, a), {a->gate, heads * 4}, {c->k, code_bytes(c)}, {c->v, code_bytes(c)},
+                         {c->k_scale, scale_bytes(c)}, {c->v_scale, scale_bytes(c)}, table(c, (int64_t)a->a + a->M)};
+  const Span writes[5] = {{a->out, heads * c->D * 2}, {a->out_f32, heads * c->D * 4}, {a->lse, heads * 4}, {a->workspace, need},
+                          {a->arrivals, (size_t)c->KVH * DSPARK_B8_ARRIVALS * 4}};
+  if (!apart(reads, writes)) return DSPARK_EINVAL;
   p.part_acc = static_cast<float*>(a->workspace);
   p.part_ml = reinterpret_cast<f32x2*>(p.part_acc + (size_t)p.c.KVH * p.R * p.S * c->D);
   return b8_attn_launch(p, c->D, c->code == DSPARK_B8_E4M3, S(stream));
@@ -160,8 +203,12 @@ int dspark_attention_mass_b8(const dspark_b8_cache* c, const dspark_b8_attn_args
                              const float* mass_in, float* mass_out, int64_t mass_stride, dspark_stream_t stream) {
   if (!rows_ok(c, a) || !query_ok(c, a) || !on(lse, 4) || !on(mass_out, 4) || (rows && !on(rows, 4))) return DSPARK_EINVAL;
   if (mass_stride < (int64_t)a->a + a->M) return DSPARK_EINVAL;
+  if (mass_in && !on(mass_in, 4)) return DSPARK_EINVAL;
   const size_t bytes = ((size_t)(c->KVH - 1) * mass_stride + a->a + a->M) * sizeof(float);
-  if (mass_in && (!on(mass_in, 4) || (mass_in != mass_out && overlap(mass_in, bytes, mass_out, bytes)))) return DSPARK_EINVAL;
+  const Span reads[7] = {{mass_in == mass_out ? nullptr : mass_in, bytes}, query(c, a), {lse, (size_t)a->M * a->QH * 4}, {rows, 4},
+                         {c->k, code_bytes(c)}, {c->k_scale, scale_bytes(c)}, table(c, (int64_t)a->a + a->M)};
+  const Span writes[1] = {{mass_out, bytes}};
+  if (!apart(reads, writes)) return DSPARK_EINVAL;
   B8Attn p = attn(c, a);
   p.lse_in = lse;
   p.rows = rows;
@@ -184,24 +231,16 @@ int dspark_kv_evict_b8(const dspark_b8_cache* src, const dspark_b8_cache* dst, i
   if (length > 1 << 30 || !fits(src, length) || !fits(dst, keep) || !waves_fit(dst, pages_of(keep))) return DSPARK_EINVAL;
   if (keep == 0) return 0;
   if (!on(mass, 4) || !on(kept, 4) || !on(mass_out, 4) || mass_stride < length || mass_out_stride < keep) return DSPARK_EINVAL;
-  // the rows move between pools that share nothing: a destination page may be written while other rows are still read
-  const size_t from[2] = {(size_t)src->kv_pages * src->KVH, (size_t)src->kv_pages * src->KVH * DSPARK_PAGE_TOKENS * src->D};
-  const size_t to[2] = {(size_t)dst->kv_pages * dst->KVH, (size_t)dst->kv_pages * dst->KVH * DSPARK_PAGE_TOKENS * dst->D};
-  const struct { const void* p; size_t n; } reads[7] = {
-      {src->k, from[1]}, {src->v, from[1]}, {src->k_scale, from[0] * 4}, {src->v_scale, from[0] * 4},
-      {mass, ((size_t)(src->KVH - 1) * mass_stride + length) * 4}, {src->block_table, src->block_table ? (size_t)pages_of(length) * 4 : 0},
-      {dst->block_table, dst->block_table ? (size_t)pages_of(keep) * 4 : 0}};
   const size_t need = b8_evict_workspace(src->KVH, length);
   if (need && (!on(workspace, 16) || workspace_bytes < need)) return DSPARK_ENOSPACE;
-  const struct { const void* p; size_t n; } writes[7] = {
-      {dst->k, to[1]}, {dst->v, to[1]}, {dst->k_scale, to[0] * 4}, {dst->v_scale, to[0] * 4},
-      {mass_out, ((size_t)(src->KVH - 1) * mass_out_stride + keep) * 4}, {kept, (size_t)src->KVH * keep * 4}, {workspace, need}};
-  for (const auto& r : reads)
-    for (const auto& w : writes)
-      if (r.n && w.n && overlap(r.p, r.n, w.p, w.n)) return DSPARK_EINVAL;
-  for (const auto& v : writes)
-    for (const auto& w : writes)
-      if (&v < &w && v.n && w.n && overlap(v.p, v.n, w.p, w.n)) return DSPARK_EINVAL;
+  // a destination page may be written while other rows are still read
+  const Span reads[7] = {{src->k, code_bytes(src)}, {src->v, code_bytes(src)}, {src->k_scale, scale_bytes(src)},
+                         {src->v_scale, scale_bytes(src)}, {mass, ((size_t)(src->KVH - 1) * mass_stride + length) * 4},
+                         table(src, length), table(dst, keep)};
+  const Span writes[7] = {{dst->k, code_bytes(dst)}, {dst->v, code_bytes(dst)}, {dst->k_scale, scale_bytes(dst)},
+                          {dst->v_scale, scale_bytes(dst)}, {mass_out, ((size_t)(src->KVH - 1) * mass_out_stride + keep) * 4},
+                          {kept, (size_t)src->KVH * keep * 4}, {workspace, need}};
+  if (!apart(reads, writes)) return DSPARK_EINVAL;
   B8Evict p;
   p.src = pool(src);
   p.dst = pool(dst);

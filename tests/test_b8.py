@@ -175,3 +175,50 @@ def test_scales_and_codes_of_the_restatement(code):
     best = np.abs(x[:, None] - inside[None] * 0.37).min(1)
     assert np.allclose(np.abs(got - x), best, rtol=0, atol=1e-12)
     assert np.array_equal(b8.codes_of("int8", np.array([0.5, 1.5, -0.5, 2.5, np.nan, np.inf]), 1.0).view(np.int8), [0, 2, 0, 2, 0, 127])
+
+
+def test_calls_refuse_memory_that_meets():
+    """Every output against every input and the other outputs, by a word at either end."""
+    L = load_host().lib()
+    MB = 1 << 20
+    pools = dict(k=16 * MB, v=32 * MB, k_scale=48 * MB, v_scale=49 * MB, block_table=50 * MB)
+    codes, scales, table = 100 * 8 * 32 * 64, 100 * 8 * 4, 32 * 4
+    c = ctypes.byref(cache(**pools))
+    held = [(16 * MB, codes), (32 * MB, codes), (48 * MB, scales), (49 * MB, scales)]
+
+    def over(spans, n):  # outputs of n bytes that reach a span's last and its first byte, on 16-byte boundaries
+        return [x for at, size in spans for x in ((at + size - 1) // 16 * 16, (at - n) // 16 * 16 + 16)]
+
+    # append: rows of 512 halves 600 apart, 10 of them; the table inside a pool
+    n = (9 * 600 + 512) * 2
+    for at in over(held, n):
+        assert L.dspark_kv_write_b8(c, at, 60 * MB, 600, 990, 10, None) == EINVAL
+        assert L.dspark_kv_write_b8(c, 60 * MB, at, 600, 990, 10, None) == EINVAL
+    for at in (16 * MB + codes - 4, 16 * MB - table + 4):
+        bad = ctypes.byref(cache(**{**pools, "block_table": at}))
+        assert L.dspark_kv_write_b8(bad, 60 * MB, 61 * MB, 600, 990, 10, None) == EINVAL
+    for bad in (dict(v=16 * MB + 64), dict(v=16 * MB), dict(v_scale=48 * MB), dict(k_scale=32 * MB + 64)):
+        assert L.dspark_kv_write_b8(ctypes.byref(cache(**{**pools, **bad})), 60 * MB, 61 * MB, 600, 990, 10, None) == EINVAL
+    # read back: rows of 512 words 1024 apart; k and v in each other's rows
+    n = (9 * 1024 + 512) * 4
+    for at in over(held + [(50 * MB, table)], n):
+        assert L.dspark_kv_read_b8(c, 990, 10, at, 60 * MB, 1024, None) == EINVAL
+        assert L.dspark_kv_read_b8(c, 990, 10, 60 * MB, at, 1024, None) == EINVAL
+    for d in (0, 16, 2048 - 16, 4096 * 9, 4096 * 9 + 2032, 4096 - 2032, 4096 * 8 + 2064):
+        assert L.dspark_kv_read_b8(c, 990, 10, 60 * MB, 60 * MB + d, 1024, None) == EINVAL
+        assert L.dspark_kv_read_b8(c, 990, 10, 60 * MB + d, 60 * MB, 1024, None) == EINVAL
+    # attention
+    base = dict(q=60 * MB, out=61 * MB, out_f32=62 * MB, lse=63 * MB, gate=64 * MB, workspace=128 * MB, arrivals=65 * MB)
+    out, heads, words = 16 * 2048, 16 * 32 * 4, 8 * 64 * 4
+    need = L.dspark_verify_attention_b8_workspace(c, ctypes.byref(attn(**base)))
+    reads = held + [(50 * MB, table), (60 * MB, 2 * out), (64 * MB, heads)]
+    sizes = dict(out=2 * out, out_f32=4 * out, lse=heads, workspace=need, arrivals=words)
+    for name, size in sizes.items():
+        others = [(base[x], s) for x, s in sizes.items() if x != name]
+        for at in over(reads + others, size):
+            assert L.dspark_verify_attention_b8(c, ctypes.byref(attn(**{**base, name: at})), None) == EINVAL, (name, at)
+    # accounts
+    ok = ctypes.byref(attn(**base))
+    bytes_ = (7 * 1100 + 1016) * 4
+    for at in over([held[0], held[2], (50 * MB, table), (60 * MB, 2 * out), (63 * MB, heads), (70 * MB, 4), (80 * MB, bytes_)], bytes_):
+        assert L.dspark_attention_mass_b8(c, ok, 63 * MB, 70 * MB, 80 * MB, at, 1100, None) == EINVAL, at

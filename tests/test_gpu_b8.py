@@ -157,6 +157,23 @@ def test_read_into_wider_rows_leaves_the_rest():
         assert bool((o[39:] == 7).all()) and bool((o[:, 192:] == 7).all())
 
 
+@pytest.mark.parametrize("n", [1, 39])
+def test_reads_and_appends_of_rows_side_by_side(n):
+    h = load_host()
+    c = filled("e4m3", 77, 3, 64, 2)
+    wide = torch.full((n, 2, 3, 64), 7.0, device="cuda")
+    h.kv_read_b8(gpu_cache(c), 30, n, wide[:, 0], wide[:, 1])
+    for x, want in zip(wide.unbind(1), c.read(30, n)):
+        np.testing.assert_array_equal(x.cpu().numpy(), want.astype(np.float32))
+    half = wide.half()
+    g = h.b8_cache_alloc(2, 3, 64, torch.float8_e4m3fn)
+    h.kv_write_b8(half[:, 0], half[:, 1], g, 5)
+    w = b8.Cache("e4m3", 2, 3, 64)
+    w.write(*half.cpu().numpy().transpose(1, 0, 2, 3), 5)
+    for x, want in zip(h.kv_read_b8(g, 5, n), w.read(5, n)):
+        np.testing.assert_array_equal(x.cpu().numpy(), want.astype(np.float32))
+
+
 # ------------------------------------------------------------------------------------------------ attention
 # Of a result o = sum p v with A = sum p |v| (p the softmax): V's scale vs goes into the exponent and p vs, times a power of two
 # that takes the row's largest to at least 2^8, is rounded to fp16 once: by 2^-11 of itself where that is a normal half, and
