@@ -4,7 +4,7 @@
 // blocks of 32 (a page) whose codes carry one scale: x = (q . code) ks log2(e) / sqrt(D). V's scale goes into the exponent:
 // P = 2^(x + log2 vs - ref) with the row's running reference over x + log2 vs, so that o += P . codes accumulates in the matrix
 // cores whatever the blocks' scales, and l += (sum of P) / vs keeps the softmax sum in the same units (with o += vs (P . codes)
-// instead, D / 4 multiply-adds a row block and page: 79 -> 58 us at 128k keys and 33 tokens). Codes (int8 or e4m3) are exact
+// instead, D / 4 multiply-adds a row block and page: 79 -> 69 us at 128k keys and 33 tokens). Codes (int8 or e4m3) are exact
 // in fp16, so the products are of exact operands but for P, which is rounded to fp16 once; scales, references, sums and
 // outputs are fp32.
 //
@@ -279,25 +279,26 @@ __device__ __forceinline__ float b8_gate(const B8Attn& p, int h, int row) {
 }
 
 // The splits of a row are added in an order of its own, whoever adds them: split lane j takes splits j, j + 4, ... in batches
-// of 8, each batch rescaled to the largest reference so far; then the lanes in order.
+// of 8, each batch rescaled to the largest reference so far; then the lanes in order. (With no more than BATCH splits a lane a
+// smaller batch gives the same bits: the missing ones add zeros.)
 constexpr int SPLIT_LANES = 4, SPLIT_BATCH = 8;
-template <int D>
-__device__ __forceinline__ void b8_add_splits(const B8Attn& p, __amdgpu_buffer_rsrc_t racc, __amdgpu_buffer_rsrc_t rml, int first, int j,
-                                              int c, float* o, f32x2* ml_out) {
-  float m = REF_INIT, l = 0.f;
-  f32x4 acc = {0, 0, 0, 0};
-  for (int s0 = j; s0 < p.S; s0 += SPLIT_LANES * SPLIT_BATCH) {
-    f32x2 ml[SPLIT_BATCH];
-    f32x4 v[SPLIT_BATCH];
+template <int D, int BATCH>
+struct B8Splits {
+  f32x2 ml[BATCH];
+  f32x4 v[BATCH];
+  // Splits s0, s0 + 4, ... of a row whose sums start at `first` (past the last split: the last again; past the rows: zeros).
+  __device__ __forceinline__ void load(const B8Attn& p, __amdgpu_buffer_rsrc_t racc, __amdgpu_buffer_rsrc_t rml, int first, int s0, int c) {
 #pragma unroll
-    for (int i = 0; i < SPLIT_BATCH; ++i) {  // (past the last split: the last again)
+    for (int i = 0; i < BATCH; ++i) {
       const int at = first + min(s0 + i * SPLIT_LANES, p.S - 1);
       ml[i] = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(rml, at * (int)sizeof(f32x2), 0, B8_COHERENT));
       v[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(racc, (at * D + 4 * c) * (int)sizeof(float), 0, B8_COHERENT));
     }
+  }
+  __device__ __forceinline__ void add(const B8Attn& p, int s0, float& m, float& l, f32x4& acc) {
     float to = m;
 #pragma unroll
-    for (int i = 0; i < SPLIT_BATCH; ++i) {
+    for (int i = 0; i < BATCH; ++i) {
       if (s0 + i * SPLIT_LANES >= p.S) ml[i] = f32x2{REF_INIT, 0.f}, v[i] = f32x4{0, 0, 0, 0};
       to = max_of(to, ml[i][0]);
     }
@@ -305,12 +306,23 @@ __device__ __forceinline__ void b8_add_splits(const B8Attn& p, __amdgpu_buffer_r
     acc *= f0;
     l *= f0;
 #pragma unroll
-    for (int i = 0; i < SPLIT_BATCH; ++i) {
+    for (int i = 0; i < BATCH; ++i) {
       const float f = fast_exp2(ml[i][0] - to);
       acc += v[i] * f;
       l = fmaf(ml[i][1], f, l);
     }
     m = to;
+  }
+};
+template <int D>
+__device__ __forceinline__ void b8_add_splits(const B8Attn& p, __amdgpu_buffer_rsrc_t racc, __amdgpu_buffer_rsrc_t rml, int first, int j,
+                                              int c, float* o, f32x2* ml_out) {
+  float m = REF_INIT, l = 0.f;
+  f32x4 acc = {0, 0, 0, 0};
+  for (int s0 = j; s0 < p.S; s0 += SPLIT_LANES * SPLIT_BATCH) {
+    B8Splits<D, SPLIT_BATCH> some;
+    some.load(p, racc, rml, first, s0, c);
+    some.add(p, s0, m, l, acc);
   }
   *reinterpret_cast<f32x4*>(o) = acc;
   if (c == 0) *ml_out = f32x2{m, l};
@@ -395,7 +407,8 @@ __global__ __launch_bounds__(64 * b8_waves(D, RB), b8_waves(D, RB) / 4) void att
   }
 
   // Every wave's sums into LDS at once, then each thread adds up some rows' quads, rescaled to the row's largest reference,
-  // in wave order. (Row block by row block with 16 rows of LDS: two more barriers and a drain each, 5 us instead of 1.5.)
+  // in wave order. (Row block by row block with 16 rows of LDS: two more barriers and a drain each; 16 tokens of
+  // 32768 keys took 17.5 us instead of 15.2.)
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
     const float l = row_sum(st.l[rb]);
@@ -462,17 +475,30 @@ __global__ __launch_bounds__(64 * b8_waves(D, RB), b8_waves(D, RB) / 4) void att
     }
     __syncthreads();
     if (!last_s) return;
-    constexpr int RP = PER / SPLIT_LANES;  // rows side by side
-    static_assert(RP >= 1 && NW >= SPLIT_LANES, "the split lanes' sums fit where the waves' were");
+    constexpr int RP = PER / SPLIT_LANES, ROUNDS = (ROWS + RP - 1) / RP, FEW = 2;  // rows side by side
+    static_assert(PER % SPLIT_LANES == 0 && NW >= SPLIT_LANES, "the split lanes' sums fit where the waves' were");
     const int u = threadIdx.x / QUADS, j = u / RP;
+    if (p.S <= FEW * SPLIT_LANES) {  // the sums of all rows in flight at once (8 tokens, 16/4/128, 1001 keys: 14.0 -> 11.0 us)
+      B8Splits<D, FEW> some[ROUNDS];
+#pragma unroll
+      for (int k = 0; k < ROUNDS; ++k) some[k].load(p, racc, rml, (k * RP + u % RP) * p.S, j, c);
+#pragma unroll
+      for (int k = 0; k < ROUNDS; ++k) {
+        const int r = k * RP + u % RP;
+        if (r >= ROWS) continue;
+        float m = REF_INIT, l = 0.f;
+        f32x4 acc = {0, 0, 0, 0};
+        some[k].add(p, j, m, l, acc);
+        *reinterpret_cast<f32x4*>(&s_o[j][r][4 * c]) = acc;
+        if (c == 0) s_ml[j][r] = f32x2{m, l};
+      }
+    } else {
 #pragma unroll 1
-    for (int r0 = 0; r0 < ROWS && row0 + r0 < p.R; r0 += RP) {
-      const int r = r0 + u % RP;
-      const bool mine = j < SPLIT_LANES && r < ROWS && row0 + r < p.R;
-      if (mine) b8_add_splits<D>(p, racc, rml, r * p.S, j, c, &s_o[j][r][4 * c], &s_ml[j][r]);
-      lds_barrier();
-      if (mine && j == 0) b8_finish_row<D>(p, h, row0 + r, c, &s_o[0][r][4 * c], &s_ml[0][r], ROWS * (D + 4), ROWS);
+      for (int r = u % RP; r < ROWS && row0 + r < p.R; r += RP) b8_add_splits<D>(p, racc, rml, r * p.S, j, c, &s_o[j][r][4 * c], &s_ml[j][r]);
     }
+    lds_barrier();
+    for (int r = u; r < ROWS && row0 + r < p.R; r += PER)
+      b8_finish_row<D>(p, h, row0 + r, c, &s_o[0][r][4 * c], &s_ml[0][r], ROWS * (D + 4), ROWS);
   }
 }
 
@@ -499,7 +525,7 @@ __global__ __launch_bounds__(256) void attn_b8_merge_kernel(B8Attn p) {
 // pages, so every key's sum is one wave's, in a fixed order and without atomics. K alone is read. The score product has its
 // operands the other way round than the attention's (A = Q, B = K): a lane holds one key's scores of rows 4 g + i, adds them
 // up in place over all row blocks, and only the four lanes of a key are added across (sums over the rows' lanes instead, with
-// A = K: eight row reductions a page, 39 -> 25 us at 128k keys and 64 rows a head).
+// A = K, are eight row reductions a page: 39 us at 128k keys and 64 rows a head, 31 so).
 template <int D, int RB, bool FP8>
 __global__ __launch_bounds__(64 * MASS_WAVES, 2) void mass_b8_kernel(B8Attn p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
@@ -618,15 +644,16 @@ void b8_attn_plan(B8Attn& p, int D, int splits, int cus) {
   const int blocks = (p.R + 15) / 16, most = D == 64 ? B8_ROW_BLOCKS : 2;
   p.RG = (blocks + most - 1) / most;
   p.rb = (blocks + p.RG - 1) / p.RG;
-  // Few pages: a row block a workgroup, and splits of a page a wave as far as there are CUs -- at D = 64 up to four pages a wave
-  // (16 tokens, 32/8/64 heads: 1000 keys 9.8 -> 8.0 us, 4000 10.3 -> 8.9, 8000 11.5 -> 10.4, 16000 13.1 -> 12.7), at
-  // D = 128 to one (8 tokens, 16/4/128: 250 keys 10.5 -> 7.0, 1001 10.7 -> 10.9 but without a second launch, 16000 13.1 -> 14.2
-  // with two).
+  // Few pages: a row block a workgroup, up to two pages a wave in one split (16 tokens, 32/8/64 heads, 500 keys: 5.7 us, 7.6 with
+  // a page a wave; three and four a wave lose to splits at 16/4/128, 1001 keys 11.6 against 10.9), then splits of a page a wave
+  // as far as there are CUs -- at D = 64 up to four pages a wave (1000 keys 9.8 -> 8.0 us against row groups of four blocks,
+  // 4000 10.3 -> 8.9, 8000 11.5 -> 10.4, 16000 13.1 -> 12.7), at D = 128 to one (8 tokens, 16/4/128: 250 keys 10.5 -> 7.0,
+  // 1001 10.7 -> 10.9 but without a second launch, 16000 13.1 -> 14.2 with two).
   const int w1 = b8_waves(D, 1), most1 = cus / (p.c.KVH * blocks);
   if (splits == 0 && most1 > 0 && p.npages <= (D == 64 ? 4 : 1) * w1 * most1) {
     p.rb = 1;
     p.RG = blocks;
-    splits = std::min(most1, (p.npages + w1 - 1) / w1);
+    splits = p.npages <= 2 * w1 ? 1 : std::min(most1, (p.npages + w1 - 1) / w1);
   }
   const int waves = b8_waves(D, p.rb);
   int S = splits > 0 ? splits : std::max(1, cus / (p.c.KVH * p.RG));
@@ -692,7 +719,7 @@ int b8_mass_launch(const B8Attn& q, int D, bool fp8, int cus, hipStream_t s) {
   p.seen_lo = p.page0;
   p.page0 = 0;  // every account is carried over, those of keys out of sight too
   p.npages = (p.a + p.M - 1) / PAGE + 1;
-  // as many pages a wave as let every workgroup start at once (a few over: 27.8 us instead of MASSNEW)
+  // as many pages a wave as let every workgroup start at once (131088 keys, 64 rows a head: 26.0 us, 27.8 with a few over)
   const int64_t waves = (int64_t)cus * (p.rb > 2 ? 12 : 16);
   p.pps = (int)std::max<int64_t>(1, ((int64_t)p.npages * p.c.KVH + waves - 1) / waves);
   const dim3 grid((p.npages + p.pps * MASS_WAVES - 1) / (p.pps * MASS_WAVES), p.c.KVH);

@@ -187,8 +187,8 @@ int dspark_verify_attention_b8(const dspark_b8_cache* c, const dspark_b8_attn_ar
   if ((a->out && !on(a->out, 16)) || (a->out_f32 && !on(a->out_f32, 16))) return DSPARK_EINVAL;
   B8Attn p = attn(c, a);
   b8_attn_plan(p, c->D, a->splits, device_cus());
-  const size_t need = b8_attn_workspace(p, c->D), heads = (size_t)a->M * a->QH;
-  if (!on(a->workspace, 16) || a->workspace_bytes < std::max(need, (size_t)256)) return DSPARK_ENOSPACE;
+  const size_t need = std::max(b8_attn_workspace(p, c->D), (size_t)256), heads = (size_t)a->M * a->QH;
+  if (!on(a->workspace, 16) || a->workspace_bytes < need) return DSPARK_ENOSPACE;
   const Span reads[7] = {query(c, a), {a->gate, heads * 4}, {c->k, code_bytes(c)}, {c->v, code_bytes(c)},
                          {c->k_scale, scale_bytes(c)}, {c->v_scale, scale_bytes(c)}, table(c, (int64_t)a->a + a->M)};
   const Span writes[5] = {{a->out, heads * c->D * 2}, {a->out_f32, heads * c->D * 4}, {a->lse, heads * 4}, {a->workspace, need},
