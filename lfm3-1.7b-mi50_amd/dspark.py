@@ -19,7 +19,8 @@ STATE_FIELDS = ["a", "anchor", "count", "rounds_left", "limit", "budget", "eos",
                 "run", "force_m", "rounds_done", "accepted", "verified", "miss", "skip", "skip_after", "skip_rounds",
                 "stop_at", "ckpt_slot"]
 
-ERRORS = {1001: "DSPARK_EINVAL", 1002: "DSPARK_ENOSPACE", 1003: "DSPARK_EUNSUPPORTED"}
+ENOSPACE = 1002
+ERRORS = {1001: "DSPARK_EINVAL", ENOSPACE: "DSPARK_ENOSPACE", 1003: "DSPARK_EUNSUPPORTED"}
 
 
 class DsparkError(RuntimeError):
@@ -435,15 +436,15 @@ def kv_read_b8(cache, pos0, n, k=None, v=None, stream=None):
     return _b8_on(cache, stream, _kv_read_b8, pos0, n, k, v)
 
 
-def _b8_attn_args(q, cache, a, start, window, causal):
+def _b8_attn_args(q, cache, a, start, window, causal, splits=0):
     shape, stride = q.shape, q.stride()
     if len(shape) != 3 or shape[2] != cache.D or q.dtype != _torch().float16 or stride[2] != 1 \
             or (shape[1] > 1 and stride[1] != cache.D):
         raise DsparkError("q is fp16 [M][QH][D] of contiguous rows, D the cache's")
     M, QH, D = shape
     cache.check(a + M, q)
-    return B8AttnArgs(q=q.data_ptr(), q_stride=stride[0] if M > 1 else max(stride[0], QH * D), M=M, QH=QH, a=a, start=start,
-                      window=window, causal=int(causal))
+    return B8AttnArgs(q.data_ptr(), stride[0] if M > 1 else max(stride[0], QH * D), None, None, None, None, None, 0, None,
+                      M, QH, a, start, window, 1 if causal else 0, splits)
 
 
 def _b8_full(t, shape, dtype, cache, what):
@@ -465,21 +466,27 @@ def _b8_workspace(cache, workspace, need):
 def _verify_attention_b8(s, cache, q, args, out, out_f32, workspace):
     torch = _torch()
     if out is None and out_f32 is None:
-        out = torch.empty(q.shape, dtype=torch.float16, device=q.device)
+        out = q.new_empty(q.shape)
     args.out = _b8_full(out, q.shape, torch.float16, cache, "out")
     args.out_f32 = _b8_full(out_f32, q.shape, torch.float32, cache, "out_f32")
-    ref = ctypes.byref(args)
-    need = lib().dspark_verify_attention_b8_workspace(cache.ref, ref)
-    if need == 0:
-        raise DsparkError("dspark_verify_attention_b8_workspace rejected the arguments")
-    ws = _b8_workspace(cache, workspace, need)
-    args.workspace, args.workspace_bytes = ws.data_ptr(), ws.numel()
     # The counters save a launch, which costs the host more than the last split's work the GPU; a graph's launch costs little,
     # and zeroing counters for one call a launch itself.
     if workspace is not None and not torch.cuda.is_current_stream_capturing():
         args.arrivals = workspace.arrivals(cache.KVH * B8_ARRIVALS).data_ptr()
-    check(lib().dspark_verify_attention_b8(cache.ref, ref, s), "dspark_verify_attention_b8")
-    return out, out_f32
+    ref, ws = ctypes.byref(args), workspace and workspace.buf
+    while True:  # with the workspace as it is first, then with one that is large enough
+        if ws is not None:
+            if ws.get_device() != cache.index:
+                raise DsparkError("workspace and cache are on different devices")
+            args.workspace, args.workspace_bytes = ws.data_ptr(), ws.numel()
+        rc = lib().dspark_verify_attention_b8(cache.ref, ref, s)
+        if rc != ENOSPACE:
+            check(rc, "dspark_verify_attention_b8")
+            return out, out_f32
+        need = lib().dspark_verify_attention_b8_workspace(cache.ref, ref)
+        if need <= args.workspace_bytes:
+            check(rc, "dspark_verify_attention_b8")
+        ws = _b8_workspace(cache, workspace, need)
 
 
 def verify_attention_b8(q, cache, a, start=0, window=0, causal=True, out=None, out_f32=None, lse=None, gate=None, splits=0,
@@ -487,11 +494,10 @@ def verify_attention_b8(q, cache, a, start=0, window=0, causal=True, out=None, o
     """verify_attention over a B8Cache that holds positions 0..a+M-1. q fp16 [M][QH][D]; lse (optional) fp32 [M][QH] receives
     the log-sum-exp of the scores. A workspace that is kept saves a launch for few rows: it holds the counters by which the
     last key split to finish adds them all. Returns (out fp16, out_f32) tensors as given/created."""
-    args = _b8_attn_args(q, cache, a, start, window, causal)
+    args = _b8_attn_args(q, cache, a, start, window, causal, splits)
     f32 = _torch().float32
     args.lse = _b8_full(lse, q.shape[:2], f32, cache, "lse")
     args.gate = _b8_full(gate, q.shape[:2], f32, cache, "gate")
-    args.splits = splits
     return _b8_on(cache, stream, _verify_attention_b8, q, args, out, out_f32, workspace)
 
 
