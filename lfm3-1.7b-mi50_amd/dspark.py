@@ -168,6 +168,7 @@ class Workspace:
         self.device = device
         self.buf = None
         self.words = None
+        self.captured = []  # buffers that captured graphs write to: kept when the workspace grows past them
 
     def get(self, nbytes):
         torch = _torch()
@@ -175,7 +176,14 @@ class Workspace:
         if self.buf is None or self.buf.numel() < nbytes:
             # zero-filled: the split-K GEMM keeps its arrival counters here (left at zero by every call)
             self.buf = torch.zeros(nbytes, dtype=torch.uint8, device=self.device)
+        if self.buf.is_cuda and torch.cuda.is_current_stream_capturing():
+            self.hold()
         return self.buf
+
+    def hold(self):
+        """The buffer stays allocated as long as the workspace: a graph that is being captured will write to it."""
+        if not any(self.buf is b for b in self.captured):
+            self.captured.append(self.buf)
 
     def arrivals(self, n):
         """n words apart from the buffer, zeroed once: arrival counters, which their user leaves at zero."""
@@ -471,8 +479,11 @@ def _verify_attention_b8(s, cache, q, args, out, out_f32, workspace):
     args.out_f32 = _b8_full(out_f32, q.shape, torch.float32, cache, "out_f32")
     # The counters save a launch, which costs the host more than the last split's work the GPU; a graph's launch costs little,
     # and zeroing counters for one call a launch itself.
-    if workspace is not None and not torch.cuda.is_current_stream_capturing():
-        args.arrivals = workspace.arrivals(cache.KVH * B8_ARRIVALS).data_ptr()
+    if workspace is not None:
+        if not torch.cuda.is_current_stream_capturing():
+            args.arrivals = workspace.arrivals(cache.KVH * B8_ARRIVALS).data_ptr()
+        elif workspace.buf is not None:
+            workspace.hold()
     ref, ws = ctypes.byref(args), workspace and workspace.buf
     while True:  # with the workspace as it is first, then with one that is large enough
         if ws is not None:

@@ -695,3 +695,75 @@ def test_graph_replays():
                      (dst.v.view(torch.uint8), dst_e.v.view(torch.uint8)), (dst.k.view(torch.uint8), dst_e.k.view(torch.uint8)),
                      (g.k.view(torch.uint8), eager.k.view(torch.uint8))):
             assert torch.equal(x, y), r
+
+
+def test_workspace_grows_after_a_capture():
+    """A graph's workspace stays its own when an eager call makes the Workspace grow past it."""
+    h = load_host()
+    rng = np.random.default_rng(12)
+    c = filled("int8", 9000 + 4, 2, 64, 3)
+    g = gpu_cache(c)
+    q = dev(rng.standard_normal((4, 8, 64)).astype(np.float16))
+    ws = h.Workspace("cuda")
+    out, _ = h.verify_attention_b8(q, g, 9000, workspace=ws)
+    want, small = out.clone(), ws.buf.numel()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        h.verify_attention_b8(q, g, 9000, out=out, workspace=ws)
+    h.verify_attention_b8(q.repeat(8, 1, 1), g, 8900, workspace=ws)
+    assert ws.buf.numel() > small
+    fill = [torch.full((small,), 7, dtype=torch.uint8, device="cuda") for _ in range(8)]  # would take a freed buffer
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and all(bool((f == 7).all()) for f in fill)
+
+
+@pytest.mark.parametrize("code", KINDS)
+def test_pages_shared_by_readers(code):
+    """Logical pages that share a physical one (a prefix read twice) are read like any other."""
+    rng = np.random.default_rng(31)
+    c = filled(code, 5 * 32, 2, 64, 6)
+    c.table = np.array([0, 1, 0, 2, 2, 3, 0, 4], np.int32)
+    M, a = 5, 8 * 32 - 5
+    q = rng.standard_normal((M, 8, 64)).astype(np.float16)
+    check_attention(c, q, a)
+    check_mass(c, q, a, 3)
+    check_evict(c, 8 * 32, 150, rng.exponential(1.0, (2, 8 * 32)).astype(np.float32), 3, 20)
+
+
+def test_as_many_heads_as_there_may_be():
+    rng = np.random.default_rng(8)
+    KVH, D, M, a = 1024, 64, 2, 40
+    c = filled("e4m3", a + M, KVH, D, 7)
+    q = rng.standard_normal((M, KVH, D)).astype(np.float16)
+    check_attention(c, q, a)
+    check_mass(c, q, a, 1)
+    check_evict(c, a + M, 35, rng.exponential(1.0, (KVH, a + M)).astype(np.float32), 2, 3)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_last_positions(D):
+    """Positions up to the last one allowed give what the same rows give at the start of a cache."""
+    h = load_host()
+    END, M, n, KVH = (1 << 31) - 64, 9, 300, 2
+    first = (END - n) // 32 * 32  # position of the rows' first page
+    table = torch.full((END // 32,), -1, dtype=torch.int32, device="cuda")
+    pages = (END - first) // 32
+    table[first // 32:] = torch.arange(pages, dtype=torch.int32, device="cuda").flip(0)
+    far, near = (h.b8_cache_alloc(pages, KVH, D, torch.int8, block_table=t) for t in (table, None))
+    n = END - first
+    kv = torch.randn((2, n, KVH, D), device="cuda").half()
+    q = torch.randn((M, 8, D), device="cuda").half()
+    got = []
+    for c, at in ((far, first), (near, 0)):
+        h.kv_write_b8(kv[0, :-M], kv[1, :-M], c, at)
+        h.kv_write_b8(kv[0, -M:], kv[1, -M:], c, at + n - M)
+        lse = torch.empty((M, 8), device="cuda")
+        o, _ = h.verify_attention_b8(q, c, at + n - M, start=at + 3, window=250, lse=lse)
+        got.append([o, lse, *h.kv_read_b8(c, at, n)])
+    for x, y in zip(*got):
+        assert torch.equal(x, y)
+    with pytest.raises(h.DsparkError):
+        h.kv_write_b8(kv[0], kv[1], far, first + 1)
