@@ -408,7 +408,7 @@ def _b8_row(t, cache, what):
     shape, stride, H, D = t.shape, t.stride(), cache.KVH, cache.D
     if len(shape) == 3 and shape[1] == H and shape[2] == D and stride[2] == 1 and (H == 1 or stride[1] == D) \
             or len(shape) == 2 and shape[1] >= H * D and stride[1] == 1:
-        return stride[0] if shape[0] > 1 else max(stride[0], H * D)
+        return stride[0] if shape[0] > 1 else H * D
     raise DsparkError(f"{what}: rows of {H} heads x {D}")
 
 
@@ -451,7 +451,7 @@ def _b8_attn_args(q, cache, a, start, window, causal, splits=0):
         raise DsparkError("q is fp16 [M][QH][D] of contiguous rows, D the cache's")
     M, QH, D = shape
     cache.check(a + M, q)
-    return B8AttnArgs(q.data_ptr(), stride[0] if M > 1 else max(stride[0], QH * D), None, None, None, None, None, 0, None,
+    return B8AttnArgs(q.data_ptr(), stride[0] if M > 1 else QH * D, None, None, None, None, None, 0, None,
                       M, QH, a, start, window, 1 if causal else 0, splits)
 
 
@@ -518,7 +518,7 @@ def _b8_accounts(t, n, cache, what):
     if len(shape) != 2 or shape[0] != cache.KVH or shape[1] < n or t.dtype != _torch().float32 \
             or (shape[1] > 1 and stride[1] != 1) or t.get_device() != cache.index:
         raise DsparkError(f"{what} is fp32 [KVH][>= {n}] on the cache's device")
-    return stride[0] if shape[0] > 1 else max(stride[0], shape[1])
+    return stride[0] if shape[0] > 1 else n
 
 
 def _attention_mass_b8(s, cache, args, lse, rows, mass_in, mass_out, stride):

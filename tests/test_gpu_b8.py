@@ -767,3 +767,26 @@ def test_last_positions(D):
         assert torch.equal(x, y)
     with pytest.raises(h.DsparkError):
         h.kv_write_b8(kv[0], kv[1], far, first + 1)
+
+
+def test_one_row_and_one_head_of_any_stride():
+    """The stride of a dimension of one says nothing: single rows, tokens and heads cut from tensors of odd widths."""
+    h = load_host()
+    g, w = h.b8_cache_alloc(2, 1, 64), h.b8_cache_alloc(2, 1, 64)
+    wide = torch.randn((3, 1, 64 * 3 + 1), device="cuda").half()
+    k, v, q = wide[:1, :, :64], wide[:1, :, 64:128], wide[:1, :, 128:192]
+    h.kv_write_b8(k, v, g, 0)
+    h.kv_write_b8(k.contiguous(), v.contiguous(), w, 0)
+    rows = torch.zeros((2, 64 * 2 + 3), device="cuda")
+    h.kv_read_b8(g, 0, 1, rows[:1, :64], rows[:1, 64:128])
+    for x, y in zip(h.kv_read_b8(w, 0, 1), (rows[0, :64], rows[0, 64:128])):
+        assert torch.equal(x.view(-1), y)
+    assert bool((rows[1:] == 0).all()) and bool((rows[:, 128:] == 0).all())
+    lse = torch.empty((1, 1), device="cuda")
+    o, _ = h.verify_attention_b8(q, g, 0, lse=lse)
+    assert torch.equal(o, h.verify_attention_b8(q.contiguous(), w, 0)[0])
+    acc, start = torch.full((1, 9), -1.0, device="cuda"), torch.ones((1, 5), device="cuda")
+    h.attention_mass_b8(q, g, 0, lse, acc, mass_in=start)
+    assert abs(float(acc[0, 0]) - 1) < 2.0 ** -15 and bool((acc[0, 1:] == -1).all())
+    kept, m = h.kv_evict_b8(g, w, 1, 1, acc)
+    assert kept.tolist() == [[0]] and torch.equal(m, acc[:, :1])
