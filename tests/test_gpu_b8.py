@@ -252,6 +252,17 @@ def test_attention_masks(code, start, window, causal, M, D):
     check_attention(c, rng.standard_normal((M, 6, D)).astype(np.float16), a, start=start, window=window, causal=causal)
 
 
+@pytest.mark.parametrize("code", KINDS)
+@pytest.mark.parametrize("QH,KVH,D,M,a", [(16, 4, 128, 8, 1001), (16, 4, 128, 9, 2000), (16, 4, 128, 12, 2900), (8, 4, 128, 2, 8000),
+                                          (32, 8, 64, 16, 2100), (32, 8, 64, 16, 4100), (10, 2, 64, 5, 1500), (2, 1, 64, 1, 9000),
+                                          (32, 8, 64, 3, 1020), (16, 4, 128, 3, 760)])
+def test_attention_few_pages(code, QH, KVH, D, M, a):
+    """One split of up to two pages a wave, and splits of a page a wave that the last of them adds: few and many of them."""
+    rng = np.random.default_rng(a)
+    c = filled(code, a + M, KVH, D, M, table=rng.permutation((a + M + 31) // 32).astype(np.int32))
+    check_attention(c, rng.standard_normal((M, QH, D)).astype(np.float16), a, gate=rng.standard_normal((M, QH)).astype(np.float32))
+
+
 @pytest.mark.parametrize("splits", [0, 1, 2, 3, 7, 64, 4096])
 @pytest.mark.parametrize("M,QH,KVH,D", [(1, 8, 2, 64), (16, 16, 2, 64), (9, 16, 2, 128), (64, 32, 2, 64), (64, 32, 2, 128),
                                         (64, 16, 1, 64), (64, 16, 1, 128), (3, 40, 2, 64), (3, 70, 2, 128)])
