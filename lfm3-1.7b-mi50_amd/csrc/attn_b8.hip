@@ -547,16 +547,25 @@ __global__ __launch_bounds__(64 * MASS_WAVES, 2) void mass_b8_kernel(B8Attn p) {
     half8 q[RB][D / 32];
     int tok[RB];
     b8_load_q<D, RB>(p, h, row0, lane, q, tok);
+    // A row past the rows, or with lse -inf, adds nothing: l2 is -inf and its q zeros, so that its weights are 2^(0 - inf)
+    // whatever q holds (a rejected draft's may be infinite or no number, and so would the score be).
+    auto draws = [&](int row, float l) { return row < R && l != -INFINITY; };
+    auto lse_of = [&](int row) {
+      const int rc = min(row, p.R - 1), t = div_by(rc, p.g_div);
+      return ldg(p.lse_in + (size_t)t * p.QH + h * p.G + rc - t * p.G);
+    };
+    float own[RB];  // of the row whose q the lane holds
     f32x4 l2[RB];
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb)
+    for (int rb = 0; rb < RB; ++rb) {
+      own[rb] = lse_of(row0 + 16 * rb + n);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int row = row0 + 16 * rb + 4 * g + i, rc = min(row, p.R - 1), t = div_by(rc, p.g_div);
-        const float l = ldg(p.lse_in + (size_t)t * p.QH + h * p.G + rc - t * p.G);
-        // past the rows, or a row that saw nothing: 2^(x - inf) adds nothing
-        l2[rb][i] = row < R && l != -INFINITY ? l * -1.44269504088896341f : -INFINITY;
+        const int row = row0 + 16 * rb + 4 * g + i;
+        const float l = lse_of(row);
+        l2[rb][i] = draws(row, l) ? l * -1.44269504088896341f : -INFINITY;
       }
+    }
     for (int b0 = w0; b0 < w1; b0 += 64) {
       const int nb = min(64, w1 - b0);
       const int pgl = b8_page(p.c, b0 + min(lane, nb - 1));
@@ -571,6 +580,12 @@ __global__ __launch_bounds__(64 * MASS_WAVES, 2) void mass_b8_kernel(B8Attn p) {
         was = from && kp < (row0 ? live : p.a) ? ldg(from + kp) : 0.f;
       };
       load(0, k[0], old[0]);
+      if (b0 == w0)  // (behind the first page's loads: ahead of them it held them back by 0.5 us)
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+          if (!draws(row0 + 16 * rb + n, own[rb]))
+#pragma unroll
+            for (int e = 0; e < D / 32; ++e) q[rb][e] = half8{0, 0, 0, 0, 0, 0, 0, 0};
       auto step = [&](int i, const u32x4 (&now)[2][D / 64], float was, u32x4 (&next)[2][D / 64], float& then) {
         load(min(i + 1, nb - 1), next, then);
         const int lp = b0 + i;

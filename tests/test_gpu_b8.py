@@ -801,3 +801,29 @@ def test_one_row_and_one_head_of_any_stride():
     assert abs(float(acc[0, 0]) - 1) < 2.0 ** -15 and bool((acc[0, 1:] == -1).all())
     kept, m = h.kv_evict_b8(g, w, 1, 1, acc)
     assert kept.tolist() == [[0]] and torch.equal(m, acc[:, :1])
+
+
+@pytest.mark.parametrize("code", KINDS)
+@pytest.mark.parametrize("QH,KVH,D,M,a,window", [(8, 2, 64, 9, 300, 0), (16, 4, 128, 8, 300, 0), (16, 1, 64, 16, 200, 0), (8, 2, 64, 5, 600, 200)])
+def test_mass_rows_that_draw_nothing(code, QH, KVH, D, M, a, window):
+    """Rejected rows and rows of lse -inf draw nothing, whatever their q and lse hold: the accounts are those of zeros there."""
+    h = load_host()
+    rng = np.random.default_rng(M)
+    g = gpu_cache(filled(code, a + M, KVH, D, 7))
+    q = rng.standard_normal((M, QH, D)).astype(np.float16)
+    lse = torch.empty((M, QH), device="cuda")
+    h.verify_attention_b8(dev(q), g, a, window=window, lse=lse)
+    n = M - 3
+    word = torch.tensor([n], dtype=torch.int32, device="cuda")
+    lse[0, 1] = -float("inf")  # a committed row that is to draw nothing
+
+    def accounts(bad_q, bad_lse):
+        x, l = q.copy(), lse.clone()
+        x[n:], x[0, 1], l[n:] = bad_q, bad_q, bad_lse
+        out = torch.full((KVH, a + M), 2.0, device="cuda")
+        return h.attention_mass_b8(dev(x), g, a, l, out, mass_in=out, rows=word, window=window)
+    want = accounts(0, 0)
+    assert bool((want[:, :a + n] > 0).all())
+    for bad in (np.nan, np.inf, -np.inf, 65504):
+        for l in (0.0, float("nan"), float("inf"), -float("inf")):
+            assert torch.equal(accounts(bad, l), want), (bad, l)
