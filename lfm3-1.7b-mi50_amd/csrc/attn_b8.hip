@@ -381,7 +381,8 @@ __global__ __launch_bounds__(64 * b8_waves(D, RB), b8_waves(D, RB) / 4) void att
     const size_t sat = (size_t)max(pgl, 0) * p.c.KVH + h;
     B8Tile<D> t[2];
     b8_load_tile<D>(p, h, __builtin_amdgcn_readlane(pgl, 0), lane, t[0]);
-    const float ksl = ldg(p.c.ks + sat) * p.c2, vsl = ldg(p.c.vs + sat);
+    const float ksl = ldg(p.c.ks + sat) * p.c2, vat = ldg(p.c.vs + sat);
+    const float vsl = pgl < 0 ? 0.f : vat;  // (what an absent page's lane loaded is another page's: infinite, it made NaN of -inf)
     // log2 vs, and 1 / vs as its very inverse. A block of zeros (scale 0) takes the smallest scale about: any will do for its
     // sum, and the smallest moves no reference.
     float lvl = __builtin_amdgcn_logf(vsl);

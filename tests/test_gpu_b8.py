@@ -827,3 +827,20 @@ def test_mass_rows_that_draw_nothing(code, QH, KVH, D, M, a, window):
     for bad in (np.nan, np.inf, -np.inf, 65504):
         for l in (0.0, float("nan"), float("inf"), -float("inf")):
             assert torch.equal(accounts(bad, l), want), (bad, l)
+
+
+@pytest.mark.parametrize("code", KINDS)
+@pytest.mark.parametrize("scale", [np.inf, np.nan, 1e-20, 1e30])
+def test_absent_pages_have_no_scale(code, scale):
+    """No entry points to physical page 0, and whatever it holds changes nothing of what is computed beside absent pages."""
+    rng = np.random.default_rng(3)
+    M, KVH, D, a = 5, 2, 64, 300
+    q = rng.standard_normal((M, 4, D)).astype(np.float16)
+    for gone in ([0], [1, 2, 3], [9], list(range(1, 9))):
+        c = filled(code, a + M, KVH, D, 3, table=np.arange(1, 11).astype(np.int32), pages=11)
+        c.table[gone] = -1
+        for x in "kv":
+            c.scale[x][0] = scale
+        c.scale["v"][c.table[9]], c.raw["v"][c.table[9]] = 0, 0  # (a block of zeros beside them)
+        check_attention(c, q, a)
+        check_mass(c, q, a, 3)
