@@ -27,6 +27,8 @@ constexpr int B8_FUSED_BYTES = 64 << 10;  // sums of one row block's splits that
 // Running reference in log2 units, set to the row's largest x + log2 vs less 8 when one passes ref + 15: P stays under 2^15,
 // and a P of 2^-22 of the largest is still a normal half (one below is off by 2^-33 of the largest at most).
 constexpr float REF_INIT = -1e30f, REF_BELOW = 8.f, REF_SLACK = 15.f;
+// log2 of the scale that stands in for a block of zeros': scales are at least 2^-33 (2^-24, the least half, over 127 or 448).
+constexpr float ZERO_LOG2 = -40.f;
 
 template <int D>
 struct B8Tile {
@@ -383,14 +385,9 @@ __global__ __launch_bounds__(64 * b8_waves(D, RB), b8_waves(D, RB) / 4) void att
     b8_load_tile<D>(p, h, __builtin_amdgcn_readlane(pgl, 0), lane, t[0]);
     const float ksl = ldg(p.c.ks + sat) * p.c2, vat = ldg(p.c.vs + sat);
     const float vsl = pgl < 0 ? 0.f : vat;  // (what an absent page's lane loaded is another page's: infinite, it made NaN of -inf)
-    // log2 vs, and 1 / vs as its very inverse. A block of zeros (scale 0) takes the smallest scale about: any will do for its
-    // sum, and the smallest moves no reference.
-    float lvl = __builtin_amdgcn_logf(vsl);
-    const bool none = !(vsl > 1e-30f);  // (no scale of a block that holds anything is as small)
-    if (__ballot(none)) {
-      const float low = -wave_max(none ? -INFINITY : -lvl);
-      if (none) lvl = low < INFINITY ? low : 0.f;
-    }
+    // log2 vs, and 1 / vs as its very inverse. A block of zeros (scale 0), which counts in the sum alone, takes one below every
+    // scale that holds anything: it moves no reference above what a later block of small values needs.
+    const float lvl = vsl > 1e-30f ? __builtin_amdgcn_logf(vsl) : ZERO_LOG2;
     const float ivl = fast_exp2(-lvl);
     // the next page's loads are in flight while a page is worked on (past the last one: that page again, from L2)
     auto step = [&](int i, const B8Tile<D>& now, B8Tile<D>& next) {

@@ -844,3 +844,15 @@ def test_absent_pages_have_no_scale(code, scale):
         c.scale["v"][c.table[9]], c.raw["v"][c.table[9]] = 0, 0  # (a block of zeros beside them)
         check_attention(c, q, a)
         check_mass(c, q, a, 3)
+
+
+def test_zeros_before_small_values():
+    """Pages of nothing but zeros in V, then small values: the running reference after the former does not lift the latter's
+    probabilities out of the half's range. 124 pages a wave, all of whose first 64 are zeros."""
+    M, QH, D, waves, pages = 8, 4, 128, 8, 124
+    a = waves * pages * 32 - M
+    c = b8.Cache("int8", waves * pages, 1, D)
+    zero = np.arange(waves * pages) % pages < 64
+    c.scale["k"][:], c.scale["v"][:] = 1, np.where(zero, 0, 1.4140625 * 2.0 ** -26)[:, None]
+    c.raw["v"][~zero] = 127
+    check_attention(c, np.zeros((M, QH, D), np.float16), a, splits=1)
