@@ -428,8 +428,12 @@ def kv_write_b8(k, v, cache, pos0, stream=None):
 
 def _kv_read_b8(s, cache, pos0, n, k, v):
     torch = _torch()
-    if k is None or v is None:
+    if k is None and v is None:
         k, v = torch.empty((2, n, cache.KVH, cache.D), dtype=torch.float32, device=cache.device).unbind()
+    elif k is None or v is None:  # the other one laid out alike
+        given = k if v is None else v
+        made = torch.empty_strided(given.shape, given.stride(), dtype=torch.float32, device=cache.device)
+        k, v = (given, made) if v is None else (made, given)
     row = _b8_row(k, cache, "kv_read_b8")
     if k.dtype != torch.float32 or v.dtype != torch.float32 or k.shape[0] < n or v.shape != k.shape \
             or _b8_row(v, cache, "kv_read_b8") != row:
@@ -439,7 +443,8 @@ def _kv_read_b8(s, cache, pos0, n, k, v):
 
 
 def kv_read_b8(cache, pos0, n, k=None, v=None, stream=None):
-    """The values of positions pos0 .. pos0+n-1 as fp32 [n][KVH][D] tensors (given, as rows, or created)."""
+    """The values of positions pos0 .. pos0+n-1 as fp32 [n][KVH][D] tensors, given (as rows) or created; one of them alone
+    given, the other is created of its shape and strides."""
     cache.check(pos0 + n, k, v)
     return _b8_on(cache, stream, _kv_read_b8, pos0, n, k, v)
 

@@ -856,3 +856,18 @@ def test_zeros_before_small_values():
     c.scale["k"][:], c.scale["v"][:] = 1, np.where(zero, 0, 1.4140625 * 2.0 ** -26)[:, None]
     c.raw["v"][~zero] = 127
     check_attention(c, np.zeros((M, QH, D), np.float16), a, splits=1)
+
+
+def test_reads_into_one_given_tensor():
+    """K or V alone given: it is filled, and the other one created."""
+    h = load_host()
+    c = filled("int8", 77, 3, 64, 1)
+    g, want = gpu_cache(c), c.read(30, 40)
+    for i, x in enumerate("kv"):
+        for given in (torch.full((40, 3, 64), 7.0, device="cuda"), torch.full((41, 200), 7.0, device="cuda")):
+            got = h.kv_read_b8(g, 30, 40, **{x: given})
+            assert got[i] is given
+            for y, w in zip(got, want):
+                y = y[:40, :192] if y.dim() == 2 else y
+                np.testing.assert_array_equal(y.reshape(40, 3, 64).cpu().numpy(), w.astype(np.float32))
+            assert given.dim() == 3 or (bool((given[40:] == 7).all()) and bool((given[:, 192:] == 7).all()))
