@@ -183,7 +183,7 @@ size_t dspark_verify_attention_b8_workspace(const dspark_b8_cache* c, const dspa
 int dspark_verify_attention_b8(const dspark_b8_cache* c, const dspark_b8_attn_args* a, dspark_stream_t stream) {
   if (!rows_ok(c, a) || !query_ok(c, a)) return DSPARK_EINVAL;
   if (!a->out && !a->out_f32) return DSPARK_EINVAL;
-  if (a->arrivals && !on(a->arrivals, 4)) return DSPARK_EINVAL;
+  if ((a->arrivals && !on(a->arrivals, 4)) || (a->lse && !on(a->lse, 4)) || (a->gate && !on(a->gate, 4))) return DSPARK_EINVAL;
   if ((a->out && !on(a->out, 16)) || (a->out_f32 && !on(a->out_f32, 16))) return DSPARK_EINVAL;
   B8Attn p = attn(c, a);
   b8_attn_plan(p, c->D, a->splits, device_cus());

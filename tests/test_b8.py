@@ -222,3 +222,12 @@ def test_calls_refuse_memory_that_meets():
     bytes_ = (7 * 1100 + 1016) * 4
     for at in over([held[0], held[2], (50 * MB, table), (60 * MB, 2 * out), (63 * MB, heads), (70 * MB, 4), (80 * MB, bytes_)], bytes_):
         assert L.dspark_attention_mass_b8(c, ok, 63 * MB, 70 * MB, 80 * MB, at, 1100, None) == EINVAL, at
+
+
+def test_attention_checks_the_alignment_of_lse_and_gate():
+    L = load_host().lib()
+    MB = 1 << 20
+    c = ctypes.byref(cache(k=16 * MB, v=32 * MB, k_scale=48 * MB, v_scale=49 * MB))
+    for bad in (dict(lse=63 * MB + 2), dict(lse=63 * MB + 1), dict(gate=64 * MB + 2), dict(gate=64 * MB + 3)):
+        a = attn(**{**dict(q=60 * MB, out=61 * MB, lse=63 * MB, gate=64 * MB, workspace=128 * MB), **bad})
+        assert L.dspark_verify_attention_b8(c, ctypes.byref(a), None) == EINVAL, bad
