@@ -388,6 +388,13 @@ def b8_cache_alloc(n_pages, KVH, D, dtype=None, device="cuda", block_table=None)
     return B8Cache(*codes, *scales, block_table)
 
 
+def _b8_words(every, what):
+    """`every`, the bitwise or of a call's counts and positions, says whether one is negative or past the 31 bits of the C ABI's
+    (ctypes would cut it to its low 32 in silence)."""
+    if every >> 31:
+        raise DsparkError(f"{what}: counts and positions are from 0 to 2^31 - 1")
+
+
 def _b8_on(cache, stream, call, *args):
     """call(handle of the stream, cache, *args) with the cache's device current and `stream` (default: that device's current
     one) the stream that allocations belong to."""
@@ -420,6 +427,7 @@ def kv_write_b8(k, v, cache, pos0, stream=None):
     """Append k, v fp16 [n][KVH][D] (or [n][row >= KVH*D]; rows may lie inside wider ones) as positions pos0 .. pos0+n-1."""
     f16 = _torch().float16
     row, n = _b8_row(k, cache, "kv_write_b8"), k.shape[0]
+    _b8_words(pos0 | n, "kv_write_b8")
     if v.shape != k.shape or _b8_row(v, cache, "kv_write_b8") != row or k.dtype != f16 or v.dtype != f16:
         raise DsparkError("kv_write_b8: k and v are fp16, of one shape and row stride")
     cache.check(pos0 + n, k, v)
@@ -445,6 +453,7 @@ def _kv_read_b8(s, cache, pos0, n, k, v):
 def kv_read_b8(cache, pos0, n, k=None, v=None, stream=None):
     """The values of positions pos0 .. pos0+n-1 as fp32 [n][KVH][D] tensors, given (as rows) or created; one of them alone
     given, the other is created of its shape and strides."""
+    _b8_words(pos0 | n, "kv_read_b8")
     cache.check(pos0 + n, k, v)
     return _b8_on(cache, stream, _kv_read_b8, pos0, n, k, v)
 
@@ -455,6 +464,7 @@ def _b8_attn_args(q, cache, a, start, window, causal, splits=0):
             or (shape[1] > 1 and stride[1] != cache.D):
         raise DsparkError("q is fp16 [M][QH][D] of contiguous rows, D the cache's")
     M, QH, D = shape
+    _b8_words(a | start | window | splits, "b8 attention")
     cache.check(a + M, q)
     return B8AttnArgs(q.data_ptr(), stride[0] if M > 1 else QH * D, None, None, None, None, None, 0, None,
                       M, QH, a, start, window, 1 if causal else 0, splits)
@@ -567,6 +577,7 @@ def kv_evict_b8(cache, dst, length, keep, mass, sinks=0, recent=0, kept=None, ma
     """Keep `keep` of the cache's `length` positions per KV head -- the first `sinks`, the last `recent`, and the rest by mass
     (fp32 [KVH][>= length]) -- as positions 0..keep-1 of `dst`, another B8Cache of the same heads and codes. Returns
     (kept int32 [KVH][keep] ascending, their mass), as given/created."""
+    _b8_words(length | keep | sinks | recent, "kv_evict_b8")
     cache.check(length, dst.k)
     dst.check(keep)
     stride = _b8_accounts(mass, length, cache, "mass")

@@ -231,3 +231,22 @@ def test_attention_checks_the_alignment_of_lse_and_gate():
     for bad in (dict(lse=63 * MB + 2), dict(lse=63 * MB + 1), dict(gate=64 * MB + 2), dict(gate=64 * MB + 3)):
         a = attn(**{**dict(q=60 * MB, out=61 * MB, lse=63 * MB, gate=64 * MB, workspace=128 * MB), **bad})
         assert L.dspark_verify_attention_b8(c, ctypes.byref(a), None) == EINVAL, bad
+
+
+@pytest.mark.parametrize("far", [1 << 31, 1 << 32, (1 << 32) + 3, -1, -(1 << 32)])
+def test_the_binding_refuses_positions_past_32_bits(far):
+    """ctypes would hand over their low 32 bits, a position or count somewhere else."""
+    import torch
+    h = load_host()
+    c, d = (h.b8_cache_alloc(4, 2, 64, device="cpu") for _ in "cd")
+    row, q = torch.zeros((4, 2, 64), dtype=torch.float16), torch.zeros((4, 8, 64), dtype=torch.float16)
+    lse, acc = torch.zeros((4, 8)), torch.zeros((2, 128))
+    for call in (lambda: h.kv_write_b8(row, row, c, far), lambda: h.kv_read_b8(c, far, 4), lambda: h.kv_read_b8(c, 0, far),
+                 lambda: h.verify_attention_b8(q, c, far), lambda: h.verify_attention_b8(q, c, 9, start=far),
+                 lambda: h.verify_attention_b8(q, c, 9, window=far), lambda: h.verify_attention_b8(q, c, 9, splits=far),
+                 lambda: h.attention_mass_b8(q, c, far, lse, acc), lambda: h.attention_mass_b8(q, c, 9, lse, acc, start=far),
+                 lambda: h.attention_mass_b8(q, c, 9, lse, acc, window=far), lambda: h.kv_evict_b8(c, d, far, 5, acc),
+                 lambda: h.kv_evict_b8(c, d, 90, far, acc), lambda: h.kv_evict_b8(c, d, 90, 5, acc, sinks=far),
+                 lambda: h.kv_evict_b8(c, d, 90, 5, acc, recent=far)):
+        with pytest.raises(h.DsparkError, match="counts and positions"):
+            call()
