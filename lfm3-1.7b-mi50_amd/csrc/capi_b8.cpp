@@ -91,14 +91,26 @@ B8Attn attn(const dspark_b8_cache* c, const dspark_b8_attn_args* a) {
   return p;
 }
 
-// Memory that a call reads or writes; p NULL or n 0: none.
+// Memory that a call reads or writes: `rows` pieces of n bytes, `stride` apart (stride >= n); p NULL or n 0: none.
 struct Span {
   const void* p;
   size_t n;
+  size_t rows = 1, stride = 0;
 };
+// A piece of n bytes at `at` and some row of y share a byte: of y's rows the first that ends behind `at` begins before the piece ends.
+bool meets(uintptr_t at, size_t n, const Span& y) {
+  const uintptr_t b = reinterpret_cast<uintptr_t>(y.p);
+  const size_t i = at < b + y.n ? 0 : y.rows > 1 ? (at - b - y.n) / y.stride + 1 : 1;
+  return i < y.rows && b + i * y.stride < at + n;
+}
 bool overlap(const Span& x, const Span& y) {
+  if (!x.p || !y.p || !x.n || !y.n) return false;
   const uintptr_t a = reinterpret_cast<uintptr_t>(x.p), b = reinterpret_cast<uintptr_t>(y.p);
-  return a && b && x.n && y.n && a < b + y.n && b < a + x.n;
+  if (a >= b + (y.rows - 1) * y.stride + y.n || b >= a + (x.rows - 1) * x.stride + x.n) return false;
+  if (x.rows > y.rows) return overlap(y, x);  // (of two spans here one has at most 1024 rows, heads or tokens)
+  for (size_t i = 0; i < x.rows; ++i)
+    if (meets(a + i * x.stride, x.n, y)) return true;
+  return false;
 }
 // Nothing that is written shares a byte with what is read, nor with anything else that is written: workgroups read and store in
 // no order among each other.
@@ -117,10 +129,14 @@ size_t code_bytes(const dspark_b8_cache* c) { return (size_t)c->kv_pages * c->KV
 Span table(const dspark_b8_cache* c, int64_t positions) { return {c->block_table, (size_t)pages_of(positions) * sizeof(int32_t)}; }
 // Rows of KVH D elements, row_stride apart.
 Span rows_of(const dspark_b8_cache* c, const void* p, int64_t n, int64_t row_stride, size_t element) {
-  return {p, ((size_t)(n - 1) * row_stride + (size_t)c->KVH * c->D) * element};
+  return {p, (size_t)c->KVH * c->D * element, (size_t)n, (size_t)row_stride * element};
 }
 Span query(const dspark_b8_cache* c, const dspark_b8_attn_args* a) {
-  return {a->q, ((size_t)(a->M - 1) * a->q_stride + (size_t)a->QH * c->D) * 2};
+  return {a->q, (size_t)a->QH * c->D * 2, (size_t)a->M, (size_t)a->q_stride * 2};
+}
+// Accounts of n positions of every head.
+Span accounts(const dspark_b8_cache* c, const float* p, int64_t n, int64_t stride) {
+  return {p, (size_t)n * sizeof(float), (size_t)c->KVH, (size_t)stride * sizeof(float)};
 }
 // Two sets of n such rows share a byte (they may lie in turn in wider rows).
 bool rows_meet(const Span& x, const Span& y, int64_t n, size_t row, size_t stride) {
@@ -204,10 +220,10 @@ int dspark_attention_mass_b8(const dspark_b8_cache* c, const dspark_b8_attn_args
   if (!rows_ok(c, a) || !query_ok(c, a) || !on(lse, 4) || !on(mass_out, 4) || (rows && !on(rows, 4))) return DSPARK_EINVAL;
   if (mass_stride < (int64_t)a->a + a->M) return DSPARK_EINVAL;
   if (mass_in && !on(mass_in, 4)) return DSPARK_EINVAL;
-  const size_t bytes = ((size_t)(c->KVH - 1) * mass_stride + a->a + a->M) * sizeof(float);
-  const Span reads[7] = {{mass_in == mass_out ? nullptr : mass_in, bytes}, query(c, a), {lse, (size_t)a->M * a->QH * 4}, {rows, 4},
+  const int64_t n = (int64_t)a->a + a->M;
+  const Span reads[7] = {accounts(c, mass_in == mass_out ? nullptr : mass_in, n, mass_stride), query(c, a), {lse, (size_t)a->M * a->QH * 4}, {rows, 4},
                          {c->k, code_bytes(c)}, {c->k_scale, scale_bytes(c)}, table(c, (int64_t)a->a + a->M)};
-  const Span writes[1] = {{mass_out, bytes}};
+  const Span writes[1] = {accounts(c, mass_out, n, mass_stride)};
   if (!apart(reads, writes)) return DSPARK_EINVAL;
   B8Attn p = attn(c, a);
   p.lse_in = lse;
@@ -235,10 +251,10 @@ int dspark_kv_evict_b8(const dspark_b8_cache* src, const dspark_b8_cache* dst, i
   if (need && (!on(workspace, 16) || workspace_bytes < need)) return DSPARK_ENOSPACE;
   // a destination page may be written while other rows are still read
   const Span reads[7] = {{src->k, code_bytes(src)}, {src->v, code_bytes(src)}, {src->k_scale, scale_bytes(src)},
-                         {src->v_scale, scale_bytes(src)}, {mass, ((size_t)(src->KVH - 1) * mass_stride + length) * 4},
+                         {src->v_scale, scale_bytes(src)}, accounts(src, mass, length, mass_stride),
                          table(src, length), table(dst, keep)};
   const Span writes[7] = {{dst->k, code_bytes(dst)}, {dst->v, code_bytes(dst)}, {dst->k_scale, scale_bytes(dst)},
-                          {dst->v_scale, scale_bytes(dst)}, {mass_out, ((size_t)(src->KVH - 1) * mass_out_stride + keep) * 4},
+                          {dst->v_scale, scale_bytes(dst)}, accounts(src, mass_out, keep, mass_out_stride),
                           {kept, (size_t)src->KVH * keep * 4}, {workspace, need}};
   if (!apart(reads, writes)) return DSPARK_EINVAL;
   B8Evict p;

@@ -871,3 +871,28 @@ def test_reads_into_one_given_tensor():
                 y = y[:40, :192] if y.dim() == 2 else y
                 np.testing.assert_array_equal(y.reshape(40, 3, 64).cpu().numpy(), w.astype(np.float32))
             assert given.dim() == 3 or (bool((given[40:] == 7).all()) and bool((given[:, 192:] == 7).all()))
+
+
+def test_accounts_in_the_gaps_of_others():
+    """Rows of accounts that lie in turn in one buffer share no byte and are taken; rows that meet are refused."""
+    h = load_host()
+    rng = np.random.default_rng(3)
+    KVH, D, M, a, keep = 3, 64, 4, 300, 70
+    n = a + M
+    g = gpu_cache(filled("int8", n, KVH, D, 7))
+    q, lse = dev(rng.standard_normal((M, 6, D)).astype(np.float16)), torch.empty((M, 6), device="cuda")
+    h.verify_attention_b8(q, g, a, lse=lse)
+    both = torch.rand((KVH, 2, n + keep), device="cuda")
+    start = both[:, 0].clone()
+    want = h.attention_mass_b8(q, g, a, lse, torch.zeros_like(start), mass_in=start)
+    got = h.attention_mass_b8(q, g, a, lse, both[:, 1], mass_in=both[:, 0])
+    assert torch.equal(got[:, :n], want[:, :n]) and torch.equal(both[:, 0], start)
+    d = [h.b8_cache_alloc(3, KVH, D) for _ in "ab"]
+    kept, m = h.kv_evict_b8(g, d[0], n, keep, want, sinks=2, recent=4)
+    kept2, m2 = h.kv_evict_b8(g, d[1], n, keep, both[:, 1, :n], sinks=2, recent=4, mass_out=both[:, 1, n:])
+    assert torch.equal(kept, kept2) and torch.equal(m, m2) and torch.equal(d[0].k, d[1].k)
+    for mass_in, mass_out in ((both[:, 0], both[:, 0, 4:]), (both[:, 0, keep:], both[:, 0]), (both.view(KVH, -1)[:, n - 1:], both[:, 0])):
+        with pytest.raises(h.DsparkError):
+            h.attention_mass_b8(q, g, a, lse, mass_out, mass_in=mass_in)
+    with pytest.raises(h.DsparkError):
+        h.kv_evict_b8(g, d[1], n, keep, both[:, 1, :n], mass_out=both[:, 1, n - 1:n - 1 + keep])
