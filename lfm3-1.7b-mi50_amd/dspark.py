@@ -174,11 +174,19 @@ class Workspace:
         torch = _torch()
         nbytes = max(int(nbytes), 256)
         if self.buf is None or self.buf.numel() < nbytes:
+            self.let_go(self.buf)
             # zero-filled: the split-K GEMM keeps its arrival counters here (left at zero by every call)
             self.buf = torch.zeros(nbytes, dtype=torch.uint8, device=self.device)
         if self.buf.is_cuda and torch.cuda.is_current_stream_capturing():
             self.hold()
         return self.buf
+
+    @staticmethod
+    def let_go(t):
+        """Work on the current stream may still use the buffer that is about to be replaced, which can belong to another one:
+        its memory is not handed out before that work is done."""
+        if t is not None and t.is_cuda:
+            t.record_stream(_torch().cuda.current_stream(t.device))
 
     def hold(self):
         """The buffer stays allocated as long as the workspace: a graph that is being captured will write to it."""
@@ -189,6 +197,7 @@ class Workspace:
         """n words apart from the buffer, zeroed once: arrival counters, which their user leaves at zero."""
         torch = _torch()
         if self.words is None or self.words.numel() < n:
+            self.let_go(self.words)
             self.words = torch.zeros(n, dtype=torch.int32, device=self.device)
         return self.words
 

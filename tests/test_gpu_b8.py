@@ -896,3 +896,24 @@ def test_accounts_in_the_gaps_of_others():
             h.attention_mass_b8(q, g, a, lse, mass_out, mass_in=mass_in)
     with pytest.raises(h.DsparkError):
         h.kv_evict_b8(g, d[1], n, keep, both[:, 1, :n], mass_out=both[:, 1, n - 1:n - 1 + keep])
+
+
+@pytest.mark.parametrize("words", [False, True])
+def test_workspace_grows_on_another_stream(words):
+    """A buffer that work on the current stream still uses is not handed to its own stream when the workspace outgrows it."""
+    h = load_host()
+    side, ws = torch.cuda.Stream(), h.Workspace("cuda")
+    old = ws.arrivals(1 << 18) if words else ws.get(1 << 20)
+    at, size = old.data_ptr(), old.numel()
+    x = torch.randn((8192, 8192), device="cuda")
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(4):  # work of some milliseconds that the buffer's last use stands behind
+            x = (x @ x).clamp_(-1, 1)
+        old.fill_(3)
+        del old
+        ws.arrivals(2 * size) if words else ws.get(2 * size)
+    taken = [torch.empty(size, dtype=torch.int32 if words else torch.uint8, device="cuda") for _ in range(4)]
+    busy = not side.query()
+    assert busy and all(t.data_ptr() != at for t in taken)
+    torch.cuda.synchronize()
