@@ -250,3 +250,40 @@ def test_the_binding_refuses_positions_past_32_bits(far):
                  lambda: h.kv_evict_b8(c, d, 90, 5, acc, recent=far)):
         with pytest.raises(h.DsparkError, match="counts and positions"):
             call()
+
+
+def test_each_refusal_stands_alone():
+    """Arguments that are refused for one reason, beside ones that nothing is wrong with (no memory meets other memory there)."""
+    import torch
+    L = load_host().lib()
+    MB = 1 << 20
+    c = ctypes.byref(cache(k=16 * MB, v=32 * MB, k_scale=48 * MB, v_scale=49 * MB))
+    base = dict(q=60 * MB, out=61 * MB, out_f32=62 * MB, lse=63 * MB, gate=64 * MB, workspace=128 * MB, arrivals=65 * MB)
+
+    def attend(**bad):
+        return L.dspark_verify_attention_b8(c, ctypes.byref(attn(**{**base, **bad})), None)
+
+    def mass(lse=63 * MB, rows=70 * MB, mi=80 * MB, mo=90 * MB, stride=1100):
+        return L.dspark_attention_mass_b8(c, ctypes.byref(attn(**base)), lse, rows, mi, mo, stride, None)
+
+    def write(k=60 * MB, v=61 * MB, row=600, pos0=990, n=10):
+        return L.dspark_kv_write_b8(c, k, v, row, pos0, n, None)
+
+    def read(k=60 * MB, v=61 * MB, row=600, pos0=990, n=10):
+        return L.dspark_kv_read_b8(c, pos0, n, k, v, row, None)
+    need = L.dspark_verify_attention_b8_workspace(c, ctypes.byref(attn(**base)))
+    for bad in (dict(q=None), dict(q=60 * MB + 8), dict(q_stride=2040), dict(q_stride=2052), dict(out=None, out_f32=None),
+                dict(out=61 * MB + 8), dict(out_f32=62 * MB + 8), dict(arrivals=65 * MB + 2), dict(M=0), dict(M=65), dict(QH=12),
+                dict(a=-1), dict(a=3190), dict(start=-1), dict(window=-1), dict(splits=-1)):
+        assert attend(**bad) == EINVAL, bad
+    for bad in (dict(workspace=None), dict(workspace=128 * MB + 8), dict(workspace_bytes=need - 1)):
+        assert attend(**bad) == ENOSPACE, bad
+    for bad in (dict(lse=None), dict(lse=63 * MB + 2), dict(rows=70 * MB + 2), dict(mi=80 * MB + 2), dict(mo=None), dict(mo=90 * MB + 2),
+                dict(stride=1015)):
+        assert mass(**bad) == EINVAL, bad
+    for bad in (dict(k=None), dict(v=None), dict(k=60 * MB + 8), dict(v=61 * MB + 8), dict(row=504), dict(pos0=-1), dict(n=-1),
+                dict(pos0=3191)):
+        assert write(**bad) == EINVAL and read(**bad) == EINVAL, bad
+    assert write(row=516) == EINVAL and read(row=514) == EINVAL
+    if not torch.cuda.is_available():  # (the launch itself fails here)
+        assert not {0, EINVAL, ENOSPACE} & {attend(), mass(), mass(rows=None), mass(mi=None), mass(mi=90 * MB), write(), read()}

@@ -917,3 +917,104 @@ def test_workspace_grows_on_another_stream(words):
     busy = not side.query()
     assert busy and all(t.data_ptr() != at for t in taken)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("code", KINDS)
+@pytest.mark.parametrize("D,M,waves", [(64, 4, 16), (64, 8, 12), (64, 12, 12), (64, 16, 8), (128, 3, 12), (128, 8, 8), (128, 16, 8)])
+@pytest.mark.parametrize("extra", [0.4, 40])
+def test_attention_many_pages_a_wave(code, D, M, waves, extra):
+    """A split of 64 pages a wave, of one more for some of them, and of over 100, with blocks of zeros and absent pages
+    anywhere."""
+    rng = np.random.default_rng(int(extra) + M)
+    pages = int(waves * (64 + extra))
+    a, QH = pages * 32 - M - 3, 4
+    c = b8.Cache(code, pages, 1, D, rng.permutation(pages).astype(np.int32))
+    top = 127 if code == "int8" else 126  # (the largest code as a byte)
+    for x in "kv":
+        raw = rng.integers(0, top + 1, c.raw[x].shape).astype(np.uint8)
+        if code == "int8":
+            raw = (raw.astype(np.int8) * rng.choice([-1, 1], raw.shape).astype(np.int8)).view(np.uint8)
+        else:
+            raw |= rng.choice([0, 128], raw.shape).astype(np.uint8)
+        c.raw[x][:] = raw
+        c.scale[x][:] = b8.scale_of(code, rng.uniform(0.5, 4, c.scale[x].shape))
+        none = rng.random(pages) < 0.15
+        c.scale[x][none], c.raw[x][none] = 0, 0
+    c.table[rng.random(pages) < 0.1] = -1
+    check_attention(c, rng.standard_normal((M, QH, D)).astype(np.float16), a, splits=1)
+
+
+@pytest.mark.parametrize("code", KINDS)
+def test_mass_many_pages_a_wave(code):
+    """So many heads that a wave has over 64 pages, against the accounts in float64 on the GPU."""
+    h = load_host()
+    KVH, D, M, pages = 1024, 64, 2, 270
+    a = pages * 32 - 37
+    kind = torch.randint(0, 127, (pages, KVH, 32, D), dtype=torch.uint8, device="cuda")
+    v = torch.zeros((pages, KVH, 32, D), dtype=torch.uint8, device="cuda")
+    scale = torch.rand((pages, KVH), device="cuda").mul_(2).sub_(8).exp2_() / (127 if code == "int8" else 448)
+    scale = (scale.view(torch.int32) & ~0xffff).view(torch.float32)  # (8 significant bits: values are exact in fp32)
+    table = torch.randperm(pages, device="cuda").int()
+    table[[5, 63, 64, 200]] = -1
+    c = h.B8Cache(kind.view(TYPES[code]), v.view(TYPES[code]), scale, scale.clone(), table)
+    q = torch.randn((M, KVH, D), device="cuda").half()
+    lse = torch.empty((M, KVH), device="cuda")
+    h.verify_attention_b8(q, c, a, lse=lse)
+    start = torch.rand((KVH, a + M), device="cuda")
+    got = h.attention_mass_b8(q, c, a, lse, torch.zeros_like(start), mass_in=start)
+    p, want = torch.arange(a + M, device="cuda"), torch.where(torch.arange(a + M, device="cuda") < a, start.double(), 0)
+    here = (table >= 0)[p // 32]
+    k = h.kv_read_b8(c, 0, a + M)[0]
+    for t in range(M):
+        see = here & (p <= a + t)
+        for h0 in range(0, KVH, 128):
+            x = (k[:, h0:h0 + 128].double() * q[t, h0:h0 + 128].double()).sum(-1).t() / D ** 0.5
+            want[h0:h0 + 128] += torch.where(see, (x - lse[t, h0:h0 + 128, None].double()).exp(), 0)
+    assert bool(((got - want).abs() <= 2.0 ** -16 * want + 1e-9).all())
+
+
+def accounts_of(name, rng, shape):
+    m = np.ones(shape, np.float32)
+    if name == "few":
+        m = rng.integers(0, 3, shape).astype(np.float32)
+    elif name == "special":
+        m = rng.choice(np.array([np.nan, np.inf, -np.inf, 0.0, -0.0, 1.0], np.float32), shape)
+        m.view(np.uint32)[:, 5] = 0xFFC00001  # a NaN with its sign bit set
+    elif name == "negative":
+        m = -rng.exponential(1.0, shape).astype(np.float32)
+    elif name == "subnormal":
+        m = rng.integers(0, 1 << 22, shape).astype(np.uint32).view(np.float32)
+    elif name == "bits":
+        m = (np.uint32(0x3F800000) + rng.integers(0, 700, shape).astype(np.uint32)).view(np.float32)
+    return m
+
+
+def coded(code, T, KVH, D, rng):
+    """A cache of random codes and scales."""
+    n = (T + 31) // 32
+    c = b8.Cache(code, n, KVH, D, rng.permutation(n).astype(np.int32))
+    for x in "kv":
+        c.raw[x][:] = rng.integers(-127, 128, c.raw[x].shape).astype(np.int8).view(np.uint8)
+        if code == "e4m3":
+            c.raw[x][c.raw[x] & 127 == 127] = 0
+        c.scale[x][:] = b8.scale_of(code, rng.integers(1, 5, c.scale[x].shape).astype(np.float64))
+    return c
+
+
+@pytest.mark.parametrize("name,T", [(x, 40000) for x in ("equal", "few", "special", "negative", "subnormal", "bits")]
+                         + [("few", 270011), ("special", 270011)])
+def test_evict_order_by_parts(name, T):
+    """The accounts of test_evict_order over several workgroups a head, of one tile and of two; the rows moved with them."""
+    rng = np.random.default_rng(T)
+    c = coded("int8" if T == 40000 else "e4m3", T, 2, 64, rng)
+    m = accounts_of(name, rng, (2, T + 1))
+    for keep, sinks, recent in ((T // 2, 3, 40), (T - 100, 0, 0), (1044, 4, 39)):
+        check_evict(c, T, keep, m, sinks, recent)
+
+
+@pytest.mark.parametrize("T,sinks,recent", [(40000, 4, 1020), (40000, 0, 33), (17000, 64, 0), (16400, 1, 2), (16384, 5, 7)])
+def test_evict_all_but_the_ends(T, sinks, recent):
+    """Nothing of the middle is kept, from few positions and from many."""
+    rng = np.random.default_rng(recent)
+    c = coded("int8", T, 3, 64, rng)
+    check_evict(c, T, sinks + recent, accounts_of("few", rng, (3, T)), sinks, recent)
