@@ -546,7 +546,8 @@ def _b8_accounts(t, n, cache, what):
 
 
 def _attention_mass_b8(s, cache, args, lse, rows, mass_in, mass_out, stride):
-    check(lib().dspark_attention_mass_b8(cache.ref, ctypes.byref(args), lse, None if rows is None else rows.data_ptr(),
+    lse = lse.contiguous()
+    check(lib().dspark_attention_mass_b8(cache.ref, ctypes.byref(args), lse.data_ptr(), None if rows is None else rows.data_ptr(),
                                          None if mass_in is None else mass_in.data_ptr(), mass_out.data_ptr(), stride, s),
           "dspark_attention_mass_b8")
     return mass_out
@@ -554,16 +555,18 @@ def _attention_mass_b8(s, cache, args, lse, rows, mass_in, mass_out, stride):
 
 def attention_mass_b8(q, cache, a, lse, mass_out, mass_in=None, rows=None, start=0, window=0, causal=True, stream=None):
     """Add the attention weights of tokens t < rows (an int32 device word, None = all of q's) to the accounts of the keys they
-    see: mass_out fp32 [KVH][>= a+M] from mass_in (None = zeros, or mass_out itself) and verify_attention_b8's lse."""
+    see: mass_out fp32 [KVH][>= a+M] from mass_in (None = zeros, or mass_out itself) and verify_attention_b8's lse (copied
+    if its strides are others)."""
     torch = _torch()
     args = _b8_attn_args(q, cache, a, start, window, causal)
-    lse_ptr = _b8_full(lse, q.shape[:2], torch.float32, cache, "lse")
+    if lse is None or lse.shape != q.shape[:2] or lse.dtype != torch.float32 or lse.get_device() != cache.index:
+        raise DsparkError(f"lse is fp32 of shape {tuple(q.shape[:2])} on the cache's device")
     stride = _b8_accounts(mass_out, a + args.M, cache, "mass_out")
-    if lse_ptr is None or (mass_in is not None and _b8_accounts(mass_in, a + args.M, cache, "mass_in") != stride):
-        raise DsparkError("attention_mass_b8: lse is given, and mass_in and mass_out have one stride")
+    if mass_in is not None and _b8_accounts(mass_in, a + args.M, cache, "mass_in") != stride:
+        raise DsparkError("attention_mass_b8: mass_in and mass_out have one stride")
     if rows is not None and (rows.dtype != torch.int32 or rows.numel() < 1 or rows.get_device() != cache.index):
         raise DsparkError("attention_mass_b8: rows is an int32 word on the cache's device")
-    return _b8_on(cache, stream, _attention_mass_b8, args, lse_ptr, rows, mass_in, mass_out, stride)
+    return _b8_on(cache, stream, _attention_mass_b8, args, lse, rows, mass_in, mass_out, stride)
 
 
 def _kv_evict_b8(s, cache, dst, length, keep, mass, stride, sinks, recent, kept, mass_out, workspace):

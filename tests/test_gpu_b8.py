@@ -1018,3 +1018,24 @@ def test_evict_all_but_the_ends(T, sinks, recent):
     rng = np.random.default_rng(recent)
     c = coded("int8", T, 3, 64, rng)
     check_evict(c, T, sinks + recent, accounts_of("few", rng, (3, T)), sinks, recent)
+
+
+@pytest.mark.parametrize("QH,KVH,M", [(8, 8, 16), (8, 2, 5), (1, 1, 7), (4, 4, 1)])
+def test_mass_takes_lse_of_any_strides(QH, KVH, M):
+    """Heads before tokens in memory, and cut from wider rows; on the current stream and on another."""
+    h = load_host()
+    rng = np.random.default_rng(M)
+    a, side = 300, torch.cuda.Stream()
+    g = gpu_cache(filled("e4m3", a + M, KVH, 64, 7))
+    q, lse = dev(rng.standard_normal((M, QH, 64)).astype(np.float16)), torch.empty((M, QH), device="cuda")
+    h.verify_attention_b8(q, g, a, lse=lse)
+    want = h.attention_mass_b8(q, g, a, lse, torch.zeros((KVH, a + M), device="cuda"))
+    wide = torch.zeros((M, 2 * QH + 1), device="cuda")
+    wide[:, 1::2] = lse
+    for x in (lse.t().contiguous().t(), wide[:, 1::2]):
+        assert x.shape == lse.shape and torch.equal(h.attention_mass_b8(q, g, a, x, torch.zeros_like(want)), want)
+        got = torch.zeros_like(want)
+        torch.cuda.synchronize()
+        h.attention_mass_b8(q, g, a, x, got, stream=side)
+        side.synchronize()
+        assert torch.equal(got, want)
