@@ -33,8 +33,8 @@ bool fits(const dspark_b8_cache* c, int64_t end) {
   return end <= POS_MAX && (c->block_table || pages_of(end) <= c->kv_pages);
 }
 
-// A launch of a wave per (page, K or V, head).
-bool waves_fit(const dspark_b8_cache* c, int64_t pages) { return pages * 2 * c->KVH < (int64_t)1 << 30; }
+// A launch of a wave per (page, K or V, head), four a workgroup: under 2^32 threads.
+bool waves_fit(const dspark_b8_cache* c, int64_t pages) { return pages * 2 * c->KVH <= ((int64_t)1 << 26) - 4; }
 
 B8Pool pool(const dspark_b8_cache* c) {
   B8Pool p;

@@ -287,3 +287,17 @@ def test_each_refusal_stands_alone():
     assert write(row=516) == EINVAL and read(row=514) == EINVAL
     if not torch.cuda.is_available():  # (the launch itself fails here)
         assert not {0, EINVAL, ENOSPACE} & {attend(), mass(), mass(rows=None), mass(mi=None), mass(mi=90 * MB), write(), read()}
+
+
+def test_no_launch_past_what_a_grid_holds():
+    """A wave of 64 threads for each page, K or V, and head: under 2^32 threads. Sparse tables reach it with little memory."""
+    L = load_host().lib()
+    MB, GB = 1 << 20, 1 << 30
+    for KVH, page in ((1, 1 << 25), (2, 1 << 24), (8, 1 << 22), (1024, 1 << 15), (1, (1 << 25) - 1)):
+        n = 32 * page
+        src = cache(k=16 * MB, v=32 * MB, k_scale=48 * MB, v_scale=49 * MB, block_table=GB, KVH=KVH, kv_pages=1)
+        dst = cache(k=17 * MB, v=33 * MB, k_scale=50 * MB, v_scale=51 * MB, block_table=2 * GB, KVH=KVH, kv_pages=1)
+        far = 1 << 50
+        assert L.dspark_kv_evict_b8(ctypes.byref(src), ctypes.byref(dst), n, n, 0, 0, far, n, 2 * far, 3 * far, n, 4 * far, far, None) == EINVAL
+        assert L.dspark_kv_write_b8(ctypes.byref(src), far, 2 * far, 64 * KVH, 0, n, None) == EINVAL
+        assert L.dspark_kv_read_b8(ctypes.byref(src), 0, n, far, 2 * far, 64 * KVH, None) == EINVAL
