@@ -170,7 +170,8 @@ typedef struct dspark_b8_cache {
 /* Append: K/V rows of positions pos0 .. pos0 + n - 1 from fp16 k, v [n][row_stride] (head h at h D; both on 16-byte
  * boundaries, row_stride a multiple of 8 and >= KVH D). A page entered at its first slot starts anew. In a page entered
  * further on the rows before pos0 stay, the scale becomes the larger of the old one and the new rows', and where it grew the
- * rows that stay are re-coded to it (rounded once more). The cache then ends at pos0 + n: the slots behind it in the last
+ * rows that stay are re-coded to it (rounded once more: free for e4m3 but where a code falls below its normal range; int8 rows
+ * may be some steps off after many appends of ever larger ones). The cache then ends at pos0 + n: the slots behind it in the last
  * page are cleared. A verify block is appended before its attention; rejected rows are dropped by the next append, which
  * starts before them (their part in the page's scale stays until the page is entered at its first slot). Positions stay
  * under 2^31 - 64, and one call takes at most 2^25 - 2 blocks of K: KVH (ceil(n / 32) + 1) (a launch holds no more; reading
@@ -230,8 +231,8 @@ int dspark_attention_mass_b8(const dspark_b8_cache* cache, const dspark_b8_attn_
  * cache of `keep` positions for every head (keys keep the rotation they were written with; later calls count positions
  * from keep). A dst block's scale is the largest of its rows' scales; rows from blocks of a smaller one are re-coded to it
  * (rounded once more). The slots behind keep in the last page are cleared. mass_out[h][j] = mass[h][kept[h][j]]. dst has
- * src's KVH, D and code, and pools of its own. sinks + recent <= keep <= length <= 2^30, KVH ceil(keep / 32) <=
- * 2^25 - 2. keep = 0 does nothing. The workspace (a size of 0: none is needed) needs no clearing. */
+ * src's KVH, D and code, and pools of its own. sinks + recent <= keep <= length <= 2^30, KVH ceil(keep / 32) <= 2^25 - 2.
+ * keep = 0 does nothing. The workspace (a size of 0: none is needed) needs no clearing. */
 int dspark_kv_evict_b8(const dspark_b8_cache* src, const dspark_b8_cache* dst, int32_t length, int32_t keep, int32_t sinks,
                        int32_t recent, const float* mass, int64_t mass_stride, int32_t* kept, float* mass_out,
                        int64_t mass_out_stride, void* workspace, size_t workspace_bytes, dspark_stream_t stream);

@@ -348,11 +348,13 @@ __device__ __forceinline__ void b8_finish_row(const B8Attn& p, int h, int row, i
 }
 
 // One workgroup per (KV head, key split, row group), the split's pages spread evenly over its waves. Splits go to the
-// workspace, where the last of them (RB = 1) or a second kernel adds them; a single split is finished here. Bound by the codes'
-// bytes up to two row blocks (131072 keys of 4 heads of 128, 36 rows: 34.0 us, 134 MB, 3.9 TB/s) and by issue above: a page costs
-// 16 rows 8 exponentials and about 25 other vector instructions a lane, beside 8 products (D = 64) that hardly overlap with them
-// (131072 keys of 8 heads of 64, 132 rows: 58.1 us, 610 TFLOP/s, vector units busy 60 % of it, matrix cores 26 %). 32768 keys
-// of 8 heads of 64, 64 rows: 14.3 us.
+// workspace, where the last of them (RB = 1) or a second kernel adds them; a single split is finished here. Bound by first loads,
+// the sums and bytes for one row group (32768 keys of 8 heads of 64, 64 rows: 13.4-14.3 us) and by issue for more, since every
+// row group loads and converts a page anew. D = 64, e4m3: 65 vector instructions a page and 16 rows, of them 8 products, 8
+// exponentials and 13 conversions (40 a page, for three row blocks); products hardly overlap with the others (131072 keys of 8
+// heads of 64, 132 rows: 58-63 us, 560-610 TFLOP/s, vector units busy 60 % of it, matrix cores 26 %). D = 128, int8: 156, of
+// them 16 products and 88 conversions (176 a page, for two row blocks), and 36 rows are computed as 64 (131072 keys of 4 heads of
+// 128: 34-35 us, 134 MB, 3.9 TB/s; vector units busy 44 %).
 template <int D, int RB, bool FP8>
 __global__ __launch_bounds__(64 * b8_waves(D, RB), b8_waves(D, RB) / 4) void attn_b8_kernel(B8Attn p) {
   constexpr int ND = D / 16, NW = b8_waves(D, RB), ROWS = 16 * RB, NT = 64 * NW;
@@ -529,7 +531,7 @@ __global__ __launch_bounds__(256) void attn_b8_merge_kernel(B8Attn p) {
 // operands the other way round than the attention's (A = Q, B = K): a lane holds one key's scores of rows 4 g + i, adds them
 // up in place over all row blocks, and only the four lanes of a key are added across (sums over the rows' lanes instead, with
 // A = K, are eight row reductions a page: 39 us at 128k keys and 64 rows a head, 31 so). Bound by K's bytes and a fixed 4 us
-// (131088 keys of 8 heads of 64, 64 rows: 21.4 us, 76 MB; 4107 keys 5.0).
+// (131088 keys of 8 heads of 64, 64 rows: 21.4-22.0 us, 76 MB; 4107 keys 5.0). K is read of pages out of sight too.
 template <int D, int RB, bool FP8>
 __global__ __launch_bounds__(64 * MASS_WAVES, 2) void mass_b8_kernel(B8Attn p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
@@ -738,7 +740,8 @@ int b8_mass_launch(const B8Attn& q, int D, bool fp8, int cus, hipStream_t s) {
   p.seen_lo = p.page0;
   p.page0 = 0;  // every account is carried over, those of keys out of sight too
   p.npages = (p.a + p.M - 1) / PAGE + 1;
-  // as many pages a wave as let every workgroup start at once (131088 keys, 64 rows a head: 26.0 us, 27.8 with a few over)
+  // as many pages a wave as let every workgroup start at once (131088 keys, 64 rows a head, when a page still cost more: 26.0 us,
+  // 27.8 with a few workgroups over)
   const int64_t waves = (int64_t)cus * (p.rb > 2 ? 12 : 16);
   p.pps = (int)std::max<int64_t>(1, ((int64_t)p.npages * p.c.KVH + waves - 1) / waves);
   const dim3 grid((p.npages + p.pps * MASS_WAVES - 1) / (p.pps * MASS_WAVES), p.c.KVH);

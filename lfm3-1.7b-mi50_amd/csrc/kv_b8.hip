@@ -2,8 +2,8 @@
 //
 // A block is the 32 positions of one (page, KV head), of K or of V: 32 x D one-byte codes, rows of D bytes in position
 // order, and one fp32 scale; value = code * scale (b8.h has the arithmetic). Rows are kept whole and in order -- the
-// attention transposes V in registers, which costs it under a tenth of its issue -- so that a position is D contiguous
-// bytes to the writer, the reader and the eviction.
+// attention transposes V in registers, by D / 8 of the 220 to 370 vector instructions that a page costs a wave -- so that a
+// position is D contiguous bytes to the writer, the reader and the eviction.
 #include "b8.h"
 #include "dspark.h"
 
@@ -245,8 +245,8 @@ __device__ __forceinline__ uint32_t sel_before(const uint32_t* wc, int wave, uin
 }
 
 // One workgroup per KV head finds the keep - sinks - recent largest accounts of up to 1024 NPL middle positions, held in
-// registers, and lists what is kept in position order. Bound by its chain of phases (three digits of clear, count, scan): 9.9 us
-// for 8449 positions.
+// registers, and lists what is kept in position order. Bound by its chain of phases (three digits of clear, count, scan):
+// 9.9-10.1 us for 8449 positions.
 template <int NPL>
 __global__ __launch_bounds__(SEL_T) void evict_select_kernel(B8Evict p) {
   __shared__ SelLds s;
@@ -290,7 +290,7 @@ __global__ __launch_bounds__(SEL_T) void evict_select_kernel(B8Evict p) {
 // digit. A workgroup stores its own histogram; the next launch's workgroups each add up all of the head's (from L2), find the
 // digit, and count the next one among their keys that match so far. The last launch knows from the parts' counts where each
 // part's first kept key goes. No atomics in memory, and no state from one call to the next. Each launch is a chain (histograms
-// or keys, counts in LDS, a scan, a store): 3.4 + 5.8 + 5.6 + 5.8 us for 130044 positions of 4 heads.
+// or keys, counts in LDS, a scan, a store): 3.4-3.7 us, then 5.6-6.1 each, for 130044 positions of 4 heads.
 constexpr int SEL_NPL = 8, SEL_TILE = SEL_T * SEL_NPL, SEL_PARTS = 32;
 struct SelHead {  // a head's part of the workspace, a u32 each
   uint32_t hist[3][SEL_PARTS][SEL_BINS];
@@ -396,7 +396,7 @@ __global__ __launch_bounds__(SEL_T) void evict_edges_kernel(B8Evict p) {
 
 // One wave per (destination page, K or V, head): 32 kept rows gathered 16 bytes a lane into one block. Its scale is the
 // largest of its rows' scales: rows that had it keep their codes, the others are re-coded to it. Bound by the chain kept ->
-// table -> rows and the gather (16384 rows of 4 heads of 128: 8.8 us, 33.6 MB, 3.8 TB/s; 8192 of 8 heads of 64: 9.8; with the
+// table -> rows and the gather (16384 rows of 4 heads of 128: 8.8-9.0 us, 37 MB, 4.2 TB/s; 8192 of 8 heads of 64, int8: 9.8-10.1; with the
 // rows' loads ahead of the scales' use the same).
 template <int D, bool FP8>
 __global__ __launch_bounds__(64 * WPB) void evict_move_kernel(B8Evict p, int nwaves) {
