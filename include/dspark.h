@@ -238,6 +238,128 @@ int dspark_kv_evict_b8(const dspark_b8_cache* src, const dspark_b8_cache* dst, i
                        int64_t mass_out_stride, void* workspace, size_t workspace_bytes, dspark_stream_t stream);
 size_t dspark_kv_evict_b8_workspace(int32_t KVH, int32_t length);
 
+/* ---------------------------------------------------------------- a batch of sequences: rotary positions and K/V by slot
+ * Rows of n tokens at any positions: the first `rot` values of each head are turned in pairs -- (i, i + rot / 2), or (2 i,
+ * 2 i + 1) with interleaved -- by the angle positions[t] * freq[i]:
+ *   y_i = s (x_i cos - x_j sin), y_j = s (x_j cos + x_i sin)     (inverse: by the negative angle: the rotation's backward pass)
+ * and the rest of the head is passed on. Angles are products in 64 bits, sines and cosines rounded to fp32 once, products fp32,
+ * one rounding to the type. q and k (either may be NULL with 0 heads) have one type, n rows of heads x D values each, rows their
+ * stride apart; a stride may be any number of elements >= heads x D. An output may be its input itself (same address and
+ * stride); otherwise nothing written shares a byte with anything else (DSPARK_EINVAL).
+ * With k_pages (fp16 only, D in {64, 128}, not inverse) the turned K rows and the rows of v go into the fp16 pages instead of
+ * k_out (NULL then): row t to slot slots[t] = 32 x physical page + position within it; a slot outside [0, 32 kv_pages) is not
+ * written. Pools may pass 4 GiB; no two rows may have the same slot. One launch for a batch's q, K and V. n = 0 does nothing.
+ * The engine's own rotation reads dspark_rope_table; this one takes its angles where the reference has an fp16 table
+ * (internal/model/engine.go:428-461). */
+enum { DSPARK_F16 = 0, DSPARK_BF16 = 1, DSPARK_F32 = 2 };
+typedef struct dspark_rope_args {
+  const void* q;               /* [n][q_stride] or NULL */
+  void* q_out;
+  const void* k;               /* [n][k_stride] or NULL */
+  void* k_out;
+  int64_t q_stride, q_out_stride, k_stride, k_out_stride; /* elements between rows */
+  const int32_t* positions;    /* [n], any sign */
+  const double* freq;          /* [rot / 2] radians a position (dspark_rope_freqs) */
+  const void* v;               /* append: fp16 [n][v_stride] */
+  int64_t v_stride;
+  void* k_pages;               /* append: the page pools */
+  void* v_pages;
+  const int64_t* slots;        /* append: [n] */
+  int64_t kv_pages;
+  double scale;                /* s */
+  int32_t n, QH, KVH, D, rot;  /* n < 2^30; QH, KVH <= 1024; D even, <= 1024; rot even, 2 <= rot <= D */
+  int32_t interleaved, inverse, type; /* DSPARK_F16 | BF16 | F32 */
+} dspark_rope_args;
+int dspark_rope(const dspark_rope_args* args, dspark_stream_t stream);
+
+/* Host helper: freq[i] = base^(-2 i / rot), i < rot / 2, scaled for contexts beyond the trained ones:
+ *   DSPARK_ROPE_PLAIN   as they are;   DSPARK_ROPE_LINEAR   divided by factor;
+ *   DSPARK_ROPE_BASE    with base x factor^(rot / (rot - 2)) instead of base: the slowest pair divided by factor, the first kept;
+ *   DSPARK_ROPE_RAMP    pairs that make at most `low` turns in `trained` positions divided by factor, those of at least `high`
+ *                       turns kept, a linear ramp between; *scale (else 1) = 0.1 ln(factor) + 1 for factor > 1.
+ * scale may be NULL. factor >= 1. */
+enum { DSPARK_ROPE_PLAIN = 0, DSPARK_ROPE_LINEAR = 1, DSPARK_ROPE_BASE = 2, DSPARK_ROPE_RAMP = 3 };
+int dspark_rope_freqs(int32_t rot, double base, int32_t scaling, double factor, double trained, double low, double high,
+                      double* freq, double* scale);
+
+/* ---------------------------------------------------------------- verify attention behind a shared prefix
+ * `seqs` sequences that begin with the same `prefix` positions, each with pages of its own behind them, all in the fp16 pages of
+ * dspark_kv_write (pools may pass 4 GiB): prefix position p in page prefix_table[p / 32] (NULL = identity), own position j of
+ * sequence r in page own_table[r * own_stride + j / 32]. Sequence r's rows of q are q_start[r] .. q_start[r + 1] - 1
+ * (m_r <= max_tokens of them), its own keys 0 .. own_len[r] - 1, these tokens' among them: token i is own position
+ * own_len[r] - m_r + i and sees the prefix and the own keys before the call's first token -- with window > 0 those of the last
+ * `window` positions up to itself, counted through the prefix -- and the call's own keys up to itself (causal) or all. The
+ * masks of dspark_verify_attention with a = prefix + own_len[r] - m_r.
+ * out and/or out_f32 [tokens][QH][D] = softmax(q k^T / sqrt(D)) v, times sigmoid(gate[t][qh]) if given; lse as in
+ * dspark_verify_attention_b8. A table entry outside [0, kv_pages) is an absent page: no row sees its positions. A row that
+ * sees no key gives zeros and lse -inf. Rows of q before q_start[0] and behind q_start[seqs], and a sequence's rows past
+ * max_tokens, are left as they are in the outputs. Keys that a row does not see may hold anything; where it sees a value of V
+ * that is not finite on a page it does not see whole, its output is NaN there. q_start must not decrease; it is cut to
+ * [0, tokens], own_len to [0, 32 own_pages]. The prefix's keys are read once for all rows (in groups of up to 256). P is
+ * rounded to fp16 once; scores, sums and outputs are fp32. The workspace needs no clearing and may be shared by stream-ordered
+ * calls. What is written shares no byte with anything else (DSPARK_EINVAL). tokens = 0 or seqs = 0 does nothing. */
+typedef struct dspark_shared_attn_args {
+  const void* q;               /* fp16 [tokens][q_stride] (head qh at qh D; 16-byte boundary, q_stride a multiple of 8) */
+  int64_t q_stride;            /* >= QH D */
+  const void* k_pages;         /* on 16-byte boundaries */
+  const void* v_pages;
+  int64_t kv_pages;            /* pages in each pool, < 2^31 */
+  const int32_t* prefix_table; /* [ceil(prefix / 32)] or NULL */
+  const int32_t* q_start;      /* device [seqs + 1] */
+  const int32_t* own_len;      /* device [seqs] */
+  const int32_t* own_table;    /* device [seqs][own_stride] */
+  int64_t own_stride;          /* >= own_pages */
+  void* out;                   /* fp16 or NULL; outputs on 16-byte boundaries */
+  float* out_f32;              /* or NULL */
+  float* lse;                  /* fp32 [tokens][QH] or NULL */
+  const float* gate;           /* fp32 [tokens][QH] or NULL */
+  void* workspace;             /* on a 16-byte boundary */
+  size_t workspace_bytes;      /* dspark_verify_attention_shared_workspace */
+  int32_t prefix, tokens, seqs, max_tokens; /* prefix < 2^30; tokens (QH / KVH) <= 2^20; seqs <= 2^20;
+                                  1 <= max_tokens <= tokens; seqs max_tokens QH < 2^26 */
+  int32_t own_pages;           /* columns of own_table, <= 2^24 */
+  int32_t QH, KVH, D;          /* D in {64, 128}; KVH <= 1024, QH <= 4096 */
+  int32_t window, causal;
+  int32_t splits;              /* key ranges of the prefix; 0 = automatic */
+} dspark_shared_attn_args;
+size_t dspark_verify_attention_shared_workspace(const dspark_shared_attn_args* args); /* 0: refused */
+int dspark_verify_attention_shared(const dspark_shared_attn_args* args, dspark_stream_t stream);
+
+/* ---------------------------------------------------------------- sampled verify (temperature, top-k, top-p, min-p)
+ * One token for each of n rows of logits [n][V] from the row's random number u in [0, 1). With T the row's temperature and
+ * w_i = exp((z_i - max z) / T), tokens are ranked by z descending, the lowest index first among equal ones; kept are those of
+ *   rank < top_k (top_k <= 0 or >= V: all), then with less than top_p x (the weight of those) in front of them (top_p >= 1: all;
+ *   the first always), and z_i >= max z + T ln(min_p) (min_p <= 0: all);
+ * the token is the first kept one, by index, at which the kept weights' running sum exceeds u times their whole sum. T <= 0 is
+ * greedy: the first maximum. NaN and -inf are never drawn; +inf shares the weight with the other +inf alone. A row with
+ * nothing to draw gives token -1, kept 0, logprob -inf, key 0. Weights are fixed-point numbers of 44 bits behind the point and their
+ * sums whole 64-bit ones, so a draw does not depend on the order of the work: the same inputs give the same token always.
+ * keys are what dspark_accept_commit takes: the round of drafts that agree with their row's draw is accepted. For drafts that are
+ * chosen without randomness, as the drafter's are, that is speculative sampling exactly: a draft is accepted with its
+ * probability under the target, and the first token that differs is distributed as the target's with the draft taken out.
+ * Per-row settings are device arrays [n]; where a pointer is NULL the value beside it holds for every row. n = 0 does nothing.
+ * The workspace needs no clearing. The reference samples on the host (internal/sample, Draw, sample.go:176-234). */
+typedef struct dspark_sample_args {
+  const void* logits;          /* [n][row_stride] of `type` */
+  int64_t row_stride;          /* elements between rows, >= V */
+  const float* u;              /* [n]; cut to [0, 1) (NaN: 0) */
+  const float* temperature;    /* [n] or NULL */
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  int32_t* tokens;             /* [n] or NULL */
+  uint64_t* keys;              /* [n] or NULL: argmax-style keys, dspark_key_token() gives the token */
+  int32_t* kept;               /* [n] or NULL: how many tokens could have been drawn */
+  float* logprob;              /* [n] or NULL: ln of the probability with which the token was drawn */
+  void* workspace;             /* on a 16-byte boundary */
+  size_t workspace_bytes;      /* dspark_verify_sample_workspace(n, V) */
+  float temperature_all, top_p_all, min_p_all;
+  int32_t top_k_all;
+  int32_t n, V, type;          /* n <= 65535, V <= 2^20; DSPARK_F16 | BF16 | F32 */
+} dspark_sample_args;
+size_t dspark_verify_sample_workspace(int32_t n, int32_t V); /* 0: refused */
+int dspark_verify_sample(const dspark_sample_args* args, dspark_stream_t stream);
+
 /* ---------------------------------------------------------------- verify argmax (greedy head)
  * best_keys[t] = max over r < V of key(pv, r), pv the repetition-penalised fp16-rounded logit (seen[] bitmap, plus
  * drafts tokens[1..t] not yet seen), key = ordered float bits << 32 | (0xFFFFFFFF - r). logits fp32 [M][V] or fp16

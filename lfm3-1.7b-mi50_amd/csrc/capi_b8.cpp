@@ -3,11 +3,11 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <atomic>
 
 #include "dspark.h"
 #include "dspark_internal.h"
 #include "b8.h"
+#include "spans.h"
 
 using namespace dspark;
 
@@ -17,7 +17,6 @@ constexpr int64_t POS_MAX = ((int64_t)1 << 31) - 2 * DSPARK_PAGE_TOKENS;  // pos
 constexpr int HEADS_MAX = 1024;
 
 hipStream_t S(dspark_stream_t s) { return reinterpret_cast<hipStream_t>(s); }
-bool on(const void* p, uintptr_t bytes) { return p && (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 int64_t pages_of(int64_t positions) { return (positions + DSPARK_PAGE_TOKENS - 1) / DSPARK_PAGE_TOKENS; }
 
 bool cache_ok(const dspark_b8_cache* c) {
@@ -46,19 +45,6 @@ B8Pool pool(const dspark_b8_cache* c) {
   p.pages = c->kv_pages;
   p.KVH = c->KVH;
   return p;
-}
-
-// Compute units of the current device (queried once per device).
-int device_cus() {
-  static std::atomic<int> cached[64];
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
-  int n = cached[dev].load(std::memory_order_relaxed);
-  if (!n) {
-    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
-    cached[dev].store(n, std::memory_order_relaxed);
-  }
-  return n;
 }
 
 bool rows_ok(const dspark_b8_cache* c, const dspark_b8_attn_args* a) {
@@ -91,39 +77,6 @@ B8Attn attn(const dspark_b8_cache* c, const dspark_b8_attn_args* a) {
   return p;
 }
 
-// Memory that a call reads or writes: `rows` pieces of n bytes, `stride` apart (stride >= n); p NULL or n 0: none.
-struct Span {
-  const void* p;
-  size_t n;
-  size_t rows = 1, stride = 0;
-};
-// A piece of n bytes at `at` and some row of y share a byte: of y's rows the first that ends behind `at` begins before the piece ends.
-bool meets(uintptr_t at, size_t n, const Span& y) {
-  const uintptr_t b = reinterpret_cast<uintptr_t>(y.p);
-  const size_t i = at < b + y.n ? 0 : y.rows > 1 ? (at - b - y.n) / y.stride + 1 : 1;
-  return i < y.rows && b + i * y.stride < at + n;
-}
-bool overlap(const Span& x, const Span& y) {
-  if (!x.p || !y.p || !x.n || !y.n) return false;
-  const uintptr_t a = reinterpret_cast<uintptr_t>(x.p), b = reinterpret_cast<uintptr_t>(y.p);
-  if (a >= b + (y.rows - 1) * y.stride + y.n || b >= a + (x.rows - 1) * x.stride + x.n) return false;
-  if (x.rows > y.rows) return overlap(y, x);  // (of two spans here one has at most 1024 rows, heads or tokens)
-  for (size_t i = 0; i < x.rows; ++i)
-    if (meets(a + i * x.stride, x.n, y)) return true;
-  return false;
-}
-// Nothing that is written shares a byte with what is read, nor with anything else that is written: workgroups read and store in
-// no order among each other.
-template <size_t NR, size_t NW>
-bool apart(const Span (&reads)[NR], const Span (&writes)[NW]) {
-  for (size_t i = 0; i < NW; ++i) {
-    for (const Span& r : reads)
-      if (overlap(r, writes[i])) return false;
-    for (size_t j = 0; j < i; ++j)
-      if (overlap(writes[j], writes[i])) return false;
-  }
-  return true;
-}
 size_t scale_bytes(const dspark_b8_cache* c) { return (size_t)c->kv_pages * c->KVH * sizeof(float); }
 size_t code_bytes(const dspark_b8_cache* c) { return (size_t)c->kv_pages * c->KVH * DSPARK_PAGE_TOKENS * c->D; }
 Span table(const dspark_b8_cache* c, int64_t positions) { return {c->block_table, (size_t)pages_of(positions) * sizeof(int32_t)}; }

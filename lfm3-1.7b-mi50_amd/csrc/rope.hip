@@ -1,0 +1,183 @@
+// Rotary positions of a batch's q and k rows, and its K and V rows into the fp16 pages by slot.
+//
+// A pair (x_i, x_j) turns by the angle p f: y_i = s (x_i cos - x_j sin), y_j = s (x_j cos + x_i sin). The angle is taken in
+// turns, p (f / 2 pi) in 64 bits, less its nearest whole number (exact), then as a quarter turn and a rest within an eighth,
+// whose sine and cosine are their series in 64 bits (the first term left out is under 2e-14): fp32 loses the angle itself
+// from some ten thousand positions on. 64-bit multiply-adds run at the rate of 32-bit ones here, and an angle serves every
+// head of its token: a workgroup computes its tokens' sines and cosines once, into LDS.
+//
+// Bound by memory: each value is read and written once, in pieces of 16 bytes where sizes and addresses allow (VEC), else value
+// by value. A unit of work is a piece (half layout: the piece and its partner rot / 2 further) or a piece of what is not turned.
+#include "batch.h"
+#include "dspark.h"
+
+namespace dspark {
+
+constexpr int ROPE_THREADS = 256;
+constexpr int ROPE_TOKENS = 8;  // of a workgroup at most
+
+__device__ __forceinline__ float rope_to_f32(float x) { return x; }
+__device__ __forceinline__ float rope_to_f32(_Float16 x) { return (float)x; }
+__device__ __forceinline__ float rope_to_f32(__bf16 x) { return (float)x; }
+
+// (cos, sin) of `turns` turns times scale.
+__device__ __forceinline__ f32x2 rope_cos_sin(double turns, double scale, bool inverse) {
+  const double r = turns - rint(turns);
+  const double quarter = rint(4 * r);
+  const double a = (r - 0.25 * quarter) * 6.283185307179586476925, b = a * a;  // |a| <= pi / 4
+  const double s = a * fma(b, fma(b, fma(b, fma(b, fma(b, fma(b, 1.0 / 6227020800.0, -1.0 / 39916800.0), 1.0 / 362880.0), -1.0 / 5040.0), 1.0 / 120.0), -1.0 / 6.0), 1.0);
+  const double c = fma(b, fma(b, fma(b, fma(b, fma(b, fma(b, fma(b, -1.0 / 87178291200.0, 1.0 / 479001600.0), -1.0 / 3628800.0), 1.0 / 40320.0), -1.0 / 720.0), 1.0 / 24.0), -0.5), 1.0);
+  const int q = (int)quarter & 3;  // (-2 .. 2, or of a NaN anything: the values are NaN)
+  double cs = q & 1 ? s : c, sn = q & 1 ? c : s;
+  if (q == 1 || q == 2) cs = -cs;
+  if (q >= 2) sn = -sn;
+  return f32x2{(float)(cs * scale), (float)((inverse ? -sn : sn) * scale)};
+}
+
+template <typename T, int VEC>
+struct RopePiece {
+  T x[VEC];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (VEC * sizeof(T) == 16) {
+      const u32x4 u = ldg(reinterpret_cast<const u32x4*>(p));
+      __builtin_memcpy(x, &u, 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) x[i] = p[i];
+    }
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (VEC * sizeof(T) == 16) {
+      u32x4 u;
+      __builtin_memcpy(&u, x, 16);
+      *reinterpret_cast<u32x4*>(p) = u;
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) p[i] = x[i];
+    }
+  }
+};
+
+// VEC: values of a piece, 16 bytes' worth or (sizes or addresses off 16 bytes) 1, interleaved pairs 2.
+template <typename T, int VEC, bool IL>
+__global__ __launch_bounds__(ROPE_THREADS) void rope_kernel(RopeBatch p) {
+  extern __shared__ f32x2 cs[];  // [tok][rot / 2]
+  const int P = p.rot / 2, t0 = (int)blockIdx.x * p.tok, nt = min(p.tok, p.n - t0);
+  for (int e = threadIdx.x; e < nt * P; e += ROPE_THREADS) {
+    const int t = e / P, i = e - t * P;
+    cs[e] = rope_cos_sin((double)ldg(p.pos + t0 + t) * (ldg(p.freq + i) * 0.15915494309189533577), p.scale, p.inverse != 0);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < nt * p.upt; e += ROPE_THREADS) {
+    const int tl = div_by(e, p.upt_div), r = e - tl * p.upt, t = t0 + tl;
+    int h = div_by(r, p.uph_div), u = r - h * p.uph;
+    // units of a head: what turns first, then the rest
+    const int turning = IL ? p.rot / VEC : P / VEC;
+    RopePiece<T, VEC> a;
+    const bool in_q = h < p.q.heads, in_k = !in_q && h < p.q.heads + p.k.heads;
+    if (!in_q && !in_k) continue;
+    const RopeTensor& x = in_q ? p.q : p.k;
+    if (!in_q) h -= p.q.heads;
+    const T* src = static_cast<const T*>(x.x) + (size_t)t * x.x_stride + (size_t)h * p.D;
+    T* dst = static_cast<T*>(x.y) + (size_t)t * x.y_stride + (size_t)h * p.D;
+    // append: a K piece of up to 8 values from a multiple of its size lies together in the page
+    const bool paged = in_k && p.kp;
+    int64_t slot = 0;
+    if constexpr (sizeof(T) == 2) {
+      if (paged) {
+        slot = ldg(p.slots + t);
+        if (slot < 0 || slot >= p.n_slots) continue;
+        dst = reinterpret_cast<T*>(p.kp) + (size_t)((slot / PAGE) * p.KVH + h) * (PAGE * p.D);
+      }
+    }
+    auto at = [&](int d) { return paged ? k_page_elem((int)(slot % PAGE), d, p.D) : d; };
+    if (u >= turning) {  // passed on
+      const int d = p.rot + (u - turning) * VEC;
+      if (!paged && dst == src) continue;
+      a.load(src + d);
+      a.store(dst + at(d));
+      continue;
+    }
+    const f32x2* c = cs + tl * P;
+    if constexpr (IL) {
+      const int d = u * VEC;
+      a.load(src + d);
+#pragma unroll
+      for (int i = 0; i < VEC; i += 2) {
+        const f32x2 w = c[d / 2 + i / 2];
+        const float xi = rope_to_f32(a.x[i]), xj = rope_to_f32(a.x[i + 1]);
+        a.x[i] = (T)(xi * w[0] - xj * w[1]);
+        a.x[i + 1] = (T)(xj * w[0] + xi * w[1]);
+      }
+      a.store(dst + at(d));
+    } else {
+      const int d = u * VEC;
+      RopePiece<T, VEC> b;
+      a.load(src + d);
+      b.load(src + P + d);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const f32x2 w = c[d + i];
+        const float xi = rope_to_f32(a.x[i]), xj = rope_to_f32(b.x[i]);
+        a.x[i] = (T)(xi * w[0] - xj * w[1]);
+        b.x[i] = (T)(xj * w[0] + xi * w[1]);
+      }
+      a.store(dst + at(d));
+      b.store(dst + at(P + d));
+    }
+  }
+  if constexpr (sizeof(T) == 2) {
+    if (!p.vp) return;
+    // V rows into the transposed pages, 8 values of a row each: [d][slot]
+    const int upv = p.KVH * p.D / 8;
+    for (int e = threadIdx.x; e < nt * upv; e += ROPE_THREADS) {
+      const int tl = e / upv, d8 = (e - tl * upv) * 8, h = d8 / p.D, d = d8 - h * p.D;
+      const int64_t slot = ldg(p.slots + t0 + tl);
+      if (slot < 0 || slot >= p.n_slots) continue;
+      const _Float16* src = static_cast<const _Float16*>(p.v.x) + (size_t)(t0 + tl) * p.v.x_stride + d8;
+      _Float16* dst = p.vp + (size_t)((slot / PAGE) * p.KVH + h) * (PAGE * p.D);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) dst[v_page_elem((int)(slot % PAGE), d + i)] = src[i];
+    }
+  }
+}
+
+int rope_batch_launch(RopeBatch& p, int type, bool interleaved, hipStream_t s) {
+  const int size = type == DSPARK_F32 ? 4 : 2, vec16 = 16 / size;
+  // whole 16-byte pieces everywhere: the head and its turned part (half layout: half of it) in pieces, rows and heads on
+  // 16-byte boundaries (D a multiple of a piece keeps every head on one)
+  bool wide = p.D % vec16 == 0 && p.rot % vec16 == 0 && (interleaved || p.rot / 2 % vec16 == 0);
+  for (const RopeTensor* x : {&p.q, &p.k}) {
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(x->x) | reinterpret_cast<uintptr_t>(x->y) |
+                           (uintptr_t)(x->x_stride * size) | (uintptr_t)(x->y_stride * size);
+    if (x->heads && bits & 15) wide = false;
+  }
+  const int vec = wide ? vec16 : interleaved ? 2 : 1;
+  p.uph = interleaved ? p.D / vec : p.rot / 2 / vec + (p.D - p.rot) / vec;
+  p.upt = (p.q.heads + p.k.heads) * p.uph;
+  p.uph_div = div_magic(p.uph);
+  p.upt_div = div_magic(p.upt);
+  // tokens of a workgroup: several where that leaves over 4 workgroups a CU, whose one round of angles then serves more work
+  p.tok = 1;
+  while (p.tok < ROPE_TOKENS && (p.n + 2 * p.tok - 1) / (2 * p.tok) >= 1024 && (int64_t)2 * p.tok * p.upt * p.upt < (int64_t)1 << 32) p.tok *= 2;
+  const dim3 grid((p.n + p.tok - 1) / p.tok), block(ROPE_THREADS);
+  const size_t lds = (size_t)p.tok * (p.rot / 2) * sizeof(f32x2);
+#define ROPE_GO(T, V, IL) hipLaunchKernelGGL((rope_kernel<T, V, IL>), grid, block, lds, s, p)
+#define ROPE_TYPE(T, V16)                    \
+  if (wide && interleaved) ROPE_GO(T, V16, true);  \
+  else if (wide) ROPE_GO(T, V16, false);     \
+  else if (interleaved) ROPE_GO(T, 2, true); \
+  else ROPE_GO(T, 1, false)
+  if (type == DSPARK_F32) {
+    ROPE_TYPE(float, 4);
+  } else if (type == DSPARK_BF16) {
+    ROPE_TYPE(__bf16, 8);
+  } else {
+    ROPE_TYPE(_Float16, 8);
+  }
+#undef ROPE_TYPE
+#undef ROPE_GO
+  return (int)hipGetLastError();
+}
+
+}  // namespace dspark

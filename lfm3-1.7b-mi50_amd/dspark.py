@@ -55,6 +55,37 @@ class B8AttnArgs(ctypes.Structure):
                 ("splits", ctypes.c_int32)]
 
 
+class RopeArgs(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("q_out", ctypes.c_void_p), ("k", ctypes.c_void_p), ("k_out", ctypes.c_void_p),
+                ("q_stride", ctypes.c_int64), ("q_out_stride", ctypes.c_int64), ("k_stride", ctypes.c_int64),
+                ("k_out_stride", ctypes.c_int64), ("positions", ctypes.c_void_p), ("freq", ctypes.c_void_p),
+                ("v", ctypes.c_void_p), ("v_stride", ctypes.c_int64), ("k_pages", ctypes.c_void_p),
+                ("v_pages", ctypes.c_void_p), ("slots", ctypes.c_void_p), ("kv_pages", ctypes.c_int64),
+                ("scale", ctypes.c_double), ("n", ctypes.c_int32), ("QH", ctypes.c_int32), ("KVH", ctypes.c_int32),
+                ("D", ctypes.c_int32), ("rot", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+                ("inverse", ctypes.c_int32), ("type", ctypes.c_int32)]
+
+
+class SharedAttnArgs(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("q_stride", ctypes.c_int64), ("k_pages", ctypes.c_void_p), ("v_pages", ctypes.c_void_p),
+                ("kv_pages", ctypes.c_int64), ("prefix_table", ctypes.c_void_p), ("q_start", ctypes.c_void_p),
+                ("own_len", ctypes.c_void_p), ("own_table", ctypes.c_void_p), ("own_stride", ctypes.c_int64),
+                ("out", ctypes.c_void_p), ("out_f32", ctypes.c_void_p), ("lse", ctypes.c_void_p), ("gate", ctypes.c_void_p),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("prefix", ctypes.c_int32),
+                ("tokens", ctypes.c_int32), ("seqs", ctypes.c_int32), ("max_tokens", ctypes.c_int32),
+                ("own_pages", ctypes.c_int32), ("QH", ctypes.c_int32), ("KVH", ctypes.c_int32), ("D", ctypes.c_int32),
+                ("window", ctypes.c_int32), ("causal", ctypes.c_int32), ("splits", ctypes.c_int32)]
+
+
+class SampleArgs(ctypes.Structure):
+    _fields_ = [("logits", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("u", ctypes.c_void_p),
+                ("temperature", ctypes.c_void_p), ("top_k", ctypes.c_void_p), ("top_p", ctypes.c_void_p),
+                ("min_p", ctypes.c_void_p), ("tokens", ctypes.c_void_p), ("keys", ctypes.c_void_p), ("kept", ctypes.c_void_p),
+                ("logprob", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+                ("temperature_all", ctypes.c_float), ("top_p_all", ctypes.c_float), ("min_p_all", ctypes.c_float),
+                ("top_k_all", ctypes.c_int32), ("n", ctypes.c_int32), ("V", ctypes.c_int32), ("type", ctypes.c_int32)]
+
+
 _lib = None
 
 _SIGS = {
@@ -92,6 +123,13 @@ _SIGS = {
                                           ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
                                           ctypes.c_size_t, ctypes.c_void_p]),
     "dspark_kv_evict_b8_workspace": (ctypes.c_size_t, [ctypes.c_int32, ctypes.c_int32]),
+    "dspark_rope": (ctypes.c_int, [ctypes.POINTER(RopeArgs), ctypes.c_void_p]),
+    "dspark_rope_freqs": (ctypes.c_int, [ctypes.c_int32, ctypes.c_double, ctypes.c_int32, ctypes.c_double, ctypes.c_double,
+                                         ctypes.c_double, ctypes.c_double, ctypes.c_void_p, ctypes.c_void_p]),
+    "dspark_verify_attention_shared_workspace": (ctypes.c_size_t, [ctypes.POINTER(SharedAttnArgs)]),
+    "dspark_verify_attention_shared": (ctypes.c_int, [ctypes.POINTER(SharedAttnArgs), ctypes.c_void_p]),
+    "dspark_verify_sample_workspace": (ctypes.c_size_t, [ctypes.c_int32, ctypes.c_int32]),
+    "dspark_verify_sample": (ctypes.c_int, [ctypes.POINTER(SampleArgs), ctypes.c_void_p]),
     "dspark_rope_table": (ctypes.c_int, [ctypes.c_float, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
                                          ctypes.c_void_p]),
     "dspark_verify_argmax_workspace": (ctypes.c_size_t, [ctypes.c_int32, ctypes.c_int32]),
@@ -594,6 +632,251 @@ def kv_evict_b8(cache, dst, length, keep, mass, sinks=0, recent=0, kept=None, ma
     dst.check(keep)
     stride = _b8_accounts(mass, length, cache, "mass")
     return _b8_on(cache, stream, _kv_evict_b8, dst, length, keep, mass, stride, sinks, recent, kept, mass_out, workspace)
+
+
+# ---------------------------------------------------------------- a batch of sequences
+F16, BF16, F32 = 0, 1, 2
+ROPE_SCALING = {None: 0, "linear": 1, "base": 2, "ramp": 3}
+
+
+def _type_of(dtype, what):
+    torch = _torch()
+    code = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32}.get(dtype)
+    if code is None:
+        raise DsparkError(f"{what} is fp16, bf16 or fp32")
+    return code
+
+
+def _on_device(t, stream, call, *args):
+    """call(stream handle, *args) with t's device current and `stream` (default: that device's current one) the stream that
+    allocations belong to."""
+    torch = _torch()
+    index = t.get_device()
+    if index < 0:
+        raise DsparkError("tensors are on a GPU")
+    if stream is None and torch.cuda.current_device() == index:
+        return call(torch._C._cuda_getCurrentRawStream(index), *args)
+    stream = stream if stream is not None else torch.cuda.current_stream(t.device)
+    if stream.device_index != index:
+        raise DsparkError("the stream belongs to another device than the tensors")
+    with torch.cuda.stream(stream):
+        return call(stream.cuda_stream, *args)
+
+
+def _flat(t, shape, dtype, index, what):
+    """The data pointer of an optional contiguous tensor of this shape and type (shape None: any) on device `index`."""
+    if t is None:
+        return None
+    if t.dtype != dtype or (shape is not None and t.shape != shape) or not t.is_contiguous() or t.get_device() != index:
+        raise DsparkError(f"{what} is a contiguous {dtype} tensor" + ("" if shape is None else f" of shape {tuple(shape)}") + " on the call's device")
+    return t.data_ptr()
+
+
+def _heads(t, what):
+    """n, heads, D and the elements between the rows of a [n][heads][D] tensor whose rows are contiguous."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or (shape[2] > 1 and stride[2] != 1) or (shape[1] > 1 and stride[1] != shape[2]):
+        raise DsparkError(f"{what} is [n][heads][D] of contiguous rows")
+    return shape[0], shape[1], shape[2], stride[0] if shape[0] > 1 else shape[1] * shape[2]
+
+
+def rope_freqs(rot, base=10000.0, scaling=None, factor=1.0, trained=0.0, low=1.0, high=32.0):
+    """(frequencies, scale) of dspark_rope for `rot` turned values of a head: float64 [rot / 2] radians a position (numpy; to be
+    moved to the device once) and the factor of the turned values. scaling None, "linear", "base" or "ramp" (include/dspark.h)."""
+    import numpy as np
+    if scaling not in ROPE_SCALING:
+        raise DsparkError(f"rope_freqs: scaling is one of {list(ROPE_SCALING)}")
+    out, scale = np.empty(max(rot, 0) // 2, np.float64), ctypes.c_double()
+    check(lib().dspark_rope_freqs(rot, base, ROPE_SCALING[scaling], factor, trained, low, high, out.ctypes.data_as(ctypes.c_void_p),
+                                  ctypes.byref(scale)), "dspark_rope_freqs")
+    return out, scale.value
+
+
+def _rope_args(q, k, positions, freqs, interleaved, inverse, scale):
+    torch = _torch()
+    first = q if q is not None else k
+    if first is None:
+        raise DsparkError("rope: q or k")
+    a, index = RopeArgs(), first.get_device()
+    a.type = _type_of(first.dtype, "rope: q and k")
+    for name, t in (("q", q), ("k", k)):
+        if t is None:
+            continue
+        n, heads, D, stride = _heads(t, "rope: " + name)
+        if t.dtype != first.dtype or n != first.shape[0] or D != first.shape[2] or t.get_device() != index:
+            raise DsparkError("rope: q and k have one type, device, number of rows and head size")
+        if name == "q":
+            a.q, a.q_stride, a.QH = t.data_ptr(), stride, heads
+        else:
+            a.k, a.k_stride, a.KVH = t.data_ptr(), stride, heads
+    a.n, a.D, a.rot = first.shape[0], first.shape[2], 2 * freqs.numel()
+    a.positions = _flat(positions, first.shape[:1], torch.int32, index, "positions")
+    a.freq = _flat(freqs, freqs.shape[:1], torch.float64, index, "freqs")
+    a.interleaved, a.inverse, a.scale = int(interleaved), int(inverse), scale
+    return a
+
+
+def _rope_out(t, out, index, what):
+    if out is None:
+        out = t.new_empty(t.shape)
+    n, heads, D, stride = _heads(out, what)
+    if out.shape != t.shape or out.dtype != t.dtype or out.get_device() != index:
+        raise DsparkError(f"{what} has its input's shape, type and device")
+    return out, out.data_ptr(), stride
+
+
+def _rope(s, a, q, k, q_out, k_out):
+    if q is not None:
+        q_out, a.q_out, a.q_out_stride = _rope_out(q, q_out, q.get_device(), "q_out")
+    if k is not None:
+        k_out, a.k_out, a.k_out_stride = _rope_out(k, k_out, k.get_device(), "k_out")
+    check(lib().dspark_rope(ctypes.byref(a), s), "dspark_rope")
+    return q_out, k_out
+
+
+def rope(q, k, positions, freqs, interleaved=False, inverse=False, scale=1.0, q_out=None, k_out=None, stream=None):
+    """Turn the first 2 * len(freqs) values of every head of q and k (either may be None; [n][heads][D] fp16, bf16 or fp32, rows may
+    lie inside wider ones) by positions (int32 [n]) times freqs (float64, rope_freqs). inverse: by the negative angles, which is
+    the gradient's way back. Returns (q_out, k_out) as given (q itself: in place) or created."""
+    a = _rope_args(q, k, positions, freqs, interleaved, inverse, scale)
+    return _on_device(q if q is not None else k, stream, _rope, a, q, k, q_out, k_out)
+
+
+def _rope_append(s, a, q, q_out):
+    q_out, a.q_out, a.q_out_stride = _rope_out(q, q_out, q.get_device(), "q_out")
+    check(lib().dspark_rope(ctypes.byref(a), s), "dspark_rope")
+    return q_out
+
+
+def rope_append(q, k, v, positions, freqs, k_pages, v_pages, slots, interleaved=False, scale=1.0, q_out=None, stream=None):
+    """rope of q, with the turned k and v (fp16 [n][KVH][D]) written into the fp16 pages instead: row t to slot slots[t] (int64,
+    32 * physical page + position in it; outside the pools: nowhere). Returns q_out."""
+    torch = _torch()
+    if q is None or k is None or v is None or k.dtype != torch.float16:
+        raise DsparkError("rope_append: q, k and v are fp16")
+    a, index = _rope_args(q, k, positions, freqs, interleaved, False, scale), q.get_device()
+    KVH, D, P = a.KVH, a.D, k_pages.shape[0]
+    n, heads, dv, a.v_stride = _heads(v, "rope_append: v")
+    if v.shape != k.shape or v.dtype != torch.float16 or v.get_device() != index:
+        raise DsparkError("rope_append: k and v have one shape, type and device")
+    a.v, a.kv_pages = v.data_ptr(), P
+    a.k_pages = _flat(k_pages, (P, KVH, PAGE, D), torch.float16, index, "k_pages")
+    a.v_pages = _flat(v_pages, (P, KVH, D, PAGE), torch.float16, index, "v_pages")
+    a.slots = _flat(slots, q.shape[:1], torch.int64, index, "slots")
+    return _on_device(q, stream, _rope_append, a, q, q_out)
+
+
+def _with_workspace(s, t, a, workspace, call, need, what):
+    """call(a, stream) with the workspace as it is first, then with one that is large enough."""
+    torch, ref = _torch(), ctypes.byref(a)
+    if workspace is not None and workspace.buf is not None and torch.cuda.is_current_stream_capturing():
+        workspace.hold()
+    ws = workspace and workspace.buf
+    while True:
+        if ws is not None:
+            if ws.get_device() != t.get_device():
+                raise DsparkError("workspace and tensors are on different devices")
+            a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        rc = call(ref, s)
+        if rc != ENOSPACE:
+            return check(rc, what)
+        n = need(ref)
+        if n <= a.workspace_bytes:
+            check(rc, what)
+        ws = (workspace or Workspace(t.device)).get(n)
+
+
+def _verify_attention_shared(s, a, q, out, out_f32, workspace):
+    torch = _torch()
+    if out is None and out_f32 is None:
+        out = q.new_empty(q.shape)
+    a.out = _flat(out, q.shape, torch.float16, q.get_device(), "out")
+    a.out_f32 = _flat(out_f32, q.shape, torch.float32, q.get_device(), "out_f32")
+    L = lib()
+    _with_workspace(s, q, a, workspace, L.dspark_verify_attention_shared, L.dspark_verify_attention_shared_workspace,
+                    "dspark_verify_attention_shared")
+    return out, out_f32
+
+
+def verify_attention_shared(q, k_pages, v_pages, prefix, q_start, own_len, own_table, max_tokens, prefix_table=None, window=0,
+                            causal=True, out=None, out_f32=None, lse=None, gate=None, splits=0, workspace=None, stream=None):
+    """verify_attention of a batch of sequences behind a shared prefix (include/dspark.h): q fp16 [tokens][QH][D], sequence r's rows
+    q_start[r] .. q_start[r + 1] - 1 (int32 [seqs + 1] on the device, at most max_tokens each), the prefix in the pages of
+    prefix_table (int32, None = identity), sequence r's own own_len[r] keys (int32) in those of own_table[r] (int32 [seqs][pages]).
+    Returns (out fp16, out_f32) as given/created; rows in no sequence are not written."""
+    torch = _torch()
+    T, QH, D, stride = _heads(q, "q")
+    index = q.get_device()
+    if q.dtype != torch.float16 or k_pages.dim() != 4:
+        raise DsparkError("q is fp16, pages are [n_pages][KVH][32][D]")
+    if (prefix | max_tokens | window | splits) >> 31:
+        raise DsparkError("verify_attention_shared: counts are from 0 to 2^31 - 1")
+    P, KVH, R = k_pages.shape[0], k_pages.shape[1], own_len.shape[0]
+    if prefix_table is not None and prefix_table.numel() * PAGE < prefix:
+        raise DsparkError(f"{prefix} positions need {(prefix + PAGE - 1) // PAGE} entries in the prefix table")
+    if own_table.dim() != 2 or own_table.shape[0] != R or own_table.dtype != torch.int32 or own_table.get_device() != index \
+            or (own_table.shape[1] > 1 and own_table.stride(1) != 1):
+        raise DsparkError("own_table is int32 [seqs][pages] on q's device")
+    a = SharedAttnArgs()
+    a.q, a.q_stride, a.kv_pages = q.data_ptr(), stride, P
+    a.k_pages = _flat(k_pages, (P, KVH, PAGE, D), torch.float16, index, "k_pages")
+    a.v_pages = _flat(v_pages, (P, KVH, D, PAGE), torch.float16, index, "v_pages")
+    a.prefix_table = _flat(prefix_table, None, torch.int32, index, "prefix_table")
+    a.q_start = _flat(q_start, (R + 1,), torch.int32, index, "q_start")
+    a.own_len = _flat(own_len, (R,), torch.int32, index, "own_len")
+    a.own_table, a.own_pages = own_table.data_ptr(), own_table.shape[1]
+    a.own_stride = own_table.stride(0) if R > 1 else a.own_pages
+    a.lse = _flat(lse, (T, QH), torch.float32, index, "lse")
+    a.gate = _flat(gate, (T, QH), torch.float32, index, "gate")
+    a.prefix, a.tokens, a.seqs, a.max_tokens = prefix, T, R, min(max_tokens, T)
+    a.QH, a.KVH, a.D, a.window, a.causal, a.splits = QH, KVH, D, window, int(bool(causal)), splits
+    return _on_device(q, stream, _verify_attention_shared, a, q, out, out_f32, workspace)
+
+
+class Sampled:
+    """What verify_sample returned: tokens, keys, kept, logprob (None where not asked for)."""
+
+    def __init__(self, tokens, keys, kept, logprob):
+        self.tokens, self.keys, self.kept, self.logprob = tokens, keys, kept, logprob
+
+
+def _verify_sample(s, a, logits, outs, workspace):
+    torch, n, index = _torch(), a.n, logits.get_device()
+    types = (torch.int32, torch.int64, torch.int32, torch.float32)
+    made = []
+    for name, t, dtype in zip(("tokens", "keys", "kept", "logprob"), outs, types):
+        if t is True:
+            t = torch.empty(n, dtype=dtype, device=logits.device)
+        elif t is False:
+            t = None
+        setattr(a, name, _flat(t, (n,), dtype, index, name))
+        made.append(t)
+    L = lib()
+    _with_workspace(s, logits, a, workspace, L.dspark_verify_sample, lambda ref: L.dspark_verify_sample_workspace(n, a.V), "dspark_verify_sample")
+    return Sampled(*made)
+
+
+def verify_sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, tokens=True, keys=False, kept=False, logprob=False,
+                  workspace=None, stream=None):
+    """A token for each row of logits ([n][V] fp16, bf16 or fp32; rows may lie inside wider ones) from u (fp32 [n], in [0, 1)):
+    the definition is in include/dspark.h. temperature, top_p, min_p (fp32) and top_k (int32) are numbers or [n] tensors. Each
+    of tokens, keys, kept, logprob is a tensor to fill, True (made) or False; keys are what accept_commit takes. Returns a Sampled."""
+    torch = _torch()
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise DsparkError("logits are [n][V] of contiguous rows")
+    a, (n, V), index = SampleArgs(), logits.shape, logits.get_device()
+    a.type = _type_of(logits.dtype, "logits")
+    a.logits, a.row_stride, a.n, a.V = logits.data_ptr(), logits.stride(0) if n > 1 else V, n, V
+    a.u = _flat(u, (n,), torch.float32, index, "u")
+    for name, x, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
+                           ("min_p", min_p, torch.float32)):
+        if isinstance(x, torch.Tensor):
+            setattr(a, name, _flat(x, (n,), dtype, index, name))
+        elif dtype is torch.int32 and not -(1 << 31) <= x < 1 << 31:
+            raise DsparkError("verify_sample: top_k is a 32-bit number")
+        else:
+            setattr(a, name + "_all", x)
+    return _on_device(logits, stream, _verify_sample, a, logits, (tokens, keys, kept, logprob), workspace)
 
 
 # ---------------------------------------------------------------- argmax / accept
