@@ -62,13 +62,24 @@ size_t shared_workspace(const SharedAttn& p, int D);
 int shared_launch(SharedAttn& p, int D, hipStream_t s);
 
 // Sampling (sample.hip).
-constexpr int SP_BINS = 2048, SP_LIST = 2048, SP_PARTS = 256;
-// What is known of a row between the launches.
+// A row's settings, and what is known of it between the launches.
+struct SampleLocals {
+  double inv_t, inv_t2;  // 1 / T, log2(e) / T
+  double low;            // min-p's bound of (z - m) / T
+  float m;               // the row's maximum
+  uint32_t first;        // where it is first
+  float p;               // top-p (1: none)
+  int k;                 // top-k (0: none)
+  bool greedy, empty, cut_low, inf;  // inf: the maximum is +inf, differences to it are no numbers
+};
+struct SampleBegun {
+  SampleLocals s;        // without what needs the maximum
+};
 struct SampleRow {
-  uint32_t mode, bin;    // bin in which the cut lies
-  uint32_t above;        // tokens in the bins above it, and their weight
-  uint32_t by_mass;      // the cut is top-p's (else top-k's)
-  uint64_t mass_above, limit;  // limit: tokens (top-k) or weight (top-p) of what is kept, before min-p
+  SampleLocals s;
+  uint32_t mode, bin;     // bin in which the cut lies
+  uint32_t by_mass, pad;  // the cut is top-p's (else top-k's)
+  uint64_t above, limit;  // weight (else tokens) in the bins above it, and of what is kept, before min-p
 };
 struct SampleParams {
   const void* logits;
@@ -84,18 +95,22 @@ struct SampleParams {
   uint64_t* keys;
   int32_t* kept;
   float* logprob;
-  int n, V, P, ps, wide;  // parts of a row and their tokens (a multiple of a workgroup's step); rows on 16-byte boundaries
+  int n, V, wide;         // rows on 16-byte boundaries
+  int P, ps;              // parts of a row in the first launch and their tokens (a multiple of a workgroup's step),
+  int P2, ps2, P3, ps3;   // in the second and the third
+  int chunks;             // of a row: as many tokens as a wave takes at a time
   // workspace
-  uint64_t* part_key;     // [n][P]
-  uint64_t* part_sum;     // [n][P]
-  uint64_t* hist_mass;    // [n][SP_BINS]
-  SampleRow* rows;        // [n]
-  uint32_t* hist_count;   // [n][SP_BINS]
-  uint32_t* part_count;   // [n][P]
-  uint32_t* part_at;      // [n][P] where the part's tokens are in the list
-  uint32_t* part_listed;  // [n][P] and how many
-  uint32_t* list;         // [n][SP_LIST]
-  uint32_t* marks;        // [n][4]: arrivals of the two launches, tokens listed
+  uint64_t* part_key;     // [n][P] the part's largest key
+  uint64_t* chunk_sum;    // [n][chunks] weight that is kept whatever the cut in the bin
+  uint64_t* hist_mass;    // [n][bins]
+  uint64_t* whole;        // [n] the row's weight
+  SampleBegun* rows;      // [n] after the first launch
+  SampleRow* result;      // [n] after the second
+  float* part_sum;        // [n][P] about the part's weight, in units of its largest
+  uint32_t* hist_count;   // [n][bins]
+  uint64_t* list;         // [n][list] tokens: argmax keys
+  uint64_t* taken;        // [n] tokens listed, and above bit 32 tokens kept above the bin
+  uint32_t* marks;        // [n][2] arrivals of the second and the third launch
 };
 void sample_plan(SampleParams& p);
 size_t sample_workspace(SampleParams& p, void* ws);

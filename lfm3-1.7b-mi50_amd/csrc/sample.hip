@@ -8,14 +8,14 @@
 //
 // Top-k and top-p both keep a prefix of the tokens ranked by (z descending, index), min-p one by z alone: what is kept is
 // "key above key*, or equal to it and index up to idx*" and z at least the min-p bound. The cut is found without sorting:
-//   1 sample_max    a part of a row each: the largest key; clears the row's histogram
-//   2 sample_hist   a part each: tokens by bins of max - z, logarithmic (128 an octave), counts and weights by LDS atomics, added
-//                   to the row's; the last part to finish finds the bin in which the cut lies
-//   3 sample_pick   a part each: the tokens down to that bin into the row's list if they are at most LIST of them (as for most
-//                   settings), else the bin's own and the weight above it by parts; the last part finds the cut in the list by
-//                   digits of the key, then the token.
-// Rows that need no cut take no histogram; a row whose bin alone passes LIST (a flat one) is finished by one workgroup from
-// the row itself.
+//   1 sample_max    a part of a row each: the largest key, and about the part's weight; clears the row's histogram
+//   2 sample_hist   a part each: tokens by bins of max - z, logarithmic (128 an octave), counts (top-k) or weights too (top-p)
+//                   by LDS atomics, added to the row's; the last part to finish finds the bin in which the cut lies
+//   3 sample_pick   a part each: that bin's tokens into the row's list, and the weight above it by chunks of 512 tokens (top-k of few:
+//                   all tokens down to the bin into the list); the last part finds the cut in the list, then the token. SP_SMALL
+//                   tokens are ranked by comparing all with all, more narrowed to that by a second division of the bin.
+// Rows that need no cut take no histogram but sums by chunks, and one workgroup then the draw. A row whose bin alone passes
+// SP_LIST tokens (a flat one), or whose top-k does with top-p behind it, is finished by one workgroup from the row itself.
 #include <algorithm>
 #include <type_traits>
 
@@ -24,255 +24,434 @@
 
 namespace dspark {
 
-constexpr int SP_THREADS = 256, SP_UNIT = 8, SP_STEP = SP_THREADS * SP_UNIT;  // tokens of a thread and of a workgroup at a time
+// Tokens of a thread and of a workgroup at a time. The second and third launch have workgroups of 1024 threads: adds of many workgroups to
+// one word go one after the other, some 50 ns each (with workgroups of 256, a word a wave, 9 rows of 128000 tokens 45 us).
+constexpr int SP_UNIT = 8, SP_MAX_THREADS = 256, SP_THREADS = 512, SP_STEP = SP_THREADS * SP_UNIT;
+constexpr int SP_CHUNK = 64 * SP_UNIT;
+constexpr int SP_BINS = 2048, SP_LIST = 3584, SP_SMALL = 256, SP_PARTS = 256, SP_CHUNKS = 2048;
 constexpr uint32_t SP_BIN0 = (127 - 9) << 7;  // bin 1 begins at max - z = 2^-9, the last one at 2^7
-constexpr double SP_ONE = 17592186044416.0;   // 2^44
 
 enum : uint32_t { SP_EMPTY, SP_GREEDY, SP_ALL, SP_LISTED, SP_BELOW, SP_ROW };
 
-struct SampleLocals {
-  float m;               // the row's maximum
-  uint32_t first;        // where it is first
-  double inv_t, low;     // 1 / T; min-p's bound of (z - m) / T
-  bool greedy, empty, cut_low;
-  int k;                 // top-k (0: none)
-  float p;               // top-p (1: none)
-};
-
 __device__ __forceinline__ float sp_value(float z) { return z != z ? -INFINITY : z == 0.f ? 0.f : z; }  // (-0 is 0)
+// What an argmax key was made of.
+__device__ __forceinline__ float sp_logit(uint32_t ord) { return __uint_as_float(ord & 0x80000000u ? ord ^ 0x80000000u : ~ord); }
+__device__ __forceinline__ uint32_t sp_index(uint64_t key) { return 0xffffffffu - (uint32_t)key; }
+// max - z, rounded but in the order of z. (s.inf is the same in every lane: the other side of its branches costs nothing.)
+__device__ __forceinline__ float sp_dist(float z, const SampleLocals& s) {
+  if (s.inf) return z == INFINITY ? 0.f : INFINITY;
+  return s.m - z;
+}
 
+// Eight logits from `at` as they are (those from `end` on are -inf), and as numbers.
 template <typename T>
-__device__ __forceinline__ float sp_to_f32(T x) { return (float)x; }
-
-// Eight logits from `at`; those from `end` on are -inf.
-template <typename T>
-__device__ __forceinline__ void sp_load(const T* row, int at, int end, bool wide, float (&z)[SP_UNIT]) {
-  if (wide && at + SP_UNIT <= end) {
-    T x[SP_UNIT];
+struct SampleUnit {
+  T x[SP_UNIT];
+  __device__ __forceinline__ void load(const T* row, int at, int end, bool wide) {
+    if (wide && at + SP_UNIT <= end) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(x) / 16; ++i) {
-      const u32x4 u = ldg(reinterpret_cast<const u32x4*>(row + at) + i);
-      __builtin_memcpy(reinterpret_cast<char*>(x) + 16 * i, &u, 16);
+      for (int i = 0; i < (int)sizeof(x) / 16; ++i) {
+        const u32x4 u = ldg(reinterpret_cast<const u32x4*>(row + at) + i);
+        __builtin_memcpy(reinterpret_cast<char*>(x) + 16 * i, &u, 16);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < SP_UNIT; ++i) x[i] = at + i < end ? row[at + i] : (T)-INFINITY;
     }
+  }
+  __device__ __forceinline__ void values(float (&z)[SP_UNIT]) const {
 #pragma unroll
-    for (int i = 0; i < SP_UNIT; ++i) z[i] = sp_value(sp_to_f32(x[i]));
-  } else {
-#pragma unroll
-    for (int i = 0; i < SP_UNIT; ++i) z[i] = at + i < end ? sp_value(sp_to_f32(row[at + i])) : -INFINITY;
+    for (int i = 0; i < SP_UNIT; ++i) z[i] = sp_value((float)x[i]);
+  }
+};
+// f(at, z) for this thread's units of [begin, end), a step of the workgroup at a time, the next step's loads in flight meanwhile. Every
+// wave that has a unit there calls it with all its lanes (at >= end: -inf).
+template <typename T, int THREADS = SP_THREADS, typename F>
+__device__ __forceinline__ void sp_units(const T* row, int begin, int end, bool wide, F f) {
+  const int lane0 = (threadIdx.x & ~63) * SP_UNIT;
+  int at = begin + threadIdx.x * SP_UNIT;
+  SampleUnit<T> now, next;
+  now.load(row, at, end, wide);
+  constexpr int STEP = THREADS * SP_UNIT;
+  for (int wave = begin + lane0; wave < end; wave += STEP, at += STEP) {
+    if (wave + STEP < end) next.load(row, at + STEP, end, wide);
+    f(at, now);
+    now = next;
   }
 }
 
-__device__ __forceinline__ uint32_t sp_bin(float z, float m) {
-  const float d = m - z;  // rounded, but the bins stay in the order of z
-  if (!(d > 0.f)) return 0;  // (also +inf - +inf)
-  const uint32_t b = __float_as_uint(d) >> 16;
-  return b < SP_BIN0 ? 0 : min(b - SP_BIN0 + 1, (uint32_t)SP_BINS - 1);
+// The bin of d = max - z >= 0 (rounded, but the bins stay in the order of z).
+__device__ __forceinline__ uint32_t sp_bin(float d) {
+  const int b = (int)(__float_as_uint(d) >> 16);
+  return (uint32_t)(min(max(b, (int)SP_BIN0 - 1), (int)SP_BIN0 + SP_BINS - 2) - ((int)SP_BIN0 - 1));
 }
+// Bins up to b hold what is not at least this (the last bin: everything).
+__device__ __forceinline__ float sp_edge(uint32_t b) { return b >= SP_BINS - 1 ? NAN : __uint_as_float((SP_BIN0 + b) << 16); }
 
-// 2^44 exp((z - m) / T) as a whole number: 2^x by its whole part and the series of 2^f = e^(f ln 2), |f| <= 1/2, to the 11th
-// power (the next term is under 7e-15 = 2^-47).
-__device__ __forceinline__ uint64_t sp_weight(float z, const SampleLocals& s) {
-  if (z == s.m) return (uint64_t)1 << 44;
-  const double x = ((double)z - (double)s.m) * s.inv_t * 1.4426950408889634074;
-  if (!(x > -46.0)) return 0;
-  const double k = rint(x), f = (x - k) * 0.69314718055994530942;
-  double e = 1.0 / 39916800.0;
-  e = fma(e, f, 1.0 / 3628800.0);
-  e = fma(e, f, 1.0 / 362880.0);
-  e = fma(e, f, 1.0 / 40320.0);
-  e = fma(e, f, 1.0 / 5040.0);
-  e = fma(e, f, 1.0 / 720.0);
-  e = fma(e, f, 1.0 / 120.0);
-  e = fma(e, f, 1.0 / 24.0);
-  e = fma(e, f, 1.0 / 6.0);
-  e = fma(e, f, 0.5);
+// a b + c for a constant c that stays in scalar registers (the compiler copies it into the accumulator of a two-address form
+// instead: a third of a weight's instructions).
+__device__ __forceinline__ double sp_fma(double a, double b, double c) {
+  double d;
+  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "s"(c));
+  return d;
+}
+// 2^44 exp((z - m) / T) as a whole number, m finite: 2^x by its whole part and a polynomial of 2^f, |f| <= 1/2, of degree 10 (through
+// the Chebyshev nodes; off by 2^-51). -inf and NaN weigh nothing: they end as x = -46, a quarter of a unit.
+__device__ __forceinline__ uint64_t sp_weight_finite(float z, const SampleLocals& s) {
+  const double x = fmax(((double)z - (double)s.m) * s.inv_t2, -46.0);
+  const double k = rint(x), f = x - k;
+  double e = sp_fma(f, 7.072585949269223e-09, 1.0208690299958306e-07);
+  e = sp_fma(e, f, 1.321544258792169e-06);
+  e = sp_fma(e, f, 1.5252657260200837e-05);
+  e = sp_fma(e, f, 0.0001540353044173605);
+  e = sp_fma(e, f, 0.0013333558230164974);
+  e = sp_fma(e, f, 0.009618129107606888);
+  e = sp_fma(e, f, 0.05550410866444772);
+  e = sp_fma(e, f, 0.24022650695910097);
+  e = sp_fma(e, f, 0.69314718055995);
   e = fma(e, f, 1.0);
-  e = fma(e, f, 1.0);
-  // the weight in units of one, rounded to a whole number by the unit of 2^52
+  // in units of one and rounded to a whole number by the unit of 2^52
   const double y = __builtin_ldexp(e, (int)k + 44) + 4503599627370496.0;
   return (uint64_t)__double_as_longlong(y) & 0xfffffffffffffull;
 }
+__device__ __forceinline__ uint64_t sp_weight(float z, const SampleLocals& s) {
+  if (s.inf) return z == INFINITY ? (uint64_t)1 << 44 : 0;
+  return sp_weight_finite(z, s);
+}
 __device__ __forceinline__ bool sp_high(float z, const SampleLocals& s) {  // min-p
-  return !s.cut_low || z == s.m || ((double)z - (double)s.m) * s.inv_t >= s.low;
+  if (s.inf) return !s.cut_low || z == INFINITY;
+  return !s.cut_low || ((double)z - (double)s.m) * s.inv_t >= s.low;
 }
 
-// A wave's and a workgroup's sums of whole numbers. scratch: 4 words.
-__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v, int lane) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const uint32_t lo = __shfl_up((uint32_t)v, d), hi = __shfl_up((uint32_t)(v >> 32), d);
-    if (lane >= d) v += ((uint64_t)hi << 32) | lo;
-  }
+// Sums of whole numbers over a wave, inclusive in lane order (by row moves, no LDS: 16, then across the rows), and the whole.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t wave_moved_u64(uint64_t v) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xf, false);
+  return ((uint64_t)hi << 32) | lo;
+}
+__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {
+  v += wave_moved_u64<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8
+  v += wave_moved_u64<0x112, 0xf>(v);
+  v += wave_moved_u64<0x114, 0xf>(v);
+  v += wave_moved_u64<0x118, 0xf>(v);
+  v += wave_moved_u64<0x142, 0xa>(v);  // lane 15 of rows 0 and 2 to rows 1 and 3
+  v += wave_moved_u64<0x143, 0xc>(v);  // lane 31 to rows 2 and 3
   return v;
 }
-// Inclusive sums over the workgroup in thread order; *total the whole. Ends with every thread past the scratch.
+__device__ __forceinline__ uint64_t wave_last_u64(uint64_t v) {
+  return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), 63) << 32) |
+         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, 63);
+}
+__device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) { return wave_last_u64(wave_scan_u64(v)); }
+// The same over a workgroup in thread order (*total the whole), and the whole alone: eight lanes add the eight waves' sums.
+static_assert(SP_THREADS / 64 == 8, "a wave's sum a lane of half a row");
+__device__ __forceinline__ uint64_t row_sum_u64(uint64_t v) {  // of values that repeat after eight lanes
+  v += wave_moved_u64<0x124, 0xf>(v);  // row_ror:4, 2, 1
+  v += wave_moved_u64<0x122, 0xf>(v);
+  return v + wave_moved_u64<0x121, 0xf>(v);
+}
 __device__ __forceinline__ uint64_t block_scan_u64(uint64_t v, uint64_t* scratch, uint64_t* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  v = wave_scan_u64(v, lane);
+  v = wave_scan_u64(v);
   if (lane == 63) scratch[wave] = v;
   __syncthreads();
-  uint64_t before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    if (w < wave) before += scratch[w];
-    all += scratch[w];
-  }
-  *total = all;
+  const uint64_t w = scratch[lane & 7];
+  *total = row_sum_u64(w);
+  v += row_sum_u64((lane & 7) < wave ? w : 0);
+  __syncthreads();  // (the scratch is free again)
+  return v;
+}
+__device__ __forceinline__ uint64_t block_sum_u64(uint64_t v, uint64_t* scratch) {
+  v = wave_sum_u64(v);
+  if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
   __syncthreads();
-  return before + v;
+  v = row_sum_u64(scratch[threadIdx.x & 7]);
+  __syncthreads();
+  return v;
+}
+__device__ __forceinline__ void sp_add(uint64_t* to, uint64_t v) {
+  atomicAdd(reinterpret_cast<unsigned long long*>(to), (unsigned long long)v);
 }
 
 template <typename T>
 __device__ __forceinline__ const T* sp_row(const SampleParams& p, int row) {
   return static_cast<const T*>(p.logits) + (size_t)row * p.stride;
 }
+__device__ __forceinline__ uint64_t sp_limit(float p, uint64_t whole) {  // of weight in front of a kept token: less than this
+  return max((uint64_t)ceil((double)p * (double)whole), (uint64_t)1);
+}
 
-// The row's settings and maximum (the same in every thread; called by whole workgroups, after sample_max).
-__device__ __forceinline__ SampleLocals sp_locals(const SampleParams& p, int row) {
-  SampleLocals s;
-  uint64_t key = 0;
-  for (int i = threadIdx.x & 63; i < p.P; i += 64) key = max(key, ldg(p.part_key + (size_t)row * p.P + i));
-  key = wave_max_u64(key);
-  const uint32_t ord = (uint32_t)(key >> 32), bits = ord & 0x80000000u ? ord ^ 0x80000000u : ~ord;
-  s.m = __uint_as_float(bits);
-  s.first = 0xffffffffu - (uint32_t)key;
-  s.empty = !(s.m > -INFINITY);
-  const float t = p.temperature ? p.temperature[row] : p.temperature_all;
+// The row's settings without its maximum.
+__device__ __forceinline__ SampleLocals sp_settings(const SampleParams& p, int row) {
+  SampleLocals s = {};
+  const float t = p.temperature ? ldc(p.temperature + row) : p.temperature_all;
   s.greedy = !(t > 0.f);
   s.inv_t = s.greedy ? 1.0 : 1.0 / (double)t;
-  s.k = p.top_k ? p.top_k[row] : p.top_k_all;
+  s.inv_t2 = s.inv_t * 1.4426950408889634074;
+  s.k = p.top_k ? ldc(p.top_k + row) : p.top_k_all;
   if (s.k <= 0 || s.k >= p.V) s.k = 0;
-  s.p = p.top_p ? p.top_p[row] : p.top_p_all;
+  s.p = p.top_p ? ldc(p.top_p + row) : p.top_p_all;
   if (!(s.p < 1.f)) s.p = 1.f;
   s.p = fmaxf(s.p, 0.f);
-  const float low = p.min_p ? p.min_p[row] : p.min_p_all;
+  const float low = p.min_p ? ldc(p.min_p + row) : p.min_p_all;
   s.cut_low = low > 0.f;
   s.low = s.cut_low ? log((double)fminf(low, 1.f)) : 0.0;
   return s;
 }
+// Sets the row's maximum (after sample_max; every lane of a wave together, the same in all).
+__device__ __forceinline__ void sp_maximum(const SampleParams& p, int row, SampleLocals& s) {
+  uint64_t key = 0;
+  for (int i = threadIdx.x & 63; i < p.P; i += 64) key = max(key, ldg(p.part_key + (size_t)row * p.P + i));
+  key = wave_max_u64(key);
+  s.m = sp_logit((uint32_t)(key >> 32));
+  s.first = sp_index(key);
+  s.empty = !(s.m > -INFINITY);
+  s.inf = s.m == INFINITY;
+}
+// A record that an earlier launch wrote, the same in every lane.
+template <typename T>
+__device__ __forceinline__ T sp_read(const T* from) {
+  T x;
+  uint32_t w[sizeof(T) / 4];
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(T) / 4); ++i) w[i] = ldc(reinterpret_cast<const uint32_t*>(from) + i);
+  __builtin_memcpy(&x, w, sizeof(T));
+  return x;
+}
 
-// One of a row's parts is done; true in the last one, which then sees what the others wrote.
+// What a row's workgroups leave for the last of them goes past the XCDs' own L2s, by atomic adds and these; a fence would write a whole L2
+// back in every workgroup (measured: 9 rows of 128000 tokens 102 -> 40 us without).
+template <typename T>
+__device__ __forceinline__ void sp_put(T* to, T v) {
+  __hip_atomic_store(to, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename T>
+__device__ __forceinline__ T sp_get(const T* from) {
+  return __hip_atomic_load(const_cast<T*>(from), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// One of a row's parts is done: everything this workgroup put and added has arrived before its own arrival counts. True in the last one.
 __device__ __forceinline__ bool sp_last(uint32_t* mark, int parts) {
   __shared__ uint32_t arrived;
-  __threadfence();
+  __builtin_amdgcn_s_waitcnt(0);
+  asm volatile("" ::: "memory");
   __syncthreads();
   if (threadIdx.x == 0) arrived = atomicAdd(mark, 1u);
   __syncthreads();
-  const bool last = arrived == (uint32_t)parts - 1;
-  if (last) __threadfence();
-  return last;
+  return arrived == (uint32_t)parts - 1;
 }
 
 template <typename T>
-__global__ __launch_bounds__(SP_THREADS) void sample_max_kernel(SampleParams p) {
+__global__ __launch_bounds__(SP_MAX_THREADS) void sample_max_kernel(SampleParams p) {
   const int part = blockIdx.x % p.P, row = blockIdx.x / p.P;
   const T* z0 = sp_row<T>(p, row);
   const int end = min((part + 1) * p.ps, p.V);
-  for (int i = part * SP_THREADS + threadIdx.x; i < SP_BINS; i += p.P * SP_THREADS) {
+  const SampleLocals s = sp_settings(p, row);
+  const bool sums = !s.greedy && s.k == 0 && s.p < 1.f;  // (what sample_hist makes use of)
+  const float c = (float)s.inv_t2;
+  for (int i = part * SP_MAX_THREADS + threadIdx.x; i < SP_BINS; i += p.P * SP_MAX_THREADS) {
     p.hist_count[(size_t)row * SP_BINS + i] = 0;
     p.hist_mass[(size_t)row * SP_BINS + i] = 0;
   }
-  if (part == 0 && threadIdx.x < 4) p.marks[row * 4 + threadIdx.x] = 0;
-  uint64_t key = 0;
-  for (int at = part * p.ps + threadIdx.x * SP_UNIT; at < end; at += SP_STEP) {
-    float z[SP_UNIT];
-    sp_load<T>(z0, at, end, p.wide, z);
+  if (part == 0 && threadIdx.x < 2) p.marks[row * 2 + threadIdx.x] = 0;
+  if (part == 0 && threadIdx.x == 2) p.whole[row] = p.taken[row] = 0;
+  if (part == 0 && threadIdx.x == 3) p.rows[row].s = s;
+  float top = -3e38f, sum = 0.f;  // this thread's maximum and its weight in units of that one's
+  uint32_t at_top = 0xffffffffu;
+  bool none = true;
+  sp_units<T, SP_MAX_THREADS>(z0, part * p.ps, end, p.wide, [&](int at, const SampleUnit<T>& x) {
+    float z[SP_UNIT], u = -INFINITY;
+    int i0 = 0;
 #pragma unroll
-    for (int i = 0; i < SP_UNIT; ++i) key = max(key, argmax_key(z[i], (uint32_t)(at + i)));
-  }
+    for (int i = 0; i < SP_UNIT; ++i) {
+      z[i] = sp_value((float)x.x[i]);
+      if (z[i] > u) {
+        u = z[i];
+        i0 = i;
+      }
+    }
+    if (u > top || (none && u > -INFINITY)) {
+      sum *= fast_exp2((top - u) * c);
+      top = u;
+      at_top = at + i0;
+      none = false;
+    }
+    if (sums)
+#pragma unroll
+      for (int i = 0; i < SP_UNIT; ++i) sum += fast_exp2((z[i] - top) * c);
+  });
   __shared__ uint64_t best[4];
-  key = wave_max_u64(key);
+  __shared__ float weight[4];
+  const uint64_t mine = none ? 0 : argmax_key(top, at_top);
+  uint64_t key = wave_max_u64(mine);
   if ((threadIdx.x & 63) == 0) best[threadIdx.x >> 6] = key;
   __syncthreads();
-  if (threadIdx.x == 0) p.part_key[(size_t)row * p.P + part] = max(max(best[0], best[1]), max(best[2], best[3]));
+  key = max(max(best[0], best[1]), max(best[2], best[3]));
+  if (sums) {
+    const float w = wave_sum(none ? 0.f : sum * fast_exp2((top - sp_logit((uint32_t)(key >> 32))) * c));
+    if ((threadIdx.x & 63) == 0) weight[threadIdx.x >> 6] = w;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    p.part_key[(size_t)row * p.P + part] = key;
+    if (sums) p.part_sum[(size_t)row * p.P + part] = (weight[0] + weight[1]) + (weight[2] + weight[3]);
+  }
 }
 
 template <typename T>
 __global__ __launch_bounds__(SP_THREADS) void sample_hist_kernel(SampleParams p) {
-  __shared__ uint64_t mass[SP_BINS];
-  __shared__ uint32_t count[SP_BINS];
-  __shared__ uint64_t scratch[4];
-  const int part = blockIdx.x % p.P, row = blockIdx.x / p.P;
-  const SampleLocals s = sp_locals(p, row);
-  if (s.empty || s.greedy || (s.k == 0 && s.p >= 1.f)) {
-    if (part == 0 && threadIdx.x == 0) p.rows[row].mode = s.empty ? SP_EMPTY : s.greedy ? SP_GREEDY : SP_ALL;
+  __shared__ uint64_t mass[SP_BINS];  // top-p
+  uint32_t* const count = reinterpret_cast<uint32_t*>(mass);  // top-k
+  __shared__ uint64_t scratch[SP_THREADS / 64];
+  __shared__ uint32_t cut_at;
+  const int part = blockIdx.x % p.P2, row = blockIdx.x / p.P2, lane = threadIdx.x & 63;
+  SampleLocals s = sp_read(&p.rows[row].s);
+  sp_maximum(p, row, s);
+  const T* z0 = sp_row<T>(p, row);
+  const int begin = part * p.ps2, end = min(begin + p.ps2, p.V);
+  const bool all_kept = s.k == 0 && s.p >= 1.f;  // (but what min-p cuts)
+  if (s.empty || s.greedy || s.inf || all_kept) {
+    // (an infinite maximum is rare: by the general way, so that the loops need not ask)
+    SampleRow r = {};
+    r.mode = s.empty ? SP_EMPTY : s.greedy ? SP_GREEDY : s.inf ? SP_ROW : SP_ALL;
+    r.s = s;
+    if (part == 0 && threadIdx.x == 0) p.result[row] = r;
+    if (r.mode != SP_ALL) return;
+    // the kept weight by chunks
+    uint32_t number = 0;
+    sp_units<T>(z0, begin, end, p.wide, [&](int at, const SampleUnit<T>& x) {
+      float z[SP_UNIT];
+      x.values(z);
+      uint64_t sum = 0;
+#pragma unroll
+      for (int i = 0; i < SP_UNIT; ++i) {
+        const bool in = z[i] > -INFINITY && sp_high(z[i], s);
+        sum += in ? sp_weight_finite(z[i], s) : 0;
+        number += in;
+      }
+      sum = wave_sum_u64(sum);
+      if (lane == 0) p.chunk_sum[(size_t)row * p.chunks + at / SP_CHUNK] = sum;
+    });
+    number = (uint32_t)block_sum_u64(number, scratch);
+    if (threadIdx.x == 0 && number) sp_add(p.taken + row, (uint64_t)number << 32);
     return;
   }
-  for (int i = threadIdx.x; i < SP_BINS; i += SP_THREADS) {
-    mass[i] = 0;
-    count[i] = 0;
-  }
+  for (int i = threadIdx.x; i < SP_BINS; i += SP_THREADS) mass[i] = 0;
   __syncthreads();
-  const T* z0 = sp_row<T>(p, row);
-  const int end = min((part + 1) * p.ps, p.V);
-  for (int at = part * p.ps + threadIdx.x * SP_UNIT; at < end; at += SP_STEP) {
-    float z[SP_UNIT];
-    sp_load<T>(z0, at, end, p.wide, z);
-#pragma unroll
-    for (int i = 0; i < SP_UNIT; ++i) {
-      if (!(z[i] > -INFINITY)) continue;
-      const uint32_t b = sp_bin(z[i], s.m);
-      atomicAdd(&count[b], 1u);
-      if (s.p < 1.f) {
-        const uint64_t w = sp_weight(z[i], s);
-        if (w) atomicAdd(reinterpret_cast<unsigned long long*>(&mass[b]), (unsigned long long)w);
-      }
+  // Tokens past `far` are in no cut and need no bin. Top-p: those lighter than (1 - p) / V of the whole weigh less than 1 - p of
+  // it together, so the cut is above them (a thousandth less, for what fp32 sums and the logarithm lose). Top-k: what is
+  // past a bin that k tokens of this part reach, looked up once the first step is through.
+  const bool by_k = s.k > 0;
+  float far = INFINITY;
+  if (!by_k) {
+    float whole = 0.f;
+    const float c = (float)s.inv_t2;
+    for (int i = lane; i < p.P; i += 64) {
+      const uint64_t key = ldg(p.part_key + (size_t)row * p.P + i);
+      if (key) whole += ldg(p.part_sum + (size_t)row * p.P + i) * fast_exp2((sp_logit((uint32_t)(key >> 32)) - s.m) * c);
     }
+    whole = wave_sum(whole);
+    const float x = log2f((1.f - s.p) * whole * 0.999f / (float)p.V);
+    if (x < 0.f) far = -x / c;  // (not where it is no number)
+  }
+  uint64_t all = 0;
+  if (by_k) {
+    auto add = [&](int, const SampleUnit<T>& x) {
+      float z[SP_UNIT];
+      x.values(z);
+#pragma unroll
+      for (int i = 0; i < SP_UNIT; ++i) {
+        const float d = s.m - z[i];
+        if (z[i] > -INFINITY && d <= far) atomicAdd(&count[sp_bin(d)], 1u);
+      }
+    };
+    const int first = min(begin + SP_STEP, end);
+    sp_units<T>(z0, begin, first, p.wide, add);
+    if (first < end) {
+      if (threadIdx.x == 0) cut_at = SP_BINS;
+      __syncthreads();
+      constexpr int EACH = SP_BINS / SP_THREADS;
+      uint64_t n = 0, total;
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) n += count[threadIdx.x * EACH + i];
+      const uint64_t before = block_scan_u64(n, scratch, &total) - n;
+      if (before < (uint64_t)s.k && before + n >= (uint64_t)s.k) cut_at = threadIdx.x * EACH + EACH - 1;  // (its bins whole)
+      __syncthreads();
+      if (cut_at < SP_BINS - 1) far = sp_edge(cut_at);
+      sp_units<T>(z0, first, end, p.wide, add);
+    }
+  } else {
+    sp_units<T>(z0, begin, end, p.wide, [&](int, const SampleUnit<T>& x) {
+#pragma unroll
+      for (int i = 0; i < SP_UNIT; ++i) {
+        const float z = (float)x.x[i];
+        const uint64_t w = sp_weight_finite(z, s);  // (0 for a NaN)
+        const float d = s.m - z;
+        all += w;
+        if (d <= far) sp_add(&mass[sp_bin(d)], w);
+      }
+    });
+  }
+  if (!by_k) {
+    all = block_sum_u64(all, scratch);
+    if (threadIdx.x == 0) sp_add(&p.whole[row], all);
   }
   __syncthreads();
   for (int i = threadIdx.x; i < SP_BINS; i += SP_THREADS) {
-    if (count[i]) atomicAdd(&p.hist_count[(size_t)row * SP_BINS + i], count[i]);
-    if (mass[i]) atomicAdd(reinterpret_cast<unsigned long long*>(&p.hist_mass[(size_t)row * SP_BINS + i]), (unsigned long long)mass[i]);
+    if (by_k && count[i]) atomicAdd(&p.hist_count[(size_t)row * SP_BINS + i], count[i]);
+    if (!by_k && mass[i]) sp_add(&p.hist_mass[(size_t)row * SP_BINS + i], mass[i]);
   }
-  if (!sp_last(&p.marks[row * 4], p.P)) return;
+  if (!sp_last(&p.marks[row * 2], p.P2)) return;
 
-  // The bin of the cut: eight bins a thread, their sums before them.
+  // The bin of the cut, by the sums before each thread's bins.
   constexpr int EACH = SP_BINS / SP_THREADS;
-  uint64_t c[EACH], w[EACH], cs = 0, ws = 0;
+  uint64_t n[EACH], ns = 0, seen;
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
     const size_t b = (size_t)row * SP_BINS + threadIdx.x * EACH + i;
-    c[i] = p.hist_count[b];
-    w[i] = p.hist_mass[b];
-    cs += c[i];
-    ws += w[i];
+    n[i] = by_k ? sp_get(p.hist_count + b) : sp_get(p.hist_mass + b);
+    ns += n[i];
   }
-  uint64_t live, whole;
-  uint64_t c0 = block_scan_u64(cs, scratch, &live) - cs, w0 = block_scan_u64(ws, scratch, &whole) - ws;
-  const bool by_k = s.k > 0 && (uint64_t)s.k < live;
-  const uint64_t limit_w = max((uint64_t)ceil((double)s.p * (double)whole), (uint64_t)1);
-  if (!by_k && s.p >= 1.f) {
-    if (threadIdx.x == 0) p.rows[row].mode = SP_ALL;
+  uint64_t before = block_scan_u64(ns, scratch, &seen) - ns;
+  SampleRow r = {};
+  r.s = s;
+  r.by_mass = !by_k;
+  r.limit = by_k ? (uint64_t)s.k : sp_limit(s.p, sp_get(p.whole + row));
+  if (seen < r.limit) {  // fewer live tokens than top-k keeps: all of them stay
+    if (threadIdx.x == 0) {
+      r.bin = SP_BINS - 1;
+      r.mode = by_k && seen <= SP_LIST ? SP_LISTED : SP_ROW;
+      p.result[row] = r;
+    }
     return;
   }
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
-    const bool here = by_k ? c0 < (uint64_t)s.k && c0 + c[i] >= (uint64_t)s.k : w0 < limit_w && w0 + w[i] >= limit_w;
-    if (here) {  // (one thread, one bin)
-      SampleRow r;
+    if (before < r.limit && before + n[i] >= r.limit) {  // (one thread, one bin)
       r.bin = threadIdx.x * EACH + i;
-      r.above = (uint32_t)c0;
-      r.mass_above = w0;
-      r.by_mass = !by_k;
-      r.limit = by_k ? (uint64_t)s.k : limit_w;
-      // (top-k and top-p with more than a list's tokens: top-p's part of the whole is of what top-k leaves)
-      r.mode = c0 + c[i] <= SP_LIST ? SP_LISTED : c[i] <= SP_LIST && !(by_k && s.p < 1.f) ? SP_BELOW : SP_ROW;
-      p.rows[row] = r;
+      r.above = before;
+      const uint64_t to = before + n[i];
+      // (top-p behind a top-k of more than a list's tokens: its part of the whole is of what top-k leaves)
+      r.mode = !by_k || (s.p >= 1.f && to > SP_SMALL && n[i] <= SP_LIST) ? SP_BELOW : to <= (s.p < 1.f ? SP_LIST : SP_SMALL) ? SP_LISTED : SP_ROW;
+      p.result[row] = r;
     }
-    c0 += c[i];
-    w0 += w[i];
+    before += n[i];
   }
 }
 
-// Tokens in index order, from the list in LDS or (ROW) the row itself.
-template <typename T, bool ROW>
-struct SampleItems {
-  const T* z0;
-  const uint32_t* idx;
-  int n;
-  __device__ __forceinline__ uint32_t index(int i) const { return ROW ? (uint32_t)i : idx[i]; }
-  __device__ __forceinline__ float value(int i) const { return sp_value(sp_to_f32(z0[index(i)])); }
-};
+// The row's outputs (one thread).
+__device__ __forceinline__ void sp_store(const SampleParams& p, int row, int token, float z, uint64_t kept, uint64_t w, uint64_t whole) {
+  if (p.tokens) p.tokens[row] = token;
+  if (p.keys) p.keys[row] = token < 0 ? 0 : argmax_key(z, (uint32_t)token);
+  if (p.kept) p.kept[row] = (int)kept;
+  if (p.logprob) p.logprob[row] = (float)log((double)w / (double)whole);
+}
+// How much weight lies in front of the draw.
+__device__ __forceinline__ uint64_t sp_target(const SampleParams& p, int row, uint64_t whole) {
+  const float u = p.u[row];
+  const double x = u > 0.f ? (double)fminf(u, 1.f - 0x1p-24f) * (double)whole : 0.0;
+  return x < (double)(whole - 1) ? (uint64_t)x : whole - 1;
+}
 
 // What is kept so far: keys above `key`, or equal to it with index <= idx.
 struct SampleCut {
@@ -281,40 +460,90 @@ struct SampleCut {
 };
 
 struct SampleShared {
-  uint64_t mass[256];
+  alignas(16) uint64_t mass[256];
+  alignas(16) uint64_t key[SP_SMALL];
   uint32_t count[256];
-  uint64_t scratch[4];
-  uint64_t c, w;         // tokens and weight above the digits found so far
-  uint32_t digit, found;
-  uint64_t w_at;
-  uint32_t at, kept;
+  uint64_t scratch[SP_THREADS / 64];
+  uint64_t c, w;
+  uint32_t digit, found, at, number;
 };
 
-// Shrinks `cut` to the first `limit` tokens (by_mass false) or to those with less than `limit` weight in front of them, of the items it
-// keeps, `above` tokens of weight `mass_above` standing in front of all of them. Digits of eight bits from the top, then ties.
-template <typename Items>
-__device__ __forceinline__ void sp_shrink(const Items& it, const SampleLocals& s, SampleShared& sh, SampleCut& cut, bool by_mass, uint64_t limit,
-                                          uint64_t above, uint64_t mass_above) {
-  uint32_t prefix = 0;
-  uint64_t c = above, w = mass_above;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    sh.mass[threadIdx.x] = 0;
-    sh.count[threadIdx.x] = 0;
+// The tokens of a list (argmax keys in LDS) or of the whole row, in any order.
+struct SampleList {
+  const uint64_t* key;
+  int n;
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    for (int i = threadIdx.x; i < n; i += SP_THREADS) f(sp_index(key[i]), sp_logit((uint32_t)(key[i] >> 32)));
+  }
+};
+template <typename T>
+struct SampleWhole {
+  const T* z0;
+  int V;
+  bool wide;
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    sp_units<T>(z0, 0, V, wide, [&](int at, const SampleUnit<T>& x) {
+      float z[SP_UNIT];
+      x.values(z);
+#pragma unroll
+      for (int i = 0; i < SP_UNIT; ++i)
+        if (z[i] > -INFINITY) f((uint32_t)(at + i), z[i]);
+    });
+  }
+};
+
+// Among the tokens that of(idx, z, &order) takes, ranked by `order` descending, behind `c` tokens of weight `w`: the order at which the
+// tokens (by_mass: their weight) reach `limit`, by digits of eight bits. c and w become what stands in front of that order, `key` the
+// order; false: they never reach it.
+template <typename Items, typename Of>
+__device__ __forceinline__ bool sp_descend(const Items& it, const SampleLocals& s, SampleShared& sh, bool by_mass, uint64_t limit, uint64_t& c,
+                                           uint64_t& w, uint32_t& key, Of of) {
+  // the bits in which the orders differ
+  if (threadIdx.x == 0) sh.digit = 0, sh.found = 0xffffffffu;
+  __syncthreads();
+  uint32_t any = 0, every = 0xffffffffu;
+  it.each([&](uint32_t idx, float z) {
+    uint32_t o;
+    if (of(idx, z, o)) any |= o, every &= o;
+  });
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    any |= __shfl_xor(any, d);
+    every &= __shfl_xor(every, d);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    atomicOr(&sh.digit, any);
+    atomicAnd(&sh.found, every);
+  }
+  __syncthreads();
+  any = sh.digit;
+  every = sh.found;
+  const uint32_t differ = any & ~every;
+  int hi = differ ? 32 - __clz(differ) : 0;       // bits from hi up are the same everywhere
+  const int lo = differ ? __ffs(differ) - 1 : 0;  // and those below lo
+  uint32_t prefix = every;                        // right outside [lo, hi)
+  __syncthreads();
+  do {
+    const int shift = max(hi - 8, lo), bits = hi - shift;
+    const uint32_t mask = bits ? (0xffffffffu >> (32 - bits)) << shift : 0;
+    const uint32_t above = hi < 32 ? 0xffffffffu << hi : 0;  // bits already settled
+    if (threadIdx.x < 256) sh.mass[threadIdx.x] = sh.count[threadIdx.x] = 0;
     if (threadIdx.x == 0) sh.found = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < it.n; i += SP_THREADS) {
-      const float z = it.value(i);
-      if (!(z > -INFINITY)) continue;
-      const uint32_t key = argmax_ord(z);
-      if (!cut.keeps(key, it.index(i)) || (shift < 24 && (key >> (shift + 8)) != prefix)) continue;
-      const uint32_t d = 255 - ((key >> shift) & 255);  // the largest digit first
+    it.each([&](uint32_t idx, float z) {
+      uint32_t o;
+      if (!of(idx, z, o) || ((o ^ prefix) & above)) return;
+      const uint32_t d = 255 - ((o & mask) >> shift);  // the largest digit first
       atomicAdd(&sh.count[d], 1u);
-      if (by_mass) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.mass[d]), (unsigned long long)sp_weight(z, s));
-    }
+      if (by_mass) sp_add(&sh.mass[d], sp_weight(z, s));
+    });
     __syncthreads();
-    const uint64_t hc = sh.count[threadIdx.x], hw = sh.mass[threadIdx.x];
-    uint64_t all;
-    const uint64_t c1 = c + block_scan_u64(hc, sh.scratch, &all), w1 = w + block_scan_u64(hw, sh.scratch, &all);
+    const bool digit = threadIdx.x < 256;
+    const uint64_t hc = digit ? sh.count[threadIdx.x] : 0, hw = digit ? sh.mass[threadIdx.x] : 0;
+    uint64_t total;
+    const uint64_t c1 = c + block_scan_u64(hc, sh.scratch, &total), w1 = by_mass ? w + block_scan_u64(hw, sh.scratch, &total) : 0;
     if (by_mass ? w1 - hw < limit && w1 >= limit : c1 - hc < limit && c1 >= limit) {
       sh.digit = 255 - threadIdx.x;
       sh.c = c1 - hc;
@@ -322,264 +551,372 @@ __device__ __forceinline__ void sp_shrink(const Items& it, const SampleLocals& s
       sh.found = 1;
     }
     __syncthreads();
-    if (!sh.found) return;  // all of them stay
-    prefix = prefix << 8 | sh.digit;
+    if (!sh.found) return false;
+    prefix = (prefix & ~mask) | (sh.digit << shift & mask);
     c = sh.c;
     w = sh.w;
+    hi = shift;
     __syncthreads();
-  }
-  // of the tokens of this key the first `more`, in index order
-  float z;
-  {
-    const uint32_t bits = prefix & 0x80000000u ? prefix ^ 0x80000000u : ~prefix;
-    z = __uint_as_float(bits);
-  }
-  const uint64_t wt = sp_weight(z, s);
-  const uint64_t more = by_mass ? (wt ? (limit - w + wt - 1) / wt : 1) : limit - c;
-  const int each = (it.n + SP_THREADS - 1) / SP_THREADS, lo = min((int)threadIdx.x * each, it.n), hi = min(lo + each, it.n);
-  auto tie = [&](int i) { return argmax_ord(it.value(i)) == prefix && cut.keeps(prefix, it.index(i)); };
-  uint64_t mine = 0, ties;
-  for (int i = lo; i < hi; ++i) mine += tie(i);
-  uint64_t before = block_scan_u64(mine, sh.scratch, &ties) - mine;
-  if (threadIdx.x == 0) sh.at = 0xffffffffu;
-  __syncthreads();
-  if (more < ties && before < more && before + mine >= more)
-    for (int i = lo; i < hi; ++i)
-      if (tie(i) && ++before == more) sh.at = it.index(i);
-  __syncthreads();
-  const uint32_t all_ties = prefix == cut.key ? cut.idx : 0xffffffffu;  // (an earlier cut among the same ties)
-  cut.idx = sh.at == 0xffffffffu ? all_ties : sh.at;
-  cut.key = prefix;
-  __syncthreads();
+  } while (hi > lo);
+  key = prefix;
+  return true;
 }
 
-// The row's outputs (one thread).
-__device__ __forceinline__ void sp_store(const SampleParams& p, int row, int token, float z, int kept, float logprob) {
-  if (p.tokens) p.tokens[row] = token;
-  if (p.keys) p.keys[row] = token < 0 ? 0 : argmax_key(z, (uint32_t)token);
-  if (p.kept) p.kept[row] = kept;
-  if (p.logprob) p.logprob[row] = logprob;
+// Shrinks `cut` to the first `limit` tokens, or (by_mass) to those with less than `limit` weight in front of them, of the items it keeps,
+// `c` tokens of weight `w` standing in front of all of them.
+template <typename Items>
+__device__ __forceinline__ void sp_shrink(const Items& it, const SampleLocals& s, SampleShared& sh, SampleCut& cut, bool by_mass, uint64_t limit,
+                                          uint64_t c, uint64_t w) {
+  uint32_t key;
+  const SampleCut old = cut;
+  if (!sp_descend(it, s, sh, by_mass, limit, c, w, key, [&](uint32_t idx, float z, uint32_t& o) {
+        o = argmax_ord(z);
+        return old.keeps(o, idx);
+      }))
+    return;
+  // of the tokens of this key the first `more`, by index
+  const uint64_t wt = by_mass ? sp_weight(sp_logit(key), s) : 0;
+  const uint64_t more = by_mass ? (limit - w + wt - 1) / max(wt, (uint64_t)1) : limit - c;
+  uint64_t c2 = 0, w2 = 0;
+  uint32_t inv;
+  cut.key = key;
+  cut.idx = key == old.key ? old.idx : 0xffffffffu;
+  if (sp_descend(it, s, sh, false, more, c2, w2, inv, [&](uint32_t idx, float z, uint32_t& o) {
+        o = ~idx;
+        return argmax_ord(z) == key && old.keeps(key, idx);
+      }))
+    cut.idx = ~inv;
 }
-__device__ __forceinline__ uint64_t sp_target(const SampleParams& p, int row, uint64_t whole) {
-  const float u = p.u[row];
-  const double x = u > 0.f ? (double)fminf(u, 1.f - 0x1p-24f) * (double)whole : 0.0;
-  return x < (double)(whole - 1) ? (uint64_t)x : whole - 1;
-}
-__device__ __forceinline__ float sp_logprob(uint64_t w, uint64_t whole) { return (float)log((double)w / (double)whole); }
 
-// The draw among items: each thread's run of them, the run that the target falls into, the item.
+// The draw among items that the cut and min-p keep.
 template <typename Items>
 __device__ __forceinline__ void sp_draw(const SampleParams& p, int row, const Items& it, const SampleLocals& s, SampleShared& sh, const SampleCut& cut) {
-  const int each = (it.n + SP_THREADS - 1) / SP_THREADS, lo = min((int)threadIdx.x * each, it.n), hi = min(lo + each, it.n);
-  uint64_t mine = 0, kept = 0, whole, all;
-  for (int i = lo; i < hi; ++i) {
-    const float z = it.value(i);
-    if (!(z > -INFINITY) || !cut.keeps(argmax_ord(z), it.index(i)) || !sp_high(z, s)) continue;
-    mine += sp_weight(z, s);
+  uint64_t whole = 0, kept = 0;
+  it.each([&](uint32_t idx, float z) {
+    if (!cut.keeps(argmax_ord(z), idx) || !sp_high(z, s)) return;
+    whole += sp_weight(z, s);
     ++kept;
-  }
-  uint64_t sum = block_scan_u64(mine, sh.scratch, &whole) - mine;
-  block_scan_u64(kept, sh.scratch, &all);
+  });
+  whole = block_sum_u64(whole, sh.scratch);
+  kept = block_sum_u64(kept, sh.scratch);
   const uint64_t target = sp_target(p, row, whole);
-  if (sum > target || sum + mine <= target) return;
-  for (int i = lo; i < hi; ++i) {  // (one thread)
-    const float z = it.value(i);
-    if (!(z > -INFINITY) || !cut.keeps(argmax_ord(z), it.index(i)) || !sp_high(z, s)) continue;
-    const uint64_t w = sp_weight(z, s);
-    sum += w;
-    if (sum > target) {
-      sp_store(p, row, (int)it.index(i), z, (int)all, sp_logprob(w, whole));
-      return;
+  uint64_t c = 0, w = 0;
+  uint32_t inv;
+  sp_descend(it, s, sh, true, target + 1, c, w, inv, [&](uint32_t idx, float z, uint32_t& o) {
+    o = ~idx;
+    return cut.keeps(argmax_ord(z), idx) && sp_high(z, s);
+  });
+  it.each([&](uint32_t idx, float z) {
+    if (idx == ~inv) sp_store(p, row, (int)idx, z, kept, sp_weight(z, s), whole);
+  });
+}
+
+// All of the cuts and the draw among items that hold every token that may be kept.
+template <typename Items>
+__device__ __forceinline__ void sp_finish(const SampleParams& p, int row, const Items& it, const SampleLocals& s, SampleShared& sh) {
+  SampleCut cut = {0, 0xffffffffu};
+  if (s.k) sp_shrink(it, s, sh, cut, false, (uint64_t)s.k, 0, 0);
+  if (s.p < 1.f) {
+    uint64_t whole = 0;
+    it.each([&](uint32_t idx, float z) { whole += cut.keeps(argmax_ord(z), idx) ? sp_weight(z, s) : 0; });
+    whole = block_sum_u64(whole, sh.scratch);
+    sp_shrink(it, s, sh, cut, true, sp_limit(s.p, whole), 0, 0);
+  }
+  sp_draw(p, row, it, s, sh, cut);
+}
+
+// Of at most SP_SMALL tokens each thread has one (the argmax key, 0: none; its weight). All of them into sh.key and sh.mass, the rest
+// of either zeros; then f(key, weight) of each, four at a time (read one by one they are a chain of LDS latencies).
+static_assert(SP_SMALL == 256, "sh.mass");
+__device__ __forceinline__ void sp_lay(SampleShared& sh, uint64_t key, uint64_t w) {
+  if (threadIdx.x < SP_SMALL) {
+    sh.key[threadIdx.x] = key;
+    sh.mass[threadIdx.x] = w;
+  }
+  __syncthreads();
+}
+template <typename F>
+__device__ __forceinline__ void sp_all(const SampleShared& sh, int n, F f) {
+  typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
+#pragma unroll 2
+  for (int j = 0; j < n; j += 4) {
+    u64x2 k[2], w[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      k[i] = *reinterpret_cast<const u64x2*>(sh.key + j + 2 * i);
+      w[i] = *reinterpret_cast<const u64x2*>(sh.mass + j + 2 * i);
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f((uint64_t)k[i / 2][i % 2], (uint64_t)w[i / 2][i % 2]);
+  }
+}
+
+// Of at most SP_SMALL tokens, `above` (tokens or weight) standing in front of all of them: the cut after `limit`. All with all.
+__device__ __forceinline__ SampleCut sp_rank(const SampleList& it, const SampleLocals& s, SampleShared& sh, bool by_mass, uint64_t limit,
+                                             uint64_t above) {
+  const int i = threadIdx.x;
+  const bool there = i < it.n, has = (i & ~63) < it.n;  // (waves without a token stay out of the loop)
+  const uint64_t key = there ? it.key[i] : 0;
+  sp_lay(sh, key, !there ? 0 : by_mass ? sp_weight(sp_logit((uint32_t)(key >> 32)), s) : 1);
+  uint32_t rank = 0;
+  uint64_t before = above;
+  if (has) sp_all(sh, it.n, [&](uint64_t k, uint64_t w) {
+    rank += k > key;
+    before += k > key ? w : 0;
+  });
+  const bool keep = there && before < limit;
+  const uint64_t kept = block_sum_u64(keep, sh.scratch);
+  if (keep && rank == (uint32_t)kept - 1) {  // the last of them
+    sh.digit = (uint32_t)(key >> 32);
+    sh.at = sp_index(key);
+  }
+  __syncthreads();
+  return SampleCut{sh.digit, sh.at};
+}
+
+// Of a longer list the tokens between max - d0 and max - d1 that hold the cut after `limit`: a 256th of the way, to `small`. above becomes what stands in front of them; false if they are more than SP_SMALL.
+__device__ __forceinline__ bool sp_narrow(const SampleList& it, const SampleLocals& s, SampleShared& sh, bool by_mass, uint64_t limit, uint64_t& above,
+                                          float d0, float d1, uint64_t* small, int* n) {
+  if (!(d1 < INFINITY)) return false;
+  const float scale = 256.f / (d1 - d0);
+  auto of = [&](float z) { return (int)fminf(fmaxf((sp_dist(z, s) - d0) * scale, 0.f), 255.f); };
+  if (threadIdx.x < 256) sh.mass[threadIdx.x] = sh.count[threadIdx.x] = 0;
+  if (threadIdx.x == 0) sh.number = 0;
+  __syncthreads();
+  it.each([&](uint32_t, float z) {
+    const int b = of(z);
+    atomicAdd(&sh.count[b], 1u);
+    if (by_mass) sp_add(&sh.mass[b], sp_weight(z, s));
+  });
+  __syncthreads();
+  const uint64_t mine = threadIdx.x >= 256 ? 0 : by_mass ? sh.mass[threadIdx.x] : sh.count[threadIdx.x];
+  uint64_t total;
+  const uint64_t after = above + block_scan_u64(mine, sh.scratch, &total);
+  if (after >= limit && after - mine < limit) {  // (one thread)
+    sh.digit = threadIdx.x;
+    sh.c = after - mine;
+  }
+  __syncthreads();
+  const int bin = (int)sh.digit;
+  if (sh.count[bin] > SP_SMALL) return false;
+  it.each([&](uint32_t i, float z) {
+    if (of(z) != bin) return;
+    const uint32_t to = atomicAdd(&sh.number, 1u);
+    small[to] = argmax_key(z, i);
+  });
+  __syncthreads();
+  above = sh.c;
+  *n = (int)sh.number;
+  return true;
+}
+
+// The cuts and the draw of a list of at most SP_SMALL tokens, of which top-k keeps some or all.
+__device__ __forceinline__ void sp_small(const SampleParams& p, int row, const SampleList& it, const SampleLocals& s, SampleShared& sh) {
+  const int i = threadIdx.x;
+  const bool there = i < it.n, has = (i & ~63) < it.n;
+  const uint64_t key = there ? it.key[i] : 0;
+  const float z = sp_logit((uint32_t)(key >> 32));
+  const uint64_t w = there ? sp_weight(z, s) : 0;
+  sp_lay(sh, key, w);
+  uint32_t rank = 0;
+  uint64_t before = 0;
+  if (has) sp_all(sh, it.n, [&](uint64_t k, uint64_t x) {
+    rank += k > key;
+    before += k > key ? x : 0;
+  });
+  bool keep = there && rank < (uint32_t)s.k;
+  if (s.p < 1.f) {
+    const uint64_t limit = sp_limit(s.p, block_sum_u64(keep ? w : 0, sh.scratch));  // (every thread)
+    keep = keep && before < limit;
+  }
+  keep = keep && sp_high(z, s);
+  __syncthreads();
+  if (i < SP_SMALL) sh.mass[i] = keep ? w : 0;
+  const uint64_t whole = block_sum_u64(keep ? w : 0, sh.scratch), kept = block_sum_u64(keep, sh.scratch);
+  const uint64_t target = sp_target(p, row, whole);
+  uint64_t sum = 0;
+  if (has) sp_all(sh, it.n, [&](uint64_t k, uint64_t x) { sum += (uint32_t)k > (uint32_t)key ? x : 0; });  // (lower indexes: larger low words)
+  if (keep && sum <= target && sum + w > target) sp_store(p, row, (int)sp_index(key), z, kept, w, whole);
+}
+
+// The draw where the kept weight lies by chunks (in LDS): the chunk, then its tokens, by one wave.
+template <typename T, typename Keep>
+__device__ __forceinline__ void sp_draw_chunk(const SampleParams& p, int row, const T* z0, uint64_t* sums, uint64_t kept, const SampleLocals& s,
+                                              SampleShared& sh, Keep keep) {
+  constexpr int EACH = SP_CHUNKS / SP_THREADS;
+  uint64_t mine = 0, whole;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int c = threadIdx.x * EACH + i;
+    mine += c < p.chunks ? sums[c] : 0;
+  }
+  uint64_t before = block_scan_u64(mine, sh.scratch, &whole) - mine;
+  const uint64_t target = sp_target(p, row, whole);
+  if (before <= target && before + mine > target) {  // (one thread)
+    int c = threadIdx.x * EACH;
+    while (before + sums[c] <= target) before += sums[c++];
+    sh.at = c;
+    sh.c = before;
+  }
+  __syncthreads();
+  if (threadIdx.x >= 64) return;
+  const int at = sh.at * SP_CHUNK + threadIdx.x * SP_UNIT;
+  SampleUnit<T> x;
+  float z[SP_UNIT];
+  uint64_t w[SP_UNIT], run = 0;
+  x.load(z0, at, p.V, p.wide);
+  x.values(z);
+#pragma unroll
+  for (int i = 0; i < SP_UNIT; ++i) {
+    w[i] = z[i] > -INFINITY && keep((uint32_t)(at + i), z[i]) && sp_high(z[i], s) ? sp_weight(z[i], s) : 0;
+    run += w[i];
+  }
+  uint64_t sum = wave_scan_u64(run);
+  sum += sh.c - run;
+#pragma unroll
+  for (int i = 0; i < SP_UNIT; ++i) {
+    if (sum <= target && sum + w[i] > target) sp_store(p, row, at + i, z[i], kept, w[i], whole);
+    sum += w[i];
   }
 }
 
 template <typename T>
 __global__ __launch_bounds__(SP_THREADS) void sample_pick_kernel(SampleParams p) {
-  __shared__ uint32_t list[SP_LIST];
+  __shared__ uint64_t list[SP_LIST];
+  extern __shared__ uint64_t sums[];  // [chunks]
+  __shared__ uint64_t small[SP_SMALL];
   __shared__ SampleShared sh;
-  const int part = blockIdx.x % p.P, row = blockIdx.x / p.P;
-  const SampleRow r = p.rows[row];
-  const SampleLocals s = sp_locals(p, row);
-  if (r.mode == SP_EMPTY || r.mode == SP_GREEDY) {
-    if (part == 0 && threadIdx.x == 0) {
-      if (r.mode == SP_EMPTY)
-        sp_store(p, row, -1, 0.f, 0, -INFINITY);
-      else
-        sp_store(p, row, (int)s.first, s.m, 1, 0.f);
-    }
-    return;
-  }
+  const int part = blockIdx.x % p.P3, row = blockIdx.x / p.P3, lane = threadIdx.x & 63;
+  const SampleRow r = sp_read(p.result + row);
+  if (part && (r.mode == SP_EMPTY || r.mode == SP_GREEDY || r.mode == SP_ALL || r.mode == SP_ROW)) return;
+  const SampleLocals s = r.s;
   const T* z0 = sp_row<T>(p, row);
-  const size_t mine = (size_t)row * p.P + part;
-  if (r.mode == SP_ROW) {
-    if (part) return;
-    const SampleItems<T, true> it = {z0, nullptr, p.V};
-    SampleCut cut = {0, 0xffffffffu};
-    if (s.k) sp_shrink(it, s, sh, cut, false, (uint64_t)s.k, 0, 0);
-    if (s.p < 1.f) {
-      uint64_t w = 0, whole;
-      for (int i = threadIdx.x; i < p.V; i += SP_THREADS) {
-        const float z = it.value(i);
-        if (z > -INFINITY && cut.keeps(argmax_ord(z), (uint32_t)i)) w += sp_weight(z, s);
-      }
-      block_scan_u64(w, sh.scratch, &whole);
-      sp_shrink(it, s, sh, cut, true, max((uint64_t)ceil((double)s.p * (double)whole), (uint64_t)1), 0, 0);
+  if (r.mode == SP_EMPTY || r.mode == SP_GREEDY) {
+    if (threadIdx.x == 0) {
+      if (r.mode == SP_EMPTY)
+        sp_store(p, row, -1, 0.f, 0, 0, 1);
+      else
+        sp_store(p, row, (int)s.first, s.m, 1, 1, 1);
     }
-    sp_draw(p, row, it, s, sh, cut);
     return;
   }
-  // This part's listed tokens in index order, and the weight and number of its tokens above the bin
-  const int end = min((part + 1) * p.ps, p.V);
-  const bool listed = r.mode == SP_LISTED, all = r.mode == SP_ALL;
-  uint64_t sum = 0, number = 0;
-  uint32_t here = 0;
-  for (int at0 = part * p.ps; at0 < end; at0 += SP_STEP) {
-    const int at = at0 + threadIdx.x * SP_UNIT;
+  if (r.mode == SP_ALL) {
+    for (int c = threadIdx.x; c < p.chunks; c += SP_THREADS) sums[c] = p.chunk_sum[(size_t)row * p.chunks + c];
+    __syncthreads();
+    sp_draw_chunk<T>(p, row, z0, sums, p.taken[row] >> 32, s, sh, [](uint32_t, float) { return true; });
+    return;
+  }
+  if (r.mode == SP_ROW) {
+    sp_finish(p, row, SampleWhole<T>{z0, p.V, p.wide != 0}, s, sh);
+    return;
+  }
+  // This part's tokens for the list, and (SP_BELOW) the kept weight above the bin by chunks
+  const int begin = part * p.ps3, end = min(begin + p.ps3, p.V);
+  const bool listed = r.mode == SP_LISTED;
+  const float edge = sp_edge(r.bin), inner = r.bin ? sp_edge(r.bin - 1) : 0.f;  // (bin 0 has nothing above it)
+  if (threadIdx.x == 0) sh.number = 0;
+  __syncthreads();
+  uint32_t number = 0;
+  sp_units<T>(z0, begin, end, p.wide, [&](int at, const SampleUnit<T>& x) {
     float z[SP_UNIT];
-    if (at < end) {
-      sp_load<T>(z0, at, end, p.wide, z);
-    } else {
-#pragma unroll
-      for (int i = 0; i < SP_UNIT; ++i) z[i] = -INFINITY;
-    }
-    uint32_t take = 0;
+    x.values(z);
+    uint32_t take = 0, over = 0;
 #pragma unroll
     for (int i = 0; i < SP_UNIT; ++i) {
-      if (!(z[i] > -INFINITY)) continue;
-      const uint32_t b = all ? 0 : sp_bin(z[i], s.m);
-      if (!all && (listed ? b <= r.bin : b == r.bin)) take |= 1u << i;
-      if (!listed && (all || b < r.bin) && sp_high(z[i], s)) {
-        sum += sp_weight(z[i], s);
-        ++number;
-      }
+      const float d = s.m - z[i];
+      const bool up = z[i] > -INFINITY && !(d >= edge), above = !listed && r.bin && !(d >= inner);
+      take |= up && !above ? 1u << i : 0u;
+      over |= up && above ? 1u << i : 0u;
     }
-    if (all) continue;
-    uint64_t total;
-    uint32_t to = here + (uint32_t)(block_scan_u64((uint64_t)__popc(take), sh.scratch, &total) - __popc(take));
+    if (__builtin_amdgcn_ballot_w64(take != 0)) {  // the wave's ones side by side
+      const uint32_t mine = (uint32_t)__popc(take);
+      const uint64_t upto = wave_scan_u64(mine);
+      uint32_t to = 0;
+      if (lane == 63) to = atomicAdd(&sh.number, (uint32_t)upto);
+      to = (uint32_t)__builtin_amdgcn_readlane((int)to, 63) + (uint32_t)upto - mine;
 #pragma unroll
-    for (int i = 0; i < SP_UNIT; ++i)
-      if (take >> i & 1) list[to++] = (uint32_t)(at + i);  // (at most SP_LIST in the whole row)
-    here += (uint32_t)total;
-  }
+      for (int i = 0; i < SP_UNIT; ++i)
+        if (take >> i & 1) {
+          if (to < SP_LIST) list[to] = argmax_key(z[i], (uint32_t)(at + i));
+          ++to;
+        }
+    }
+    if (!listed) {
+      uint64_t sum = 0;
+      if (__builtin_amdgcn_ballot_w64(over != 0)) {
+#pragma unroll
+        for (int i = 0; i < SP_UNIT; ++i) {
+          const bool in = (over >> i & 1) && sp_high(z[i], s);
+          sum += in ? sp_weight_finite(z[i], s) : 0;
+          number += in;
+        }
+        sum = wave_sum_u64(sum);
+      }
+      if (lane == 0) sp_put(p.chunk_sum + (size_t)row * p.chunks + at / SP_CHUNK, sum);
+    }
+  });
+  number = (uint32_t)block_sum_u64(number, sh.scratch);  // (a barrier too)
+  const uint32_t here = sh.number;
+  if (threadIdx.x == 0)
+    sh.at = here || number ? (uint32_t)atomicAdd(reinterpret_cast<unsigned long long*>(p.taken + row), (unsigned long long)number << 32 | here) : 0;
   __syncthreads();
-  if (!all) {
-    if (threadIdx.x == 0) {
-      sh.at = here ? atomicAdd(&p.marks[row * 4 + 2], here) : 0;
-      p.part_at[mine] = sh.at;
-      p.part_listed[mine] = here;
-    }
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < here; i += SP_THREADS) p.list[(size_t)row * SP_LIST + sh.at + i] = list[i];
-  }
-  if (!listed) {
-    uint64_t s_all, n_all;
-    block_scan_u64(sum, sh.scratch, &s_all);
-    block_scan_u64(number, sh.scratch, &n_all);
-    if (threadIdx.x == 0) {
-      p.part_sum[mine] = s_all;
-      p.part_count[mine] = (uint32_t)n_all;
-    }
-  }
-  if (!sp_last(&p.marks[row * 4 + 1], p.P)) return;
+  for (uint32_t i = threadIdx.x; i < here && sh.at + i < SP_LIST; i += SP_THREADS) sp_put(p.list + (size_t)row * SP_LIST + sh.at + i, list[i]);
+  if (!sp_last(&p.marks[row * 2 + 1], p.P3)) return;
 
-  // The last part finishes the row. The list, part by part, so that it is in index order:
-  const bool mine_is = (int)threadIdx.x < p.P;
-  const size_t of = (size_t)row * p.P + threadIdx.x;
-  SampleItems<T, false> it = {z0, list, 0};
-  if (!all) {
-    const uint64_t n = mine_is ? p.part_listed[of] : 0;
-    uint64_t total;
-    const uint32_t to = (uint32_t)(block_scan_u64(n, sh.scratch, &total) - n);
-    sh.count[threadIdx.x] = to - (n ? p.part_at[of] : 0);  // from an entry's place in the row's list to its place here
-    __syncthreads();
-    it.n = (int)total;
-    for (int i = threadIdx.x; i < it.n; i += SP_THREADS) {
-      const uint32_t idx = p.list[(size_t)row * SP_LIST + i];
-      list[(uint32_t)i + sh.count[idx / (uint32_t)p.ps]] = idx;
-    }
-    __syncthreads();
+  // The last part finishes the row
+  const uint64_t taken = sp_get(p.taken + row);
+  const int n = (int)(uint32_t)taken;
+  if (n > SP_LIST) {  // (top-p's bin: only its weight was known)
+    sp_finish(p, row, SampleWhole<T>{z0, p.V, p.wide != 0}, s, sh);
+    return;
+  }
+  for (int i = threadIdx.x; i < n; i += SP_THREADS) list[i] = sp_get(p.list + (size_t)row * SP_LIST + i);
+  __syncthreads();
+  const SampleList it = {list, n};
+  if (listed && n <= SP_SMALL) {
+    sp_small(p, row, it, s, sh);
+    return;
+  }
+  if (listed) {  // more than SP_SMALL tokens, by top-k
+    sp_finish(p, row, it, s, sh);
+    return;
   }
   SampleCut cut = {0, 0xffffffffu};
-  if (listed) {
-    if (s.k && (!r.by_mass)) sp_shrink(it, s, sh, cut, false, r.limit, 0, 0);
-    if (s.p < 1.f) {
-      uint64_t limit = r.limit;
-      if (!r.by_mass) {
-        uint64_t w = 0, whole;
-        for (int i = threadIdx.x; i < it.n; i += SP_THREADS) {
-          const float z = it.value(i);
-          if (cut.keeps(argmax_ord(z), it.index(i))) w += sp_weight(z, s);
-        }
-        block_scan_u64(w, sh.scratch, &whole);
-        limit = max((uint64_t)ceil((double)s.p * (double)whole), (uint64_t)1);
-      }
-      sp_shrink(it, s, sh, cut, true, limit, 0, 0);
-    }
-    sp_draw(p, row, it, s, sh, cut);
-    return;
-  }
-  // Weights by parts: above the bin, and the bin's kept ones
-  if (!all) sp_shrink(it, s, sh, cut, r.by_mass != 0, r.limit, r.above, r.mass_above);
-  sh.mass[threadIdx.x] = mine_is ? p.part_sum[of] : 0;
-  sh.count[threadIdx.x] = mine_is ? p.part_count[of] : 0;
+  SampleList few = {small, 0};
+  uint64_t front = r.above;
+  if (n <= SP_SMALL)
+    cut = sp_rank(it, s, sh, r.by_mass != 0, r.limit, front);
+  else if (sp_narrow(it, s, sh, r.by_mass != 0, r.limit, front, r.bin ? inner : 0.f, edge, small, &few.n))
+    cut = sp_rank(few, s, sh, r.by_mass != 0, r.limit, front);
+  else
+    sp_shrink(it, s, sh, cut, r.by_mass != 0, r.limit, r.above, r.above);
+  for (int c = threadIdx.x; c < p.chunks; c += SP_THREADS) sums[c] = sp_get(p.chunk_sum + (size_t)row * p.chunks + c);
   __syncthreads();
-  for (int i = threadIdx.x; i < it.n; i += SP_THREADS) {
-    const float z = it.value(i);
-    const uint32_t idx = it.index(i);
-    if (!cut.keeps(argmax_ord(z), idx) || !sp_high(z, s)) continue;
-    atomicAdd(reinterpret_cast<unsigned long long*>(&sh.mass[idx / (uint32_t)p.ps]), (unsigned long long)sp_weight(z, s));
-    atomicAdd(&sh.count[idx / (uint32_t)p.ps], 1u);
-  }
-  __syncthreads();
-  const uint64_t w = sh.mass[threadIdx.x], cnt = sh.count[threadIdx.x];
-  uint64_t whole, kept;
-  const uint64_t after = block_scan_u64(w, sh.scratch, &whole);
-  block_scan_u64(cnt, sh.scratch, &kept);
-  const uint64_t target = sp_target(p, row, whole);
-  if (after > target && after - w <= target) {  // (one thread)
-    sh.found = threadIdx.x;
-    sh.c = after - w;
-  }
-  __syncthreads();
-  // the part, in index order, a workgroup's step at a time
-  uint64_t base = sh.c;
-  const int first = (int)sh.found * p.ps, last = min(first + p.ps, p.V);
-  for (int at0 = first; at0 < last; at0 += SP_STEP) {
-    const int at = at0 + threadIdx.x * SP_UNIT;
-    float z[SP_UNIT];
-    uint64_t ws[SP_UNIT], run = 0, step;
-    if (at < last) {
-      sp_load<T>(z0, at, last, p.wide, z);
-    } else {
-#pragma unroll
-      for (int i = 0; i < SP_UNIT; ++i) z[i] = -INFINITY;
-    }
-#pragma unroll
-    for (int i = 0; i < SP_UNIT; ++i) {
-      const bool in = z[i] > -INFINITY && (all || sp_bin(z[i], s.m) < r.bin || cut.keeps(argmax_ord(z[i]), (uint32_t)(at + i))) && sp_high(z[i], s);
-      ws[i] = in ? sp_weight(z[i], s) : 0;
-      run += ws[i];
-    }
-    uint64_t sum0 = base + block_scan_u64(run, sh.scratch, &step) - run;
-    if (sum0 <= target && sum0 + run > target) {
-#pragma unroll
-      for (int i = 0; i < SP_UNIT; ++i) {
-        if (sum0 <= target && sum0 + ws[i] > target) sp_store(p, row, at + i, z[i], (int)kept, sp_logprob(ws[i], whole));
-        sum0 += ws[i];
-      }
-    }
-    base += step;
-    if (base > target) return;
-  }
+  uint64_t more = 0;
+  it.each([&](uint32_t i, float z) {
+    if (!cut.keeps(argmax_ord(z), i) || !sp_high(z, s)) return;
+    sp_add(&sums[i / SP_CHUNK], sp_weight(z, s));
+    ++more;
+  });
+  more = block_sum_u64(more, sh.scratch);
+  sp_draw_chunk<T>(p, row, z0, sums, (taken >> 32) + more, s, sh, [&](uint32_t i, float z) {
+    return (r.bin && !(sp_dist(z, s) >= inner)) || cut.keeps(argmax_ord(z), i);
+  });
 }
 
-// Parts of a row: about 1024 workgroups in all, none of less than a step.
+// Parts of a row: up to about 1024 workgroups in the first launch, 2048 in the others (rows differ most in their work there), none of
+// less than a step.
 void sample_plan(SampleParams& p) {
-  const int steps = (p.V + SP_STEP - 1) / SP_STEP;
-  const int parts = std::min({SP_PARTS, steps, std::max(1, 1024 / p.n)});
-  p.ps = (steps + parts - 1) / parts * SP_STEP;
-  p.P = (p.V + p.ps - 1) / p.ps;
+  auto parts = [&](int step, int most, int& n, int& size) {
+    const int steps = (p.V + step - 1) / step;
+    const int want = std::min(steps, std::max(1, most / p.n));
+    size = (steps + want - 1) / want * step;
+    n = (p.V + size - 1) / size;
+  };
+  parts(SP_MAX_THREADS * SP_UNIT, std::min(1024, SP_PARTS * p.n), p.P, p.ps);
+  parts(SP_STEP, 1024, p.P2, p.ps2);
+  parts(SP_STEP, 1024, p.P3, p.ps3);
+  p.chunks = (p.V + SP_CHUNK - 1) / SP_CHUNK;
 }
 
 // Carves the workspace (nullptr: its size alone), the 8-byte pieces first.
@@ -591,25 +928,26 @@ size_t sample_workspace(SampleParams& p, void* ws) {
     at += count * sizeof(*to);
   };
   piece(p.part_key, parts);
-  piece(p.part_sum, parts);
+  piece(p.chunk_sum, n * p.chunks);
   piece(p.hist_mass, n * SP_BINS);
-  piece(p.rows, n);
-  piece(p.hist_count, n * SP_BINS);
-  piece(p.part_count, parts);
-  piece(p.part_at, parts);
-  piece(p.part_listed, parts);
+  piece(p.whole, n);
+  piece(p.taken, n);
   piece(p.list, n * SP_LIST);
-  piece(p.marks, n * 4);
+  piece(p.rows, n);
+  piece(p.result, n);
+  piece(p.part_sum, parts);
+  piece(p.hist_count, n * SP_BINS);
+  piece(p.marks, n * 2);
   return (size_t)(at - static_cast<char*>(ws));
 }
 
 int sample_launch(const SampleParams& p, int type, hipStream_t s) {
-  const dim3 grid((unsigned)p.n * p.P), block(SP_THREADS);
-#define SP_GO(T)                                                  \
-  do {                                                            \
-    hipLaunchKernelGGL((sample_max_kernel<T>), grid, block, 0, s, p);  \
-    hipLaunchKernelGGL((sample_hist_kernel<T>), grid, block, 0, s, p); \
-    hipLaunchKernelGGL((sample_pick_kernel<T>), grid, block, 0, s, p); \
+  const dim3 block(SP_THREADS);
+#define SP_GO(T)                                                       \
+  do {                                                                 \
+    hipLaunchKernelGGL((sample_max_kernel<T>), dim3((unsigned)p.n * p.P), dim3(SP_MAX_THREADS), 0, s, p);  \
+    hipLaunchKernelGGL((sample_hist_kernel<T>), dim3((unsigned)p.n * p.P2), block, 0, s, p); \
+    hipLaunchKernelGGL((sample_pick_kernel<T>), dim3((unsigned)p.n * p.P3), block, p.chunks * sizeof(uint64_t), s, p); \
   } while (0)
   if (type == DSPARK_F32)
     SP_GO(float);
