@@ -294,7 +294,7 @@ int dspark_rope_freqs(int32_t rot, double base, int32_t scaling, double factor, 
  * dspark_verify_attention_b8. A table entry outside [0, kv_pages) is an absent page: no row sees its positions. A row that
  * sees no key gives zeros and lse -inf. Rows of q before q_start[0] and behind q_start[seqs], and a sequence's rows past
  * max_tokens, are left as they are in the outputs. Keys that a row does not see may hold anything; where it sees a value of V
- * that is not finite on a page it does not see whole, its output is NaN there. q_start must not decrease; it is cut to
+ * that is not finite, its output is not finite there. q_start must not decrease; it is cut to
  * [0, tokens], own_len to [0, 32 own_pages]. The prefix's keys are read once for all rows (in groups of up to 256). P is
  * rounded to fp16 once; scores, sums and outputs are fp32. The workspace needs no clearing and may be shared by stream-ordered
  * calls. What is written shares no byte with anything else (DSPARK_EINVAL). tokens = 0 or seqs = 0 does nothing. */

@@ -13,6 +13,7 @@
 // or, with few rows, page waves (each a page of the slot), whose sums meet in LDS. Partial sums go to the workspace, a second
 // launch adds a row's in split order: no atomics, the same bits every call.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "batch.h"
@@ -21,14 +22,16 @@
 namespace dspark {
 
 constexpr float SA_TAU = 8.f;
-constexpr float SA_M_INIT = -1e30f;  // reference of a row that has seen no key
 constexpr int SA_THREADS = 256;
 
-// Pages of a ring slot of the row-wave form: two slots are 64 KB, two workgroups a CU.
-constexpr int sa_np(int D) { return D == 64 ? 4 : 2; }
-constexpr int SA_LDS = 64 << 10;
-static_assert(2 * sa_np(64) * PAGE * 64 * 4 == SA_LDS && 2 * sa_np(128) * PAGE * 128 * 4 == SA_LDS && 4 * 32 * 128 * 4 == SA_LDS,
-              "the ring, and the sums of four page waves of 32 rows");
+// The row-wave form's ring: two slots of two pages. At D = 64 that leaves room for four workgroups a CU, at 128 for two, as many as the
+// registers do.
+constexpr int SA_NP = 2;
+constexpr int sa_slot(int D) { return SA_NP * PAGE * D * 4; }
+constexpr int sa_waves(int D) { return D == 64 ? 4 : 2; }  // of a SIMD
+// The two slots are two LDS objects: the compiler then knows that loads in flight into one do not touch what is read from the other
+// (in one array it waits for all loads before the first read of a step). The page-wave form keeps K in the first, V in the second.
+static_assert(sa_slot(128) == 4 * PAGE * 128 * 2 && sa_slot(64) == 2 * 32 * 64 * 4, "four page waves' K; two waves' sums of 32 rows");
 
 // Which keys the lane's rows see: lo <= key <= hi, and the pages on which every row of the wave sees all keys.
 template <int QB>
@@ -41,8 +44,8 @@ template <int D, int QB>
 struct SaState {
   f32x4 o[QB][D / 16];
   f32x4 l[QB];
-  float m[QB];    // reference in log2 units
-  float thr[QB];  // raw score from which it moves: (m + TAU) / c, -inf before the first key
+  float m[QB];    // reference in log2 units, 0 before the row's first key
+  float thr[QB];  // an exponent above this moves it: TAU, -inf before the first key
 };
 
 // Scores of one page for the wave's row blocks, from K at `kt` in LDS (operand order).
@@ -65,9 +68,12 @@ __device__ __forceinline__ void sa_scores(const char* kt, const half8 (&q)[QB][D
 // Is a page one on which some row of the wave does not see some key?
 template <int QB>
 __device__ __forceinline__ bool sa_edge(const SaMask<QB>& mk, int key0) {
-  return key0 < mk.full_lo || key0 + PAGE - 1 > mk.full_hi;
+  return key0 < mk.full_lo || key0 + PAGE - 1 > mk.full_hi;  // (scalars)
 }
 
+__device__ __forceinline__ float sa_top(const f32x4 (&x)[2]) {
+  return fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+}
 // Masks, the references' moves, and P.
 template <int D, int QB>
 __device__ __forceinline__ void sa_softmax(f32x4 (&s)[QB][2], int key0, const SaMask<QB>& mk, float c, SaState<D, QB>& st,
@@ -83,27 +89,33 @@ __device__ __forceinline__ void sa_softmax(f32x4 (&s)[QB][2], int key0, const Sa
         s[qb][1][i] = b >= mk.lo[qb] && b <= mk.hi[qb] ? s[qb][1][i] : -INFINITY;
       }
   }
-  float top[QB];
+  // exponents against the reference as it is; it moves only where one passes TAU (or at a row's first key, from 0)
   bool need = false;
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
-    const f32x4 a = s[qb][0], b = s[qb][1];
-    top[qb] = fmaxf(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])), fmaxf(fmaxf(b[0], b[1]), fmaxf(b[2], b[3])));
-    need = need | (top[qb] > st.thr[qb]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[qb][0][i] = fmaf(s[qb][0][i], c, -st.m[qb]);
+      s[qb][1][i] = fmaf(s[qb][1][i], c, -st.m[qb]);
+    }
+    need = need | (sa_top(s[qb]) > st.thr[qb]);
   }
   if (__builtin_amdgcn_ballot_w64(need) != 0) {
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
-      float rm = fmaxf(top[qb], __shfl_xor(top[qb], 16));  // the row's four lanes
+      float rm = sa_top(s[qb]);
+      rm = fmaxf(rm, __shfl_xor(rm, 16));  // the row's four lanes
       rm = fmaxf(rm, __shfl_xor(rm, 32));
       if (rm > st.thr[qb]) {
-        const float m = rm * c;
-        const float alpha = fast_exp2(st.m[qb] - m);  // (0 before the first key: st.m is -1e30)
+        const float m = st.m[qb] + rm, move = m - st.m[qb];
+        const float alpha = st.thr[qb] == SA_TAU ? fast_exp2(-move) : 0.f;
 #pragma unroll
         for (int cc = 0; cc < D / 16; ++cc) st.o[qb][cc] *= alpha;
         st.l[qb] *= alpha;
         st.m[qb] = m;
-        st.thr[qb] = rm + SA_TAU / c;
+        st.thr[qb] = SA_TAU;
+        s[qb][0] -= move;
+        s[qb][1] -= move;
       }
     }
   }
@@ -111,58 +123,59 @@ __device__ __forceinline__ void sa_softmax(f32x4 (&s)[QB][2], int key0, const Sa
   for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      pp[qb][i] = (_Float16)fast_exp2(fmaf(s[qb][0][i], c, -st.m[qb]));
-      pp[qb][4 + i] = (_Float16)fast_exp2(fmaf(s[qb][1][i], c, -st.m[qb]));
+      pp[qb][i] = (_Float16)fast_exp2(s[qb][0][i]);
+      pp[qb][4 + i] = (_Float16)fast_exp2(s[qb][1][i]);
     }
 }
 
-// O^T += V^T P^T and the row sums, from V's operands at `vt` in LDS.
+// V's operands of a page in LDS.
+template <int D>
+__device__ __forceinline__ void sa_v(const char* vt, u32x4 (&v)[D / 16], int lane) {
+#pragma unroll
+  for (int cc = 0; cc < D / 16; ++cc) v[cc] = *reinterpret_cast<const u32x4*>(vt + cc * 1024 + lane * 16);
+}
+// O^T += V^T P^T and the row sums. On an edge page, where some row does not see some key, a value of V that is not finite would spoil
+// every row (0 x inf): it counts as zero in the product, and afterwards the rows that do see one get an infinity: a product of
+// where it stands with which keys they see, times 2^254.
 template <int D, int QB>
-__device__ __forceinline__ void sa_values(const char* vt, int key0, const half8 (&pp)[QB], const SaMask<QB>& mk, SaState<D, QB>& st,
-                                          int lane) {
-  const int g = lane >> 4;
+__device__ __forceinline__ void sa_values(const char* vt, u32x4 (&v)[D / 16], int key0, const half8 (&pp)[QB], const SaMask<QB>& mk,
+                                          SaState<D, QB>& st, int lane) {
+  const bool edge = sa_edge<QB>(mk, key0);
+  if (edge) {
+#pragma unroll
+    for (int cc = 0; cc < D / 16; ++cc)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)  // two halves a word
+        v[cc][i] &= ((v[cc][i] & 0x7c00u) == 0x7c00u ? 0u : 0xffffu) | ((v[cc][i] & 0x7c000000u) == 0x7c000000u ? 0u : 0xffff0000u);
+  }
   const half8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) st.l[qb] = mfma16x16x32(ones, pp[qb], st.l[qb]);
-  if (sa_edge<QB>(mk, key0)) {
-    // Keys that some row does not see: a V value there that is not finite would spoil every row (0 x inf). It counts as zero, and
-    // the rows that do see one get NaN: a product of where it stands with which keys they see.
-    half8 sees[QB];
 #pragma unroll
-    for (int qb = 0; qb < QB; ++qb)
+  for (int cc = 0; cc < D / 16; ++cc)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int key = key0 + 8 * g + i;
-        sees[qb][i] = key >= mk.lo[qb] && key <= mk.hi[qb] ? (_Float16)1 : (_Float16)0;
-      }
+    for (int qb = 0; qb < QB; ++qb) st.o[qb][cc] = mfma16x16x32(as_half8(v[cc]), pp[qb], st.o[qb][cc]);
+  if (edge) {
+    asm volatile("" ::: "memory");  // (V is read again: nothing of this is worked out for the pages that do not come here)
 #pragma unroll
     for (int cc = 0; cc < D / 16; ++cc) {
-      u32x4 v = *reinterpret_cast<const u32x4*>(vt + cc * 1024 + lane * 16), bad;
-      bool any = false;
+      u32x4 bad = *reinterpret_cast<const u32x4*>(vt + cc * 1024 + lane * 16);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {  // two halves a word; 0x3c00 is one
-        const bool lo = (v[i] & 0x7c00u) == 0x7c00u, hi = (v[i] & 0x7c000000u) == 0x7c000000u;
-        bad[i] = (lo ? 0x3c00u : 0u) | (hi ? 0x3c000000u : 0u);
-        v[i] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
-        any = any | lo | hi;
-      }
-      const bool mark = __builtin_amdgcn_ballot_w64(any) != 0;
+      for (int i = 0; i < 4; ++i)  // 0x3c00 is one
+        bad[i] = ((bad[i] & 0x7c00u) == 0x7c00u ? 0x3c00u : 0u) | ((bad[i] & 0x7c000000u) == 0x7c000000u ? 0x3c000000u : 0u);
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) {
-        st.o[qb][cc] = mfma16x16x32(as_half8(v), pp[qb], st.o[qb][cc]);
-        if (mark) {
-          const f32x4 n = mfma16x16x32(as_half8(bad), sees[qb], f32x4{0, 0, 0, 0});
+        half8 sees;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) st.o[qb][cc][i] = n[i] > 0.f ? NAN : st.o[qb][cc][i];
+        for (int i = 0; i < 8; ++i) {
+          const int key = key0 + 8 * (lane >> 4) + i;
+          sees[i] = key >= mk.lo[qb] && key <= mk.hi[qb] ? (_Float16)1 : (_Float16)0;
         }
+        const f32x4 n = mfma16x16x32(as_half8(bad), sees, f32x4{0, 0, 0, 0});
+#pragma unroll
+        for (int i = 0; i < 4; ++i) st.o[qb][cc][i] = fmaf(n[i] * 0x1p127f, 0x1p127f, st.o[qb][cc][i]);
       }
-    }
-  } else {
-#pragma unroll
-    for (int cc = 0; cc < D / 16; ++cc) {
-      const half8 v = *reinterpret_cast<const half8*>(vt + cc * 1024 + lane * 16);
-#pragma unroll
-      for (int qb = 0; qb < QB; ++qb) st.o[qb][cc] = mfma16x16x32(v, pp[qb], st.o[qb][cc]);
+      asm volatile("" ::: "memory");  // (one operand at a time: these pages are few, registers are too)
     }
   }
 }
@@ -174,9 +187,10 @@ struct SaWork {
   int h, row0, rows, pb, pe, split;
 };
 
-__device__ __forceinline__ int sa_physical(const SharedAttn& p, const SaWork& w, int i) {  // -1: absent
-  const int pg = w.tab ? ldc(w.tab + i) : i;
-  return pg >= 0 && pg < p.pages ? pg : -1;
+// The table's entry of page i, unlooked-at (the load may be in flight), and the page it stands for: -1 absent, or past the range.
+__device__ __forceinline__ int sa_entry(const SaWork& w, int i) { return w.tab ? ldc(w.tab + min(i, w.pe - 1)) : i; }
+__device__ __forceinline__ int sa_physical(const SharedAttn& p, const SaWork& w, int i, int entry) {
+  return i < w.pe && (uint32_t)entry < (uint32_t)p.pages ? entry : -1;
 }
 
 // K or V of a page into LDS, 1 KB a load. An absent page (-1) is fetched as page 0, which exists, and not used: every page costs
@@ -211,50 +225,76 @@ __device__ __forceinline__ void sa_begin(const SharedAttn& p, const SaWork& w, i
     mk.full_lo = max(mk.full_lo, (int)wave_max_u32((uint32_t)max(mk.lo[qb], 0)));
     mk.full_hi = min(mk.full_hi, 0x7fffffff - (int)wave_max_u32(0x7fffffffu - (uint32_t)max(mk.hi[qb], 0)));
     if (__builtin_amdgcn_ballot_w64(mk.hi[qb] < 0)) mk.full_hi = -1;
+    mk.full_lo = __builtin_amdgcn_readfirstlane(mk.full_lo);
+    mk.full_hi = __builtin_amdgcn_readfirstlane(mk.full_hi);
 #pragma unroll
     for (int cc = 0; cc < D / 16; ++cc) st.o[qb][cc] = f32x4{0, 0, 0, 0};
     st.l[qb] = f32x4{0, 0, 0, 0};
-    st.m[qb] = SA_M_INIT;
+    st.m[qb] = 0.f;
     st.thr[qb] = -INFINITY;
   }
 }
 
-// Many rows: four waves of 16 QB rows each take every page of a slot of NP pages.
+// Many rows: four waves of 16 QB rows each take every page.
 template <int D, int QB, typename Mask>
-__device__ __forceinline__ void sa_run_rows(const SharedAttn& p, char* lds, const SaWork& w, Mask row_mask) {
-  constexpr int NP = sa_np(D), PAGE_BYTES = PAGE * D * 4, SLOT = NP * PAGE_BYTES;
+__device__ __forceinline__ void sa_run_rows(const SharedAttn& p, char (&lds0)[sa_slot(D)], char (&lds1)[sa_slot(D)], const SaWork& w, Mask row_mask) {
+  constexpr int PAGE_BYTES = PAGE * D * 4;
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // a wave's share of a slot: NP = 4, K and V of page `wave`; NP = 2, K (even waves) or V of page wave / 2
-  const int mine = NP == 4 ? wave : wave >> 1;
-  auto issue = [&](int first, char* slot) {
-    if (first + mine >= w.pe) return;
-    const int pg = sa_physical(p, w, first + mine);
-    char* dst = slot + mine * PAGE_BYTES;
-    if (NP == 4 || !(wave & 1)) sa_fetch<D>(p, false, pg, w.h, dst, lane);
-    if (NP == 4 || (wave & 1)) sa_fetch<D>(p, true, pg, w.h, dst + PAGE * D * 2, lane);
+  // a wave's share of a slot: K (even waves) or V of page wave / 2. Table entries are read a step before their pages are fetched.
+  const int mine = wave >> 1;
+  const bool isv = wave & 1;
+  int here[SA_NP], next[SA_NP];
+  auto entries = [&](int first, int (&e)[SA_NP]) {
+#pragma unroll
+    for (int i = 0; i < SA_NP; ++i) e[i] = sa_entry(w, first + i);
   };
-  if (w.pb < w.pe) issue(w.pb, lds);
+  auto issue = [&](int first, const int (&e)[SA_NP], char* slot) {  // (past the range: page 0, into a slot nobody reads)
+    sa_fetch<D>(p, isv, sa_physical(p, w, first + mine, mine ? e[1] : e[0]), w.h, slot + mine * PAGE_BYTES + (isv ? PAGE * D * 2 : 0), lane);
+  };
+  if (w.pb < w.pe) {
+    entries(w.pb, here);
+    entries(w.pb + SA_NP, next);
+    issue(w.pb, here, lds0);
+  }
   const int wrow = w.row0 + wave * 16 * QB;
   half8 q[QB][D / 32];
   SaMask<QB> mk;
   SaState<D, QB> st;
   sa_begin<D, QB>(p, w, wrow, q, mk, st, lane, row_mask);
-  for (int first = w.pb, k = 0; first < w.pe; first += NP, ++k) {
-    char* cur = lds + (k & 1) * SLOT;
+  const bool rows = wrow < w.rows;  // (a wave without any fetches its share alone)
+  auto step = [&](int first, const char* cur, char* nxt) {
     ring_barrier<0>();  // this slot is in LDS, every wave is done with the other one
-    if (first + NP < w.pe) issue(first + NP, lds + ((k + 1) & 1) * SLOT);
+    issue(first + SA_NP, next, nxt);
+    int after[SA_NP];
+    entries(first + 2 * SA_NP, after);
+    if (rows) {
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      if (first + i >= w.pe || sa_physical(p, w, first + i) < 0) continue;
-      const char* kt = cur + i * PAGE_BYTES;
-      f32x4 s[QB][2];
-      half8 pp[QB];
-      sa_scores<D, QB>(kt, q, s, lane);
-      sa_softmax<D, QB>(s, (first + i) * PAGE, mk, p.c, st, pp, lane);
-      sa_values<D, QB>(kt + PAGE * D * 2, (first + i) * PAGE, pp, mk, st, lane);
+      for (int i = 0; i < SA_NP; ++i) {
+        if (sa_physical(p, w, first + i, here[i]) < 0) continue;
+        const char* kt = cur + i * PAGE_BYTES;
+        f32x4 s[QB][2];
+        half8 pp[QB];
+        u32x4 v[D / 16];
+        sa_scores<D, QB>(kt, q, s, lane);
+        if (D == 128) sa_v<D>(kt + PAGE * D * 2, v, lane);  // (early where the registers allow it)
+        sa_softmax<D, QB>(s, (first + i) * PAGE, mk, p.c, st, pp, lane);
+        if (D == 64) sa_v<D>(kt + PAGE * D * 2, v, lane);
+        sa_values<D, QB>(kt + PAGE * D * 2, v, (first + i) * PAGE, pp, mk, st, lane);
+      }
     }
+#pragma unroll
+    for (int i = 0; i < SA_NP; ++i) {
+      here[i] = next[i];
+      next[i] = after[i];
+    }
+  };
+  for (int first = w.pb; first < w.pe; first += 2 * SA_NP) {
+    step(first, lds0, lds1);
+    if (first + SA_NP >= w.pe) break;
+    step(first + SA_NP, lds1, lds0);
   }
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // (the last step's fetch: LDS is not given up before it has arrived)
   const size_t out0 = (size_t)w.h * p.T * p.G;
   const int S = p.Sp + p.So;
 #pragma unroll
@@ -276,15 +316,15 @@ __device__ __forceinline__ void sa_run_rows(const SharedAttn& p, char* lds, cons
 // are no barriers: K's half of the wave's LDS page is fetched anew while the page's P and products are computed, V's half
 // while the next page's scores are.
 template <int D, int QB, typename Mask>
-__device__ __forceinline__ void sa_run_pages(const SharedAttn& p, char* lds, const SaWork& w, Mask row_mask) {
+__device__ __forceinline__ void sa_run_pages(const SharedAttn& p, char (&lds0)[sa_slot(D)], char (&lds1)[sa_slot(D)], const SaWork& w, Mask row_mask) {
   constexpr int HALF = PAGE * D * 2, LOADS = D / 16;
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  char* kt = lds + wave * 2 * HALF;
-  char* vt = kt + HALF;
+  char* kt = lds0 + wave * HALF;
+  char* vt = lds1 + wave * HALF;
   int i = w.pb + wave, pg = -1;
   if (i < w.pe) {
-    pg = sa_physical(p, w, i);
+    pg = sa_physical(p, w, i, sa_entry(w, i));
     sa_fetch<D>(p, false, pg, w.h, kt, lane);
     sa_fetch<D>(p, true, pg, w.h, vt, lane);
   }
@@ -301,13 +341,15 @@ __device__ __forceinline__ void sa_run_pages(const SharedAttn& p, char* lds, con
   while (i < w.pe) {
     const int nxt = i + 4;
     const bool more = nxt < w.pe;
-    const int npg = more ? sa_physical(p, w, nxt) : -1;
+    const int entry = sa_entry(w, nxt);
     f32x4 s[QB][2];
     half8 pp[QB];
+    int npg = -1;
     loads_but(Half{});
     sa_scores<D, QB>(kt, q, s, lane);
     if (more) {
       loads_but(std::integral_constant<int, 63>{});  // (the reads of K)
+      npg = sa_physical(p, w, nxt, entry);
       sa_fetch<D>(p, false, npg, w.h, kt, lane);
     }
     if (pg >= 0) sa_softmax<D, QB>(s, i * PAGE, mk, p.c, st, pp, lane);
@@ -315,7 +357,11 @@ __device__ __forceinline__ void sa_run_pages(const SharedAttn& p, char* lds, con
       loads_but(Half{});
     else
       loads_but(Zero{});
-    if (pg >= 0) sa_values<D, QB>(vt, i * PAGE, pp, mk, st, lane);
+    if (pg >= 0) {
+      u32x4 v[D / 16];
+      sa_v<D>(vt, v, lane);
+      sa_values<D, QB>(vt, v, i * PAGE, pp, mk, st, lane);
+    }
     if (more) {
       loads_but(std::integral_constant<int, 63>{});
       sa_fetch<D>(p, true, npg, w.h, vt, lane);
@@ -327,16 +373,16 @@ __device__ __forceinline__ void sa_run_pages(const SharedAttn& p, char* lds, con
   // the four waves' sums through LDS, values in 16-byte pieces at c ^ (row % 16) so that rows lie on different banks
   __shared__ float sm_m[4][16 * QB], sm_l[4][16 * QB];
   lds_barrier();
-  f32x4* sums = reinterpret_cast<f32x4*>(lds);
+  auto sums = [&](int v) { return reinterpret_cast<f32x4*>(v < 2 ? lds0 : lds1) + (v & 1) * (16 * QB * D / 4); };  // of wave v
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
     const int r = 16 * qb + n;
     if (g == 0) {
-      sm_m[wave][r] = st.m[qb];
+      sm_m[wave][r] = st.thr[qb] == SA_TAU ? st.m[qb] : -1e30f;  // (no key: a reference below all others)
       sm_l[wave][r] = st.l[qb][0];
     }
 #pragma unroll
-    for (int cc = 0; cc < D / 16; ++cc) sums[(wave * 16 * QB + r) * (D / 4) + ((4 * cc + g) ^ n)] = st.o[qb][cc];
+    for (int cc = 0; cc < D / 16; ++cc) sums(wave)[r * (D / 4) + ((4 * cc + g) ^ n)] = st.o[qb][cc];
   }
   lds_barrier();
   const size_t out0 = (size_t)w.h * p.T * p.G;
@@ -350,7 +396,7 @@ __device__ __forceinline__ void sa_run_pages(const SharedAttn& p, char* lds, con
     for (int v = 0; v < 4; ++v) {
       const float f = fast_exp2(sm_m[v][r] - m);
       l += f * sm_l[v][r];
-      o += sums[(v * 16 * QB + r) * (D / 4) + (c4 ^ (r & 15))] * f;
+      o += sums(v)[r * (D / 4) + (c4 ^ (r & 15))] * f;
     }
     const size_t at = (out0 + w.row0 + r) * (p.Sp + p.So) + w.split;
     if (c4 == 0) p.part_ml[at] = f32x2{l != 0.f ? m : -INFINITY, l};
@@ -373,14 +419,14 @@ __device__ __forceinline__ SaSeq sa_seq(const SharedAttn& p, int r) {
 
 // ROWS: prefix workgroups of four row waves, else of four page waves.
 template <int D, int QB, bool ROWS, int QBO>
-__global__ __launch_bounds__(SA_THREADS, 2) void shared_attn_kernel(SharedAttn p) {
-  __shared__ __attribute__((aligned(16))) char lds[SA_LDS];
+__global__ __launch_bounds__(SA_THREADS, sa_waves(D)) void shared_attn_kernel(SharedAttn p) {
+  __shared__ __attribute__((aligned(16))) char lds0[sa_slot(D)], lds1[sa_slot(D)];
   constexpr int BLOCK = 16 * QB * (ROWS ? 4 : 1);
   auto go = [&](const SaWork& w, auto mask) {
     if constexpr (ROWS)
-      sa_run_rows<D, QB>(p, lds, w, mask);
+      sa_run_rows<D, QB>(p, lds0, lds1, w, mask);
     else
-      sa_run_pages<D, QB>(p, lds, w, mask);
+      sa_run_pages<D, QB>(p, lds0, lds1, w, mask);
   };
   const int prefix_groups = (p.KVH * p.Sp + 7) / 8 * 8 * p.RBp;
   int id = blockIdx.x;
@@ -442,7 +488,7 @@ __global__ __launch_bounds__(SA_THREADS, 2) void shared_attn_kernel(SharedAttn p
   const int ctx = s.len - s.m;  // own keys before the call's first token
   if (p.window) pb = max(pb, min(max(ctx + div_by(rb * 16 * QBO, p.g_div) - p.window + 1, 0), max(ctx, 0)) / PAGE);
   const SaWork w = {p.own_tab + (size_t)r * p.own_stride, h, s.t0 * p.G + rb * 16 * QBO, (s.t0 + m) * p.G, pb, pe, p.Sp + split};
-  sa_run_pages<D, QBO>(p, lds, w,
+  sa_run_pages<D, QBO>(p, lds0, lds1, w,
                     [&](int row, int& lo, int& hi) {
                       const int pos = ctx + div_by(row, p.g_div) - s.t0;
                       lo = p.window ? min(max(pos - p.window + 1, 0), max(ctx, 0)) : 0;
@@ -450,47 +496,71 @@ __global__ __launch_bounds__(SA_THREADS, 2) void shared_attn_kernel(SharedAttn p
                     });
 }
 
-// A row's partial sums in split order: one wave a row, D / 4 lanes for the values by 256 / D for the splits.
-template <int D>
+// A row's partial sums: W waves a row, D / 4 lanes for the values by 256 W / D for the splits, whose sums meet in a fixed order (lanes,
+// then waves). Everything a lane loads is asked for before the first of it is used, up to SA_ROUND splits at a time.
+constexpr int SA_ROUND = 8;
+template <int D, int W>
 __global__ __launch_bounds__(SA_THREADS) void shared_merge_kernel(SharedAttn p) {
-  constexpr int CH = D / 4, SL = 64 / CH;
+  constexpr int CH = D / 4, SL = 64 / CH * W;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t unit = (int64_t)blockIdx.x * 4 + wave;
+  const int64_t unit = (int64_t)blockIdx.x * (4 / W) + wave / W;
   const int qh = (int)(unit % p.QH);
   const int64_t ri = unit / p.QH;
   const int i = (int)(ri % p.max_tokens), r = (int)(ri / p.max_tokens);
-  if (r >= p.R) return;
+  if (r >= p.R) return;  // (W = 4: the whole workgroup)
   const SaSeq s = sa_seq(p, r);
   if (i >= s.m) return;
   const int t = s.t0 + i, h = div_by(qh, p.g_div), S = p.Sp + p.So;
   const size_t row = ((size_t)h * p.T + t) * p.G + (qh - h * p.G);
   const f32x2* ml = p.part_ml + row * S;
+  const f32x4* po = reinterpret_cast<const f32x4*>(p.part_o + row * S * D);
+  const int c4 = lane % CH, s0 = (wave % W) * (64 / CH) + lane / CH;
+  f32x2 x[SA_ROUND];
+  f32x4 v[SA_ROUND];
+  auto load = [&](int k0) {
+#pragma unroll
+    for (int j = 0; j < SA_ROUND; ++j) {
+      const int k = min(k0 + j * SL, S - 1);
+      x[j] = ldg(ml + k);
+      v[j] = ldg(po + (size_t)k * CH + c4);
+    }
+  };
+  load(s0);
   float m = -INFINITY;
   for (int k = lane; k < S; k += 64) m = fmaxf(m, ldg(ml + k)[0]);
   m = wave_max(m);
   float l = 0.f;
   f32x4 o = {0, 0, 0, 0};
-  const int c4 = lane % CH, s0 = lane / CH;
-  if (m > -INFINITY) {
-    const f32x4* po = reinterpret_cast<const f32x4*>(p.part_o + row * S * D);
-    for (int k = s0; k < S; k += SL) {
-      const f32x2 x = ldg(ml + k);
-      if (x[1] == 0.f) continue;
-      const float f = fast_exp2(x[0] - m);
-      l += f * x[1];
-      o += ldg(po + (size_t)k * CH + c4) * f;
+  for (int k0 = s0; k0 < S; k0 += SA_ROUND * SL) {
+    if (k0 != s0) load(k0);
+#pragma unroll
+    for (int j = 0; j < SA_ROUND; ++j) {
+      const bool in = k0 + j * SL < S && x[j][1] != 0.f;  // (a split that saw nothing left no values)
+      const float f = in ? fast_exp2(x[j][0] - m) : 0.f;
+      l += in ? f * x[j][1] : 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += in ? f * v[j][e] : 0.f;
     }
   }
-  // the other lanes' splits
 #pragma unroll
   for (int d = CH; d < 64; d *= 2) {
     l += __shfl_xor(l, d);
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[j] += __shfl_xor(o[j], d);
   }
-  if (s0) return;
+  if constexpr (W > 1) {
+    __shared__ f32x4 so[W][CH];
+    __shared__ float sl[W];
+    if (lane < CH) so[wave][lane] = o;
+    if (lane == 0) sl[wave] = l;
+    __syncthreads();
+    if (wave) return;
+    l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+    o = (so[0][c4] + so[1][c4]) + (so[2][c4] + so[3][c4]);
+  }
+  if (lane >= CH) return;
   const size_t at = (size_t)t * p.QH + qh;
-  float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : NAN;
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : NAN;
   if (p.lse && c4 == 0) p.lse[at] = l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : l == 0.f ? -INFINITY : NAN;
   o *= inv;
   if (p.gate) o *= 1.f / (1.f + __expf(-ldg(p.gate + at)));
@@ -508,25 +578,28 @@ struct SaCfg {
   int qb;
   bool rows;
 };
-constexpr SaCfg SA_CFG[5] = {{1, false}, {2, false}, {1, true}, {2, true}, {4, true}};
+constexpr SaCfg SA_CFG[4] = {{1, false}, {2, false}, {1, true}, {2, true}};
 
 void shared_plan(SharedAttn& p, int D, int splits, int cus) {
   const int64_t rows = (int64_t)p.T * p.G;
-  // the least block that holds all rows; past 128, blocks of 256 where the registers take four row blocks a wave (D = 64)
-  p.cfg = rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 || D == 128 ? 3 : 4;
+  // the least block that holds all rows, else blocks of 128
+  p.cfg = rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 3;
   const int per = 16 * SA_CFG[p.cfg].qb * (SA_CFG[p.cfg].rows ? 4 : 1), wp = SA_CFG[p.cfg].rows ? 1 : 4;
   p.RBp = (int)((rows + per - 1) / per);
   const int pages = (p.prefix + PAGE - 1) / PAGE;
   p.own_qb = p.max_tokens * p.G <= 16 ? 1 : 2;
   p.RBo = (p.max_tokens * p.G + 16 * p.own_qb - 1) / (16 * p.own_qb);
-  // Two workgroups a CU in all; a prefix split has at least two pages a page wave, so that its start is not most of its time
+  // Splits: a start and a share of the merge cost each of them some pages' time, and so does each further page of a split: about as many
+  // splits as pages of one, at least half as many workgroups as CUs, at most as many as run at once. (Graph replays, 1024 pages of 8 x 64,
+  // 128 rows: 16 splits 43 us, 32 29, 64 32, 128 39; 256 pages of 4 x 128, 320 rows: 8 splits 37, 16 28, 32 32.)
   const int64_t units = (int64_t)p.KVH * p.RBp;
-  int64_t sp = pages ? splits ? splits : std::max<int64_t>(1, 2 * cus / units) : 0;
+  int64_t sp = pages ? splits ? splits : std::max<int64_t>((int64_t)std::ceil(std::sqrt((double)pages)), cus / (2 * units)) : 0;
+  if (!splits) sp = std::min(sp, std::max<int64_t>(1, sa_waves(D) * cus / units));
   sp = std::min<int64_t>(sp, splits ? pages : (pages + 2 * wp - 1) / (2 * wp));
   p.pps = sp ? (int)((pages + sp - 1) / sp) : 0;
   p.Sp = p.pps ? (pages + p.pps - 1) / p.pps : 0;
   const int64_t own = (int64_t)p.R * p.KVH * p.RBo;
-  p.So = (int)std::max<int64_t>(1, std::min<int64_t>({2 * cus / own, (p.own_pages + 7) / 8, 64}));
+  p.So = (int)std::max<int64_t>(1, std::min<int64_t>({sa_waves(D) * cus / own, (p.own_pages + 15) / 16, 64}));
 }
 
 size_t shared_workspace(const SharedAttn& p, int D) {
@@ -550,8 +623,7 @@ int shared_launch(SharedAttn& p, int D, hipStream_t s) {
       case 0: SA_GO(64, 1, false); break;
       case 1: SA_GO(64, 2, false); break;
       case 2: SA_GO(64, 1, true); break;
-      case 3: SA_GO(64, 2, true); break;
-      default: SA_GO(64, 4, true); break;
+      default: SA_GO(64, 2, true); break;
     }
   } else {
     switch (p.cfg) {
@@ -563,11 +635,18 @@ int shared_launch(SharedAttn& p, int D, hipStream_t s) {
   }
 #undef SA_GO
   if (const hipError_t e = hipGetLastError(); e != hipSuccess) return (int)e;
-  const int64_t waves = (int64_t)p.R * p.max_tokens * p.QH;
-  if (D == 64)
-    hipLaunchKernelGGL(shared_merge_kernel<64>, dim3((unsigned)((waves + 3) / 4)), block, 0, s, p);
+  // four waves for a row whose splits one wave would take in more than two rounds
+  const int64_t units = (int64_t)p.R * p.max_tokens * p.QH;
+  const bool four = p.Sp + p.So > 2 * SA_ROUND * 256 / D;
+  const dim3 merge((unsigned)(four ? units : (units + 3) / 4));
+  if (D == 64 && four)
+    hipLaunchKernelGGL((shared_merge_kernel<64, 4>), merge, block, 0, s, p);
+  else if (D == 64)
+    hipLaunchKernelGGL((shared_merge_kernel<64, 1>), merge, block, 0, s, p);
+  else if (four)
+    hipLaunchKernelGGL((shared_merge_kernel<128, 4>), merge, block, 0, s, p);
   else
-    hipLaunchKernelGGL(shared_merge_kernel<128>, dim3((unsigned)((waves + 3) / 4)), block, 0, s, p);
+    hipLaunchKernelGGL((shared_merge_kernel<128, 1>), merge, block, 0, s, p);
   return (int)hipGetLastError();
 }
 
