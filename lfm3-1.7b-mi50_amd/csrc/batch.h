@@ -24,6 +24,7 @@ struct RopeBatch {
   int KVH;
   // rope_batch_launch sets: units of a head and of a token, their divisors, tokens of a workgroup
   int uph, upt, tok;
+  int fill, v_wide;    // append: workgroups that fill pages; V in pieces of 16 bytes
   uint32_t uph_div, upt_div;
 };
 int rope_batch_launch(RopeBatch& p, int type, bool interleaved, hipStream_t s);

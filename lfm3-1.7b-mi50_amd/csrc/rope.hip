@@ -8,13 +8,21 @@
 //
 // Bound by memory: each value is read and written once, in pieces of 16 bytes where sizes and addresses allow (VEC), else value
 // by value. A unit of work is a piece (half layout: the piece and its partner rot / 2 further) or a piece of what is not turned.
+//
+// Into the pages go workgroups of a KV head and 32 tokens, side by side in the lanes: tokens of a run lie in consecutive slots,
+// which K's operand order keeps 16 bytes apart and V's transposed rows 2, so that a wave's store covers whole lines. V's rows turn
+// in LDS.
 #include "batch.h"
+
+#include <algorithm>
+
 #include "dspark.h"
 
 namespace dspark {
 
 constexpr int ROPE_THREADS = 256;
 constexpr int ROPE_TOKENS = 8;  // of a workgroup at most
+constexpr int ROPE_RUN = 32;    // of a workgroup that fills pages
 
 __device__ __forceinline__ float rope_to_f32(float x) { return x; }
 __device__ __forceinline__ float rope_to_f32(_Float16 x) { return (float)x; }
@@ -58,87 +66,113 @@ struct RopePiece {
   }
 };
 
-// VEC: values of a piece, 16 bytes' worth or (sizes or addresses off 16 bytes) 1, interleaved pairs 2.
-template <typename T, int VEC, bool IL>
-__global__ __launch_bounds__(ROPE_THREADS) void rope_kernel(RopeBatch p) {
-  extern __shared__ f32x2 cs[];  // [tok][rot / 2]
-  const int P = p.rot / 2, t0 = (int)blockIdx.x * p.tok, nt = min(p.tok, p.n - t0);
+// The sines and cosines of tokens t0 .. t0 + nt - 1: cs[t][rot / 2].
+__device__ __forceinline__ void rope_angles(const RopeBatch& p, f32x2* cs, int t0, int nt) {
+  const int P = p.rot / 2;
   for (int e = threadIdx.x; e < nt * P; e += ROPE_THREADS) {
     const int t = e / P, i = e - t * P;
     cs[e] = rope_cos_sin((double)ldg(p.pos + t0 + t) * (ldg(p.freq + i) * 0.15915494309189533577), p.scale, p.inverse != 0);
   }
+}
+
+// Unit u of a head's row at src, token tl of cs, to dst + at(d). VEC: values of a piece, 16 bytes' worth or (sizes or addresses off
+// 16 bytes) 1, interleaved pairs 2.
+template <typename T, int VEC, bool IL, typename At>
+__device__ __forceinline__ void rope_unit(const RopeBatch& p, const f32x2* c, int u, const T* src, T* dst, At at) {
+  const int P = p.rot / 2, turning = IL ? p.rot / VEC : P / VEC;  // units of a head: what turns first, then the rest
+  RopePiece<T, VEC> a;
+  if (u >= turning) {  // passed on
+    const int d = p.rot + (u - turning) * VEC;
+    if (dst == src) return;
+    a.load(src + d);
+    a.store(dst + at(d));
+    return;
+  }
+  const int d = u * VEC;
+  a.load(src + d);
+  if constexpr (IL) {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) {
+      const f32x2 w = c[d / 2 + i / 2];
+      const float xi = rope_to_f32(a.x[i]), xj = rope_to_f32(a.x[i + 1]);
+      a.x[i] = (T)(xi * w[0] - xj * w[1]);
+      a.x[i + 1] = (T)(xj * w[0] + xi * w[1]);
+    }
+    a.store(dst + at(d));
+  } else {
+    RopePiece<T, VEC> b;
+    b.load(src + P + d);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const f32x2 w = c[d + i];
+      const float xi = rope_to_f32(a.x[i]), xj = rope_to_f32(b.x[i]);
+      a.x[i] = (T)(xi * w[0] - xj * w[1]);
+      b.x[i] = (T)(xj * w[0] + xi * w[1]);
+    }
+    a.store(dst + at(d));
+    b.store(dst + at(P + d));
+  }
+}
+
+// K and V of KV head h, tokens t0 .. t0 + nt - 1 (nt <= ROPE_RUN), into the pages.
+template <int VEC, bool IL>
+__device__ __forceinline__ void rope_pages(const RopeBatch& p, f32x2* cs, int h, int t0, int nt) {
+  _Float16* turn = reinterpret_cast<_Float16*>(cs + ROPE_RUN * (p.rot / 2));  // V's rows, D + 2 halves apart: odd in words
+  const int per = p.D / 8, pitch = p.D + 2;
+  for (int e = threadIdx.x; e < nt * per; e += ROPE_THREADS) {
+    const int t = e / per, d = (e - t * per) * 8;
+    const _Float16* src = static_cast<const _Float16*>(p.v.x) + (size_t)(t0 + t) * p.v.x_stride + (size_t)h * p.D + d;
+    uint32_t x[4];
+    if (p.v_wide) {
+      const u32x4 u = ldg(reinterpret_cast<const u32x4*>(src));
+      __builtin_memcpy(x, &u, 16);
+    } else {
+      __builtin_memcpy(x, src, 16);
+    }
+    uint32_t* to = reinterpret_cast<uint32_t*>(turn + t * pitch + d);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) to[i] = x[i];
+  }
+  rope_angles(p, cs, t0, nt);
+  __syncthreads();
+  const int t = threadIdx.x % ROPE_RUN;
+  if (t >= nt) return;
+  const int64_t slot = ldg(p.slots + t0 + t);
+  if (slot < 0 || slot >= p.n_slots) return;
+  const size_t block = (size_t)((slot / PAGE) * p.KVH + h) * (PAGE * p.D);
+  const int at_slot = (int)(slot % PAGE);
+  // (a piece of up to 8 values from a multiple of its size lies together in K's page)
+  const _Float16* src = static_cast<const _Float16*>(p.k.x) + (size_t)(t0 + t) * p.k.x_stride + (size_t)h * p.D;
+  for (int u = threadIdx.x / ROPE_RUN; u < p.uph; u += ROPE_THREADS / ROPE_RUN)
+    rope_unit<_Float16, VEC, IL>(p, cs + t * (p.rot / 2), u, src, p.kp + block, [&](int d) { return k_page_elem(at_slot, d, p.D); });
+  for (int d = threadIdx.x / ROPE_RUN; d < p.D; d += ROPE_THREADS / ROPE_RUN)
+    p.vp[block + v_page_elem(at_slot, d)] = turn[t * pitch + d];
+}
+
+template <typename T, int VEC, bool IL>
+__global__ __launch_bounds__(ROPE_THREADS) void rope_kernel(RopeBatch p) {
+  extern __shared__ f32x2 cs[];  // [tokens][rot / 2]
+  int wg = (int)blockIdx.x;
+  if constexpr (__is_same(T, _Float16)) {
+    if (wg < p.fill) {
+      const int run = wg / p.KVH, t0 = run * ROPE_RUN;
+      rope_pages<VEC, IL>(p, cs, wg - run * p.KVH, t0, min(ROPE_RUN, p.n - t0));
+      return;
+    }
+    wg -= p.fill;
+  }
+  const int t0 = wg * p.tok, nt = min(p.tok, p.n - t0);
+  rope_angles(p, cs, t0, nt);
   __syncthreads();
   for (int e = threadIdx.x; e < nt * p.upt; e += ROPE_THREADS) {
     const int tl = div_by(e, p.upt_div), r = e - tl * p.upt, t = t0 + tl;
-    int h = div_by(r, p.uph_div), u = r - h * p.uph;
-    // units of a head: what turns first, then the rest
-    const int turning = IL ? p.rot / VEC : P / VEC;
-    RopePiece<T, VEC> a;
-    const bool in_q = h < p.q.heads, in_k = !in_q && h < p.q.heads + p.k.heads;
-    if (!in_q && !in_k) continue;
+    int h = div_by(r, p.uph_div);
+    const int u = r - h * p.uph;
+    const bool in_q = h < p.q.heads;
     const RopeTensor& x = in_q ? p.q : p.k;
     if (!in_q) h -= p.q.heads;
-    const T* src = static_cast<const T*>(x.x) + (size_t)t * x.x_stride + (size_t)h * p.D;
-    T* dst = static_cast<T*>(x.y) + (size_t)t * x.y_stride + (size_t)h * p.D;
-    // append: a K piece of up to 8 values from a multiple of its size lies together in the page
-    const bool paged = in_k && p.kp;
-    int64_t slot = 0;
-    if constexpr (sizeof(T) == 2) {
-      if (paged) {
-        slot = ldg(p.slots + t);
-        if (slot < 0 || slot >= p.n_slots) continue;
-        dst = reinterpret_cast<T*>(p.kp) + (size_t)((slot / PAGE) * p.KVH + h) * (PAGE * p.D);
-      }
-    }
-    auto at = [&](int d) { return paged ? k_page_elem((int)(slot % PAGE), d, p.D) : d; };
-    if (u >= turning) {  // passed on
-      const int d = p.rot + (u - turning) * VEC;
-      if (!paged && dst == src) continue;
-      a.load(src + d);
-      a.store(dst + at(d));
-      continue;
-    }
-    const f32x2* c = cs + tl * P;
-    if constexpr (IL) {
-      const int d = u * VEC;
-      a.load(src + d);
-#pragma unroll
-      for (int i = 0; i < VEC; i += 2) {
-        const f32x2 w = c[d / 2 + i / 2];
-        const float xi = rope_to_f32(a.x[i]), xj = rope_to_f32(a.x[i + 1]);
-        a.x[i] = (T)(xi * w[0] - xj * w[1]);
-        a.x[i + 1] = (T)(xj * w[0] + xi * w[1]);
-      }
-      a.store(dst + at(d));
-    } else {
-      const int d = u * VEC;
-      RopePiece<T, VEC> b;
-      a.load(src + d);
-      b.load(src + P + d);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const f32x2 w = c[d + i];
-        const float xi = rope_to_f32(a.x[i]), xj = rope_to_f32(b.x[i]);
-        a.x[i] = (T)(xi * w[0] - xj * w[1]);
-        b.x[i] = (T)(xj * w[0] + xi * w[1]);
-      }
-      a.store(dst + at(d));
-      b.store(dst + at(P + d));
-    }
-  }
-  if constexpr (sizeof(T) == 2) {
-    if (!p.vp) return;
-    // V rows into the transposed pages, 8 values of a row each: [d][slot]
-    const int upv = p.KVH * p.D / 8;
-    for (int e = threadIdx.x; e < nt * upv; e += ROPE_THREADS) {
-      const int tl = e / upv, d8 = (e - tl * upv) * 8, h = d8 / p.D, d = d8 - h * p.D;
-      const int64_t slot = ldg(p.slots + t0 + tl);
-      if (slot < 0 || slot >= p.n_slots) continue;
-      const _Float16* src = static_cast<const _Float16*>(p.v.x) + (size_t)(t0 + tl) * p.v.x_stride + d8;
-      _Float16* dst = p.vp + (size_t)((slot / PAGE) * p.KVH + h) * (PAGE * p.D);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) dst[v_page_elem((int)(slot % PAGE), d + i)] = src[i];
-    }
+    rope_unit<T, VEC, IL>(p, cs + tl * (p.rot / 2), u, static_cast<const T*>(x.x) + (size_t)t * x.x_stride + (size_t)h * p.D,
+                          static_cast<T*>(x.y) + (size_t)t * x.y_stride + (size_t)h * p.D, [](int d) { return d; });
   }
 }
 
@@ -154,14 +188,17 @@ int rope_batch_launch(RopeBatch& p, int type, bool interleaved, hipStream_t s) {
   }
   const int vec = wide ? vec16 : interleaved ? 2 : 1;
   p.uph = interleaved ? p.D / vec : p.rot / 2 / vec + (p.D - p.rot) / vec;
-  p.upt = (p.q.heads + p.k.heads) * p.uph;
+  p.upt = (p.q.heads + (p.kp ? 0 : p.k.heads)) * p.uph;
   p.uph_div = div_magic(p.uph);
-  p.upt_div = div_magic(p.upt);
+  p.upt_div = div_magic(max(p.upt, 1));
   // tokens of a workgroup: several where that leaves over 4 workgroups a CU, whose one round of angles then serves more work
   p.tok = 1;
   while (p.tok < ROPE_TOKENS && (p.n + 2 * p.tok - 1) / (2 * p.tok) >= 1024 && (int64_t)2 * p.tok * p.upt * p.upt < (int64_t)1 << 32) p.tok *= 2;
-  const dim3 grid((p.n + p.tok - 1) / p.tok), block(ROPE_THREADS);
-  const size_t lds = (size_t)p.tok * (p.rot / 2) * sizeof(f32x2);
+  p.fill = p.kp ? (p.n + ROPE_RUN - 1) / ROPE_RUN * p.KVH : 0;
+  p.v_wide = !((reinterpret_cast<uintptr_t>(p.v.x) | (uintptr_t)(p.v.x_stride * 2)) & 15);
+  const dim3 grid((p.upt ? (p.n + p.tok - 1) / p.tok : 0) + p.fill), block(ROPE_THREADS);
+  size_t lds = (size_t)p.tok * (p.rot / 2) * sizeof(f32x2);
+  if (p.fill) lds = std::max(lds, (size_t)ROPE_RUN * (p.rot / 2) * sizeof(f32x2) + (size_t)ROPE_RUN * (p.D + 2) * 2);
 #define ROPE_GO(T, V, IL) hipLaunchKernelGGL((rope_kernel<T, V, IL>), grid, block, lds, s, p)
 #define ROPE_TYPE(T, V16)                    \
   if (wide && interleaved) ROPE_GO(T, V16, true);  \
