@@ -79,7 +79,8 @@ struct SampleBegun {
 struct SampleRow {
   SampleLocals s;
   uint32_t mode, bin;     // bin in which the cut lies
-  uint32_t by_mass, pad;  // the cut is top-p's (else top-k's)
+  uint32_t by_mass;       // the cut is top-p's (else top-k's)
+  float u;                // (set by the third launch)
   uint64_t above, limit;  // weight (else tokens) in the bins above it, and of what is kept, before min-p
 };
 struct SampleParams {

@@ -412,11 +412,12 @@ __global__ __launch_bounds__(SP_THREADS) void sample_hist_kernel(SampleParams p)
     n[i] = by_k ? sp_get(p.hist_count + b) : sp_get(p.hist_mass + b);
     ns += n[i];
   }
+  const uint64_t whole = by_k ? 0 : sp_get(p.whole + row);
   uint64_t before = block_scan_u64(ns, scratch, &seen) - ns;
   SampleRow r = {};
   r.s = s;
   r.by_mass = !by_k;
-  r.limit = by_k ? (uint64_t)s.k : sp_limit(s.p, sp_get(p.whole + row));
+  r.limit = by_k ? (uint64_t)s.k : sp_limit(s.p, whole);
   if (seen < r.limit) {  // fewer live tokens than top-k keeps: all of them stay
     if (threadIdx.x == 0) {
       r.bin = SP_BINS - 1;
@@ -447,8 +448,8 @@ __device__ __forceinline__ void sp_store(const SampleParams& p, int row, int tok
   if (p.logprob) p.logprob[row] = (float)log((double)w / (double)whole);
 }
 // How much weight lies in front of the draw.
-__device__ __forceinline__ uint64_t sp_target(const SampleParams& p, int row, uint64_t whole) {
-  const float u = p.u[row];
+__device__ __forceinline__ uint64_t sp_target(const SampleRow& r, uint64_t whole) {
+  const float u = r.u;
   const double x = u > 0.f ? (double)fminf(u, 1.f - 0x1p-24f) * (double)whole : 0.0;
   return x < (double)(whole - 1) ? (uint64_t)x : whole - 1;
 }
@@ -590,7 +591,8 @@ __device__ __forceinline__ void sp_shrink(const Items& it, const SampleLocals& s
 
 // The draw among items that the cut and min-p keep.
 template <typename Items>
-__device__ __forceinline__ void sp_draw(const SampleParams& p, int row, const Items& it, const SampleLocals& s, SampleShared& sh, const SampleCut& cut) {
+__device__ __forceinline__ void sp_draw(const SampleParams& p, int row, const Items& it, const SampleRow& r, SampleShared& sh, const SampleCut& cut) {
+  const SampleLocals& s = r.s;
   uint64_t whole = 0, kept = 0;
   it.each([&](uint32_t idx, float z) {
     if (!cut.keeps(argmax_ord(z), idx) || !sp_high(z, s)) return;
@@ -599,7 +601,7 @@ __device__ __forceinline__ void sp_draw(const SampleParams& p, int row, const It
   });
   whole = block_sum_u64(whole, sh.scratch);
   kept = block_sum_u64(kept, sh.scratch);
-  const uint64_t target = sp_target(p, row, whole);
+  const uint64_t target = sp_target(r, whole);
   uint64_t c = 0, w = 0;
   uint32_t inv;
   sp_descend(it, s, sh, true, target + 1, c, w, inv, [&](uint32_t idx, float z, uint32_t& o) {
@@ -613,7 +615,8 @@ __device__ __forceinline__ void sp_draw(const SampleParams& p, int row, const It
 
 // All of the cuts and the draw among items that hold every token that may be kept.
 template <typename Items>
-__device__ __forceinline__ void sp_finish(const SampleParams& p, int row, const Items& it, const SampleLocals& s, SampleShared& sh) {
+__device__ __forceinline__ void sp_finish(const SampleParams& p, int row, const Items& it, const SampleRow& r, SampleShared& sh) {
+  const SampleLocals& s = r.s;
   SampleCut cut = {0, 0xffffffffu};
   if (s.k) sp_shrink(it, s, sh, cut, false, (uint64_t)s.k, 0, 0);
   if (s.p < 1.f) {
@@ -622,7 +625,7 @@ __device__ __forceinline__ void sp_finish(const SampleParams& p, int row, const 
     whole = block_sum_u64(whole, sh.scratch);
     sp_shrink(it, s, sh, cut, true, sp_limit(s.p, whole), 0, 0);
   }
-  sp_draw(p, row, it, s, sh, cut);
+  sp_draw(p, row, it, r, sh, cut);
 }
 
 // Of at most SP_SMALL tokens each thread has one (the argmax key, 0: none; its weight). All of them into sh.key and sh.mass, the rest
@@ -711,7 +714,8 @@ __device__ __forceinline__ bool sp_narrow(const SampleList& it, const SampleLoca
 }
 
 // The cuts and the draw of a list of at most SP_SMALL tokens, of which top-k keeps some or all.
-__device__ __forceinline__ void sp_small(const SampleParams& p, int row, const SampleList& it, const SampleLocals& s, SampleShared& sh) {
+__device__ __forceinline__ void sp_small(const SampleParams& p, int row, const SampleList& it, const SampleRow& r, SampleShared& sh) {
+  const SampleLocals& s = r.s;
   const int i = threadIdx.x;
   const bool there = i < it.n, has = (i & ~63) < it.n;
   const uint64_t key = there ? it.key[i] : 0;
@@ -733,7 +737,7 @@ __device__ __forceinline__ void sp_small(const SampleParams& p, int row, const S
   __syncthreads();
   if (i < SP_SMALL) sh.mass[i] = keep ? w : 0;
   const uint64_t whole = block_sum_u64(keep ? w : 0, sh.scratch), kept = block_sum_u64(keep, sh.scratch);
-  const uint64_t target = sp_target(p, row, whole);
+  const uint64_t target = sp_target(r, whole);
   uint64_t sum = 0;
   if (has) sp_all(sh, it.n, [&](uint64_t k, uint64_t x) { sum += (uint32_t)k > (uint32_t)key ? x : 0; });  // (lower indexes: larger low words)
   if (keep && sum <= target && sum + w > target) sp_store(p, row, (int)sp_index(key), z, kept, w, whole);
@@ -741,8 +745,9 @@ __device__ __forceinline__ void sp_small(const SampleParams& p, int row, const S
 
 // The draw where the kept weight lies by chunks (in LDS): the chunk, then its tokens, by one wave.
 template <typename T, typename Keep>
-__device__ __forceinline__ void sp_draw_chunk(const SampleParams& p, int row, const T* z0, uint64_t* sums, uint64_t kept, const SampleLocals& s,
+__device__ __forceinline__ void sp_draw_chunk(const SampleParams& p, int row, const T* z0, uint64_t* sums, uint64_t kept, const SampleRow& r,
                                               SampleShared& sh, Keep keep) {
+  const SampleLocals& s = r.s;
   constexpr int EACH = SP_CHUNKS / SP_THREADS;
   uint64_t mine = 0, whole;
 #pragma unroll
@@ -751,7 +756,7 @@ __device__ __forceinline__ void sp_draw_chunk(const SampleParams& p, int row, co
     mine += c < p.chunks ? sums[c] : 0;
   }
   uint64_t before = block_scan_u64(mine, sh.scratch, &whole) - mine;
-  const uint64_t target = sp_target(p, row, whole);
+  const uint64_t target = sp_target(r, whole);
   if (before <= target && before + mine > target) {  // (one thread)
     int c = threadIdx.x * EACH;
     while (before + sums[c] <= target) before += sums[c++];
@@ -787,7 +792,8 @@ __global__ __launch_bounds__(SP_THREADS) void sample_pick_kernel(SampleParams p)
   __shared__ uint64_t small[SP_SMALL];
   __shared__ SampleShared sh;
   const int part = blockIdx.x % p.P3, row = blockIdx.x / p.P3, lane = threadIdx.x & 63;
-  const SampleRow r = sp_read(p.result + row);
+  SampleRow r = sp_read(p.result + row);
+  r.u = ldc(p.u + row);
   if (part && (r.mode == SP_EMPTY || r.mode == SP_GREEDY || r.mode == SP_ALL || r.mode == SP_ROW)) return;
   const SampleLocals s = r.s;
   const T* z0 = sp_row<T>(p, row);
@@ -803,11 +809,11 @@ __global__ __launch_bounds__(SP_THREADS) void sample_pick_kernel(SampleParams p)
   if (r.mode == SP_ALL) {
     for (int c = threadIdx.x; c < p.chunks; c += SP_THREADS) sums[c] = p.chunk_sum[(size_t)row * p.chunks + c];
     __syncthreads();
-    sp_draw_chunk<T>(p, row, z0, sums, p.taken[row] >> 32, s, sh, [](uint32_t, float) { return true; });
+    sp_draw_chunk<T>(p, row, z0, sums, p.taken[row] >> 32, r, sh, [](uint32_t, float) { return true; });
     return;
   }
   if (r.mode == SP_ROW) {
-    sp_finish(p, row, SampleWhole<T>{z0, p.V, p.wide != 0}, s, sh);
+    sp_finish(p, row, SampleWhole<T>{z0, p.V, p.wide != 0}, r, sh);
     return;
   }
   // This part's tokens for the list, and (SP_BELOW) the kept weight above the bin by chunks
@@ -865,20 +871,24 @@ __global__ __launch_bounds__(SP_THREADS) void sample_pick_kernel(SampleParams p)
 
   // The last part finishes the row
   const uint64_t taken = sp_get(p.taken + row);
+  if (!listed)
+    for (int c = threadIdx.x; c < p.chunks; c += SP_THREADS) sums[c] = sp_get(p.chunk_sum + (size_t)row * p.chunks + c);
   const int n = (int)(uint32_t)taken;
   if (n > SP_LIST) {  // (top-p's bin: only its weight was known)
-    sp_finish(p, row, SampleWhole<T>{z0, p.V, p.wide != 0}, s, sh);
+    sp_finish(p, row, SampleWhole<T>{z0, p.V, p.wide != 0}, r, sh);
     return;
   }
-  for (int i = threadIdx.x; i < n; i += SP_THREADS) list[i] = sp_get(p.list + (size_t)row * SP_LIST + i);
+  const uint64_t first = sp_get(p.list + (size_t)row * SP_LIST + threadIdx.x);  // (there or not: asked for along with their number)
+  if ((int)threadIdx.x < n) list[threadIdx.x] = first;
+  for (int i = threadIdx.x + SP_THREADS; i < n; i += SP_THREADS) list[i] = sp_get(p.list + (size_t)row * SP_LIST + i);
   __syncthreads();
   const SampleList it = {list, n};
   if (listed && n <= SP_SMALL) {
-    sp_small(p, row, it, s, sh);
+    sp_small(p, row, it, r, sh);
     return;
   }
   if (listed) {  // more than SP_SMALL tokens, by top-k
-    sp_finish(p, row, it, s, sh);
+    sp_finish(p, row, it, r, sh);
     return;
   }
   SampleCut cut = {0, 0xffffffffu};
@@ -890,8 +900,6 @@ __global__ __launch_bounds__(SP_THREADS) void sample_pick_kernel(SampleParams p)
     cut = sp_rank(few, s, sh, r.by_mass != 0, r.limit, front);
   else
     sp_shrink(it, s, sh, cut, r.by_mass != 0, r.limit, r.above, r.above);
-  for (int c = threadIdx.x; c < p.chunks; c += SP_THREADS) sums[c] = sp_get(p.chunk_sum + (size_t)row * p.chunks + c);
-  __syncthreads();
   uint64_t more = 0;
   it.each([&](uint32_t i, float z) {
     if (!cut.keeps(argmax_ord(z), i) || !sp_high(z, s)) return;
@@ -899,7 +907,7 @@ __global__ __launch_bounds__(SP_THREADS) void sample_pick_kernel(SampleParams p)
     ++more;
   });
   more = block_sum_u64(more, sh.scratch);
-  sp_draw_chunk<T>(p, row, z0, sums, (taken >> 32) + more, s, sh, [&](uint32_t i, float z) {
+  sp_draw_chunk<T>(p, row, z0, sums, (taken >> 32) + more, r, sh, [&](uint32_t i, float z) {
     return (r.bin && !(sp_dist(z, s) >= inner)) || cut.keeps(argmax_ord(z), i);
   });
 }
