@@ -2,8 +2,10 @@
 // all sequences, each sequence's own keys for its rows.
 //
 // o = sum_j P_j v_j / l with P_j = 2^(c q.k_j - m), c = log2(e) / sqrt(D), l = sum_j P_j and m the row's running reference (it
-// moves only when a score passes it by more than TAU, so P <= 2^TAU and a page mostly needs no rescale). Tiles are those of the
-// page format: S^T[keys][rows] = K Q^T, a lane holds one row's scores of eight keys, which in this order are its operand of
+// moves only when a score passes it by more than TAU, so P <= 2^TAU and a page mostly needs no rescale). It is set BASE below the
+// largest score: fp16 then holds weights down to 2^-31 of the largest, and a long tail of keys far below one of them keeps its
+// share (with the reference at the largest itself a weight of 2^-26 is nothing, 2^17 such keys 2^-9 of the whole). Tiles are those
+// of the page format: S^T[keys][rows] = K Q^T, a lane holds one row's scores of eight keys, which in this order are its operand of
 // O^T += V^T P^T; the row sums are a product with ones. Scores, sums and outputs are fp32, P is rounded to fp16 once (V's
 // products take fp16 operands); q is taken as it is, the scale in the exponent's multiply-add (scaled in fp16 it would be rounded).
 //
@@ -21,7 +23,7 @@
 
 namespace dspark {
 
-constexpr float SA_TAU = 8.f;
+constexpr float SA_TAU = 15.f, SA_BASE = 7.f;  // (2^15 < 65504)
 constexpr int SA_THREADS = 256;
 
 // The row-wave form's ring: two slots of two pages. At D = 64 that leaves room for four workgroups a CU, at 128 for two, as many as the
@@ -107,7 +109,7 @@ __device__ __forceinline__ void sa_softmax(f32x4 (&s)[QB][2], int key0, const Sa
       rm = fmaxf(rm, __shfl_xor(rm, 16));  // the row's four lanes
       rm = fmaxf(rm, __shfl_xor(rm, 32));
       if (rm > st.thr[qb]) {
-        const float m = st.m[qb] + rm, move = m - st.m[qb];
+        const float m = st.m[qb] + (rm - SA_BASE), move = m - st.m[qb];
         const float alpha = st.thr[qb] == SA_TAU ? fast_exp2(-move) : 0.f;
 #pragma unroll
         for (int cc = 0; cc < D / 16; ++cc) st.o[qb][cc] *= alpha;

@@ -360,6 +360,29 @@ def test_shared_growing_and_falling_scores(D, seqs):
     assert np.all(np.abs(f64(lse) - wlse) <= 2.0 ** -11 + score + 740 * 2.0 ** -25 + 2.0 ** -22 * np.abs(wlse))
 
 
+@pytest.mark.parametrize("seqs", [1, 20])
+@pytest.mark.parametrize("D,b", [(64, 12.0), (128, 17.0)])
+def test_shared_long_tail(D, b, seqs):
+    """One key 18 above all others, with V of 0 where they have 1000: their share is n e^-18. P of a tail key is off by 2^-25 of a largest of 2^7
+    at least, n 2^-32 of the whole; the rest as in Batch.close, of the output itself (the tail's weights are all alike)."""
+    x = Batch(D, 2, 1, D, 20000, [1] * seqs, [1] * seqs)
+    x.q_np[:] = 0
+    x.q_np[:, :, 0] = 12
+    for k, v in zip(x.k, x.v):
+        k[:], v[:] = 0, 1000
+    x.k[0][777, :, 0], x.v[0][777] = b, 0
+    h, first = x.h, x.prefix_table.cpu().numpy()
+    for t, k, v in zip([first] + list(x.own_table.cpu().numpy()), x.k, x.v):
+        h.kv_write(dev(k).view(len(k), -1), dev(v).view(len(v), -1), x.kp, x.vp, 0, dev(t[:(len(k) + 31) // 32].copy()))
+    x.q = dev(x.q_np)
+    _, f32, lse = x.run()
+    want, wlse, _ = x.oracle()
+    score = 2 * D ** 1.5 * 2.0 ** -24 * 12 * b / 2 + 2.0 ** -22
+    assert want.min() > 0.25
+    assert np.all(np.abs(f64(f32) - want) <= 20001 * 2.0 ** -32 * 1000 + (2.0 ** -10 + score) * want)
+    assert np.all(np.abs(f64(lse) - wlse) <= 20001 * 2.0 ** -32 + score + 2.0 ** -22 * np.abs(wlse))
+
+
 def test_shared_is_verify_attention_of_each():
     """One sequence behind a prefix is the paged verify attention of the whole: both within their bounds, so within their sum."""
     h = load_host()
