@@ -639,9 +639,14 @@ F16, BF16, F32 = 0, 1, 2
 ROPE_SCALING = {None: 0, "linear": 1, "base": 2, "ramp": 3}
 
 
+_types = {}
+
+
 def _type_of(dtype, what):
-    torch = _torch()
-    code = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32}.get(dtype)
+    if not _types:
+        torch = _torch()
+        _types.update({torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32})
+    code = _types.get(dtype)
     if code is None:
         raise DsparkError(f"{what} is fp16, bf16 or fp32")
     return code
@@ -654,7 +659,7 @@ def _on_device(t, stream, call, *args):
     index = t.get_device()
     if index < 0:
         raise DsparkError("tensors are on a GPU")
-    if stream is None and torch.cuda.current_device() == index:
+    if stream is None and torch._C._cuda_getDevice() == index:
         return call(torch._C._cuda_getCurrentRawStream(index), *args)
     stream = stream if stream is not None else torch.cuda.current_stream(t.device)
     if stream.device_index != index:
@@ -694,42 +699,44 @@ def rope_freqs(rot, base=10000.0, scaling=None, factor=1.0, trained=0.0, low=1.0
 
 def _rope_args(q, k, positions, freqs, interleaved, inverse, scale):
     torch = _torch()
-    first = q if q is not None else k
-    if first is None:
+    if q is None and k is None:
         raise DsparkError("rope: q or k")
-    a, index = RopeArgs(), first.get_device()
-    a.type = _type_of(first.dtype, "rope: q and k")
-    for name, t in (("q", q), ("k", k)):
-        if t is None:
-            continue
-        n, heads, D, stride = _heads(t, "rope: " + name)
-        if t.dtype != first.dtype or n != first.shape[0] or D != first.shape[2] or t.get_device() != index:
+    a = RopeArgs()
+    if q is not None:
+        n, a.QH, D, a.q_stride = _heads(q, "rope: q")
+        a.q, index, dtype = q.data_ptr(), q.get_device(), q.dtype
+    if k is not None:
+        m, a.KVH, E, a.k_stride = _heads(k, "rope: k")
+        a.k = k.data_ptr()
+        if q is None:
+            n, D, index, dtype = m, E, k.get_device(), k.dtype
+        elif k.dtype != dtype or m != n or E != D or k.get_device() != index:
             raise DsparkError("rope: q and k have one type, device, number of rows and head size")
-        if name == "q":
-            a.q, a.q_stride, a.QH = t.data_ptr(), stride, heads
-        else:
-            a.k, a.k_stride, a.KVH = t.data_ptr(), stride, heads
-    a.n, a.D, a.rot = first.shape[0], first.shape[2], 2 * freqs.numel()
-    a.positions = _flat(positions, first.shape[:1], torch.int32, index, "positions")
-    a.freq = _flat(freqs, freqs.shape[:1], torch.float64, index, "freqs")
+    a.type = _type_of(dtype, "rope: q and k")
+    pairs = freqs.numel()
+    a.n, a.D, a.rot = n, D, 2 * pairs
+    a.positions = _flat(positions, (n,), torch.int32, index, "positions")
+    a.freq = _flat(freqs, (pairs,), torch.float64, index, "freqs")
     a.interleaved, a.inverse, a.scale = int(interleaved), int(inverse), scale
     return a
 
 
-def _rope_out(t, out, index, what):
+def _rope_out(t, out, what):
+    """`out` or a new one for t, its address and row stride."""
     if out is None:
-        out = t.new_empty(t.shape)
+        out = _torch().empty_like(t)  # (its rows one after the other, those of a t inside wider rows too)
+        return out, out.data_ptr(), t.shape[1] * t.shape[2]
     n, heads, D, stride = _heads(out, what)
-    if out.shape != t.shape or out.dtype != t.dtype or out.get_device() != index:
+    if out is not t and (out.shape != t.shape or out.dtype != t.dtype or out.get_device() != t.get_device()):
         raise DsparkError(f"{what} has its input's shape, type and device")
     return out, out.data_ptr(), stride
 
 
 def _rope(s, a, q, k, q_out, k_out):
     if q is not None:
-        q_out, a.q_out, a.q_out_stride = _rope_out(q, q_out, q.get_device(), "q_out")
+        q_out, a.q_out, a.q_out_stride = _rope_out(q, q_out, "q_out")
     if k is not None:
-        k_out, a.k_out, a.k_out_stride = _rope_out(k, k_out, k.get_device(), "k_out")
+        k_out, a.k_out, a.k_out_stride = _rope_out(k, k_out, "k_out")
     check(lib().dspark_rope(ctypes.byref(a), s), "dspark_rope")
     return q_out, k_out
 
@@ -743,7 +750,7 @@ def rope(q, k, positions, freqs, interleaved=False, inverse=False, scale=1.0, q_
 
 
 def _rope_append(s, a, q, q_out):
-    q_out, a.q_out, a.q_out_stride = _rope_out(q, q_out, q.get_device(), "q_out")
+    q_out, a.q_out, a.q_out_stride = _rope_out(q, q_out, "q_out")
     check(lib().dspark_rope(ctypes.byref(a), s), "dspark_rope")
     return q_out
 
@@ -756,20 +763,20 @@ def rope_append(q, k, v, positions, freqs, k_pages, v_pages, slots, interleaved=
         raise DsparkError("rope_append: q, k and v are fp16")
     a, index = _rope_args(q, k, positions, freqs, interleaved, False, scale), q.get_device()
     KVH, D, P = a.KVH, a.D, k_pages.shape[0]
-    n, heads, dv, a.v_stride = _heads(v, "rope_append: v")
-    if v.shape != k.shape or v.dtype != torch.float16 or v.get_device() != index:
+    n, heads, E, a.v_stride = _heads(v, "rope_append: v")
+    if n != a.n or heads != KVH or E != D or v.dtype != torch.float16 or v.get_device() != index:
         raise DsparkError("rope_append: k and v have one shape, type and device")
     a.v, a.kv_pages = v.data_ptr(), P
     a.k_pages = _flat(k_pages, (P, KVH, PAGE, D), torch.float16, index, "k_pages")
     a.v_pages = _flat(v_pages, (P, KVH, D, PAGE), torch.float16, index, "v_pages")
-    a.slots = _flat(slots, q.shape[:1], torch.int64, index, "slots")
+    a.slots = _flat(slots, (n,), torch.int64, index, "slots")
     return _on_device(q, stream, _rope_append, a, q, q_out)
 
 
 def _with_workspace(s, t, a, workspace, call, need, what):
     """call(a, stream) with the workspace as it is first, then with one that is large enough."""
     torch, ref = _torch(), ctypes.byref(a)
-    if workspace is not None and workspace.buf is not None and torch.cuda.is_current_stream_capturing():
+    if workspace is not None and workspace.buf is not None and torch._C._cuda_isCurrentStreamCapturing():
         workspace.hold()
     ws = workspace and workspace.buf
     while True:
@@ -789,8 +796,10 @@ def _with_workspace(s, t, a, workspace, call, need, what):
 def _verify_attention_shared(s, a, q, out, out_f32, workspace):
     torch = _torch()
     if out is None and out_f32 is None:
-        out = q.new_empty(q.shape)
-    a.out = _flat(out, q.shape, torch.float16, q.get_device(), "out")
+        out = torch.empty_like(q)
+        a.out = out.data_ptr()
+    else:
+        a.out = _flat(out, q.shape, torch.float16, q.get_device(), "out")
     a.out_f32 = _flat(out_f32, q.shape, torch.float32, q.get_device(), "out_f32")
     L = lib()
     _with_workspace(s, q, a, workspace, L.dspark_verify_attention_shared, L.dspark_verify_attention_shared_workspace,
@@ -847,9 +856,11 @@ def _verify_sample(s, a, logits, outs, workspace):
     for name, t, dtype in zip(("tokens", "keys", "kept", "logprob"), outs, types):
         if t is True:
             t = torch.empty(n, dtype=dtype, device=logits.device)
+            setattr(a, name, t.data_ptr())
         elif t is False:
             t = None
-        setattr(a, name, _flat(t, (n,), dtype, index, name))
+        else:
+            setattr(a, name, _flat(t, (n,), dtype, index, name))
         made.append(t)
     L = lib()
     _with_workspace(s, logits, a, workspace, L.dspark_verify_sample, lambda ref: L.dspark_verify_sample_workspace(n, a.V), "dspark_verify_sample")
