@@ -66,12 +66,12 @@ struct RopePiece {
   }
 };
 
-// The sines and cosines of tokens t0 .. t0 + nt - 1: cs[t][rot / 2].
-__device__ __forceinline__ void rope_angles(const RopeBatch& p, f32x2* cs, int t0, int nt) {
+// The sines and cosines of tokens t0 .. t0 + nt - 1: cs[t][rot / 2], tokens `pitch` apart.
+__device__ __forceinline__ void rope_angles(const RopeBatch& p, f32x2* cs, int pitch, int t0, int nt) {
   const int P = p.rot / 2;
   for (int e = threadIdx.x; e < nt * P; e += ROPE_THREADS) {
     const int t = e / P, i = e - t * P;
-    cs[e] = rope_cos_sin((double)ldg(p.pos + t0 + t) * (ldg(p.freq + i) * 0.15915494309189533577), p.scale, p.inverse != 0);
+    cs[t * pitch + i] = rope_cos_sin((double)ldg(p.pos + t0 + t) * (ldg(p.freq + i) * 0.15915494309189533577), p.scale, p.inverse != 0);
   }
 }
 
@@ -117,8 +117,9 @@ __device__ __forceinline__ void rope_unit(const RopeBatch& p, const f32x2* c, in
 // K and V of KV head h, tokens t0 .. t0 + nt - 1 (nt <= ROPE_RUN), into the pages.
 template <int VEC, bool IL>
 __device__ __forceinline__ void rope_pages(const RopeBatch& p, f32x2* cs, int h, int t0, int nt) {
-  _Float16* turn = reinterpret_cast<_Float16*>(cs + ROPE_RUN * (p.rot / 2));  // V's rows, D + 2 halves apart: odd in words
-  const int per = p.D / 8, pitch = p.D + 2;
+  // (lanes are tokens: angles of two words an odd number of them apart, V's rows an odd number of words)
+  const int angles = p.rot / 2 | 1, per = p.D / 8, pitch = p.D + 2;
+  _Float16* turn = reinterpret_cast<_Float16*>(cs + ROPE_RUN * angles);
   for (int e = threadIdx.x; e < nt * per; e += ROPE_THREADS) {
     const int t = e / per, d = (e - t * per) * 8;
     const _Float16* src = static_cast<const _Float16*>(p.v.x) + (size_t)(t0 + t) * p.v.x_stride + (size_t)h * p.D + d;
@@ -133,7 +134,7 @@ __device__ __forceinline__ void rope_pages(const RopeBatch& p, f32x2* cs, int h,
 #pragma unroll
     for (int i = 0; i < 4; ++i) to[i] = x[i];
   }
-  rope_angles(p, cs, t0, nt);
+  rope_angles(p, cs, angles, t0, nt);
   __syncthreads();
   const int t = threadIdx.x % ROPE_RUN;
   if (t >= nt) return;
@@ -144,7 +145,7 @@ __device__ __forceinline__ void rope_pages(const RopeBatch& p, f32x2* cs, int h,
   // (a piece of up to 8 values from a multiple of its size lies together in K's page)
   const _Float16* src = static_cast<const _Float16*>(p.k.x) + (size_t)(t0 + t) * p.k.x_stride + (size_t)h * p.D;
   for (int u = threadIdx.x / ROPE_RUN; u < p.uph; u += ROPE_THREADS / ROPE_RUN)
-    rope_unit<_Float16, VEC, IL>(p, cs + t * (p.rot / 2), u, src, p.kp + block, [&](int d) { return k_page_elem(at_slot, d, p.D); });
+    rope_unit<_Float16, VEC, IL>(p, cs + t * angles, u, src, p.kp + block, [&](int d) { return k_page_elem(at_slot, d, p.D); });
   for (int d = threadIdx.x / ROPE_RUN; d < p.D; d += ROPE_THREADS / ROPE_RUN)
     p.vp[block + v_page_elem(at_slot, d)] = turn[t * pitch + d];
 }
@@ -162,7 +163,7 @@ __global__ __launch_bounds__(ROPE_THREADS) void rope_kernel(RopeBatch p) {
     wg -= p.fill;
   }
   const int t0 = wg * p.tok, nt = min(p.tok, p.n - t0);
-  rope_angles(p, cs, t0, nt);
+  rope_angles(p, cs, p.rot / 2, t0, nt);
   __syncthreads();
   for (int e = threadIdx.x; e < nt * p.upt; e += ROPE_THREADS) {
     const int tl = div_by(e, p.upt_div), r = e - tl * p.upt, t = t0 + tl;
@@ -198,7 +199,7 @@ int rope_batch_launch(RopeBatch& p, int type, bool interleaved, hipStream_t s) {
   p.v_wide = !((reinterpret_cast<uintptr_t>(p.v.x) | (uintptr_t)(p.v.x_stride * 2)) & 15);
   const dim3 grid((p.upt ? (p.n + p.tok - 1) / p.tok : 0) + p.fill), block(ROPE_THREADS);
   size_t lds = (size_t)p.tok * (p.rot / 2) * sizeof(f32x2);
-  if (p.fill) lds = std::max(lds, (size_t)ROPE_RUN * (p.rot / 2) * sizeof(f32x2) + (size_t)ROPE_RUN * (p.D + 2) * 2);
+  if (p.fill) lds = std::max(lds, (size_t)ROPE_RUN * (p.rot / 2 + 1) * sizeof(f32x2) + (size_t)ROPE_RUN * (p.D + 2) * 2);
 #define ROPE_GO(T, V, IL) hipLaunchKernelGGL((rope_kernel<T, V, IL>), grid, block, lds, s, p)
 #define ROPE_TYPE(T, V16)                    \
   if (wide && interleaved) ROPE_GO(T, V16, true);  \
