@@ -166,7 +166,7 @@ __global__ __launch_bounds__(ROPE_THREADS) void rope_kernel(RopeBatch p) {
   rope_angles(p, cs, p.rot / 2, t0, nt);
   __syncthreads();
   for (int e = threadIdx.x; e < nt * p.upt; e += ROPE_THREADS) {
-    const int tl = div_by(e, p.upt_div), r = e - tl * p.upt, t = t0 + tl;
+    const int tl = p.tok == 1 ? 0 : div_by(e, p.upt_div), r = e - tl * p.upt, t = t0 + tl;
     int h = div_by(r, p.uph_div);
     const int u = r - h * p.uph;
     const bool in_q = h < p.q.heads;
@@ -192,7 +192,8 @@ int rope_batch_launch(RopeBatch& p, int type, bool interleaved, hipStream_t s) {
   p.upt = (p.q.heads + (p.kp ? 0 : p.k.heads)) * p.uph;
   p.uph_div = div_magic(p.uph);
   p.upt_div = div_magic(max(p.upt, 1));
-  // tokens of a workgroup: several where that leaves over 4 workgroups a CU, whose one round of angles then serves more work
+  // tokens of a workgroup: several where that leaves over 4 workgroups a CU, whose one round of angles then serves more work, and where
+  // the division by upt is exact (a token alone may have more units than that)
   p.tok = 1;
   while (p.tok < ROPE_TOKENS && (p.n + 2 * p.tok - 1) / (2 * p.tok) >= 1024 && (int64_t)2 * p.tok * p.upt * p.upt < (int64_t)1 << 32) p.tok *= 2;
   p.fill = p.kp ? (p.n + ROPE_RUN - 1) / ROPE_RUN * p.KVH : 0;

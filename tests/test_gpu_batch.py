@@ -87,6 +87,19 @@ def test_rope_rows_in_wider_ones(kind, interleaved, off, stride):
     assert torch.equal(before, base)
 
 
+@pytest.mark.parametrize("QH,KVH", [(128, 8), (100, 7), (1024, 1024)])
+def test_rope_more_units_of_a_token_than_a_division_holds(QH, KVH):
+    """Heads of 1022 values, turned value by value: 109247 units of a token and more."""
+    h, rng, n, D = load_host(), np.random.default_rng(QH), 3, 1022
+    q, k = (dev(rng.standard_normal((n, heads, D)).astype(np.float16)) for heads in (QH, KVH))
+    f, pos = batch.rope_freqs(2, 1e4)[0], np.array([5, 70000, 3], np.int32)
+    spare = torch.full((n + 2, QH, D), 7.0, dtype=torch.float16, device="cuda")
+    oq, ok = h.rope(q, k, dev(pos), dev(f), q_out=spare[1:1 + n])
+    for y, x in ((oq, q), (ok, k)):
+        rope_close(y, f64(x), batch.rope(f64(x), pos, f), "f16", 1.0, 2)
+    assert bool((spare[0] == 7).all()) and bool((spare[-1] == 7).all())
+
+
 def test_rope_not_finite_and_nothing():
     h = load_host()
     f = dev(batch.rope_freqs(8, 1e4)[0])
