@@ -267,7 +267,8 @@ typedef struct dspark_rope_args {
   const int64_t* slots;        /* append: [n] */
   int64_t kv_pages;
   double scale;                /* s */
-  int32_t n, QH, KVH, D, rot;  /* n < 2^30; QH, KVH <= 1024; D even, <= 1024; rot even, 2 <= rot <= D */
+  int32_t n, QH, KVH, D, rot;  /* n < 2^23, append: n KVH < 2^27 (launches of under 2^32 threads); QH, KVH <= 1024;
+                                  D even, <= 1024; rot even, 2 <= rot <= D */
   int32_t interleaved, inverse, type; /* DSPARK_F16 | BF16 | F32 */
 } dspark_rope_args;
 int dspark_rope(const dspark_rope_args* args, dspark_stream_t stream);

@@ -101,7 +101,7 @@ int dspark_rope_freqs(int32_t rot, double base, int32_t scaling, double factor, 
 }
 
 int dspark_rope(const dspark_rope_args* a, dspark_stream_t stream) {
-  if (!a || a->n < 0 || a->n >= 1 << 30 || a->QH < 0 || a->KVH < 0 || a->QH > HEADS_MAX || a->KVH > HEADS_MAX || a->QH + a->KVH < 1)
+  if (!a || a->n < 0 || a->n >= 1 << 23 || a->QH < 0 || a->KVH < 0 || a->QH > HEADS_MAX || a->KVH > HEADS_MAX || a->QH + a->KVH < 1)
     return DSPARK_EINVAL;
   if (a->D < 2 || a->D > 1024 || a->D % 2 || a->rot < 2 || a->rot > a->D || a->rot % 2) return DSPARK_EINVAL;
   if (a->type != DSPARK_F16 && a->type != DSPARK_BF16 && a->type != DSPARK_F32) return DSPARK_EINVAL;
@@ -116,7 +116,7 @@ int dspark_rope(const dspark_rope_args* a, dspark_stream_t stream) {
   if (append) {
     if (a->KVH < 1 || a->type != DSPARK_F16 || a->inverse || (a->D != 64 && a->D != 128) || a->k_out) return DSPARK_EINVAL;
     if (!on(a->k_pages, 16) || !on(a->v_pages, 16) || !on(a->v, 2) || a->v_stride < (int64_t)a->KVH * a->D || !on(a->slots, 8)) return DSPARK_EINVAL;
-    if (a->kv_pages < 1 || a->kv_pages >= (int64_t)1 << 31) return DSPARK_EINVAL;
+    if (a->kv_pages < 1 || a->kv_pages >= (int64_t)1 << 31 || (int64_t)a->n * a->KVH >= 1 << 27) return DSPARK_EINVAL;
   } else if (a->KVH && (!on(a->k_out, size) || a->k_out_stride < (int64_t)a->KVH * a->D)) {
     return DSPARK_EINVAL;
   }

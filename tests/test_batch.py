@@ -66,6 +66,14 @@ def test_rope_append_refuses(bad):
     assert load_host().lib().dspark_rope(append_args(**bad), None) == EINVAL
 
 
+def test_rope_refuses_launches_past_what_a_grid_holds():
+    """Buffers far apart, so that nothing else is wrong with them."""
+    L, far = load_host().lib(), {k: i << 44 for i, k in enumerate(("q", "q_out", "k", "k_out", "positions", "freq"), 1)}
+    assert L.dspark_rope(rope_args(n=1 << 23, **far), None) == EINVAL
+    far.update(k_out=None, v=7 << 44, slots=8 << 44, k_pages=9 << 44, v_pages=10 << 44)
+    assert L.dspark_rope(append_args(n=1 << 20, KVH=128, k_stride=1 << 14, v_stride=1 << 14, kv_pages=1 << 20, **far), None) == EINVAL
+
+
 def test_rope_of_nothing():
     L = load_host().lib()
     assert L.dspark_rope(None, None) == EINVAL
