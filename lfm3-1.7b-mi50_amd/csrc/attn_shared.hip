@@ -637,9 +637,9 @@ int shared_launch(SharedAttn& p, int D, hipStream_t s) {
   }
 #undef SA_GO
   if (const hipError_t e = hipGetLastError(); e != hipSuccess) return (int)e;
-  // four waves for a row whose splits one wave would take in more than two rounds
+  // four waves for a row whose splits one wave would take in more than two rounds, where a workgroup a row is a launch of under 2^32 threads
   const int64_t units = (int64_t)p.R * p.max_tokens * p.QH;
-  const bool four = p.Sp + p.So > 2 * SA_ROUND * 256 / D;
+  const bool four = p.Sp + p.So > 2 * SA_ROUND * 256 / D && units < 1 << 24;
   const dim3 merge((unsigned)(four ? units : (units + 3) / 4));
   if (D == 64 && four)
     hipLaunchKernelGGL((shared_merge_kernel<64, 4>), merge, block, 0, s, p);

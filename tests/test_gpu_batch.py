@@ -408,6 +408,25 @@ def test_shared_is_verify_attention_of_each():
     assert float((f32 - ref).abs().max()) <= 2 * 2e-3
 
 
+def test_shared_many_splits_of_many_rows():
+    """64 sequences that may have 16384 tokens each, one of which has any: 2^24 rows asked for with more splits than a wave's two rounds. With
+    one split the same within both bounds (P's roundings and scores', Batch.close; values are at most 4 here)."""
+    h, T, QH, D, prefix = load_host(), 1 << 14, 16, 64, 67 * 32
+    rng = np.random.default_rng(3)
+    kp, vp = h.kv_pages_alloc(67, 1, D)
+    k, v = ((rng.standard_normal((prefix, D))).clip(-4, 4).astype(np.float16) for _ in range(2))
+    h.kv_write(dev(k), dev(v), kp, vp, 0, torch.arange(67, dtype=torch.int32, device="cuda"))
+    q = dev(rng.standard_normal((64, QH, D)).astype(np.float16)).repeat(T // 64, 1, 1)
+    start = torch.zeros(65, dtype=torch.int32, device="cuda")
+    start[33:] = T
+    none = torch.zeros(64, dtype=torch.int32, device="cuda")
+    ws = h.Workspace("cuda")
+    got = [h.verify_attention_shared(q, kp, vp, prefix, start, none, torch.zeros((64, 1), dtype=torch.int32, device="cuda"), T,
+                                     causal=False, out_f32=torch.empty((T, QH, D), device="cuda"), splits=s, workspace=ws)[1] for s in (67, 1)]
+    assert float((got[0] - got[1]).abs().max()) <= 2 * (2.0 ** -10 + 2 * (2 * D ** 1.5 * 2.0 ** -24 + 2.0 ** -22) + 2.0 ** -20) * 4 + 2 * prefix * 2.0 ** -25 * 5
+    assert torch.equal(got[0][:64], got[0][-64:])
+
+
 def test_shared_identity_table_and_strides():
     """No prefix table; q inside wider rows; own tables inside wider ones."""
     h = load_host()
