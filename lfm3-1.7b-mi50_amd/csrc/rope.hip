@@ -75,44 +75,50 @@ __device__ __forceinline__ void rope_angles(const RopeBatch& p, f32x2* cs, int p
   }
 }
 
-// Unit u of a head's row at src, token tl of cs, to dst + at(d). VEC: values of a piece, 16 bytes' worth or (sizes or addresses off
-// 16 bytes) 1, interleaved pairs 2.
-template <typename T, int VEC, bool IL, typename At>
-__device__ __forceinline__ void rope_unit(const RopeBatch& p, const f32x2* c, int u, const T* src, T* dst, At at) {
-  const int P = p.rot / 2, turning = IL ? p.rot / VEC : P / VEC;  // units of a head: what turns first, then the rest
-  RopePiece<T, VEC> a;
-  if (u >= turning) {  // passed on
-    const int d = p.rot + (u - turning) * VEC;
-    if (dst == src) return;
+// Unit u of a head's row: loaded, then turned by its token's c and stored to dst + at(d). VEC: values of a piece, 16 bytes' worth or
+// (sizes or addresses off 16 bytes) 1, interleaved pairs 2.
+template <typename T, int VEC, bool IL>
+struct RopeUnit {
+  RopePiece<T, VEC> a, b;  // (b: the half layout's partner)
+  int d;
+  bool turns, stays;
+  __device__ __forceinline__ void load(const RopeBatch& p, int u, const T* src, bool in_place) {
+    const int P = p.rot / 2, turning = IL ? p.rot / VEC : P / VEC;  // units of a head: what turns first, then the rest
+    turns = u < turning;
+    d = turns ? u * VEC : p.rot + (u - turning) * VEC;
+    stays = !turns && in_place;
+    if (stays) return;
     a.load(src + d);
-    a.store(dst + at(d));
-    return;
+    if (!IL && turns) b.load(src + P + d);
   }
-  const int d = u * VEC;
-  a.load(src + d);
-  if constexpr (IL) {
+  template <typename At>
+  __device__ __forceinline__ void store(const RopeBatch& p, const f32x2* c, T* dst, At at) {
+    const int P = p.rot / 2;
+    if (stays) return;
+    if (!turns) {
+      a.store(dst + at(d));
+    } else if constexpr (IL) {
 #pragma unroll
-    for (int i = 0; i < VEC; i += 2) {
-      const f32x2 w = c[d / 2 + i / 2];
-      const float xi = rope_to_f32(a.x[i]), xj = rope_to_f32(a.x[i + 1]);
-      a.x[i] = (T)(xi * w[0] - xj * w[1]);
-      a.x[i + 1] = (T)(xj * w[0] + xi * w[1]);
-    }
-    a.store(dst + at(d));
-  } else {
-    RopePiece<T, VEC> b;
-    b.load(src + P + d);
+      for (int i = 0; i < VEC; i += 2) {
+        const f32x2 w = c[d / 2 + i / 2];
+        const float xi = rope_to_f32(a.x[i]), xj = rope_to_f32(a.x[i + 1]);
+        a.x[i] = (T)(xi * w[0] - xj * w[1]);
+        a.x[i + 1] = (T)(xj * w[0] + xi * w[1]);
+      }
+      a.store(dst + at(d));
+    } else {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const f32x2 w = c[d + i];
-      const float xi = rope_to_f32(a.x[i]), xj = rope_to_f32(b.x[i]);
-      a.x[i] = (T)(xi * w[0] - xj * w[1]);
-      b.x[i] = (T)(xj * w[0] + xi * w[1]);
+      for (int i = 0; i < VEC; ++i) {
+        const f32x2 w = c[d + i];
+        const float xi = rope_to_f32(a.x[i]), xj = rope_to_f32(b.x[i]);
+        a.x[i] = (T)(xi * w[0] - xj * w[1]);
+        b.x[i] = (T)(xj * w[0] + xi * w[1]);
+      }
+      a.store(dst + at(d));
+      b.store(dst + at(P + d));
     }
-    a.store(dst + at(d));
-    b.store(dst + at(P + d));
   }
-}
+};
 
 // K and V of KV head h, tokens t0 .. t0 + nt - 1 (nt <= ROPE_RUN), into the pages.
 template <int VEC, bool IL>
@@ -120,6 +126,12 @@ __device__ __forceinline__ void rope_pages(const RopeBatch& p, f32x2* cs, int h,
   // (lanes are tokens: angles of two words an odd number of them apart, V's rows an odd number of words)
   const int angles = p.rot / 2 | 1, per = p.D / 8, pitch = p.D + 2;
   _Float16* turn = reinterpret_cast<_Float16*>(cs + ROPE_RUN * angles);
+  // K's first pieces are on their way while V's rows and the angles are laid down
+  const int tk = threadIdx.x % ROPE_RUN, u0 = threadIdx.x / ROPE_RUN;
+  const _Float16* k = static_cast<const _Float16*>(p.k.x) + (size_t)(t0 + min(tk, nt - 1)) * p.k.x_stride + (size_t)h * p.D;
+  const int64_t slot = ldg(p.slots + t0 + min(tk, nt - 1));
+  RopeUnit<_Float16, VEC, IL> now, next;
+  if (u0 < p.uph) now.load(p, u0, k, false);
   for (int e = threadIdx.x; e < nt * per; e += ROPE_THREADS) {
     const int t = e / per, d = (e - t * per) * 8;
     const _Float16* src = static_cast<const _Float16*>(p.v.x) + (size_t)(t0 + t) * p.v.x_stride + (size_t)h * p.D + d;
@@ -136,18 +148,16 @@ __device__ __forceinline__ void rope_pages(const RopeBatch& p, f32x2* cs, int h,
   }
   rope_angles(p, cs, angles, t0, nt);
   __syncthreads();
-  const int t = threadIdx.x % ROPE_RUN;
-  if (t >= nt) return;
-  const int64_t slot = ldg(p.slots + t0 + t);
-  if (slot < 0 || slot >= p.n_slots) return;
+  if (tk >= nt || slot < 0 || slot >= p.n_slots) return;
   const size_t block = (size_t)((slot / PAGE) * p.KVH + h) * (PAGE * p.D);
   const int at_slot = (int)(slot % PAGE);
   // (a piece of up to 8 values from a multiple of its size lies together in K's page)
-  const _Float16* src = static_cast<const _Float16*>(p.k.x) + (size_t)(t0 + t) * p.k.x_stride + (size_t)h * p.D;
-  for (int u = threadIdx.x / ROPE_RUN; u < p.uph; u += ROPE_THREADS / ROPE_RUN)
-    rope_unit<_Float16, VEC, IL>(p, cs + t * angles, u, src, p.kp + block, [&](int d) { return k_page_elem(at_slot, d, p.D); });
-  for (int d = threadIdx.x / ROPE_RUN; d < p.D; d += ROPE_THREADS / ROPE_RUN)
-    p.vp[block + v_page_elem(at_slot, d)] = turn[t * pitch + d];
+  for (int u = u0; u < p.uph; u += ROPE_THREADS / ROPE_RUN) {
+    if (u + ROPE_THREADS / ROPE_RUN < p.uph) next.load(p, u + ROPE_THREADS / ROPE_RUN, k, false);
+    now.store(p, cs + tk * angles, p.kp + block, [&](int d) { return k_page_elem(at_slot, d, p.D); });
+    now = next;
+  }
+  for (int d = u0; d < p.D; d += ROPE_THREADS / ROPE_RUN) p.vp[block + v_page_elem(at_slot, d)] = turn[tk * pitch + d];
 }
 
 template <typename T, int VEC, bool IL>
@@ -163,17 +173,39 @@ __global__ __launch_bounds__(ROPE_THREADS) void rope_kernel(RopeBatch p) {
     wg -= p.fill;
   }
   const int t0 = wg * p.tok, nt = min(p.tok, p.n - t0);
-  rope_angles(p, cs, p.rot / 2, t0, nt);
-  __syncthreads();
-  for (int e = threadIdx.x; e < nt * p.upt; e += ROPE_THREADS) {
-    const int tl = p.tok == 1 ? 0 : div_by(e, p.upt_div), r = e - tl * p.upt, t = t0 + tl;
+  // a unit's loads are on their way while the angles, then the unit before are worked on (in place too: no unit reads what another writes)
+  struct Place {
+    const T* src;
+    T* dst;
+    int u, tl;
+  };
+  auto place = [&](int e) {
+    const int tl = p.tok == 1 ? 0 : div_by(e, p.upt_div), r = e - tl * p.upt;
     int h = div_by(r, p.uph_div);
     const int u = r - h * p.uph;
     const bool in_q = h < p.q.heads;
     const RopeTensor& x = in_q ? p.q : p.k;
     if (!in_q) h -= p.q.heads;
-    rope_unit<T, VEC, IL>(p, cs + tl * (p.rot / 2), u, static_cast<const T*>(x.x) + (size_t)t * x.x_stride + (size_t)h * p.D,
-                          static_cast<T*>(x.y) + (size_t)t * x.y_stride + (size_t)h * p.D, [](int d) { return d; });
+    const size_t t = t0 + tl;
+    return Place{static_cast<const T*>(x.x) + t * x.x_stride + (size_t)h * p.D, static_cast<T*>(x.y) + t * x.y_stride + (size_t)h * p.D, u, tl};
+  };
+  const int units = nt * p.upt;
+  RopeUnit<T, VEC, IL> now, next;
+  Place here = {}, there = {};
+  if ((int)threadIdx.x < units) {
+    here = place(threadIdx.x);
+    now.load(p, here.u, here.src, here.src == here.dst);
+  }
+  rope_angles(p, cs, p.rot / 2, t0, nt);
+  __syncthreads();
+  for (int e = threadIdx.x; e < units; e += ROPE_THREADS) {
+    if (e + ROPE_THREADS < units) {
+      there = place(e + ROPE_THREADS);
+      next.load(p, there.u, there.src, there.src == there.dst);
+    }
+    now.store(p, cs + here.tl * (p.rot / 2), here.dst, [](int d) { return d; });
+    here = there;
+    now = next;
   }
 }
 
