@@ -9,11 +9,21 @@
 // O^T += V^T P^T; the row sums are a product with ones. Scores, sums and outputs are fp32, P is rounded to fp16 once (V's
 // products take fp16 operands); q is taken as it is, the scale in the exponent's multiply-add (scaled in fp16 it would be rounded).
 //
-// Work: one launch over two kinds of workgroups. Prefix: a KV head, a block of its rows (all sequences' side by side: 16 to 256)
+// Work: one launch over two kinds of workgroups. Prefix: a KV head, a block of its rows (all sequences' side by side: 16 to 128)
 // and a range of prefix pages. Own: a KV head, a sequence, a block of its rows and a range of its pages. Either streams pages
 // through a two-slot ring in LDS by direct-to-LDS loads, one slot ahead; its waves are row waves (every wave all pages of a slot)
 // or, with few rows, page waves (each a page of the slot), whose sums meet in LDS. Partial sums go to the workspace, a second
 // launch adds a row's in split order: no atomics, the same bits every call.
+//
+// What bounds it. Few rows: the chain of launch, table, first pages, sums and second launch (4 rows of 1001 + 37 keys, 4 x 128: 7.1 + 4.1
+// us). A long prefix of 128 rows (8 x 64, 32768 keys and 32 sequences' own): 82 MB fetched in 25.5 us, 3.2 TB/s, ~4 of them before the
+// first page is there. Many rows:
+// issue; 1024 rows x 131072 keys of 8 x 64 take 216-240 us, 720-800 TFLOP/s. A page of 32 rows costs a wave 93 vector
+// instructions beside 18 products of matrix instructions (16 exponentials, 16 multiply-adds, 16 roundings in pairs, 14 maxima,
+// addresses and bookkeeping), which hardly run side by side: matrix cores 41 %, vector units 62 % of the time at a clock of
+// 1.7-2.1 GHz. Measured and not kept there: a third or fourth slot in the ring (229 -> 225 us, shorter calls slower), two pages'
+// softmax at once (237, spills at D = 128), four row blocks a wave, wave priorities, one workgroup of 64 rows instead of two of 32
+// for a sequence's own keys (27.7 -> 27.7 at 36 rows a sequence).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>

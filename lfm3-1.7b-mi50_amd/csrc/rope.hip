@@ -8,10 +8,12 @@
 //
 // Bound by memory: each value is read and written once, in pieces of 16 bytes where sizes and addresses allow (VEC), else value
 // by value. A unit of work is a piece (half layout: the piece and its partner rot / 2 further) or a piece of what is not turned.
+// Measured: 4099 tokens of 16 + 4 heads of 128 in fp32, 84 MB, 13.5 us (6.2 TB/s: partly from the 256 MB cache); 8192 tokens of 16 + 4
+// heads of 128 in fp16 with K and V into pages, 101 MB, 22 us (26 from memory alone, 3.9 TB/s); 8 tokens 3.9 us.
 //
 // Into the pages go workgroups of a KV head and 32 tokens, side by side in the lanes: tokens of a run lie in consecutive slots,
-// which K's operand order keeps 16 bytes apart and V's transposed rows 2, so that a wave's store covers whole lines. V's rows turn
-// in LDS.
+// which K's operand order keeps 16 bytes apart and V's transposed rows 2, so that a wave's store covers whole lines (a token's row
+// after another's 2-byte stores 64 bytes apart: 63 us instead of 22). V's rows turn in LDS.
 #include "batch.h"
 
 #include <algorithm>

@@ -15,7 +15,15 @@
 //                   all tokens down to the bin into the list); the last part finds the cut in the list, then the token. SP_SMALL
 //                   tokens are ranked by comparing all with all, more narrowed to that by a second division of the bin.
 // Rows that need no cut take no histogram but sums by chunks, and one workgroup then the draw. A row whose bin alone passes
-// SP_LIST tokens (a flat one), or whose top-k does with top-p behind it, is finished by one workgroup from the row itself.
+// SP_LIST tokens (a flat one), or whose top-k does with top-p behind it, is finished by one workgroup from the row itself: some
+// fifteen passes of one CU over it (9 rows of 128000 tokens, top-k 5000 with top-p 0.9: 0.88 ms against 0.06 with top-k 3000).
+//
+// What bounds it: few rows, the three launches' chains of dependent reads (one row of 65536 tokens 3.8 + 7.4 + 11.5 us, each beginning
+// with ~2.5 of launch and first load and ending in round trips to memory of ~1 us: arrivals, list, sums, the drawn chunk). Many
+// rows, 64-bit multiply-adds: 256 rows of 128000 fp16 tokens read 65.5 MB three times, 20 us for the maximum (3.4 TB/s), 38 for
+// the histogram, 60-66 for the third launch, most of which is the CUs whose rows keep a third of their tokens: each of those
+// has its weight worked out again. Measured and not kept: the weights of kept tokens alone, one a lane at a time (71 -> 69 us at
+// top-p 0.9); 2048 parts instead of 1024 (mixed settings 61 -> 58 us, top-k 32 -> 37, none 10 -> 16).
 #include <algorithm>
 #include <type_traits>
 
@@ -24,9 +32,14 @@
 
 namespace dspark {
 
-// Tokens of a thread and of a workgroup at a time. The second and third launch have workgroups of 1024 threads: adds of many workgroups to
-// one word go one after the other, some 50 ns each (with workgroups of 256, a word a wave, 9 rows of 128000 tokens 45 us).
+// Tokens of a thread and of a workgroup at a time. The second and third launch have workgroups of 512 threads: adds of many workgroups to
+// one word go one after the other, some 50 ns each (9 rows of 128000 tokens: with 256 threads and a word a wave 45 us a call, with
+// 512 and a word a workgroup 29).
 constexpr int SP_UNIT = 8, SP_MAX_THREADS = 256, SP_THREADS = 512, SP_STEP = SP_THREADS * SP_UNIT;
+// Waves of a SIMD in the second launch, so that four workgroups a CU run at once: left alone the compiler takes over 96 scalar registers,
+// which leaves room for three (256 rows of 128000 tokens 43 -> 38.5 us). The third launch keeps to three: the fourth goes where one is
+// done first, and rows that keep many tokens lie on more CUs (top-p 0.9 71 us, with four at once 87).
+constexpr int SP_WAVES = 8;
 constexpr int SP_CHUNK = 64 * SP_UNIT;
 constexpr int SP_BINS = 2048, SP_LIST = 3584, SP_SMALL = 256, SP_PARTS = 256, SP_CHUNKS = 2048;
 constexpr uint32_t SP_BIN0 = (127 - 9) << 7;  // bin 1 begins at max - z = 2^-9, the last one at 2^7
@@ -299,7 +312,7 @@ __global__ __launch_bounds__(SP_MAX_THREADS) void sample_max_kernel(SampleParams
 }
 
 template <typename T>
-__global__ __launch_bounds__(SP_THREADS) void sample_hist_kernel(SampleParams p) {
+__global__ __launch_bounds__(SP_THREADS, SP_WAVES) void sample_hist_kernel(SampleParams p) {
   __shared__ uint64_t mass[SP_BINS];  // top-p
   uint32_t* const count = reinterpret_cast<uint32_t*>(mass);  // top-k
   __shared__ uint64_t scratch[SP_THREADS / 64];
@@ -912,8 +925,7 @@ __global__ __launch_bounds__(SP_THREADS) void sample_pick_kernel(SampleParams p)
   });
 }
 
-// Parts of a row: up to about 1024 workgroups in the first launch, 2048 in the others (rows differ most in their work there), none of
-// less than a step.
+// Parts of a row: up to about 1024 workgroups in each launch, which all run at once, none of less than a step.
 void sample_plan(SampleParams& p) {
   auto parts = [&](int step, int most, int& n, int& size) {
     const int steps = (p.V + step - 1) / step;
