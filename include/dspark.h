@@ -297,8 +297,8 @@ int dspark_rope_freqs(int32_t rot, double base, int32_t scaling, double factor, 
  * max_tokens, are left as they are in the outputs. Keys that a row does not see may hold anything; where it sees a value of V
  * that is not finite, its output is not finite there. q_start must not decrease; it is cut to
  * [0, tokens], own_len to [0, 32 own_pages]. The prefix's keys are read once for all rows (in groups of up to 128). P is
- * rounded to fp16 once, in the products and their sum alike (lse is good to 2^-11, what weighs less than 2^-32 of the largest
- * weighs nothing); scores, sums and outputs are fp32. The workspace needs no clearing and may be shared by stream-ordered
+ * rounded to fp16 once, for its products with V (what weighs less than 2^-32 of the largest adds nothing there); scores, sums,
+ * lse and outputs are fp32. The workspace needs no clearing and may be shared by stream-ordered
  * calls. What is written shares no byte with anything else (DSPARK_EINVAL). tokens = 0 or seqs = 0 does nothing. */
 typedef struct dspark_shared_attn_args {
   const void* q;               /* fp16 [tokens][q_stride] (head qh at qh D; 16-byte boundary, q_stride a multiple of 8) */

@@ -6,8 +6,9 @@
 // largest score: fp16 then holds weights down to 2^-31 of the largest, and a long tail of keys far below one of them keeps its
 // share (with the reference at the largest itself a weight of 2^-26 is nothing, 2^17 such keys 2^-9 of the whole). Tiles are those
 // of the page format: S^T[keys][rows] = K Q^T, a lane holds one row's scores of eight keys, which in this order are its operand of
-// O^T += V^T P^T; the row sums are a product with ones. Scores, sums and outputs are fp32, P is rounded to fp16 once (V's
-// products take fp16 operands); q is taken as it is, the scale in the exponent's multiply-add (scaled in fp16 it would be rounded).
+// O^T += V^T P^T; row sums are added up before that. Scores, sums and outputs are fp32, P is rounded to fp16 once (V's
+// products take fp16 operands; sums of the rounded P by a product with ones cost lse its digits past 2^-11, and a long call 229 us
+// instead of 224); q is taken as it is, the scale in the exponent's multiply-add (scaled in fp16 it would be rounded).
 //
 // Work: one launch over two kinds of workgroups. Prefix: a KV head, a block of its rows (all sequences' side by side: 16 to 128)
 // and a range of prefix pages. Own: a KV head, a sequence, a block of its rows and a range of its pages. Either streams pages
@@ -16,11 +17,11 @@
 // launch adds a row's in split order: no atomics, the same bits every call.
 //
 // What bounds it. Few rows: the chain of launch, table, first pages, sums and second launch (4 rows of 1001 + 37 keys, 4 x 128: 7.1 + 4.1
-// us). A long prefix of 128 rows (8 x 64, 32768 keys and 32 sequences' own): 82 MB fetched in 25.5 us, 3.2 TB/s, ~4 of them before the
+// us). A long prefix of 128 rows (8 x 64, 32768 keys and 32 sequences' own): 82 MB fetched in 26 us, 3.2 TB/s, ~4 of them before the
 // first page is there. Many rows:
-// issue; 1024 rows x 131072 keys of 8 x 64 take 216-240 us, 720-800 TFLOP/s. A page of 32 rows costs a wave 93 vector
-// instructions beside 18 products of matrix instructions (16 exponentials, 16 multiply-adds, 16 roundings in pairs, 14 maxima,
-// addresses and bookkeeping), which hardly run side by side: matrix cores 41 %, vector units 62 % of the time at a clock of
+// issue; 1024 rows x 131072 keys of 8 x 64 take 212-235 us, 740-810 TFLOP/s. A page of 32 rows costs a wave some 110 vector
+// instructions beside 16 products of matrix instructions (16 exponentials, multiply-adds, additions, 14 maxima, 16 roundings,
+// addresses and bookkeeping), which hardly run side by side: matrix cores 36 %, vector units 68 % of the time at a clock of
 // 1.7-2.1 GHz. Measured and not kept there: a third or fourth slot in the ring (229 -> 225 us, shorter calls slower), two pages'
 // softmax at once (237, spills at D = 128), four row blocks a wave, wave priorities, one workgroup of 64 rows instead of two of 32
 // for a sequence's own keys (27.7 -> 27.7 at 36 rows a sequence).
@@ -55,7 +56,7 @@ struct SaMask {
 template <int D, int QB>
 struct SaState {
   f32x4 o[QB][D / 16];
-  f32x4 l[QB];
+  float l[QB];    // of the lane's keys: a row's four lanes add theirs at the end (sa_sum)
   float m[QB];    // reference in log2 units, 0 before the row's first key
   float thr[QB];  // an exponent above this moves it: TAU, -inf before the first key
 };
@@ -135,9 +136,15 @@ __device__ __forceinline__ void sa_softmax(f32x4 (&s)[QB][2], int key0, const Sa
   for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      pp[qb][i] = (_Float16)fast_exp2(s[qb][0][i]);
-      pp[qb][4 + i] = (_Float16)fast_exp2(s[qb][1][i]);
+      const float e0 = fast_exp2(s[qb][0][i]), e1 = fast_exp2(s[qb][1][i]);
+      st.l[qb] += e0 + e1;
+      pp[qb][i] = (_Float16)e0;
+      pp[qb][4 + i] = (_Float16)e1;
     }
+}
+__device__ __forceinline__ float sa_sum(float l) {
+  l += __shfl_xor(l, 16);
+  return l + __shfl_xor(l, 32);
 }
 
 // V's operands of a page in LDS.
@@ -146,7 +153,7 @@ __device__ __forceinline__ void sa_v(const char* vt, u32x4 (&v)[D / 16], int lan
 #pragma unroll
   for (int cc = 0; cc < D / 16; ++cc) v[cc] = *reinterpret_cast<const u32x4*>(vt + cc * 1024 + lane * 16);
 }
-// O^T += V^T P^T and the row sums. On an edge page, where some row does not see some key, a value of V that is not finite would spoil
+// O^T += V^T P^T. On an edge page, where some row does not see some key, a value of V that is not finite would spoil
 // every row (0 x inf): it counts as zero in the product, and afterwards the rows that do see one get an infinity: a product of
 // where it stands with which keys they see, times 2^254.
 template <int D, int QB>
@@ -160,9 +167,6 @@ __device__ __forceinline__ void sa_values(const char* vt, u32x4 (&v)[D / 16], in
       for (int i = 0; i < 4; ++i)  // two halves a word
         v[cc][i] &= ((v[cc][i] & 0x7c00u) == 0x7c00u ? 0u : 0xffffu) | ((v[cc][i] & 0x7c000000u) == 0x7c000000u ? 0u : 0xffff0000u);
   }
-  const half8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
-#pragma unroll
-  for (int qb = 0; qb < QB; ++qb) st.l[qb] = mfma16x16x32(ones, pp[qb], st.l[qb]);
 #pragma unroll
   for (int cc = 0; cc < D / 16; ++cc)
 #pragma unroll
@@ -241,7 +245,7 @@ __device__ __forceinline__ void sa_begin(const SharedAttn& p, const SaWork& w, i
     mk.full_hi = __builtin_amdgcn_readfirstlane(mk.full_hi);
 #pragma unroll
     for (int cc = 0; cc < D / 16; ++cc) st.o[qb][cc] = f32x4{0, 0, 0, 0};
-    st.l[qb] = f32x4{0, 0, 0, 0};
+    st.l[qb] = 0.f;
     st.m[qb] = 0.f;
     st.thr[qb] = -INFINITY;
   }
@@ -312,9 +316,9 @@ __device__ __forceinline__ void sa_run_rows(const SharedAttn& p, char (&lds0)[sa
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
     const int row = wrow + 16 * qb + n;
-    if (row >= w.rows) continue;
     const size_t at = (out0 + row) * S + w.split;
-    const float l = st.l[qb][0];
+    const float l = sa_sum(st.l[qb]);
+    if (row >= w.rows) continue;
     if (g == 0) p.part_ml[at] = f32x2{l != 0.f ? st.m[qb] : -INFINITY, l};
     if (l != 0.f) {
       f32x4* dst = reinterpret_cast<f32x4*>(p.part_o + at * D);
@@ -389,9 +393,10 @@ __device__ __forceinline__ void sa_run_pages(const SharedAttn& p, char (&lds0)[s
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
     const int r = 16 * qb + n;
+    const float l = sa_sum(st.l[qb]);
     if (g == 0) {
       sm_m[wave][r] = st.thr[qb] == SA_TAU ? st.m[qb] : -1e30f;  // (no key: a reference below all others)
-      sm_l[wave][r] = st.l[qb][0];
+      sm_l[wave][r] = l;
     }
 #pragma unroll
     for (int cc = 0; cc < D / 16; ++cc) sums(wave)[r * (D / 4) + ((4 * cc + g) ^ n)] = st.o[qb][cc];

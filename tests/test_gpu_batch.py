@@ -247,7 +247,7 @@ class Batch:
         return out, f32, lse
 
     def close(self, out, f32, lse, want, wlse, size):
-        """P is rounded to fp16: each weight is off by 2^-11 of itself, in the sum and in the products alike, so an output moves by at most
+        """P is rounded to fp16: each weight is off by 2^-11 of itself in the products (were it in the sum too), so an output moves by at most
         2 x 2^-11 max |v|; a P below 2^-14 by 2^-25, of sums of at least 1, over all n keys: n 2^-25 (1 + max |v|), the one among
         the subnormals. Scores: D products of fp16 values, exact, summed in fp32: D roundings of 2^-24 of at most sum |q_i k_i|, which
         is under 2 D here (1.5 x 2 / pi D on average), over sqrt(D); the exponent's own rounding 2^-22. The gate's and the sums' own roundings are under 2^-20."""
@@ -371,6 +371,17 @@ def test_shared_growing_and_falling_scores(D, seqs):
     score = 6 * 2 * D ** 1.5 * 2.0 ** -24 + 2.0 ** -19
     assert np.all(np.abs(f64(f32) - want) <= ((2.0 ** -10 + 2 * score) * top + 740 * 2.0 ** -25 * (1 + top))[..., None])
     assert np.all(np.abs(f64(lse) - wlse) <= 2.0 ** -11 + score + 740 * 2.0 ** -25 + 2.0 ** -22 * np.abs(wlse))
+
+
+@pytest.mark.parametrize("D,seqs", [(64, 1), (128, 1), (64, 20), (128, 20), (64, 70)])
+def test_shared_lse(D, seqs):
+    """lse is of the weights before they are rounded: scores and exponents as in Batch.close, n / 4 additions a lane and a logarithm."""
+    b = Batch(seqs + D, 8, 2, D, 999, [2] * seqs, list(range(2, 2 + seqs)))
+    _, _, lse = b.run()
+    _, want, _ = b.oracle()
+    n = 999 + 2 + seqs
+    score = 2 * D ** 1.5 * 2.0 ** -24 + 2.0 ** -22
+    assert np.all(np.abs(f64(lse) - want) <= score + (n / 4 + 64) * 2.0 ** -24 + 2.0 ** -22 * np.abs(want))
 
 
 @pytest.mark.parametrize("seqs", [1, 20])
