@@ -15,8 +15,9 @@
 //                   all tokens down to the bin into the list); the last part finds the cut in the list, then the token. SP_SMALL
 //                   tokens are ranked by comparing all with all, more narrowed to that by a second division of the bin.
 // Rows that need no cut take no histogram but sums by chunks, and one workgroup then the draw. A row whose bin alone passes
-// SP_LIST tokens (a flat one), or whose top-k does with top-p behind it, is finished by one workgroup from the row itself: some
-// fifteen passes of one CU over it (9 rows of 128000 tokens, top-k 5000 with top-p 0.9: 0.88 ms against 0.06 with top-k 3000).
+// SP_LIST tokens (equal logits by thousands, as bfloat16 has far from zero) takes two passes of one workgroup more (sp_crowded: 9 rows
+// of 128000 tokens around 40, top-p 0.9, 0.57 -> 0.12 ms). One whose top-k passes a list with top-p behind it is finished by one
+// workgroup from the row itself, some fifteen passes (the same rows, top-k 5000 with top-p 0.9: 0.88 ms against 0.06 with top-k 3000).
 //
 // What bounds it: few rows, the three launches' chains of dependent reads (one row of 65536 tokens 3.8 + 7.4 + 11.5 us, each beginning
 // with ~2.5 of launch and first load and ending in round trips to memory of ~1 us: arrivals, list, sums, the drawn chunk). Many
@@ -446,7 +447,7 @@ __global__ __launch_bounds__(SP_THREADS, SP_WAVES) void sample_hist_kernel(Sampl
       r.above = before;
       const uint64_t to = before + n[i];
       // (top-p behind a top-k of more than a list's tokens: its part of the whole is of what top-k leaves)
-      r.mode = !by_k || (s.p >= 1.f && to > SP_SMALL && n[i] <= SP_LIST) ? SP_BELOW : to <= (s.p < 1.f ? SP_LIST : SP_SMALL) ? SP_LISTED : SP_ROW;
+      r.mode = !by_k || (s.p >= 1.f && to > SP_SMALL) ? SP_BELOW : to <= (s.p < 1.f ? SP_LIST : SP_SMALL) ? SP_LISTED : SP_ROW;
       p.result[row] = r;
     }
     before += n[i];
@@ -798,6 +799,177 @@ __device__ __forceinline__ void sp_draw_chunk(const SampleParams& p, int row, co
   }
 }
 
+// A row whose bin, max - z from d0 to d1, holds more tokens than a list (`sums`: the kept weight above the bin by chunks, of `kept`
+// tokens): the bin in 1024 parts, one pass to find the cut's part and one to list it. A part of more tokens than a list are equal
+// logits in all likelihood (bfloat16 has 33 values between 32 and 40): then their numbers by chunks say which is the last one kept.
+// False if they are not, or the bin is the last.
+constexpr int SP_SUB = 1024;
+static_assert(SP_SUB * 12 <= SP_LIST * 8 && SP_CHUNKS * 4 <= SP_LIST * 8, "in the list's place");
+template <typename T>
+__device__ __forceinline__ bool sp_crowded(const SampleParams& p, int row, const T* z0, const SampleRow& r, float d0, float d1, uint64_t* list,
+                                           uint64_t* sums, uint64_t kept, SampleShared& sh) {
+  if (!(d1 < INFINITY)) return false;
+  const SampleLocals& s = r.s;
+  const bool by_mass = r.by_mass != 0;
+  const int lane = threadIdx.x & 63;
+  const float scale = SP_SUB / (d1 - d0);
+  auto of = [&](float d) { return (int)fminf(fmaxf((d - d0) * scale, 0.f), SP_SUB - 1.f); };
+  uint32_t* const count = reinterpret_cast<uint32_t*>(list + SP_SUB);
+  for (int i = threadIdx.x; i < SP_SUB; i += SP_THREADS) list[i] = count[i] = 0;
+  __syncthreads();
+  sp_units<T>(z0, 0, p.V, p.wide, [&](int, const SampleUnit<T>& x) {
+    float z[SP_UNIT];
+    x.values(z);
+#pragma unroll
+    for (int i = 0; i < SP_UNIT; ++i) {
+      const float d = s.m - z[i];
+      if (!(d >= d0 && d < d1)) continue;
+      const int b = of(d);
+      atomicAdd(&count[b], 1u);
+      if (by_mass) sp_add(&list[b], sp_weight_finite(z[i], s));
+    }
+  });
+  __syncthreads();
+  constexpr int EACH = SP_SUB / SP_THREADS;
+  uint64_t n[EACH], ns = 0, total;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int b = threadIdx.x * EACH + i;
+    n[i] = by_mass ? list[b] : count[b];
+    ns += n[i];
+  }
+  if (threadIdx.x == 0) sh.found = sh.number = 0;
+  uint64_t front = r.above + block_scan_u64(ns, sh.scratch, &total) - ns;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    if (front < r.limit && front + n[i] >= r.limit) {  // (one thread, one part)
+      sh.digit = threadIdx.x * EACH + i;
+      sh.count[0] = count[threadIdx.x * EACH + i];
+      sh.c = front;
+      sh.found = 1;
+    }
+    front += n[i];
+  }
+  __syncthreads();
+  const bool found = sh.found != 0;
+  const int part = (int)sh.digit, size = (int)sh.count[0];
+  const bool alike = size > SP_LIST;
+  uint32_t* const number = reinterpret_cast<uint32_t*>(list);  // (alike) by chunks
+  front = sh.c;
+  __syncthreads();
+  if (!found) return false;  // (the same in every thread)
+  if (threadIdx.x == 0) sh.digit = 0, sh.found = 0xffffffffu;
+  __syncthreads();
+  uint32_t over = 0, any = 0, every = 0xffffffffu;
+  sp_units<T>(z0, 0, p.V, p.wide, [&](int at, const SampleUnit<T>& x) {
+    float z[SP_UNIT];
+    x.values(z);
+    uint64_t sum = 0;
+    uint32_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < SP_UNIT; ++i) {
+      const float d = s.m - z[i];
+      if (!(d >= d0 && d < d1)) continue;
+      const int b = of(d);
+      if (b < part && sp_high(z[i], s)) {
+        sum += sp_weight_finite(z[i], s);
+        ++over;
+      }
+      if (b != part) continue;
+      ++mine;
+      if (alike) {
+        any |= argmax_ord(z[i]);
+        every &= argmax_ord(z[i]);
+      } else {
+        const uint32_t to = atomicAdd(&sh.number, 1u);
+        if (to < SP_LIST) list[to] = argmax_key(z[i], (uint32_t)(at + i));
+      }
+    }
+    sum = wave_sum_u64(sum);
+    const uint64_t here = alike ? wave_sum_u64(mine) : 0;
+    if (lane == 0) {
+      sums[at / SP_CHUNK] += sum;
+      if (alike) number[at / SP_CHUNK] = (uint32_t)here;
+    }
+  });
+  kept += block_sum_u64(over, sh.scratch);  // (a barrier too)
+  SampleCut cut = {0, 0xffffffffu};
+  if (!alike) {
+    const SampleList it = {list, size};
+    if (size <= SP_SMALL)
+      cut = sp_rank(it, s, sh, by_mass, r.limit, front);
+    else
+      sp_shrink(it, s, sh, cut, by_mass, r.limit, front, front);
+    __syncthreads();
+    uint64_t more = 0;
+    it.each([&](uint32_t i, float z) {
+      if (!cut.keeps(argmax_ord(z), i) || !sp_high(z, s)) return;
+      sp_add(&sums[i / SP_CHUNK], sp_weight(z, s));
+      ++more;
+    });
+    kept += block_sum_u64(more, sh.scratch);
+  } else {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      any |= __shfl_xor(any, d);
+      every &= __shfl_xor(every, d);
+    }
+    if (lane == 0) {
+      atomicOr(&sh.digit, any);
+      atomicAnd(&sh.found, every);
+    }
+    __syncthreads();
+    cut.key = sh.digit;
+    const bool differ = sh.found != cut.key;
+    __syncthreads();
+    if (differ) return false;
+    const float z = sp_logit(cut.key);
+    const uint64_t w = sp_weight(z, s), one = by_mass ? max(w, (uint64_t)1) : 1;
+    const uint64_t m = min((r.limit - front + one - 1) / one, (uint64_t)size);  // so many of them, by index
+    const bool high = sp_high(z, s);
+    constexpr int OF = SP_CHUNKS / SP_THREADS;
+    uint64_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < OF; ++i) {
+      const int c = threadIdx.x * OF + i;
+      mine += c < p.chunks ? number[c] : 0;
+    }
+    uint64_t before = block_scan_u64(mine, sh.scratch, &total) - mine;
+#pragma unroll
+    for (int i = 0; i < OF; ++i) {
+      const int c = threadIdx.x * OF + i;
+      const uint64_t k = c < p.chunks ? number[c] : 0, take = min(k, m - min(m, before));
+      if (high && take) sums[c] += take * w;
+      if (before < m && before + k >= m) {  // (one thread, one chunk)
+        sh.at = c;
+        sh.number = (uint32_t)(m - before);
+      }
+      before += k;
+    }
+    __syncthreads();
+    if (threadIdx.x < 64) {  // the last one kept within its chunk
+      const int at = (int)sh.at * SP_CHUNK + lane * SP_UNIT;
+      SampleUnit<T> x;
+      float v[SP_UNIT];
+      uint32_t equal = 0;
+      x.load(z0, at, p.V, p.wide);
+      x.values(v);
+#pragma unroll
+      for (int i = 0; i < SP_UNIT; ++i) equal |= v[i] == z ? 1u << i : 0u;
+      uint32_t rank = (uint32_t)wave_scan_u64(__popc(equal)) - __popc(equal);
+#pragma unroll
+      for (int i = 0; i < SP_UNIT; ++i)
+        if (equal >> i & 1 && ++rank == sh.number) sh.digit = at + i;
+    }
+    __syncthreads();
+    cut.idx = sh.digit;
+    kept += high ? m : 0;
+    __syncthreads();
+  }
+  sp_draw_chunk<T>(p, row, z0, sums, kept, r, sh, [&](uint32_t i, float z) { return cut.keeps(argmax_ord(z), i); });
+  return true;
+}
+
 template <typename T>
 __global__ __launch_bounds__(SP_THREADS) void sample_pick_kernel(SampleParams p) {
   __shared__ uint64_t list[SP_LIST];
@@ -887,8 +1059,8 @@ __global__ __launch_bounds__(SP_THREADS) void sample_pick_kernel(SampleParams p)
   if (!listed)
     for (int c = threadIdx.x; c < p.chunks; c += SP_THREADS) sums[c] = sp_get(p.chunk_sum + (size_t)row * p.chunks + c);
   const int n = (int)(uint32_t)taken;
-  if (n > SP_LIST) {  // (top-p's bin: only its weight was known)
-    sp_finish(p, row, SampleWhole<T>{z0, p.V, p.wide != 0}, r, sh);
+  if (n > SP_LIST) {
+    if (!sp_crowded<T>(p, row, z0, r, r.bin ? inner : 0.f, edge, list, sums, taken >> 32, sh)) sp_finish(p, row, SampleWhole<T>{z0, p.V, p.wide != 0}, r, sh);
     return;
   }
   const uint64_t first = sp_get(p.list + (size_t)row * SP_LIST + threadIdx.x);  // (there or not: asked for along with their number)

@@ -593,6 +593,29 @@ def test_sample_wide_nuclei(kind):
         sample_check(logits, U, **how)
 
 
+@pytest.mark.parametrize("kind,V,values", [("bf16", 128001, "coarse"), ("f16", 60000, "coarse"), ("f32", 200003, "normal"), ("f32", 262144, "narrow"),
+                                           ("f32", 30011, "close"), ("f32", 30011, "ends")])
+def test_sample_crowded_bins(kind, V, values):
+    """Cuts within a bin of more tokens than a list: equal logits by thousands (far from zero, coarse types), many different ones, pairs of
+    values closer than the bin's parts, and whole rows of one value with a few above and below."""
+    rng = np.random.default_rng(V)
+    n = len(U)
+    if values == "coarse":
+        z = 40 + 2 * rng.standard_normal((n, V))
+    elif values == "normal":
+        z = 1.2 * rng.standard_normal((n, V)) + 7.0 * (rng.random((n, V)) < 1e-4)
+    elif values == "narrow":
+        z = -3 + 0.01 * rng.random((n, V)) + 3.0 * (rng.random((n, V)) < 1e-5)
+    elif values == "close":
+        z = -0.5 + 1e-6 * rng.integers(0, 2, (n, V)) + 0.5 * (np.arange(V) == 777)
+    else:
+        z = np.where(np.arange(V) % 997 == 5, 2.0, np.where(np.arange(V) % 991 == 7, -2.0, 0.0)) * np.ones((n, 1))
+    logits = rows_of(kind, z)
+    for how in (dict(p=0.3), dict(p=0.6), dict(p=0.9), dict(p=0.97, t=1.3), dict(p=0.99, low=0.3), dict(p=0.5, low=0.9), dict(k=50), dict(k=5000),
+                dict(k=V // 2), dict(k=V // 2, low=0.2), dict(k=V - 9)):
+        sample_check(logits, U, **how)
+
+
 @pytest.mark.parametrize("kind", sorted(TYPES))
 def test_sample_special_values(kind):
     inf, nan = math.inf, math.nan
