@@ -18,8 +18,7 @@
 //
 // What bounds it. Few rows: the chain of launch, table, first pages, sums and second launch (4 rows of 1001 + 37 keys, 4 x 128: 7.1 + 4.1
 // us). A long prefix of 128 rows (8 x 64, 32768 keys and 32 sequences' own): 82 MB fetched in 26 us, 3.2 TB/s, ~4 of them before the
-// first page is there. Many rows:
-// issue; 1024 rows x 131072 keys of 8 x 64 take 212-235 us, 740-810 TFLOP/s. A page of 32 rows costs a wave some 110 vector
+// first page is there. Many rows: issue; 1024 rows x 131072 keys of 8 x 64 take 212-235 us, 740-810 TFLOP/s. A page of 32 rows costs a wave some 110 vector
 // instructions beside 16 products of matrix instructions (16 exponentials, multiply-adds, additions, 14 maxima, 16 roundings,
 // addresses and bookkeeping), which hardly run side by side: matrix cores 36 %, vector units 68 % of the time at a clock of
 // 1.7-2.1 GHz. Measured and not kept there: a third or fourth slot in the ring (229 -> 225 us, shorter calls slower), two pages'
