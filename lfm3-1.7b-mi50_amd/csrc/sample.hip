@@ -566,12 +566,15 @@ __device__ __forceinline__ bool sp_descend(const Items& it, const SampleLocals& 
       sh.found = 1;
     }
     __syncthreads();
-    if (!sh.found) return false;
-    prefix = (prefix & ~mask) | (sh.digit << shift & mask);
-    c = sh.c;
-    w = sh.w;
+    const bool found = sh.found != 0;
+    const uint32_t at = sh.digit;
+    const uint64_t c0 = sh.c, w0 = sh.w;
+    __syncthreads();  // (read by every wave before any of them goes on, or back to the caller)
+    if (!found) return false;
+    prefix = (prefix & ~mask) | (at << shift & mask);
+    c = c0;
+    w = w0;
     hi = shift;
-    __syncthreads();
   } while (hi > lo);
   key = prefix;
   return true;
@@ -715,7 +718,9 @@ __device__ __forceinline__ bool sp_narrow(const SampleList& it, const SampleLoca
   }
   __syncthreads();
   const int bin = (int)sh.digit;
-  if (sh.count[bin] > SP_SMALL) return false;
+  const uint32_t size = sh.count[bin];
+  __syncthreads();  // (read by every wave before one goes back to the caller, whose next helper clears sh.digit)
+  if (size > SP_SMALL) return false;
   it.each([&](uint32_t i, float z) {
     if (of(z) != bin) return;
     const uint32_t to = atomicAdd(&sh.number, 1u);

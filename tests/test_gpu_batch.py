@@ -617,6 +617,23 @@ def test_sample_crowded_bins(kind, V, values):
 
 
 @pytest.mark.parametrize("kind", sorted(TYPES))
+@pytest.mark.parametrize("ties", [257, 700, 2000, 3500])
+def test_sample_ties_that_no_division_of_a_bin_parts(kind, ties):
+    """A list of more than 256 tokens of which one 256th of the bin holds more than 256 as well, a few in the part before it: the cut by
+    digits. Many rows, so that the waves of many workgroups come there at all kinds of times."""
+    rng = np.random.default_rng(ties)
+    n, V = 96, 9001
+    z = np.full((n, V), -30.0)
+    for r in range(n):
+        at = rng.permutation(V)
+        z[r, at[0]], z[r, at[1:11]], z[r, at[11:11 + ties]] = 0.0, -2.0, -2.0 if kind == "bf16" else -2.0 - 2.0 ** -7
+    logits, u = rows_of(kind, z), rng.random(n)
+    for how in (dict(p=0.5), dict(p=0.9, low=0.01), dict(p=rng.uniform(0.3, 0.95, n)), dict(k=20 + ties // 2), dict(k=rng.integers(12, 10 + ties, n)),
+                dict(k=ties, p=0.6)):
+        sample_check(logits, u, **how)
+
+
+@pytest.mark.parametrize("kind", sorted(TYPES))
 def test_sample_special_values(kind):
     inf, nan = math.inf, math.nan
     big = float(torch.finfo(TYPES[kind]).max)

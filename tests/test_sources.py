@@ -19,3 +19,26 @@ def test_barriers_are_fenced(name):
         body = text[text.index("ring_barrier()"):]
         assert re.search(r's_waitcnt\(vmcnt_imm\(N\) & ~0x0F00\);\s*asm volatile\("" ::: "memory"\);\s*'
                          r'__builtin_amdgcn_s_barrier\(\);\s*asm volatile\("" ::: "memory"\);', body)
+
+
+def helpers(text, param):
+    """Bodies of the device functions that take `param`, by name."""
+    for at in re.finditer(r"\b(\w+)\(([^()]*\b%s[^()]*)\) \{\n" % re.escape(param), text):
+        depth, end = 1, at.end()
+        while depth:
+            depth += {"{": 1, "}": -1}.get(text[end], 0)
+            end += 1
+        yield at.group(1), text[at.end():end]
+
+
+def test_sampling_helpers_return_behind_a_barrier():
+    """What a wave reads of the words that the sampler's helpers share it has read before any wave returns: the caller's next helper writes
+    the same words at once (a wave that is late would take another way through the barriers than the rest)."""
+    text = re.sub(r"//[^\n]*", "", open(os.path.join(CSRC, "sample.hip")).read())
+    seen = 0
+    for name, body in helpers(text, "SampleShared& sh"):
+        for at in re.finditer(r"return false;", body):
+            seen += 1
+            since = body[:at.start()].rsplit("__syncthreads();", 1)[-1]
+            assert not re.search(r"\bsh\.", since), (name, since)
+    assert seen >= 5
