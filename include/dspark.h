@@ -334,7 +334,7 @@ int dspark_verify_attention_shared(const dspark_shared_attn_args* args, dspark_s
  *   the first always), and z_i >= max z + T ln(min_p) (min_p <= 0: all);
  * the token is the first kept one, by index, at which the kept weights' running sum exceeds u times their whole sum. T <= 0 is
  * greedy: the first maximum. NaN and -inf are never drawn; +inf shares the weight with the other +inf alone. A row with
- * nothing to draw gives token -1, kept 0, logprob -inf, key 0. Weights are fixed-point numbers of 44 bits behind the point and their
+ * nothing to draw gives token -1, kept 0, logprob -inf, key 0. Weights are whole numbers, the largest 2^44 - 2^24, and their
  * sums whole 64-bit ones, so a draw does not depend on the order of the work: the same inputs give the same token always.
  * keys are what dspark_accept_commit takes: the round of drafts that agree with their row's draw is accepted. For drafts that are
  * chosen without randomness, as the drafter's are, that is speculative sampling exactly: a draft is accepted with its

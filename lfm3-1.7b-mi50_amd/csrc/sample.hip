@@ -1,10 +1,10 @@
 // Sampling a token from each row of logits: temperature, top-k, top-p, min-p and a given random number (include/dspark.h).
 //
-// A token's weight exp((z - max) / T) is a fixed-point number w = rint(2^44 exp(..)), computed in 64 bits, so that every sum of
-// weights is a whole number whatever the order it is taken in: histograms by atomic adds, partial sums of workgroups and the
-// draw itself give the same bits always, and sums of 2^20 weights stay under 2^64. (Sums of fp32 weights move the borders
-// between tokens by 2^-24 of the whole, more than most of a vocabulary's tokens have; one draw in a thousand then falls to
-// another token than the definition's.)
+// A token's weight exp((z - max) / T) is a whole number w = rint((2^44 - 2^24) exp(..)), computed in 64 bits, so that every sum of
+// weights is one too whatever the order it is taken in: histograms by atomic adds, partial sums of workgroups and the
+// draw itself give the same bits always, and sums of 2^20 weights, the longest row, reach 2^64 - 2^44 at most. (Sums of fp32
+// weights move the borders between tokens by 2^-24 of the whole, more than most of a vocabulary's tokens have; one draw in a
+// thousand then falls to another token than the definition's.)
 //
 // Top-k and top-p both keep a prefix of the tokens ranked by (z descending, index), min-p one by z alone: what is kept is
 // "key above key*, or equal to it and index up to idx*" and z at least the min-p bound. The cut is found without sorting:
@@ -43,6 +43,7 @@ constexpr int SP_UNIT = 8, SP_MAX_THREADS = 256, SP_THREADS = 512, SP_STEP = SP_
 constexpr int SP_WAVES = 8;
 constexpr int SP_CHUNK = 64 * SP_UNIT;
 constexpr int SP_BINS = 2048, SP_LIST = 3584, SP_SMALL = 256, SP_PARTS = 256, SP_CHUNKS = 2048;
+constexpr uint64_t SP_ONE = ((uint64_t)1 << 44) - ((uint64_t)1 << 24);  // the largest weight: 2^20 of them are under 2^64
 constexpr uint32_t SP_BIN0 = (127 - 9) << 7;  // bin 1 begins at max - z = 2^-9, the last one at 2^7
 
 enum : uint32_t { SP_EMPTY, SP_GREEDY, SP_ALL, SP_LISTED, SP_BELOW, SP_ROW };
@@ -109,27 +110,28 @@ __device__ __forceinline__ double sp_fma(double a, double b, double c) {
   asm("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "s"(c));
   return d;
 }
-// 2^44 exp((z - m) / T) as a whole number, m finite: 2^x by its whole part and a polynomial of 2^f, |f| <= 1/2, of degree 10 (through
-// the Chebyshev nodes; off by 2^-51). -inf and NaN weigh nothing: they end as x = -46, a quarter of a unit.
+// (2^44 - 2^24) exp((z - m) / T) as a whole number, m finite: 2^x by its whole part and a polynomial of (1 - 2^-20) 2^f, |f| <= 1/2, of
+// degree 10 (through the Chebyshev nodes; off by 2^-51; its first term is exact: a token at the maximum weighs SP_ONE). -inf and NaN
+// weigh nothing: they end as x = -46, a quarter of a unit.
 __device__ __forceinline__ uint64_t sp_weight_finite(float z, const SampleLocals& s) {
   const double x = fmax(((double)z - (double)s.m) * s.inv_t2, -46.0);
   const double k = rint(x), f = x - k;
-  double e = sp_fma(f, 7.072585949269223e-09, 1.0208690299958306e-07);
-  e = sp_fma(e, f, 1.321544258792169e-06);
-  e = sp_fma(e, f, 1.5252657260200837e-05);
-  e = sp_fma(e, f, 0.0001540353044173605);
-  e = sp_fma(e, f, 0.0013333558230164974);
-  e = sp_fma(e, f, 0.009618129107606888);
-  e = sp_fma(e, f, 0.05550410866444772);
-  e = sp_fma(e, f, 0.24022650695910097);
-  e = sp_fma(e, f, 0.69314718055995);
-  e = fma(e, f, 1.0);
+  double e = sp_fma(f, 7.072579204325653e-09, 1.0208680564192563e-07);
+  e = sp_fma(e, f, 1.3215429984693514e-06);
+  e = sp_fma(e, f, 1.5252642714133351e-05);
+  e = sp_fma(e, f, 0.00015403515751784687);
+  e = sp_fma(e, f, 0.0013333545514292945);
+  e = sp_fma(e, f, 0.009618119935044186);
+  e = sp_fma(e, f, 0.055504055731604836);
+  e = sp_fma(e, f, 0.24022627786125117);
+  e = sp_fma(e, f, 0.6931465195232863);
+  e = sp_fma(e, f, 1.0 - 0x1p-20);
   // in units of one and rounded to a whole number by the unit of 2^52
   const double y = __builtin_ldexp(e, (int)k + 44) + 4503599627370496.0;
   return (uint64_t)__double_as_longlong(y) & 0xfffffffffffffull;
 }
 __device__ __forceinline__ uint64_t sp_weight(float z, const SampleLocals& s) {
-  if (s.inf) return z == INFINITY ? (uint64_t)1 << 44 : 0;
+  if (s.inf) return z == INFINITY ? SP_ONE : 0;
   return sp_weight_finite(z, s);
 }
 __device__ __forceinline__ bool sp_high(float z, const SampleLocals& s) {  // min-p

@@ -646,6 +646,23 @@ def test_sample_special_values(kind):
     sample_check(rows_of(kind, rows), [nan, -1.0, 1.0, 2.0, inf, -inf, 0.5, 0.5, 0.5, 0.5, 0.5])
 
 
+@pytest.mark.parametrize("kind", sorted(TYPES))
+@pytest.mark.parametrize("V", [(1 << 20) - 1, 1 << 20])
+def test_sample_the_largest_rows(kind, V):
+    """2^20 tokens of the largest weight each, by every way through the launches: their sum has to fit. Flat rows, an infinite temperature
+    and rows of infinities; one token above all others; ordinary values."""
+    rng = np.random.default_rng(V)
+    u = [0.0, 0.03, 0.5, 0.9999, U[-1]]
+    flat = rows_of(kind, np.zeros((len(u), V)))
+    for how in (dict(), dict(p=0.9), dict(p=1e-6), dict(low=0.5), dict(k=V - 1), dict(k=700000, p=0.5), dict(k=300), dict(t=math.inf, p=0.999)):
+        sample_check(flat, u, **how)
+    sample_check(rows_of(kind, np.full((len(u), V), math.inf)), u)
+    sample_check(rows_of(kind, np.full((len(u), V), math.inf)), u, p=0.9)
+    logits = rows_of(kind, rng.standard_normal((len(u), V)))
+    for how in (dict(), dict(p=0.9), dict(t=math.inf), dict(k=40, p=0.9)):
+        sample_check(logits, u, **how)
+
+
 @pytest.mark.parametrize("n", [1, 3, 700, 5000])
 def test_sample_rows(n):
     """One row to thousands, rows inside wider ones and off 16-byte boundaries."""
