@@ -375,11 +375,14 @@ size_t dspark_verify_argmax_workspace(int32_t M, int32_t V);
 /* ---------------------------------------------------------------- acceptance + commit
  * On the device State: acc = longest prefix with token(best[i]) == tokens[i+1]; emit drafts[1..acc] and the bonus
  * token(best[acc]) to out_tokens[count..]; mark them in seen; advance a by acc+1; update counters, skip/miss and run
- * exactly as dspark.hip:2848-2913. `skip_now` is the round's skip flag. The KV rows of positions a..a+acc are already
- * in the pages (dspark_kv_write before attention), so the commit moves no K/V. */
+ * exactly as dspark.hip:2848-2913. A key without a token (token(key) < 0: key 0, of a row with nothing to draw) agrees
+ * with no draft; as best[acc] it ends the commit before it: drafts[1..acc] alone are emitted and marked, a advances by
+ * acc, the anchor (and tokens[0]) is tokens[acc], whose position a is the next round's first, ctx_new = acc, and
+ * run = 0. `skip_now` is the round's skip flag. The KV rows of positions a..a+acc are already in the pages
+ * (dspark_kv_write before attention), so the commit moves no K/V. */
 int dspark_accept_commit(dspark_state* st, const uint64_t* best_keys, int32_t M, int32_t skip_now, int32_t* out_tokens,
                          int32_t out_cap, uint32_t* seen, dspark_stream_t stream);
-/* out_cap: int32 slots in out_tokens (>= M). A commit that would write past it (State.count + acc + 1 > out_cap)
+/* out_cap: int32 slots in out_tokens (>= M). A commit that would write past it (State.count and what it emits > out_cap)
  * writes nothing and stops the run (State.run = 0), as a launch whose output buffer is full must stop. */
 
 /* ---------------------------------------------------------------- int8-weight verify GEMM

@@ -137,8 +137,9 @@ __device__ __forceinline__ int key_token(uint64_t k) { return (int)(0xffffffffu 
 // The books run on the whole wave: lane l holds the State's header word l, tokens[l], tokens[l + 1] and key l, all
 // requested in the kernel's first round with the run flag and the first batch of partial keys. Acceptance is a ballot
 // over the lanes (lane t < m - 1 misses when token(key t) != tokens[t + 1]; acc = the first miss, else m - 1); lanes
-// 1..acc store the accepted drafts and lane 0 the bonus token, each setting its own seen bit; the header words the
-// books change are stored by lane 0 from registers. No value is read back from memory after the first round.
+// 1..acc store the accepted drafts and lane 0 the bonus token (if that row has one), each setting its own seen bit; the
+// header words the books change are stored by lane 0 from registers. No value is read back from memory after the first
+// round.
 __global__ __launch_bounds__(64) void accept_commit_kernel(dspark_state* st, uint64_t* best, int m, int skip_now,
                                                            int32_t* out_tokens, int out_cap, uint32_t* seen,
                                                            const uint64_t* part, int nchunks, int mfold,
@@ -189,10 +190,15 @@ __global__ __launch_bounds__(64) void accept_commit_kernel(dspark_state* st, uin
   if (part && lane < mfold) best[lane] = key;  // the folded keys
   auto hdr = [&](size_t off) { return __builtin_amdgcn_readlane(hw, (int)(off / sizeof(int32_t))); };
   if (m <= 0) m = hdr(offsetof(dspark_state, M));  // rounds that drafted on the device: the verified count is in the State
-  const uint64_t miss = __builtin_amdgcn_ballot_w64(lane < m - 1 && key_token(key) != tn);
+  const int mine_token = key_token(key);
+  const uint64_t miss = __builtin_amdgcn_ballot_w64(lane < m - 1 && (mine_token != tn || mine_token < 0));
   const int acc = miss ? (int)__builtin_ctzll(miss) : max(m - 1, 0);
-  const int commit = acc + 1;
-  const int bonus = key_token((uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)key, acc));  // the token is the low word
+  // a row without a token (key 0: nothing to draw) ends the commit before it: the drafts up to there are committed, the last of
+  // them (or the anchor) is the next anchor, at the last committed position, and the run stops
+  const int drawn = __builtin_amdgcn_readlane(mine_token, acc);
+  const bool none = drawn < 0;
+  const int commit = acc + (none ? 0 : 1);
+  const int bonus = none ? __builtin_amdgcn_readlane(tk, acc) : drawn;
   const int aa = hdr(offsetof(dspark_state, a));
   const int count = hdr(offsetof(dspark_state, count));
   if (count < 0 || count + commit > out_cap) {  // no room for the commit: write nothing and stop
@@ -201,7 +207,7 @@ __global__ __launch_bounds__(64) void accept_commit_kernel(dspark_state* st, uin
   }
   // lanes 1..acc: the accepted drafts tokens[1..acc] at count..count+acc-1; lane 0: the bonus token after them
   const int val = lane == 0 ? bonus : tk;
-  const bool mine = lane <= acc;
+  const bool mine = lane <= acc && !(none && lane == 0);
   if (mine) {
     out_tokens[lane == 0 ? count + acc : count + lane - 1] = val;
     atomicOr(&seen[val >> 5], 1u << (val & 31));
@@ -227,7 +233,7 @@ __global__ __launch_bounds__(64) void accept_commit_kernel(dspark_state* st, uin
   }
   const int rounds_done = hdr(offsetof(dspark_state, rounds_done)) + 1;
   const int rounds_left = hdr(offsetof(dspark_state, rounds_left)) - 1;
-  const int run1 = (!stop && rounds_left > 0 && a1 < hdr(offsetof(dspark_state, stop_at)) &&
+  const int run1 = (!stop && !none && rounds_left > 0 && a1 < hdr(offsetof(dspark_state, stop_at)) &&
                     count1 < hdr(offsetof(dspark_state, budget)))
                        ? 1
                        : 0;

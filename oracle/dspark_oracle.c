@@ -398,24 +398,27 @@ int32_t orc_argmax_first(const float* lg, int n) {
 
 /* ------------------------------------------------------------------ accept / commit */
 
-/* dspark.hip:2852-2859 (acceptance) and 2880-2913 (books). */
+/* dspark.hip:2852-2859 (acceptance) and 2880-2913 (books). A negative token is a row without one (nothing to draw, which the
+ * reference's argmax never has): it agrees with no draft, and where the bonus would be it the commit ends before it, the last
+ * committed token is the next anchor at its own position, and the run stops. */
 int orc_accept_commit(orc_state* st, const int32_t* best_tok, int m, int skip_now, int32_t* out_tokens, uint32_t* seen) {
   int acc = 0;
   for (int t = 0; t < m - 1; ++t) {
-    if (best_tok[t] != st->tokens[t + 1]) break;
+    if (best_tok[t] < 0 || best_tok[t] != st->tokens[t + 1]) break;
     ++acc;
   }
-  const int commit = acc + 1;
-  const int32_t bonus = best_tok[acc];
+  const int none = best_tok[acc] < 0;
+  const int commit = none ? acc : acc + 1;
+  const int32_t bonus = none ? st->tokens[acc] : best_tok[acc];
   int count = st->count;
   for (int i = 1; i <= acc; ++i) out_tokens[count++] = st->tokens[i];
-  out_tokens[count++] = bonus;
+  if (!none) out_tokens[count++] = bonus;
   for (int i = 1; i <= acc; ++i) {
     const int32_t tk = st->tokens[i];
     seen[tk >> 5] |= 1u << (tk & 31);
   }
-  seen[bonus >> 5] |= 1u << (bonus & 31);
-  int stop = 0;
+  if (!none) seen[bonus >> 5] |= 1u << (bonus & 31);
+  int stop = none;
   if (st->eos >= 0)
     for (int i = count - commit; i < count; ++i) stop = stop || out_tokens[i] == st->eos;
   const int aa = st->a;

@@ -738,6 +738,38 @@ def test_sample_keys_feed_accept_commit():
         assert out[:agree + 1].tolist() == t[:agree + 1]
 
 
+@pytest.mark.parametrize("empty,agree", [(0, 5), (2, 5), (5, 5), (3, 1), (2, 2)])
+@pytest.mark.parametrize("pad", [False, True])
+def test_sample_rows_with_nothing_to_draw_end_a_commit(orc, empty, agree, pad):
+    """A masked row first, in the middle, last, behind the first miss (5 drafts, of which `agree` are their rows' draws; pad: the draft that
+    answers the masked row is -1): State, tokens and bitmap are the oracle's, and the words around the bitmap stay as they are."""
+    h, rng = load_host(), np.random.default_rng(empty)
+    M, V = 6, 4096
+    z = rng.standard_normal((M, V)) * 3
+    z[empty] = -np.inf
+    drawn = h.verify_sample(rows_of("f32", z), dev(rng.random(M).astype(np.float32)), temperature=0.8, top_k=50, keys=True)
+    t = drawn.tokens.tolist()
+    assert t[empty] == -1 and int(drawn.keys[empty]) == 0
+    tokens = [7] + [max(t[i], 0) if i < agree else (t[i] + 1) % V for i in range(M - 1)]
+    if pad and empty < M - 1:
+        tokens[empty + 1] = -1
+    base = dict(a=100, anchor=7, tokens=tokens, rounds_left=32, budget=512, eos=-1, stop_at=128, run=1, skip_rounds=1, count=3)
+    st, out = h.state_tensor(**base), torch.full((64,), -7, dtype=torch.int32, device="cuda")
+    words = torch.full((16 + V // 32 + 16,), 1 << 20, dtype=torch.int32, device="cuda")
+    h.accept_commit(st, drawn.keys, M, out, words[16:16 + V // 32])
+    got = h.state_from_tensor(st)
+    want, wout, wseen = orc.new_state(**base), np.full(64, -7, np.int32), np.full(V // 32, 1 << 20, np.uint32)
+    acc = orc.accept_commit(want, t, M, wout, wseen)
+    assert acc == min(empty, agree) and got.run == (1 if agree < empty else 0)
+    for f in h.STATE_FIELDS:
+        assert getattr(got, f) == getattr(want, f), f
+    assert [got.tokens[i] for i in range(64)] == [want.tokens[i] for i in range(64)]
+    np.testing.assert_array_equal(out.cpu().numpy(), wout)
+    words = words.cpu().numpy()
+    np.testing.assert_array_equal(words[16:-16].view(np.uint32), wseen)
+    assert np.all(words[:16] == 1 << 20) and np.all(words[-16:] == 1 << 20)
+
+
 # ------------------------------------------------------------------------------------------------ together
 @pytest.mark.parametrize("QH,KVH,D", [(32, 8, 64), (16, 4, 128)])
 def test_a_server_step(QH, KVH, D):

@@ -320,6 +320,31 @@ def test_commit_stop_rules(orc):
     assert st.run == 0 and st.rounds_left == 0
 
 
+@pytest.mark.parametrize("empty,acc", [(0, 0), (2, 2), (4, 4), (3, 2)])
+def test_commit_of_rows_without_a_token(orc, empty, acc):
+    """A row with nothing to draw (token -1), first, in the middle, last, behind a miss: the drafts before it are committed, nothing is
+    marked in front of the bitmap, the run stops with the last committed token as the anchor -- or the miss before it counts alone."""
+    tokens, best = [5, 10, 11, 12, 13], [10, 11, 12, 13, 99]
+    best[empty] = -1
+    if acc < empty:
+        best[acc] = 77
+    for draft in (tokens[empty + 1:empty + 2] and tokens[empty + 1], -1):  # a draft of -1 (padding) agrees with no row either
+        toks = list(tokens)
+        if draft == -1 and empty < 4:
+            toks[empty + 1] = -1
+        st = orc.new_state(a=1024, anchor=5, count=2, rounds_left=32, budget=512, eos=-1, stop_at=1056, tokens=toks, run=1, skip_rounds=1)
+        out, words = np.full(16, -7, np.int32), np.full(40, 1 << 31, np.uint32)
+        assert orc.accept_commit(st, best, 5, out, words[8:]) == acc
+        assert np.all(words[:8] == 1 << 31) and np.all(words[12:] == 1 << 31)
+        new = toks[1:1 + acc] + ([77] if acc < empty else [])
+        assert out.tolist() == [-7] * 2 + new + [-7] * (14 - len(new))
+        bits = {t for t in range(96) if (words[8 + t // 32] & ~np.uint32(1 << 31)) >> np.uint32(t % 32) & 1}
+        assert bits == set(new)
+        assert (st.a, st.count, st.ctx_new, st.ctx_pos) == (1024 + len(new), 2 + len(new), len(new), 1024)
+        assert st.anchor == st.tokens[0] == (new[-1] if new else 5)
+        assert st.run == (1 if acc < empty else 0) and st.rounds_done == 1 and st.verified == 5 and st.accepted == acc
+
+
 def test_kv_commit_positions(orc):
     cache = orc.normal_f16(61, (40, 2, 4))
     before = cache.copy()
