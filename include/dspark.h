@@ -290,7 +290,8 @@ int dspark_rope_freqs(int32_t rot, double base, int32_t scaling, double factor, 
  * (m_r <= max_tokens of them), its own keys 0 .. own_len[r] - 1, these tokens' among them: token i is own position
  * own_len[r] - m_r + i and sees the prefix and the own keys before the call's first token -- with window > 0 those of the last
  * `window` positions up to itself, counted through the prefix -- and the call's own keys up to itself (causal) or all. The
- * masks of dspark_verify_attention with a = prefix + own_len[r] - m_r.
+ * masks of dspark_verify_attention with a = prefix + own_len[r] - m_r. Where own_len[r] < m_r the first tokens stand in front of the
+ * own keys and see none of them; the prefix they see as any token does.
  * out and/or out_f32 [tokens][QH][D] = softmax(q k^T / sqrt(D)) v, times sigmoid(gate[t][qh]) if given; lse as in
  * dspark_verify_attention_b8. A table entry outside [0, kv_pages) is an absent page: no row sees its positions. A row that
  * sees no key gives zeros and lse -inf. Rows of q before q_start[0] and behind q_start[seqs], and a sequence's rows past

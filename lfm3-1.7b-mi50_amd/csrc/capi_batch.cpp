@@ -52,7 +52,9 @@ SharedAttn shared_params(const dspark_shared_attn_args* a) {
   p.KVH = a->KVH;
   p.G = a->QH / a->KVH;
   p.g_div = div_magic(p.G);
-  p.window = a->window;
+  // a window of all positions or more is none: the kernels' differences with those that are left (< 3 x 2^29) stay in 32 bits, also
+  // from positions below 0 (of sequences with fewer own keys than tokens)
+  p.window = a->window < (int64_t)a->prefix + (int64_t)a->own_pages * DSPARK_PAGE_TOKENS ? a->window : 0;
   p.causal = a->causal ? 1 : 0;
   shared_plan(p, a->D, a->splits, device_cus());
   return p;

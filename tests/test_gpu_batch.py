@@ -289,6 +289,20 @@ def test_shared_windows(D, window, causal):
     b.check(window=window, causal=causal)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("prefix,m,lens", [(10, [20], [0]), (300, [20, 3, 9], [0, 3, 200]), (90, [1] * 30, [0] * 30), (1, [300], [2])])
+def test_shared_windows_past_every_position(D, prefix, m, lens):
+    """A window of at least all positions is none, bit for bit, up to the largest one and for sequences with fewer own keys than tokens: those
+    in front of the first own key see the whole prefix."""
+    b = Batch(prefix, 4, 2, D, prefix, m, lens)
+    for causal in (True, False):
+        want = b.run(causal=causal)
+        if not causal:
+            b.close(*want, *b.oracle(causal=False))
+        for window in (prefix + 300, 5000, 1 << 30, 3 << 29, (1 << 31) - 5, (1 << 31) - 1):
+            assert all(torch.equal(x, y) for x, y in zip(b.run(window=window, causal=causal), want)), window
+
+
 @pytest.mark.parametrize("QH,KVH,D", [(32, 8, 64), (16, 4, 128)])
 @pytest.mark.parametrize("seqs,tokens", [(1, 4), (8, 1), (12, 2), (5, 7), (17, 4), (33, 4), (65, 3)])
 def test_shared_row_blocks(QH, KVH, D, seqs, tokens):
