@@ -244,8 +244,8 @@ size_t dspark_kv_evict_b8_workspace(int32_t KVH, int32_t length);
  *   y_i = s (x_i cos - x_j sin), y_j = s (x_j cos + x_i sin)     (inverse: by the negative angle: the rotation's backward pass)
  * and the rest of the head is passed on. Angles are products in 64 bits, sines and cosines rounded to fp32 once, products fp32,
  * one rounding to the type. q and k (either may be NULL with 0 heads) have one type, n rows of heads x D values each, rows their
- * stride apart; a stride may be any number of elements >= heads x D. An output may be its input itself (same address and
- * stride); otherwise nothing written shares a byte with anything else (DSPARK_EINVAL).
+ * stride apart; a stride may be any number of elements from heads x D to 2^30 - 1. An output may be its input itself (same
+ * address and stride); otherwise nothing written shares a byte with anything else (DSPARK_EINVAL).
  * With k_pages (fp16 only, D in {64, 128}, not inverse) the turned K rows and the rows of v go into the fp16 pages instead of
  * k_out (NULL then): row t to slot slots[t] = 32 x physical page + position within it; a slot outside [0, 32 kv_pages) is not
  * written. Pools may pass 4 GiB; no two rows may have the same slot. One launch for a batch's q, K and V. n = 0 does nothing.
@@ -303,7 +303,7 @@ int dspark_rope_freqs(int32_t rot, double base, int32_t scaling, double factor, 
  * calls. What is written shares no byte with anything else (DSPARK_EINVAL). tokens = 0 or seqs = 0 does nothing. */
 typedef struct dspark_shared_attn_args {
   const void* q;               /* fp16 [tokens][q_stride] (head qh at qh D; 16-byte boundary, q_stride a multiple of 8) */
-  int64_t q_stride;            /* >= QH D */
+  int64_t q_stride;            /* >= QH D, < 2^30 */
   const void* k_pages;         /* on 16-byte boundaries */
   const void* v_pages;
   int64_t kv_pages;            /* pages in each pool, < 2^31 */
@@ -311,7 +311,7 @@ typedef struct dspark_shared_attn_args {
   const int32_t* q_start;      /* device [seqs + 1] */
   const int32_t* own_len;      /* device [seqs] */
   const int32_t* own_table;    /* device [seqs][own_stride] */
-  int64_t own_stride;          /* >= own_pages */
+  int64_t own_stride;          /* >= own_pages, < 2^30 */
   void* out;                   /* fp16 or NULL; outputs on 16-byte boundaries */
   float* out_f32;              /* or NULL */
   float* lse;                  /* fp32 [tokens][QH] or NULL */
@@ -344,7 +344,7 @@ int dspark_verify_attention_shared(const dspark_shared_attn_args* args, dspark_s
  * The workspace needs no clearing. The reference samples on the host (internal/sample, Draw, sample.go:176-234). */
 typedef struct dspark_sample_args {
   const void* logits;          /* [n][row_stride] of `type` */
-  int64_t row_stride;          /* elements between rows, >= V */
+  int64_t row_stride;          /* elements between rows, >= V, < 2^30 */
   const float* u;              /* [n]; cut to [0, 1) (NaN: 0) */
   const float* temperature;    /* [n] or NULL */
   const int32_t* top_k;

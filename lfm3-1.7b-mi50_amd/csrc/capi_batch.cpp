@@ -107,8 +107,10 @@ int dspark_rope(const dspark_rope_args* a, dspark_stream_t stream) {
     return DSPARK_EINVAL;
   if (a->D < 2 || a->D > 1024 || a->D % 2 || a->rot < 2 || a->rot > a->D || a->rot % 2) return DSPARK_EINVAL;
   if (a->type != DSPARK_F16 && a->type != DSPARK_BF16 && a->type != DSPARK_F32) return DSPARK_EINVAL;
-  if (std::max({a->q_stride, a->q_out_stride, a->k_stride, a->k_out_stride, a->v_stride}) >= STRIDE_MAX) return DSPARK_EINVAL;
   const bool append = a->k_pages || a->v_pages;
+  // (the strides of what is not there are not looked at)
+  if ((a->QH && std::max(a->q_stride, a->q_out_stride) >= STRIDE_MAX) || (a->KVH && a->k_stride >= STRIDE_MAX)) return DSPARK_EINVAL;
+  if (a->KVH && (append ? a->v_stride : a->k_out_stride) >= STRIDE_MAX) return DSPARK_EINVAL;
   if (a->n == 0) return 0;
   const size_t size = a->type == DSPARK_F32 ? 4 : 2;
   if (!on(a->positions, 4) || !on(a->freq, 8)) return DSPARK_EINVAL;

@@ -115,6 +115,30 @@ def test_rope_not_finite_and_nothing():
     assert q.shape == (0, 2, 16) and k.shape == (0, 1, 16)
 
 
+def test_rope_strides_of_what_is_not_there():
+    """q alone, k alone and the pages: the strides of the rest may hold anything."""
+    h, n, D, any_ = load_host(), 3, 64, 1 << 40
+    x, pos, f = torch.randn((n, 2, D), device="cuda").half(), torch.arange(n, dtype=torch.int32, device="cuda"), dev(batch.rope_freqs(D, 1e4)[0])
+    want, _ = h.rope(x, None, pos, f)
+    common = dict(positions=pos.data_ptr(), freq=f.data_ptr(), scale=1.0, n=n, D=D, rot=D)
+    stream = torch.cuda.current_stream().cuda_stream
+    for t, other in (("q", "k"), ("k", "q")):
+        y = torch.zeros_like(x)
+        heads = {"QH" if t == "q" else "KVH": 2}
+        a = h.RopeArgs(**{t: x.data_ptr(), t + "_out": y.data_ptr(), t + "_stride": 128, t + "_out_stride": 128, other + "_stride": any_,
+                          other + "_out_stride": any_}, v_stride=any_, **heads, **common)
+        assert h.lib().dspark_rope(a, stream) == 0
+        assert torch.equal(y, want)
+    kp, vp = h.kv_pages_alloc(1, 2, D)
+    slots = torch.arange(n, device="cuda")
+    a = h.RopeArgs(k=x.data_ptr(), k_stride=128, k_out_stride=any_, q_stride=any_, q_out_stride=any_, v=x.data_ptr(), v_stride=128, KVH=2,
+                   k_pages=kp.data_ptr(), v_pages=vp.data_ptr(), slots=slots.data_ptr(), kv_pages=1, **common)
+    assert h.lib().dspark_rope(a, stream) == 0
+    k1, v1 = h.kv_from_pages(kp, vp, range(n))
+    np.testing.assert_array_equal(k1, want.cpu().numpy())
+    np.testing.assert_array_equal(v1, x.cpu().numpy())
+
+
 @pytest.mark.parametrize("interleaved", [False, True])
 def test_rope_gradient(interleaved):
     """The inverse is the backward pass: <rope(x), g> = <x, inverse(g)>, by the formula's autograd and by differences (rope is linear, so a
