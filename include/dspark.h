@@ -277,7 +277,7 @@ int dspark_rope(const dspark_rope_args* args, dspark_stream_t stream);
  *   DSPARK_ROPE_PLAIN   as they are;   DSPARK_ROPE_LINEAR   divided by factor;
  *   DSPARK_ROPE_BASE    with base x factor^(rot / (rot - 2)) instead of base: the slowest pair divided by factor, the first kept;
  *   DSPARK_ROPE_RAMP    pairs that make at most `low` turns in `trained` positions divided by factor, those of at least `high`
- *                       turns kept, a linear ramp between; *scale (else 1) = 0.1 ln(factor) + 1 for factor > 1.
+ *                       turns kept, a ramp linear in the turns between; *scale (else 1) = 0.1 ln(factor) + 1 for factor > 1.
  * scale may be NULL. factor >= 1. */
 enum { DSPARK_ROPE_PLAIN = 0, DSPARK_ROPE_LINEAR = 1, DSPARK_ROPE_BASE = 2, DSPARK_ROPE_RAMP = 3 };
 int dspark_rope_freqs(int32_t rot, double base, int32_t scaling, double factor, double trained, double low, double high,
@@ -333,13 +333,14 @@ int dspark_verify_attention_shared(const dspark_shared_attn_args* args, dspark_s
  * w_i = exp((z_i - max z) / T), tokens are ranked by z descending, the lowest index first among equal ones; kept are those of
  *   rank < top_k (top_k <= 0 or >= V: all), then with less than top_p x (the weight of those) in front of them (top_p >= 1: all;
  *   the first always), and z_i >= max z + T ln(min_p) (min_p <= 0: all);
- * the token is the first kept one, by index, at which the kept weights' running sum exceeds u times their whole sum. T <= 0 is
- * greedy: the first maximum. NaN and -inf are never drawn; +inf shares the weight with the other +inf alone. A row with
+ * the token is the first kept one, by index, at which the kept weights' running sum exceeds u times their whole sum. T <= 0 (or
+ * NaN) is greedy: the first maximum. NaN and -inf are never drawn; +inf shares the weight with the other +inf alone. A row with
  * nothing to draw gives token -1, kept 0, logprob -inf, key 0. Weights are whole numbers, the largest 2^44 - 2^24, and their
  * sums whole 64-bit ones, so a draw does not depend on the order of the work: the same inputs give the same token always.
- * keys are what dspark_accept_commit takes: the round of drafts that agree with their row's draw is accepted. For drafts that are
- * chosen without randomness, as the drafter's are, that is speculative sampling exactly: a draft is accepted with its
- * probability under the target, and the first token that differs is distributed as the target's with the draft taken out.
+ * keys are what dspark_accept_commit takes (a row with nothing to draw ends its commit): the round of drafts that agree
+ * with their row's draw is accepted. For drafts that are chosen without randomness, as the drafter's are, that is speculative
+ * sampling exactly: a draft is accepted with its probability under the target, and the first token that differs is
+ * distributed as the target's with the draft taken out. No repetition penalty is applied.
  * Per-row settings are device arrays [n]; where a pointer is NULL the value beside it holds for every row. n = 0 does nothing.
  * The workspace needs no clearing. The reference samples on the host (internal/sample, Draw, sample.go:176-234). */
 typedef struct dspark_sample_args {
@@ -352,7 +353,7 @@ typedef struct dspark_sample_args {
   const float* min_p;
   int32_t* tokens;             /* [n] or NULL */
   uint64_t* keys;              /* [n] or NULL: argmax-style keys, dspark_key_token() gives the token */
-  int32_t* kept;               /* [n] or NULL: how many tokens could have been drawn */
+  int32_t* kept;               /* [n] or NULL: how many tokens the cuts leave (those too light to be drawn among them) */
   float* logprob;              /* [n] or NULL: ln of the probability with which the token was drawn */
   void* workspace;             /* on a 16-byte boundary */
   size_t workspace_bytes;      /* dspark_verify_sample_workspace(n, V) */

@@ -18,12 +18,14 @@
 //
 // What bounds it. Few rows: the chain of launch, table, first pages, sums and second launch (4 rows of 1001 + 37 keys, 4 x 128: 7.1 + 4.1
 // us). A long prefix of 128 rows (8 x 64, 32768 keys and 32 sequences' own): 82 MB fetched in 26 us, 3.2 TB/s, ~4 of them before the
-// first page is there. Many rows: issue; 1024 rows x 131072 keys of 8 x 64 take 212-235 us, 740-810 TFLOP/s. A page of 32 rows costs a wave some 110 vector
-// instructions beside 16 products of matrix instructions (16 exponentials, multiply-adds, additions, 14 maxima, 16 roundings,
-// addresses and bookkeeping), which hardly run side by side: matrix cores 36 %, vector units 68 % of the time at a clock of
-// 1.7-2.1 GHz. Measured and not kept there: a third or fourth slot in the ring (229 -> 225 us, shorter calls slower), two pages'
-// softmax at once (237, spills at D = 128), four row blocks a wave, wave priorities, one workgroup of 64 rows instead of two of 32
-// for a sequence's own keys (27.7 -> 27.7 at 36 rows a sequence).
+// first page is there. Many rows: issue; 640 rows of each head x 131072 keys of 8 x 64 take 212-235 us, 740-810 TFLOP/s. A page of
+// 32 rows costs a wave some 110 vector instructions beside 16 products of matrix instructions (16 exponentials, multiply-adds,
+// additions, 14 maxima, 16 roundings, addresses and bookkeeping), which follow each other in its program and hardly run side by side:
+// matrix cores 36 %, vector units 68 % of the time at a clock of 1.7-2.1 GHz. That is the schedule's limit, neither unit's own.
+// With a window the prefix is split as without one and the workgroups before it find nothing to do: 32 rows of 131072 keys, 4096 of
+// them seen, take 77 us, all of them 84, a prefix of 4096 keys 20. Measured and not kept, of many rows: a third or fourth slot in the ring
+// (229 -> 225 us, shorter calls slower), two pages' softmax at once (237, spills at D = 128), four row blocks a wave, wave priorities,
+// one workgroup of 64 rows instead of two of 32 for a sequence's own keys (27.7 -> 27.7 at 36 rows a sequence).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>

@@ -744,7 +744,8 @@ def _rope(s, a, q, k, q_out, k_out):
 def rope(q, k, positions, freqs, interleaved=False, inverse=False, scale=1.0, q_out=None, k_out=None, stream=None):
     """Turn the first 2 * len(freqs) values of every head of q and k (either may be None; [n][heads][D] fp16, bf16 or fp32, rows may
     lie inside wider ones) by positions (int32 [n]) times freqs (float64, rope_freqs). inverse: by the negative angles, which is
-    the gradient's way back. Returns (q_out, k_out) as given (q itself: in place) or created."""
+    the gradient's way back (nothing is recorded for autograd: a training program makes that call in its own backward). Returns
+    (q_out, k_out) as given (q itself: in place) or created."""
     a = _rope_args(q, k, positions, freqs, interleaved, inverse, scale)
     return _on_device(q if q is not None else k, stream, _rope, a, q, k, q_out, k_out)
 
