@@ -476,6 +476,8 @@ struct SampleCut {
   __device__ __forceinline__ bool keeps(uint32_t k, uint32_t i) const { return k > key || (k == key && i <= idx); }
 };
 
+// What the helpers below share. Each may write any of it at once, so whoever reads a word has a barrier between that and the next helper:
+// its own before it returns false, the sums' of the code behind it after sp_rank and a narrowed list.
 struct SampleShared {
   alignas(16) uint64_t mass[256];
   alignas(16) uint64_t key[SP_SMALL];
